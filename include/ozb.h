@@ -212,6 +212,65 @@ int ozb_ddgemm_ex(int M, int N, int K, const double *Ah, const double *Al, long 
 int ozb_bf16_fp8_gemm(int M, int N, int K, const void *X, const void *W, const float *S, float *Y, int *open, int *moduli,
                       void *stream);
 
+/* ---- microscaled 4-bit operands and experts ---------------------------------------------------------------------
+ * What the reference's language-model programs use beside the FP8 product (llm/mxexact.cu works on such operands, llm/moe*.cu
+ * on experts; separate programs there, no ABI), as operators on device buffers. All are asynchronous on `stream`, allocate
+ * nothing (but one status word per device at the first product), keep nothing between calls and may be captured.
+ *
+ * Element types of dense operands: */
+enum { OZB_F32 = 0, OZB_BF16 = 1, OZB_F16 = 2 };
+/* The 4-bit format (OCP microscaling, MXFP4): vectors in blocks of 32 values; a value is a code of 4 bits (a sign, then 0, 0.5, 1,
+ * 1.5, 2, 3, 4, 6) times the block's power of two 2^(s - 127), s one byte (255: the block is not a number). Row-major: row r of
+ * the codes at codes + r * ldq (two codes to a byte, the earlier one in the low half), its scales at scales + r * lds (bytes,
+ * one to a block). `codes` 16-byte and `scales` 8-byte aligned, ldq a multiple of 16, lds of 8; a row has room for ceil(len / 32)
+ * whole blocks, and the codes behind `len` in the last one are 0.
+ *
+ * ozb_mx4_quantize: `nvec` vectors of `len` values of X to that format, nearest code, ties to the even one. by_rows = 1: the rows of
+ * X (pitch ldx); by_rows = 0: the columns of a row-major len x nvec X, which come out as rows. rule 0: the block's scale is
+ * 2^(floor(log2 amax) - 2), values above 6 of it saturate; rule 1: the smallest power of two with amax <= 6 of it. Scales stay
+ * within 2^-127 .. 2^127. A block that holds an infinity or a NaN gets s = 255 and codes 0. `slots` (may be NULL) takes the
+ * rows of X through the map of ozb_expert_sort: row r of the matrix that is quantised is row slots[r] / per of X, or zeros where
+ * slots[r] is negative or the row is not below `sources`. planes > 1 (without slots): that many matrices, plane_x elements,
+ * plane_q and plane_s bytes apart (multiples of 16 and 8). The gradient is passed through (straight-through), no call needed. */
+int ozb_mx4_quantize(const void *X, int type, int nvec, int len, long long ldx, int by_rows, int rule, const int *slots, int per, int sources,
+                     int planes, size_t plane_x, uint8_t *codes, long long ldq, size_t plane_q, uint8_t *scales, long long lds,
+                     size_t plane_s, void *stream);
+/* the values that codes and scales stand for, rounded to `type` (exact in FP32 and BF16); NaN for a block with s = 255 */
+int ozb_mx4_dequantize(const uint8_t *codes, long long ldq, const uint8_t *scales, long long lds, int nvec, int len, void *Y, int type,
+                       long long ldy, void *stream);
+/* Y = X W^T: X is M x K, W is N x K, both 4-bit with blocks along K; Y is M x N of `type`, summed in FP32 and rounded once. Gradients
+ * are the same call: dX = dY W from dY by rows and W by columns, dW = dY^T X from both by columns. */
+int ozb_mx4_gemm(int M, int N, int K, const uint8_t *X, long long ldx, const uint8_t *Xs, long long ldxs, const uint8_t *W, long long ldw,
+                 const uint8_t *Ws, long long ldws, void *Y, int type, long long ldy, void *stream);
+/* Rows [offsets[g], offsets[g + 1]) of X (R x K) with W[g] (N x K, plane_w / plane_ws bytes from one to the next). `offsets` is on the
+ * device, groups + 1 numbers that do not decrease; rows of Y outside of them stay as they were. At most 1024 groups. */
+int ozb_mx4_gemm_grouped(int groups, int R, int N, int K, const int *offsets, const uint8_t *X, long long ldx, const uint8_t *Xs, long long ldxs,
+                         const uint8_t *W, long long ldw, size_t plane_w, const uint8_t *Ws, long long ldws, size_t plane_ws, void *Y, int type,
+                         long long ldy, void *stream);
+/* Y[g] = A[:, offsets[g] : offsets[g + 1]] B[:, the same]^T: A is M x R, B is N x R, blocks along R; Y[g] is M x N, plane_y elements
+ * from one to the next, zeros for an empty segment. The offsets are multiples of 64 (they are rounded down to one). At most 1024. */
+int ozb_mx4_gemm_segments(int groups, int M, int N, int R, const int *offsets, const uint8_t *A, long long lda, const uint8_t *As, long long ldas,
+                          const uint8_t *B, long long ldb, const uint8_t *Bs, long long ldbs, void *Y, int type, long long ldy, size_t plane_y,
+                          void *stream);
+/* Each of T tokens goes to `top` experts: slot t * top + j to expert ids[t][j] (id_bytes 4 or 8; a number outside 0 .. experts - 1
+ * drops the slot). ozb_expert_sort lays the slots out by expert, in their order, each expert's segment padded to a multiple of
+ * `align` (1 .. 256) rows: offsets [experts + 1], rows [T][top] (the row of a slot, -1 if dropped), slots [R] (the slot of a row,
+ * -1 if none). R is at least ozb_expert_sort_rows; scratch at least ozb_expert_sort_scratch bytes (which may be 0). At most 1024
+ * experts. ozb_expert_sort_rows returns a negative error code for sizes that are refused. */
+long long ozb_expert_sort_rows(int T, int top, int experts, int align);
+size_t ozb_expert_sort_scratch(int T, int top, int experts);
+int ozb_expert_sort(int T, int top, int experts, const void *ids, int id_bytes, int align, int R, int *offsets, int *rows, int *slots, void *scratch,
+                    size_t scratch_bytes, void *stream);
+/* Y[r] = X[slots[r] / top] (T x H to R x H), zeros where there is no slot. Its gradient is ozb_expert_combine without weights. */
+int ozb_expert_gather(int R, int H, const void *X, int type, long long ldx, int T, const int *slots, int top, void *Y, long long ldy, void *stream);
+/* Y[t] = sum over j of weights[t][j] Z[rows[t][j]] (weights NULL: 1), in FP32 in the order of j; dropped slots count nothing. */
+int ozb_expert_combine(int T, int top, int H, const void *Z, int type, int R, long long ldz, const int *rows, const float *weights, void *Y,
+                       long long ldy, void *stream);
+/* The gradients of that: dZ[r] = weights[s] dY[s / top] with s = slots[r] (zeros where there is none), dweights[s] = <dY[s / top],
+ * Z[rows[s]]> (0 for a dropped slot). dZ is neither dY nor Z. */
+int ozb_expert_combine_grad(int T, int top, int H, const void *dY, int type, long long lddy, const void *Z, long long ldz, int R, const int *rows,
+                            const int *slots, const float *weights, void *dZ, long long lddz, float *dweights, void *stream);
+
 /* The four stages on caller-owned device buffers (what bench/phases.cu launches one by one). Asynchronous.
  * Pitches: ld of int8 planes in bytes and a multiple of 16; `plane` = distance between planes in elements. */
 /* src/ozaki2.cuh:56-78 -- scales + residues of an A-like operand (rows of `len` contiguous doubles, pitch ldx) */

@@ -63,6 +63,19 @@ lib.ozb_gemm_i8_mod.argtypes = [_p, _p, _p, _i, _i, _i, _i, _ll, _ll, _ll, _sz, 
 lib.ozb_gemm_i8_mod_beside.argtypes = [_p, _p, _p, _i, _i, _i, _i, _ll, _ll, _ll, _sz, _sz, _sz, _i, _i, _p, _p]
 lib.ozb_crt_i32.argtypes = [_i, _p, _sz, _i, _i, _ll, _p, _p, _p, _ll, _p]
 lib.ozb_crt_i8.argtypes = [_i, _p, _sz, _i, _i, _ll, _p, _p, _p, _ll, _p]
+lib.ozb_mx4_quantize.argtypes = [_p, _i, _i, _i, _ll, _i, _i, _p, _i, _i, _i, _sz, _p, _ll, _sz, _p, _ll, _sz, _p]
+lib.ozb_mx4_dequantize.argtypes = [_p, _ll, _p, _ll, _i, _i, _p, _i, _ll, _p]
+lib.ozb_mx4_gemm.argtypes = [_i] * 3 + [_p, _ll] * 4 + [_p, _i, _ll, _p]
+lib.ozb_mx4_gemm_grouped.argtypes = [_i] * 4 + [_p] + [_p, _ll] * 2 + [_p, _ll, _sz] * 2 + [_p, _i, _ll, _p]
+lib.ozb_mx4_gemm_segments.argtypes = [_i] * 4 + [_p] + [_p, _ll] * 4 + [_p, _i, _ll, _sz, _p]
+lib.ozb_expert_sort_rows.restype = _ll
+lib.ozb_expert_sort_rows.argtypes = [_i] * 4
+lib.ozb_expert_sort_scratch.restype = _sz
+lib.ozb_expert_sort_scratch.argtypes = [_i] * 3
+lib.ozb_expert_sort.argtypes = [_i] * 3 + [_p, _i, _i, _i, _p, _p, _p, _p, _sz, _p]
+lib.ozb_expert_gather.argtypes = [_i, _i, _p, _i, _ll, _i, _p, _i, _p, _ll, _p]
+lib.ozb_expert_combine.argtypes = [_i] * 3 + [_p, _i, _i, _ll, _p, _p, _p, _ll, _p]
+lib.ozb_expert_combine_grad.argtypes = [_i] * 3 + [_p, _i, _ll, _p, _ll, _i, _p, _p, _p, _p, _ll, _p, _p]
 lib.ozb_int8_peak.argtypes = [_i, _i, ctypes.POINTER(ctypes.c_float), ctypes.POINTER(ctypes.c_double)]
 lib.ozb_selftest_wait_expiry.argtypes = [_i]
 lib.ozb_dgemm_mg.argtypes = [_i] * 3 + [_p] * 3 + [_i] * 3
@@ -88,5 +101,7 @@ SYMBOLS = [
     "ozb_plan_panel", "ozb_plan_b_begin", "ozb_plan_b_rows", "ozb_plan_b_finish", "ozb_plan_multiply", "ozb_cols_absmax", "ozb_plan_b_rows_residues", "ozb_plan_view", "ozb_plan_status", "ozb_plan_profile", "ozb_plan_phase_ms", "ozb_plan_kernel_ms", "ozb_dgemm_ex", "ozb_dgemm_norm", "ozb_scales_norm", "ozb_ddgemm_ex", "ozb_bf16_fp8_gemm",
     "ozb_scale_residues_rows", "ozb_scale_residues_cols", "ozb_scale_residues_cols_static", "ozb_gemm_i8", "ozb_gemm_i8_mod", "ozb_gemm_i8_mod_beside", "ozb_crt_i32", "ozb_crt_i8",
     "ozb_status", "ozb_int8_peak", "ozb_selftest_wait_expiry", "ozb_bounds_report", "ozb_selftest_bounds",
+    "ozb_mx4_quantize", "ozb_mx4_dequantize", "ozb_mx4_gemm", "ozb_mx4_gemm_grouped", "ozb_mx4_gemm_segments",
+    "ozb_expert_sort_rows", "ozb_expert_sort_scratch", "ozb_expert_sort", "ozb_expert_gather", "ozb_expert_combine", "ozb_expert_combine_grad",
     "ozb_dgemm_mg", "ozb_mg_release", "ozb_mg_unique_id", "ozb_mg_create", "ozb_mg_destroy", "ozb_mg_dgemm", "ozb_mg_wait", "ozb_mg_info", "ozb_mg_schedule", "ozb_mg_schedule_pieces",
 ]

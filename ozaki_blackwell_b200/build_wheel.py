@@ -15,7 +15,7 @@ import zipfile
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 NAME = "ozaki_blackwell_b200"
-PY_FILES = ("__init__.py", "__main__.py", "_lib.py", "dist.py", "gemm_bench.py", "exact_f8_bench.py")
+PY_FILES = ("__init__.py", "__main__.py", "_lib.py", "dist.py", "mx4.py", "experts.py", "gemm_bench.py", "exact_f8_bench.py")
 LIB = "libozaki_blackwell.so"
 
 

@@ -404,14 +404,44 @@ template <class F> int ordered_on_cached_plan(ozb_plan *p, cudaStream_t st, F &&
     return (int)cudaEventRecord(p->evDone, st);
 }
 int finish() { const int e = (int)cudaDeviceSynchronize(); return e ? e : (int)cudaGetLastError(); }   // python/capi.cu:49
+// Made at the first call on a device, which may come while the caller captures a stream: the allocation and its clearing are kept out
+// of the capture (relaxed mode for this thread, a stream of their own).
 int *status_word() {
+    static std::mutex once;
     int dev = 0;
     if (cudaGetDevice(&dev) || dev < 0 || dev >= 64) return nullptr;
+    std::lock_guard<std::mutex> g(once);
     if (!stage_status[dev]) {
-        if (cudaMalloc(&stage_status[dev], 256) || cudaMemset(stage_status[dev], 0, 256)) { cudaGetLastError(); stage_status[dev] = nullptr; }
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+        cudaThreadExchangeStreamCaptureMode(&mode);
+        cudaStream_t st = nullptr;
+        int *p = nullptr;
+        cudaError_t e = cudaMalloc(&p, 256);
+        if (!e) e = cudaStreamCreateWithFlags(&st, cudaStreamNonBlocking);
+        if (!e) e = cudaMemsetAsync(p, 0, 256, st);
+        if (!e) e = cudaStreamSynchronize(st);
+        if (st) cudaStreamDestroy(st);
+        cudaThreadExchangeStreamCaptureMode(&mode);
+        if (e) { cudaGetLastError(); cudaFree(p); return nullptr; }
+        stage_status[dev] = p;
     }
     return stage_status[dev];
 }
+// what check_args says of the device, for the entry points whose sizes are checked apart
+int check_device() {
+    int dev, major;
+    if (cudaGetDevice(&dev) || cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev)) return (int)cudaGetLastError();
+    return major != 10 ? OZB_EARCH : 0;
+}
+bool off(const void *p, unsigned to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) != 0; }   // not aligned
+// a 4-bit operand: rows of `len` values, codes and scales
+bool bad_mx4(const void *codes, long long ldq, const void *scales, long long lds, int len) {
+    return !codes || !scales || off(codes, 16) || off(scales, 8) || (ldq & 15) || (lds & 7) || ldq < ((long long)len + 31) / 32 * 16 ||
+           lds < ((long long)len + 31) / 32;
+}
+constexpr int MAX_LEN = 0x7fffffff - 1023;   // lengths are rounded up in 32 bits
+bool bad_type(int type) { return type < OZB_F32 || type > OZB_F16; }
+bool off_type(const void *p, int type) { return off(p, type == OZB_F32 ? 4 : 2); }
 }  // namespace
 
 OZB_API const char *ozb_version(void) { return OZB_VERSION; }
@@ -826,6 +856,110 @@ OZB_API int ozb_bf16_fp8_gemm(int M, int N, int K, const void *X, const void *W,
     if (!X || !W || !S || !Y) return OZB_EARG;
     std::lock_guard<std::mutex> g(mu);
     return exact_bf16_fp8_gemm(M, N, K, (const uint16_t *)X, K, (const uint8_t *)W, N, S, Y, N, open, moduli, (cudaStream_t)stream);
+}
+
+// ---- microscaled 4-bit format -------------------------------------------------------------------------------------
+OZB_API int ozb_mx4_quantize(const void *X, int type, int nvec, int len, long long ldx, int by_rows, int rule, const int *slots, int per, int sources,
+                             int planes, size_t plane_x, uint8_t *codes, long long ldq, size_t plane_q, uint8_t *scales, long long lds,
+                             size_t plane_s, void *stream) {
+    if (nvec <= 0 || len <= 0 || len > MAX_LEN || nvec > MAX_LEN || planes <= 0 || !X || bad_type(type) || off_type(X, type) || (rule != 0 && rule != 1) ||
+        ldx < (by_rows ? len : nvec) || bad_mx4(codes, ldq, scales, lds, len))
+        return OZB_EARG;
+    if (slots && (per <= 0 || sources <= 0 || planes > 1 || off(slots, 4))) return OZB_EARG;
+    if (planes > 1 && ((plane_q & 15) || (plane_s & 7))) return OZB_EARG;
+    if (int e = check_device()) return e;
+    if (planes == 1) plane_x = plane_q = plane_s = 0;
+    return (int)(by_rows ? mx4_quantize_rows : mx4_quantize_cols)(X, type, nvec, len, ldx, plane_x, planes, rule, slots, per, sources, codes, ldq,
+                                                                 plane_q, scales, lds, plane_s, (cudaStream_t)stream);
+}
+OZB_API int ozb_mx4_dequantize(const uint8_t *codes, long long ldq, const uint8_t *scales, long long lds, int nvec, int len, void *Y, int type,
+                               long long ldy, void *stream) {
+    if (nvec <= 0 || len <= 0 || len > MAX_LEN || !Y || bad_type(type) || off_type(Y, type) || ldy < len || bad_mx4(codes, ldq, scales, lds, len)) return OZB_EARG;
+    if (int e = check_device()) return e;
+    return (int)mx4_dequantize(codes, ldq, scales, lds, nvec, len, Y, type, ldy, (cudaStream_t)stream);
+}
+static int run_mx4(const Mx4Product &g, void *stream) {
+    if (int e = check_device()) return e;
+    int *st = status_word();
+    if (!st) return (int)cudaErrorMemoryAllocation;
+    const int e = (int)mx4_product(g, st, (cudaStream_t)stream);
+    return e == (int)cudaErrorInvalidValue ? OZB_ESIZE : e;   // a tile count or an extent beyond what a launch or a tensor map holds
+}
+OZB_API int ozb_mx4_gemm(int M, int N, int K, const uint8_t *X, long long ldx, const uint8_t *Xs, long long ldxs, const uint8_t *W, long long ldw,
+                         const uint8_t *Ws, long long ldws, void *Y, int type, long long ldy, void *stream) {
+    if (M <= 0 || N <= 0 || K <= 0 || K > MAX_LEN || N > MAX_LEN || M > MAX_LEN || bad_type(type) || !Y || off_type(Y, type) || ldy < N || bad_mx4(X, ldx, Xs, ldxs, K) ||
+        bad_mx4(W, ldw, Ws, ldws, K))
+        return OZB_EARG;
+    return run_mx4({0, 1, N, M, K, type, nullptr, W, Ws, X, Xs, ldw, ldws, ldx, ldxs, 0, 0, Y, ldy, 0}, stream);
+}
+OZB_API int ozb_mx4_gemm_grouped(int groups, int R, int N, int K, const int *offsets, const uint8_t *X, long long ldx, const uint8_t *Xs, long long ldxs,
+                                 const uint8_t *W, long long ldw, size_t plane_w, const uint8_t *Ws, long long ldws, size_t plane_ws, void *Y, int type,
+                                 long long ldy, void *stream) {
+    if (groups <= 0 || R <= 0 || N <= 0 || K <= 0 || K > MAX_LEN || N > MAX_LEN || R > MAX_LEN || !offsets || off(offsets, 4) || bad_type(type) || !Y ||
+        off_type(Y, type) || ldy < N || bad_mx4(X, ldx, Xs, ldxs, K) || bad_mx4(W, ldw, Ws, ldws, K) || (groups > 1 && ((plane_w & 15) || (plane_ws & 7))))
+        return OZB_EARG;
+    if (groups > 1024) return OZB_ESIZE;
+    return run_mx4({1, groups, N, R, K, type, offsets, W, Ws, X, Xs, ldw, ldws, ldx, ldxs, plane_w, plane_ws, Y, ldy, 0}, stream);
+}
+OZB_API int ozb_mx4_gemm_segments(int groups, int M, int N, int R, const int *offsets, const uint8_t *A, long long lda, const uint8_t *As, long long ldas,
+                                  const uint8_t *B, long long ldb, const uint8_t *Bs, long long ldbs, void *Y, int type, long long ldy, size_t plane_y,
+                                  void *stream) {
+    if (groups <= 0 || M <= 0 || N <= 0 || R <= 0 || M > MAX_LEN || N > MAX_LEN || R > MAX_LEN || !offsets || off(offsets, 4) || bad_type(type) || !Y ||
+        off_type(Y, type) || ldy < N || bad_mx4(A, lda, As, ldas, R) || bad_mx4(B, ldb, Bs, ldbs, R))
+        return OZB_EARG;
+    if (groups > 1024) return OZB_ESIZE;
+    return run_mx4({2, groups, N, M, R, type, offsets, B, Bs, A, As, ldb, ldbs, lda, ldas, 0, 0, Y, ldy, plane_y}, stream);
+}
+
+// ---- tokens by expert ---------------------------------------------------------------------------------------------
+static long long sorted_rows(long long slots, int experts, int align) {   // the most rows that the padded segments take
+    return (slots + (slots < experts ? slots : experts) * (align - 1)) / align * align;
+}
+static bool bad_slots(int T, int top) { return T <= 0 || top <= 0 || (long long)T * top > MAX_LEN; }
+OZB_API long long ozb_expert_sort_rows(int T, int top, int experts, int align) {
+    if (bad_slots(T, top) || experts <= 0 || experts > 1024 || align <= 0 || align > 256) return -OZB_EARG;
+    return sorted_rows((long long)T * top, experts, align);
+}
+OZB_API size_t ozb_expert_sort_scratch(int T, int top, int experts) {
+    if (bad_slots(T, top) || experts <= 0 || experts > 1024) return 0;
+    return expert_sort_scratch(T * top, experts);
+}
+OZB_API int ozb_expert_sort(int T, int top, int experts, const void *ids, int id_bytes, int align, int R, int *offsets, int *rows, int *slots,
+                            void *scratch, size_t scratch_bytes, void *stream) {
+    if (bad_slots(T, top) || experts <= 0 || align <= 0 || align > 256 || (id_bytes != 4 && id_bytes != 8) || !ids || off(ids, id_bytes) || !offsets ||
+        !rows || !slots || off(offsets, 4) || off(rows, 4) || off(slots, 4) || off(scratch, 4))
+        return OZB_EARG;
+    if (experts > 1024) return OZB_ESIZE;
+    const long long need = sorted_rows((long long)T * top, experts, align);
+    if (need > MAX_LEN) return OZB_ESIZE;
+    const size_t bytes = expert_sort_scratch(T * top, experts);
+    if (R < need || R > MAX_LEN || scratch_bytes < bytes || (bytes && !scratch)) return OZB_EARG;
+    if (int e = check_device()) return e;
+    return (int)expert_sort(T * top, experts, ids, id_bytes, align, R, offsets, rows, slots, scratch, (cudaStream_t)stream);
+}
+OZB_API int ozb_expert_gather(int R, int H, const void *X, int type, long long ldx, int T, const int *slots, int top, void *Y, long long ldy, void *stream) {
+    if (R <= 0 || H <= 0 || H > MAX_LEN || bad_slots(T, top) || !X || !Y || !slots || X == Y || bad_type(type) || off_type(X, type) || off_type(Y, type) ||
+        off(slots, 4) || ldx < H || ldy < H)
+        return OZB_EARG;
+    if (int e = check_device()) return e;
+    return (int)expert_gather(R, H, X, type, ldx, T, slots, top, Y, ldy, (cudaStream_t)stream);
+}
+OZB_API int ozb_expert_combine(int T, int top, int H, const void *Z, int type, int R, long long ldz, const int *rows, const float *weights, void *Y,
+                               long long ldy, void *stream) {
+    if (R <= 0 || H <= 0 || H > MAX_LEN || bad_slots(T, top) || !Z || !Y || !rows || Z == Y || bad_type(type) || off_type(Z, type) || off_type(Y, type) ||
+        off(rows, 4) || off(weights, 4) || ldz < H || ldy < H)
+        return OZB_EARG;
+    if (int e = check_device()) return e;
+    return (int)expert_combine(T, top, H, Z, type, R, ldz, rows, weights, Y, ldy, (cudaStream_t)stream);
+}
+OZB_API int ozb_expert_combine_grad(int T, int top, int H, const void *dY, int type, long long lddy, const void *Z, long long ldz, int R, const int *rows,
+                                    const int *slots, const float *weights, void *dZ, long long lddz, float *dweights, void *stream) {
+    if (R <= 0 || H <= 0 || H > MAX_LEN || bad_slots(T, top) || !dY || !Z || !dZ || !rows || !slots || !dweights || dZ == Z || dZ == dY || bad_type(type) ||
+        off_type(dY, type) || off_type(Z, type) || off_type(dZ, type) || off(rows, 4) || off(slots, 4) || off(weights, 4) || off(dweights, 4) ||
+        lddy < H || ldz < H || lddz < H)
+        return OZB_EARG;
+    if (int e = check_device()) return e;
+    return (int)expert_combine_grad(T, top, H, dY, type, lddy, Z, ldz, R, rows, slots, weights, dZ, lddz, dweights, (cudaStream_t)stream);
 }
 OZB_API int ozb_int8_peak(int iters, int pair, float *ms, double *tops) {
     if (int e = check_args(1, 1, 1)) return e;

@@ -1,0 +1,267 @@
+// mx4.cu -- the microscaled 4-bit format: rounding to it by rows and by columns, and back.
+//
+// A vector is cut into blocks of 32. With amax the largest magnitude of a block, its scale is 2^e, |e| <= 127, and a value x is
+// the nearest of 0, 0.5, 1, 1.5, 2, 3, 4, 6 to |x| 2^-e (ties to the even code), with its sign:
+//     rule 0:  e = floor(log2 amax) - 2          (the largest value lands in [4, 8) and saturates at 6)
+//     rule 1:  e = ceil(log2(amax / 6))          (nothing saturates)
+// With amax = 1.f 2^p both are integer arithmetic on the bits of amax: p - 2, plus one under rule 1 if 1.f > 1.5. The scale is
+// stored as the byte e + 127, clamped at 0 (an empty block, or values below 2^-125); 255 marks a block that holds an infinity or a
+// NaN. x 2^-e is exact: it is below 8, and what falls below 2^-126 is rounded to the code of 0 either way. The rounding itself is
+// the hardware's conversion (cvt.rn.satfinite.e2m1x2.f32).
+#include "oz_common.cuh"
+#include "oz_kernels.h"
+#include "oz_types.cuh"
+
+namespace ozk {
+
+namespace {
+
+// eight values -> eight codes, the first in the lowest four bits
+__device__ __forceinline__ uint32_t codes_of(const float *v) {
+    uint32_t r;
+    asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b1, %4, %3;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b2, %6, %5;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b3, %8, %7;\n\t"
+        "mov.b32 %0, {b0, b1, b2, b3};\n\t}"
+        : "=r"(r) : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
+    return r;
+}
+// eight codes -> eight values
+__device__ __forceinline__ void values_of(uint32_t c, float *v) {
+    uint32_t h[4];
+    asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+        "mov.b32 {b0, b1, b2, b3}, %4;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %0, b0;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %1, b1;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %2, b2;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %3, b3;\n\t}"
+        : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3]) : "r"(c));
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&h[i]));
+        v[2 * i] = f.x;
+        v[2 * i + 1] = f.y;
+    }
+}
+// the block's scale byte from the bits of its largest magnitude (0 .. 255)
+__device__ __forceinline__ uint32_t scale_byte(uint32_t amax_bits, int rule) {
+    if (amax_bits >= 0x7f800000u) return 255;
+    const int field = (int)((amax_bits + (rule ? 0x3fffffu : 0u)) >> 23);   // mantissa above 1.5: the next power of two
+    return field > 2 ? (uint32_t)(field - 2) : 0u;
+}
+// 2^-e for the byte e + 127; 0 for a block that is not a number, whose codes are then 0 (its values are cleared first)
+__device__ __forceinline__ float inverse_scale(uint32_t byte) { return __uint_as_float((254u - byte) << 23); }
+__device__ __forceinline__ float scale_of(uint32_t byte) {
+    return __uint_as_float(byte == 255 ? 0x7fffffffu : byte ? byte << 23 : 0x00400000u);
+}
+__device__ __forceinline__ uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+
+// the row of X that vector or element r takes its values from; -1: none (zeros)
+__device__ __forceinline__ long long source_row(const int *slots, int per, int sources, int r) {
+    if (!slots) return r;
+    const int s = __ldg(slots + r);
+    if (s < 0) return -1;
+    const int row = s / per;
+    return row < sources ? row : -1;
+}
+
+// Blocks along the rows of X. A lane holds 16 values, two lanes a block; a warp takes 512 values of one row, so that its loads are
+// 512 or 1024 bytes in a piece and its stores 256. Bound by HBM: the codes leave as 8-byte words, the scales as bytes.
+template <class T, bool VEC>
+__global__ void __launch_bounds__(256) mx4_rows(const T *X, int nvec, int len, long long ldx, size_t plane_x, int planes, int rule,
+                                                const int *slots, int per, int sources, uint8_t *codes, long long ldq, size_t plane_q,
+                                                uint8_t *scales, long long lds, size_t plane_s) {
+    const int lane = threadIdx.x & 31;
+    const int pieces = (len + 511) / 512;
+    const long long total = (long long)planes * nvec * pieces;
+    for (long long w = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); w < total; w += (long long)gridDim.x * 8) {
+        const long long vec = w / pieces;
+        const int i0 = (int)(w - vec * pieces) * 512 + lane * 16;
+        const int z = (int)(vec / nvec), r = (int)(vec - (long long)z * nvec);
+        const long long src = source_row(slots, per, sources, r);
+        float v[16];
+        if (src < 0 || i0 >= len) {
+#pragma unroll
+            for (int i = 0; i < 16; i++) v[i] = 0.f;
+        } else {
+            const T *x = X + (size_t)z * plane_x + (size_t)src * ldx + i0;
+            if (VEC && i0 + 16 <= len) {
+                constexpr int N = Vec16<T>::N;
+                uint4 q[16 / N];
+#pragma unroll
+                for (int i = 0; i < 16 / N; i++) q[i] = __ldg(reinterpret_cast<const uint4 *>(x) + i);
+#pragma unroll
+                for (int i = 0; i < 16 / N; i++) Vec16<T>::unpack(q[i], v + i * N);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 16; i++) v[i] = i0 + i < len ? to_f32<T>(x[i]) : 0.f;
+            }
+        }
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < 16; i++) m = max(m, magnitude(v[i]));
+        m = max(m, __shfl_xor_sync(~0u, m, 1));
+        const uint32_t byte = scale_byte(m, rule);
+        const float inv = inverse_scale(byte);
+#pragma unroll
+        for (int i = 0; i < 16; i++) v[i] = byte == 255 ? 0.f : v[i] * inv;
+        if ((i0 & ~31) < len) {   // the block exists: its codes are written whole, zeros behind the last value
+            *reinterpret_cast<uint2 *>(codes + (size_t)z * plane_q + (size_t)r * ldq + (i0 >> 1)) = make_uint2(codes_of(v), codes_of(v + 8));
+            if (!(lane & 1)) scales[(size_t)z * plane_s + (size_t)r * lds + (i0 >> 5)] = (uint8_t)byte;
+        }
+    }
+}
+
+// Blocks down the columns of a row-major X (len x nvec): vector c is column c, and comes out as a row. A block of threads takes 256
+// rows of 64 columns: warp w holds rows 32w .. 32w+31, two columns to a lane, in registers (32 independent loads of a pair in
+// flight to a lane), so that a lane has a whole block of each of its columns; the codes turn through shared memory into 128
+// contiguous bytes for each column.
+constexpr int CT_COLS = 64, CT_ROWS = 256, CT_PITCH = 128 + 16;
+template <class T, bool VEC>
+__global__ void __launch_bounds__(256) mx4_cols(const T *X, int nvec, int len, long long ldx, size_t plane_x, int rule, const int *slots,
+                                                int per, int sources, uint8_t *codes, long long ldq, size_t plane_q, uint8_t *scales,
+                                                long long lds, size_t plane_s, int col_tiles, int row_tiles) {
+    __shared__ __align__(16) uint8_t tile[CT_COLS * CT_PITCH];
+    __shared__ __align__(8) uint8_t stile[CT_COLS * 8];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    long long b = blockIdx.x;
+    const int ct = (int)(b % col_tiles);
+    b /= col_tiles;
+    const int rt = (int)(b % row_tiles), z = (int)(b / row_tiles);
+    const int c = ct * CT_COLS + 2 * lane, k0 = rt * CT_ROWS + warp * 32;
+    X += (size_t)z * plane_x;
+    codes += (size_t)z * plane_q;
+    scales += (size_t)z * plane_s;
+    float v[2][32];
+    long long mine = -1;
+    if (k0 + lane < len) mine = source_row(slots, per, sources, k0 + lane);
+#pragma unroll
+    for (int i = 0; i < 32; i++) {
+        const long long src = __shfl_sync(~0u, mine, i);
+        v[0][i] = v[1][i] = 0.f;
+        if (src >= 0 && c < nvec) {
+            const T *x = X + (size_t)src * ldx + c;
+            if (VEC && c + 1 < nvec) {
+                struct alignas(2 * sizeof(T)) Pair { T a, b; };
+                const Pair p = *reinterpret_cast<const Pair *>(x);
+                v[0][i] = to_f32<T>(p.a);
+                v[1][i] = to_f32<T>(p.b);
+            } else {
+                v[0][i] = to_f32<T>(x[0]);
+                if (c + 1 < nvec) v[1][i] = to_f32<T>(x[1]);
+            }
+        }
+    }
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < 32; i++) m = max(m, magnitude(v[h][i]));
+        const uint32_t byte = scale_byte(m, rule);
+        const float inv = inverse_scale(byte);
+#pragma unroll
+        for (int i = 0; i < 32; i++) v[h][i] = byte == 255 ? 0.f : v[h][i] * inv;
+        *reinterpret_cast<uint4 *>(tile + (2 * lane + h) * CT_PITCH + warp * 16) =
+            make_uint4(codes_of(v[h]), codes_of(v[h] + 8), codes_of(v[h] + 16), codes_of(v[h] + 24));
+        stile[(2 * lane + h) * 8 + warp] = (uint8_t)byte;
+    }
+    __syncthreads();
+    const int blocks = (len + 31) / 32, kb = rt * 8;   // blocks of a column, and this tile's first
+#pragma unroll
+    for (int i = 0; i < CT_COLS * 8 / 256; i++) {
+        const int col = i * 32 + (threadIdx.x >> 3), blk = threadIdx.x & 7, g = ct * CT_COLS + col;
+        if (g < nvec && kb + blk < blocks)
+            *reinterpret_cast<uint4 *>(codes + (size_t)g * ldq + (size_t)(kb + blk) * 16) = *reinterpret_cast<const uint4 *>(tile + col * CT_PITCH + blk * 16);
+    }
+    if (threadIdx.x < CT_COLS && ct * CT_COLS + (int)threadIdx.x < nvec) {
+        uint8_t *dst = scales + (size_t)(ct * CT_COLS + threadIdx.x) * lds + kb;
+        if (kb + 8 <= blocks) *reinterpret_cast<uint2 *>(dst) = *reinterpret_cast<const uint2 *>(stile + threadIdx.x * 8);
+        else for (int i = 0; kb + i < blocks; i++) dst[i] = stile[threadIdx.x * 8 + i];
+    }
+}
+
+// Codes and scales back to values: a lane takes half a block (8 bytes of codes), a warp 512 values of one vector. Every product of a
+// code's value and a power of two is exact in FP32; T rounds it once (FP16 may overflow or lose small values, BF16 does not lose any).
+template <class T, bool VEC>
+__global__ void __launch_bounds__(256) mx4_values(const uint8_t *codes, long long ldq, const uint8_t *scales, long long lds, int nvec, int len,
+                                                  T *Y, long long ldy) {
+    const int lane = threadIdx.x & 31;
+    const int pieces = (len + 511) / 512;
+    const long long total = (long long)nvec * pieces;
+    for (long long w = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); w < total; w += (long long)gridDim.x * 8) {
+        const long long r = w / pieces;
+        const int i0 = (int)(w - r * pieces) * 512 + lane * 16;
+        if (i0 >= len) continue;
+        const uint2 q = __ldg(reinterpret_cast<const uint2 *>(codes + (size_t)r * ldq + (i0 >> 1)));
+        const float s = scale_of(__ldg(scales + (size_t)r * lds + (i0 >> 5)));
+        float v[16];
+        values_of(q.x, v);
+        values_of(q.y, v + 8);
+#pragma unroll
+        for (int i = 0; i < 16; i++) v[i] *= s;
+        T *y = Y + (size_t)r * ldy + i0;
+        if (VEC && i0 + 16 <= len) {
+            constexpr int N = Vec16<T>::N;
+#pragma unroll
+            for (int i = 0; i < 16 / N; i++) *(reinterpret_cast<uint4 *>(y) + i) = Vec16<T>::pack(v + i * N);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; i++)
+                if (i0 + i < len) y[i] = from_f32<T>(v[i]);
+        }
+    }
+}
+
+int warp_grid(long long warps) {   // eight warps to a block, at most 2^20 blocks (the kernels stride)
+    const long long blocks = (warps + 7) / 8;
+    return (int)(blocks < (1 << 20) ? blocks : (1 << 20));
+}
+
+}  // namespace
+
+cudaError_t mx4_quantize_rows(const void *X, int type, int nvec, int len, long long ldx, size_t plane_x, int planes, int rule, const int *slots,
+                              int per, int sources, uint8_t *codes, long long ldq, size_t plane_q, uint8_t *scales, long long lds,
+                              size_t plane_s, cudaStream_t st) {
+    const int size = type_size(type);
+    const bool vec = !(reinterpret_cast<uintptr_t>(X) & 15) && !(ldx * size & 15) && !(plane_x * size & 15);
+    const int grid = warp_grid((long long)planes * nvec * ((len + 511) / 512));
+    with_type(type, [&](auto t) {
+        using T = decltype(t);
+        if (vec) mx4_rows<T, true><<<grid, 256, 0, st>>>((const T *)X, nvec, len, ldx, plane_x, planes, rule, slots, per, sources, codes, ldq, plane_q, scales, lds, plane_s);
+        else mx4_rows<T, false><<<grid, 256, 0, st>>>((const T *)X, nvec, len, ldx, plane_x, planes, rule, slots, per, sources, codes, ldq, plane_q, scales, lds, plane_s);
+    });
+    return cudaGetLastError();
+}
+
+cudaError_t mx4_quantize_cols(const void *X, int type, int nvec, int len, long long ldx, size_t plane_x, int planes, int rule, const int *slots,
+                              int per, int sources, uint8_t *codes, long long ldq, size_t plane_q, uint8_t *scales, long long lds,
+                              size_t plane_s, cudaStream_t st) {
+    const int size = type_size(type);
+    const bool vec = !(reinterpret_cast<uintptr_t>(X) % (2 * size)) && !(ldx & 1) && !(plane_x & 1);
+    const int col_tiles = (nvec + CT_COLS - 1) / CT_COLS, row_tiles = (len + CT_ROWS - 1) / CT_ROWS;
+    const long long grid = (long long)col_tiles * row_tiles * planes;
+    if (grid > 0x7fffffffLL) return cudaErrorInvalidValue;
+    with_type(type, [&](auto t) {
+        using T = decltype(t);
+        if (vec) mx4_cols<T, true><<<(int)grid, 256, 0, st>>>((const T *)X, nvec, len, ldx, plane_x, rule, slots, per, sources, codes, ldq, plane_q, scales, lds, plane_s, col_tiles, row_tiles);
+        else mx4_cols<T, false><<<(int)grid, 256, 0, st>>>((const T *)X, nvec, len, ldx, plane_x, rule, slots, per, sources, codes, ldq, plane_q, scales, lds, plane_s, col_tiles, row_tiles);
+    });
+    return cudaGetLastError();
+}
+
+cudaError_t mx4_dequantize(const uint8_t *codes, long long ldq, const uint8_t *scales, long long lds, int nvec, int len, void *Y, int type,
+                           long long ldy, cudaStream_t st) {
+    const int size = type_size(type);
+    const bool vec = !(reinterpret_cast<uintptr_t>(Y) & 15) && !(ldy * size & 15);
+    const int grid = warp_grid((long long)nvec * ((len + 511) / 512));
+    with_type(type, [&](auto t) {
+        using T = decltype(t);
+        if (vec) mx4_values<T, true><<<grid, 256, 0, st>>>(codes, ldq, scales, lds, nvec, len, (T *)Y, ldy);
+        else mx4_values<T, false><<<grid, 256, 0, st>>>(codes, ldq, scales, lds, nvec, len, (T *)Y, ldy);
+    });
+    return cudaGetLastError();
+}
+
+}  // namespace ozk

@@ -47,4 +47,38 @@ int exact_bf16_fp8_gemm(int M, int N, int K, const uint16_t *X, long long ldx, c
                         long long ldy, int *open, int *moduli, cudaStream_t st);
 void exact_f8_release();
 
+
+// microscaled 4-bit format (mx4.cu): element types 0 FP32, 1 BF16, 2 FP16
+cudaError_t mx4_quantize_rows(const void *X, int type, int nvec, int len, long long ldx, size_t plane_x, int planes, int rule, const int *slots,
+                              int per, int sources, uint8_t *codes, long long ldq, size_t plane_q, uint8_t *scales, long long lds,
+                              size_t plane_s, cudaStream_t st);
+cudaError_t mx4_quantize_cols(const void *X, int type, int nvec, int len, long long ldx, size_t plane_x, int planes, int rule, const int *slots,
+                              int per, int sources, uint8_t *codes, long long ldq, size_t plane_q, uint8_t *scales, long long lds,
+                              size_t plane_s, cudaStream_t st);
+cudaError_t mx4_dequantize(const uint8_t *codes, long long ldq, const uint8_t *scales, long long lds, int nvec, int len, void *Y, int type,
+                           long long ldy, cudaStream_t st);
+// products of it (mx4_gemm.cu): C[g][j][i] = sum_k P[g][i][k] Q[j][k]; mode 0 dense, 1 segments of the rows of Q, 2 segments of k
+struct Mx4Product {
+    int mode, groups, rows_p, rows_q, K, type;
+    const int *offsets;
+    const uint8_t *p, *sp, *q, *sq;
+    long long ldp, ldsp, ldq, ldsq;
+    size_t plane_p, plane_sp;
+    void *C;
+    long long ldc;
+    size_t plane_c;
+};
+cudaError_t mx4_product(const Mx4Product &g, int *status, cudaStream_t st);
+
+// tokens by expert and back (experts.cu)
+size_t expert_sort_scratch(int slots, int experts);
+cudaError_t expert_sort(int slots, int experts, const void *ids, int id_bytes, int align, int R, int *offsets, int *rows, int *slot_of, void *scratch,
+                        cudaStream_t st);
+cudaError_t expert_gather(int R, int H, const void *X, int type, long long ldx, int T, const int *slots, int top, void *Y, long long ldy,
+                          cudaStream_t st);
+cudaError_t expert_combine(int T, int top, int H, const void *Z, int type, int R, long long ldz, const int *rows, const float *weights, void *Y,
+                           long long ldy, cudaStream_t st);
+cudaError_t expert_combine_grad(int T, int top, int H, const void *dY, int type, long long lddy, const void *Z, long long ldz, int R, const int *rows,
+                                const int *slots, const float *weights, void *dZ, long long lddz, float *dweights, cudaStream_t st);
+
 }  // namespace ozk

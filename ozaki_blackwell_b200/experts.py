@@ -1,0 +1,127 @@
+"""Tokens by expert and back, and the experts' products on 4-bit weights, over torch tensors.
+
+    sort(ids, experts, align=1)                       slots in the order of their experts -> Routing
+    gather(x, routing)                                the tokens' rows in that order
+    combine(z, routing, weights=None)                 and back: y[t] = sum_j weights[t, j] z[row of slot (t, j)]
+    combine_grad(dy, z, routing, weights=None)        the gradients of combine: (dz, dweights)
+    matmul(x, w, ids, weights)                        y[t] = sum_j weights[t, j] W[ids[t, j]] x[t], all of the above and mx4's product
+    matmul_grad(dy, x, z, wt, routing, weights)       its gradients: (dx, dweights, dw)
+
+The gradient of gather is combine without weights. What each computes, index by index, is in include/ozb.h (ozb_expert_*). Every call
+is asynchronous on the current stream of the operands' device and may be captured into a CUDA graph.
+"""
+from typing import NamedTuple
+
+import torch
+
+from . import mx4
+from ._lib import lib as _lib
+from .mx4 import _call, _dense, _pitch, _result, _same_device, _type
+
+__all__ = ["Routing", "sort", "gather", "combine", "combine_grad", "matmul", "matmul_grad"]
+
+
+class Routing(NamedTuple):
+    """Where the slots (t, j) of T tokens go: expert e has the rows offsets[e] .. offsets[e + 1] - 1; rows [T, top] is the row of a slot
+    (-1: dropped), slots [R] the slot t * top + j of a row (-1: none). All int32. align: what the segments are padded to (0: unknown)."""
+    offsets: torch.Tensor
+    rows: torch.Tensor
+    slots: torch.Tensor
+    align: int = 0
+
+
+def _routing(r, device):
+    for name, t in (("offsets", r.offsets), ("rows", r.rows), ("slots", r.slots)):
+        if t.dtype != torch.int32 or not t.is_contiguous() or t.device != device:
+            raise ValueError(f"routing.{name} must be contiguous int32 on {device}")
+    if r.rows.dim() != 2:
+        raise ValueError("routing.rows has a row for each token")
+    return r.rows.shape
+
+
+def _weights(weights, shape, device):
+    if weights is None:
+        return None
+    if weights.dtype != torch.float32 or tuple(weights.shape) != tuple(shape) or not weights.is_contiguous() or weights.device != device:
+        raise ValueError(f"weights must be contiguous float32 {tuple(shape)} on {device}")
+    return weights.data_ptr()
+
+
+def sort(ids, experts, align=1):
+    """ids [T, top] (int32 or int64) -> Routing over `experts` experts, stable, segments padded to multiples of `align` (1 to 256; products
+    along the tokens need 64). A number outside 0 .. experts - 1 drops its slot."""
+    if ids.dtype not in (torch.int32, torch.int64) or ids.dim() != 2 or not ids.is_contiguous() or not ids.is_cuda:
+        raise ValueError("ids must be a contiguous [tokens, top] matrix of int32 or int64 on a GPU")
+    tokens, top = ids.shape
+    size = _lib.ozb_expert_sort_rows(tokens, top, experts, align)
+    if size < 0:
+        raise ValueError(f"cannot sort {tokens} x {top} slots over {experts} experts in segments of {align}: sizes are positive, at most 1024 experts, align at most 256")
+    need = _lib.ozb_expert_sort_scratch(tokens, top, experts)
+    # one allocation: offsets, rows, slots and the counts of the chunks
+    n = tokens * top
+    buf = torch.empty(experts + 1 + n + size + need // 4, dtype=torch.int32, device=ids.device)
+    offsets, rows, slots = buf[: experts + 1], buf[experts + 1 : experts + 1 + n], buf[experts + 1 + n : experts + 1 + n + size]
+    at = buf.data_ptr()
+    _call(ids.device, _lib.ozb_expert_sort, tokens, top, experts, ids.data_ptr(), ids.element_size(), align, size, at, at + 4 * (experts + 1),
+          at + 4 * (experts + 1 + n), at + 4 * (experts + 1 + n + size), need)
+    return Routing(offsets, rows.view(tokens, top), slots, align)
+
+
+def gather(x, routing, out=None):
+    """The rows of x [T, h] in the order of their experts, [R, h]; zeros where a row has no slot."""
+    _dense(x, "x")
+    tokens, top = _routing(routing, x.device)
+    if x.shape[0] != tokens:
+        raise ValueError(f"x has {x.shape[0]} rows, the routing {tokens} tokens")
+    y = _result(out, (routing.slots.numel(), x.shape[1]), x.dtype, x.device)
+    _call(x.device, _lib.ozb_expert_gather, y.shape[0], y.shape[1], x.data_ptr(), _type(x.dtype), _pitch(x), tokens, routing.slots.data_ptr(), top,
+          y.data_ptr(), _pitch(y))
+    return y
+
+
+def combine(z, routing, weights=None, out=None):
+    """y[t] = sum over j of weights[t, j] z[rows[t, j]] (weights None: 1), in FP32, rounded once to z's type."""
+    _dense(z, "z")
+    tokens, top = _routing(routing, z.device)
+    y = _result(out, (tokens, z.shape[1]), z.dtype, z.device)
+    _call(z.device, _lib.ozb_expert_combine, tokens, top, z.shape[1], z.data_ptr(), _type(z.dtype), z.shape[0], _pitch(z), routing.rows.data_ptr(),
+          _weights(weights, (tokens, top), z.device), y.data_ptr(), _pitch(y))
+    return y
+
+
+def combine_grad(dy, z, routing, weights=None):
+    """(dz, dweights) of combine(z, routing, weights) for a gradient dy [T, h] of z's type; dz is zero where a row has no slot."""
+    _dense(dy, "dy")
+    _dense(z, "z")
+    _same_device(z.device, dy=dy)
+    tokens, top = _routing(routing, z.device)
+    if dy.dtype != z.dtype or tuple(dy.shape) != (tokens, z.shape[1]) or z.shape[0] != routing.slots.numel():
+        raise ValueError(f"dy {tuple(dy.shape)} of {dy.dtype} and z {tuple(z.shape)} of {z.dtype} do not fit a routing of {tokens} tokens and {routing.slots.numel()} rows")
+    dz = torch.empty(z.shape, dtype=z.dtype, device=z.device)
+    dweights = torch.empty((tokens, top), dtype=torch.float32, device=z.device)
+    _call(z.device, _lib.ozb_expert_combine_grad, tokens, top, z.shape[1], dy.data_ptr(), _type(z.dtype), _pitch(dy), z.data_ptr(), _pitch(z), z.shape[0],
+          routing.rows.data_ptr(), routing.slots.data_ptr(), _weights(weights, (tokens, top), z.device), dz.data_ptr(), _pitch(dz), dweights.data_ptr())
+    return dz, dweights
+
+
+def matmul(x, w, ids, weights=None, keep=False):
+    """y[t] = sum over j of weights[t, j] W[ids[t, j]] x[t]: tokens sorted by expert, rounded to the 4-bit format as they are gathered, one
+    product for all experts, and the rows added up by token. w: Mx4 stack [experts, n, ...] with blocks along the rows of x.
+    keep: returns (y, z, routing) for matmul_grad, with segments padded to 64."""
+    _dense(x, "x")
+    r = sort(ids, w.codes.shape[0], 64 if keep else 1)
+    z = mx4.grouped_matmul(mx4.quantize(x, routing=r), w, r.offsets, x.dtype)
+    y = combine(z, r, weights)
+    return (y, z, r) if keep else y
+
+
+def matmul_grad(dy, x, z, wt, routing, weights=None):
+    """The gradients of matmul(..., keep=True): (dx, dweights, dw) with dw [experts, n, k] of x's type. wt: the weights with blocks along n,
+    mx4.quantize(W, dim=-2), a stack [experts, k, ...]. Operands of the products are rounded to the 4-bit format, gradients pass
+    through that rounding."""
+    if routing.align % 64:
+        raise ValueError(f"the segments are padded to {routing.align}: products along the tokens need multiples of 64 (matmul with keep=True)")
+    dz, dweights = combine_grad(dy, z, routing, weights)
+    dx = combine(mx4.grouped_matmul(mx4.quantize(dz), wt, routing.offsets, z.dtype), routing)
+    dw = mx4.segment_matmul(mx4.quantize(dz, dim=-2), mx4.quantize(x, dim=-2, routing=routing), routing.offsets, x.dtype)
+    return dx, dweights, dw

@@ -1,0 +1,98 @@
+"""Argument checks of the 4-bit and expert entry points: they come before any device work, so they are tested without one."""
+import ctypes
+
+import pytest
+import torch
+
+from ozaki_blackwell_b200._lib import lib
+
+P = ctypes.c_void_p(4096)          # never dereferenced: every call below is refused
+ARG, SIZE = 10001, 10006
+
+
+def _quantize(X=P, type=0, nvec=4, len=64, ldx=64, by_rows=1, rule=0, slots=None, per=0, sources=0, planes=1, plane_x=0, codes=P, ldq=32, plane_q=0,
+              scales=P, lds=8, plane_s=0):
+    return lib.ozb_mx4_quantize(X, type, nvec, len, ldx, by_rows, rule, slots, per, sources, planes, plane_x, codes, ldq, plane_q, scales, lds, plane_s, None)
+
+
+@pytest.mark.parametrize("bad", [dict(X=None), dict(type=3), dict(type=-1), dict(nvec=0), dict(len=0), dict(len=-1), dict(len=2 ** 31 - 1), dict(ldx=63),
+                                 dict(by_rows=0, ldx=3), dict(rule=2), dict(codes=None), dict(codes=ctypes.c_void_p(4104)), dict(ldq=24), dict(ldq=16),
+                                 dict(scales=None), dict(scales=ctypes.c_void_p(4100)), dict(lds=4), dict(lds=0), dict(slots=P), dict(slots=P, per=1),
+                                 dict(slots=P, per=1, sources=4, planes=2), dict(planes=0), dict(planes=2, plane_q=8), dict(planes=2, plane_q=16, plane_s=4),
+                                 dict(X=ctypes.c_void_p(4098)), dict(X=ctypes.c_void_p(4097), type=1)])
+def test_quantize(bad):
+    assert _quantize(**bad) == ARG
+
+
+def test_dequantize():
+    call = lambda **b: lib.ozb_mx4_dequantize(*{**dict(codes=P, ldq=32, scales=P, lds=8, nvec=4, len=64, Y=P, type=1, ldy=64), **b}.values(), None)  # noqa: E731
+    for bad in (dict(codes=None), dict(scales=None), dict(Y=None), dict(nvec=0), dict(len=0), dict(len=65), dict(ldy=63), dict(type=4), dict(Y=ctypes.c_void_p(4097))):
+        assert call(**bad) == ARG, bad
+
+
+def test_products():
+    dense = dict(M=4, N=4, K=64, X=P, ldx=32, Xs=P, ldxs=8, W=P, ldw=32, Ws=P, ldws=8, Y=P, type=0, ldy=4)
+    call = lambda **b: lib.ozb_mx4_gemm(*{**dense, **b}.values(), None)  # noqa: E731
+    for bad in (dict(M=0), dict(N=0), dict(K=0), dict(K=65), dict(K=2 ** 31 - 1), dict(X=None), dict(Xs=None), dict(W=None), dict(Ws=None), dict(Y=None),
+                dict(ldx=16), dict(ldxs=4), dict(ldy=3), dict(type=3), dict(Y=ctypes.c_void_p(4098)), dict(W=ctypes.c_void_p(4104)), dict(M=-5)):
+        assert call(**bad) == ARG, bad
+    grouped = dict(groups=2, R=4, N=4, K=64, offsets=P, X=P, ldx=32, Xs=P, ldxs=8, W=P, ldw=32, plane_w=128, Ws=P, ldws=8, plane_ws=32, Y=P, type=0, ldy=4)
+    call = lambda **b: lib.ozb_mx4_gemm_grouped(*{**grouped, **b}.values(), None)  # noqa: E731
+    for bad in (dict(groups=0), dict(R=0), dict(N=0), dict(K=0), dict(offsets=None), dict(offsets=ctypes.c_void_p(4098)), dict(plane_w=8), dict(plane_ws=4), dict(ldy=3)):
+        assert call(**bad) == ARG, bad
+    assert call(groups=1025) == SIZE
+    segments = dict(groups=2, M=4, N=4, R=64, offsets=P, A=P, lda=32, As=P, ldas=8, B=P, ldb=32, Bs=P, ldbs=8, Y=P, type=0, ldy=4, plane_y=16)
+    call = lambda **b: lib.ozb_mx4_gemm_segments(*{**segments, **b}.values(), None)  # noqa: E731
+    for bad in (dict(groups=0), dict(M=0), dict(N=0), dict(R=0), dict(R=65), dict(offsets=None), dict(As=None), dict(ldb=8)):
+        assert call(**bad) == ARG, bad
+    assert call(groups=1025) == SIZE
+
+
+def test_sort():
+    assert lib.ozb_expert_sort_rows(3, 2, 4, 1) == 6
+    assert lib.ozb_expert_sort_rows(3, 2, 4, 64) == (6 + 4 * 63) // 64 * 64      # four segments of at most 64
+    assert lib.ozb_expert_sort_rows(1, 2, 100, 8) == 16                           # two slots touch two experts at most
+    for bad in ((0, 1, 1, 1), (1, 0, 1, 1), (1, 1, 0, 1), (1, 1, 1025, 1), (1, 1, 1, 0), (1, 1, 1, 257), (2 ** 20, 2 ** 12, 1, 1)):
+        assert lib.ozb_expert_sort_rows(*bad) == -ARG, bad
+    assert lib.ozb_expert_sort_scratch(1, 8, 64) == 0 and lib.ozb_expert_sort_scratch(2049, 1, 64) == 2 * 64 * 4
+    base = dict(T=3, top=2, experts=4, ids=P, id_bytes=4, align=1, R=6, offsets=P, rows=P, slots=P, scratch=None, bytes=0)
+    call = lambda **b: lib.ozb_expert_sort(*{**base, **b}.values(), None)  # noqa: E731
+    for bad in (dict(T=0), dict(top=0), dict(experts=0), dict(ids=None), dict(id_bytes=2), dict(align=0), dict(align=257), dict(R=5), dict(align=64), dict(offsets=None),
+                dict(rows=None), dict(slots=None), dict(T=3000, R=6000), dict(ids=ctypes.c_void_p(4100), id_bytes=8), dict(T=2 ** 20, top=2 ** 12)):
+        assert call(**bad) == ARG, bad
+    assert call(experts=1025) == SIZE
+
+
+def test_rows():
+    base = dict(R=6, H=8, X=P, type=0, ldx=8, T=3, slots=P, top=2, Y=ctypes.c_void_p(8192), ldy=8)
+    call = lambda **b: lib.ozb_expert_gather(*{**base, **b}.values(), None)  # noqa: E731
+    for bad in (dict(R=0), dict(H=0), dict(X=None), dict(type=5), dict(ldx=7), dict(T=0), dict(slots=None), dict(top=0), dict(Y=None), dict(Y=P), dict(ldy=7)):
+        assert call(**bad) == ARG, bad
+    base = dict(T=3, top=2, H=8, Z=P, type=0, R=6, ldz=8, rows=P, weights=None, Y=ctypes.c_void_p(8192), ldy=8)
+    call = lambda **b: lib.ozb_expert_combine(*{**base, **b}.values(), None)  # noqa: E731
+    for bad in (dict(T=0), dict(top=0), dict(H=0), dict(Z=None), dict(R=0), dict(ldz=7), dict(rows=None), dict(weights=ctypes.c_void_p(2)), dict(Y=None), dict(Y=P), dict(ldy=7)):
+        assert call(**bad) == ARG, bad
+    base = dict(T=3, top=2, H=8, dY=P, type=0, lddy=8, Z=P, ldz=8, R=6, rows=P, slots=P, weights=None, dZ=ctypes.c_void_p(8192), lddz=8, dweights=P)
+    call = lambda **b: lib.ozb_expert_combine_grad(*{**base, **b}.values(), None)  # noqa: E731
+    for bad in (dict(T=0), dict(dY=None), dict(Z=None), dict(dZ=None), dict(dZ=P), dict(rows=None), dict(slots=None), dict(dweights=None), dict(lddy=7), dict(ldz=7), dict(lddz=7), dict(R=0)):
+        assert call(**bad) == ARG, bad
+
+
+def test_host_tensors_are_refused():
+    from ozaki_blackwell_b200 import experts, mx4
+    x = torch.zeros(4, 64)
+    with pytest.raises(TypeError):
+        mx4.quantize(x)
+    with pytest.raises(TypeError):
+        mx4.dequantize(mx4.Mx4(torch.zeros(4, 32, dtype=torch.uint8), torch.zeros(4, 16, dtype=torch.uint8), 64))
+    with pytest.raises(TypeError):
+        mx4.dequantize(mx4.Mx4(torch.zeros(4, 32), torch.zeros(4, 16), 64))
+    with pytest.raises(ValueError):
+        experts.sort(torch.zeros(4, 2, dtype=torch.int32), 3)
+    with pytest.raises(TypeError):
+        experts.matmul(x, None, None)
+
+
+def test_the_wheel_carries_the_modules():
+    from ozaki_blackwell_b200 import build_wheel
+    assert {"mx4.py", "experts.py"} <= set(build_wheel.PY_FILES)
