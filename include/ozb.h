@@ -222,8 +222,8 @@ enum { OZB_F32 = 0, OZB_BF16 = 1, OZB_F16 = 2 };
 /* The 4-bit format (OCP microscaling, MXFP4): vectors in blocks of 32 values; a value is a code of 4 bits (a sign, then 0, 0.5, 1,
  * 1.5, 2, 3, 4, 6) times the block's power of two 2^(s - 127), s one byte (255: the block is not a number). Row-major: row r of
  * the codes at codes + r * ldq (two codes to a byte, the earlier one in the low half), its scales at scales + r * lds (bytes,
- * one to a block). `codes` 16-byte and `scales` 8-byte aligned, ldq a multiple of 16, lds of 8; a row has room for ceil(len / 32)
- * whole blocks, and the codes behind `len` in the last one are 0.
+ * one to a block). Both start on 16 bytes and have pitches that are multiples of 16; a row of codes has room for ceil(len / 32)
+ * whole blocks, a row of scales for that many bytes rounded up to 16, and the codes behind `len` in the last one are 0.
  *
  * ozb_mx4_quantize: `nvec` vectors of `len` values of X to that format, nearest code, ties to the even one. by_rows = 1: the rows of
  * X (pitch ldx); by_rows = 0: the columns of a row-major len x nvec X, which come out as rows. rule 0: the block's scale is
@@ -231,7 +231,7 @@ enum { OZB_F32 = 0, OZB_BF16 = 1, OZB_F16 = 2 };
  * within 2^-127 .. 2^127. A block that holds an infinity or a NaN gets s = 255 and codes 0. `slots` (may be NULL) takes the
  * rows of X through the map of ozb_expert_sort: row r of the matrix that is quantised is row slots[r] / per of X, or zeros where
  * slots[r] is negative or the row is not below `sources`. planes > 1 (without slots): that many matrices, plane_x elements,
- * plane_q and plane_s bytes apart (multiples of 16 and 8). The gradient is passed through (straight-through), no call needed. */
+ * plane_q and plane_s bytes apart (multiples of 16). The gradient is passed through (straight-through), no call needed. */
 int ozb_mx4_quantize(const void *X, int type, int nvec, int len, long long ldx, int by_rows, int rule, const int *slots, int per, int sources,
                      int planes, size_t plane_x, uint8_t *codes, long long ldq, size_t plane_q, uint8_t *scales, long long lds,
                      size_t plane_s, void *stream);

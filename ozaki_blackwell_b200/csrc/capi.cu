@@ -436,7 +436,7 @@ int check_device() {
 bool off(const void *p, unsigned to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) != 0; }   // not aligned
 // a 4-bit operand: rows of `len` values, codes and scales
 bool bad_mx4(const void *codes, long long ldq, const void *scales, long long lds, int len) {
-    return !codes || !scales || off(codes, 16) || off(scales, 8) || (ldq & 15) || (lds & 7) || ldq < ((long long)len + 31) / 32 * 16 ||
+    return !codes || !scales || off(codes, 16) || off(scales, 16) || (ldq & 15) || (lds & 15) || ldq < ((long long)len + 31) / 32 * 16 ||
            lds < ((long long)len + 31) / 32;
 }
 constexpr int MAX_LEN = 0x7fffffff - 1023;   // lengths are rounded up in 32 bits
@@ -866,7 +866,7 @@ OZB_API int ozb_mx4_quantize(const void *X, int type, int nvec, int len, long lo
         ldx < (by_rows ? len : nvec) || bad_mx4(codes, ldq, scales, lds, len))
         return OZB_EARG;
     if (slots && (per <= 0 || sources <= 0 || planes > 1 || off(slots, 4))) return OZB_EARG;
-    if (planes > 1 && ((plane_q & 15) || (plane_s & 7))) return OZB_EARG;
+    if (planes > 1 && ((plane_q & 15) || (plane_s & 15))) return OZB_EARG;
     if (int e = check_device()) return e;
     if (planes == 1) plane_x = plane_q = plane_s = 0;
     return (int)(by_rows ? mx4_quantize_rows : mx4_quantize_cols)(X, type, nvec, len, ldx, plane_x, planes, rule, slots, per, sources, codes, ldq,
@@ -890,16 +890,16 @@ OZB_API int ozb_mx4_gemm(int M, int N, int K, const uint8_t *X, long long ldx, c
     if (M <= 0 || N <= 0 || K <= 0 || K > MAX_LEN || N > MAX_LEN || M > MAX_LEN || bad_type(type) || !Y || off_type(Y, type) || ldy < N || bad_mx4(X, ldx, Xs, ldxs, K) ||
         bad_mx4(W, ldw, Ws, ldws, K))
         return OZB_EARG;
-    return run_mx4({0, 1, N, M, K, type, nullptr, W, Ws, X, Xs, ldw, ldws, ldx, ldxs, 0, 0, Y, ldy, 0}, stream);
+    return run_mx4({0, 1, M, N, K, type, nullptr, X, ldx, Xs, ldxs, W, ldw, 0, Ws, ldws, 0, Y, ldy, 0}, stream);
 }
 OZB_API int ozb_mx4_gemm_grouped(int groups, int R, int N, int K, const int *offsets, const uint8_t *X, long long ldx, const uint8_t *Xs, long long ldxs,
                                  const uint8_t *W, long long ldw, size_t plane_w, const uint8_t *Ws, long long ldws, size_t plane_ws, void *Y, int type,
                                  long long ldy, void *stream) {
     if (groups <= 0 || R <= 0 || N <= 0 || K <= 0 || K > MAX_LEN || N > MAX_LEN || R > MAX_LEN || !offsets || off(offsets, 4) || bad_type(type) || !Y ||
-        off_type(Y, type) || ldy < N || bad_mx4(X, ldx, Xs, ldxs, K) || bad_mx4(W, ldw, Ws, ldws, K) || (groups > 1 && ((plane_w & 15) || (plane_ws & 7))))
+        off_type(Y, type) || ldy < N || bad_mx4(X, ldx, Xs, ldxs, K) || bad_mx4(W, ldw, Ws, ldws, K) || (groups > 1 && ((plane_w & 15) || (plane_ws & 15))))
         return OZB_EARG;
     if (groups > 1024) return OZB_ESIZE;
-    return run_mx4({1, groups, N, R, K, type, offsets, W, Ws, X, Xs, ldw, ldws, ldx, ldxs, plane_w, plane_ws, Y, ldy, 0}, stream);
+    return run_mx4({1, groups, R, N, K, type, offsets, X, ldx, Xs, ldxs, W, ldw, plane_w, Ws, ldws, plane_ws, Y, ldy, 0}, stream);
 }
 OZB_API int ozb_mx4_gemm_segments(int groups, int M, int N, int R, const int *offsets, const uint8_t *A, long long lda, const uint8_t *As, long long ldas,
                                   const uint8_t *B, long long ldb, const uint8_t *Bs, long long ldbs, void *Y, int type, long long ldy, size_t plane_y,
@@ -908,7 +908,7 @@ OZB_API int ozb_mx4_gemm_segments(int groups, int M, int N, int R, const int *of
         off_type(Y, type) || ldy < N || bad_mx4(A, lda, As, ldas, R) || bad_mx4(B, ldb, Bs, ldbs, R))
         return OZB_EARG;
     if (groups > 1024) return OZB_ESIZE;
-    return run_mx4({2, groups, N, M, R, type, offsets, B, Bs, A, As, ldb, ldbs, lda, ldas, 0, 0, Y, ldy, plane_y}, stream);
+    return run_mx4({2, groups, M, N, R, type, offsets, A, lda, As, ldas, B, ldb, 0, Bs, ldbs, 0, Y, ldy, plane_y}, stream);
 }
 
 // ---- tokens by expert ---------------------------------------------------------------------------------------------

@@ -1,24 +1,34 @@
 // mx4_gemm.cu -- products of microscaled 4-bit operands on the block-scaled tensor-core instruction of sm_100a.
 //
-//     C[g][j][i] = sum_k P[g][i][k] Q[j][k]        values of 4-bit codes times a power of two for every 32 along k
+//     Y[t][n] = sum_k X[t][k] W[n][k]        values of 4-bit codes times a power of two for every 32 along k
 //
-// P are the lanes of the accumulator (weights: contiguous in C), Q its columns (tokens, the rows of C). Three walks over the groups g:
-//     dense      one group, every row of Q
-//     by rows    group g owns the rows [offsets[g], offsets[g + 1]) of Q and C and multiplies them by its own P[g]
-//     along k    group g owns the k in [offsets[g], offsets[g + 1]) (multiples of 64); P and Q are shared, C[g] is its own
+// X are the tokens, W the weights. Three walks over groups g:
+//     dense      one group
+//     by rows    group g owns the rows [offsets[g], offsets[g + 1]) of X and Y and multiplies them by its own W[g]
+//     along k    group g owns the k in [offsets[g], offsets[g + 1]) (multiples of 64); X and W are shared, Y[g] is its own
 // The offsets live on the device. Accumulation is in FP32 in tensor memory, one rounding to the output type at the end.
 //
-// One kernel, warp-specialised, 128 rows of P by BN rows of Q to a tile, 256 values (128 bytes) of k to a stage:
-//   warp 0     producer: one thread, TMA (128-byte swizzle) of both operands' codes into a ring of stages
-//   warp 1     issuer: one thread; tcgen05.cp of the stage's scales into tensor memory, four tcgen05.mma kind::mxf4 (K = 64) on it
-//   warps 2-3  scales: the row-major scale bytes of 128 + BN rows become the tiles of 128 rows x 4 blocks that the instruction
-//              takes (row r of a tile at byte 16 (r % 32) + 4 (r / 32)): a lane reads 8 bytes of each of the rows l, l + 32,
-//              l + 64, l + 96 and writes two 16-byte words, so the turn costs two conflict-free stores for 128 rows
+// One kernel, warp-specialised: a tile is 128 rows of P, which are the lanes of the accumulator, by BN rows of Q, its columns; 256
+// values (128 bytes) of k make a stage, 512 (16 scale bytes) a scale slot.
+//   warp 0     producer: one thread, TMA of both operands' codes (128-byte swizzle) into a ring of stages. What lies outside a matrix
+//              comes as zero codes.
+//   warps 3, 8, 9  scales, in turns of a slot: a row's 16 bytes are four words, one to 128 values of k; the instruction wants, for a
+//              word, 128 rows as 32 x 16 bytes (row r at 16 (r % 32) + 4 (r / 32)). A lane reads the rows l, l + 32, l + 64, l + 96
+//              and writes the 4 x 4 words turned: four 16-byte loads and stores for 128 rows by 512 values, without bank conflicts.
+//   warp 2     one thread; tcgen05.cp of a stage's turned scales into tensor memory, its completion counted by the stage's barrier
+//   warp 1     issuer: one thread; four tcgen05.mma kind::mxf4 (K = 64) to a stage
 //   warps 4-7  epilogue: tensor memory to registers to global memory, while the next tile accumulates
-// The scales of a stage have tensor-memory columns of their own, so a stage's release covers them too.
-// Rows of Q are few where latency counts, so BN is 16 to 192, chosen by the rows there are to a group, and with few tiles the k of
-// a tile is split over a cluster of 2, 4 or 8 CTAs, whose partial tiles are added in a fixed order through distributed shared
-// memory. Every wait is bounded: on expiry the CTA raises the status word, stops, frees its tensor memory and returns.
+// An instruction of tcgen05 takes 20 to 60 cycles to issue, whatever it does; with the four to six copies of a stage's scales in
+// the thread that issues its four products the tensor pipe waited, so the copies have a thread of their own. Bringing the scale
+// bytes by TMA was slower: boxes 16 bytes wide cost the TMA unit as much for a row as the 128 bytes of its codes (900 cycles a slot).
+//
+// Few tokens (NARROW): P = weights, Q = tokens, BN = 16 .. 128 by the tokens there are, Y's columns are the lanes, so that a warp stores
+// contiguous columns of one token. With few tiles the k of a tile is split over a cluster of 2, 4 or 8 CTAs, whose partial tiles
+// are added in a fixed order through distributed shared memory. Many tokens (WIDE): P = tokens, Q = weights, BN = 192, a lane stores
+// 32 columns of its token in 16-byte pieces; two accumulators of 192 columns leave 128 columns of tensor memory for scales. With
+// enough tiles a pair of CTAs (cta_group::2) shares a tile of 256 tokens: each loads its own 128 tokens and half of the weights'
+// rows (a seventh of the bytes in shared memory for an operation less than a third), and turns its own and all the weights' scales.
+// Every wait is bounded: on expiry the CTA raises the status word, stops, frees its tensor memory and returns.
 #include <type_traits>
 #include "oz_async.cuh"
 #include "oz_common.cuh"
@@ -29,61 +39,96 @@ namespace ozk {
 
 namespace m4 {
 
-constexpr int BP = 128;            // rows of P to a tile
+constexpr int BP = 128;            // rows of P to a CTA
 constexpr int BK = 256, BKB = 128; // k of a stage, in values and in bytes
 constexpr int UK = 64;             // k of one tcgen05.mma kind::mxf4
-constexpr int THREADS = 256;
+constexpr int THREADS = 320, TURNERS = 3;
 constexpr int MAX_GROUPS = 1024;
 
 enum { DENSE = 0, BY_ROWS = 1, ALONG_K = 2 };
+enum { NARROW = 0, SPLIT = 1, WIDE = 2, PAIR = 3 };
 
 struct Params {
     int mode, groups;
-    int rows_p, rows_q, K;          // rows of P (to a group), rows of Q, length along k
-    int tiles_p, band;              // tiles of P, and how many of them are walked before the next tile of Q
+    int tokens, weights, K;         // rows of X, rows of W (to a group), length along k
+    int band;                       // tiles of P that are walked before the next tile of Q
     const int *offsets;             // [groups + 1] on the device (BY_ROWS, ALONG_K)
-    const uint8_t *sp, *sq;         // scale bytes, row-major
+    const uint8_t *sp, *sq;         // scales of P and Q
     long long ldsp, ldsq;
-    size_t plane_sp;                // bytes between the scales of two groups of P
-    void *C;
-    long long ldc;
-    size_t plane_c;                 // elements between the results of two groups (ALONG_K)
+    size_t plane_sp, plane_sq;      // bytes between two groups' (0: shared)
+    void *Y;
+    long long ldy;
+    size_t plane_y;                 // elements between the results of two groups (ALONG_K)
     int *status;
 };
 
-template <int BN> struct Shape {
+template <int FORM, int BN> struct Shape {
+    static constexpr bool pair = FORM == PAIR, wide = FORM >= WIDE;
+    static constexpr int P_TILE = pair ? 2 * BP : BP;              // rows of P to a tile
+    static constexpr int TOKENS = wide ? P_TILE : BN, WEIGHTS = wide ? BN : P_TILE;
+    static constexpr int Q_ROWS = pair ? BN / 2 : BN;              // rows of Q whose codes this CTA loads
     static constexpr int Q_TILES = (BN + 127) / 128;               // scale tiles of 128 rows of Q
-    static constexpr int P_BYTES = BP * BKB, Q_BYTES = BN * BKB;
-    static constexpr int SP_BYTES = 2 * 512, SQ_BYTES = 2 * 512 * Q_TILES;
-    static constexpr int STAGE = P_BYTES + Q_BYTES + SP_BYTES + SQ_BYTES;
+    static constexpr int P_BYTES = BP * BKB, Q_BYTES = Q_ROWS * BKB, STAGE = P_BYTES + Q_BYTES;
+    static constexpr int SLOT = 4 * 512 * (1 + Q_TILES);           // turned scales of 512 values of k: four words of P's tile, then of Q's
     static constexpr int SCALE_COLS = 8 + 8 * Q_TILES;             // tensor-memory columns of a stage's scales
-    static constexpr int STAGES = BN <= 32 ? 8 : BN <= 64 ? 7 : BN <= 128 ? 6 : 5;
+    static constexpr int STAGES = pair ? 5 : BN <= 32 ? 8 : BN <= 64 ? 7 : BN <= 128 ? 5 : 4;
+    static constexpr int SLOTS = TURNERS;                          // a slot is always the same warp's
     static constexpr int COLS = 2 * BN + STAGES * SCALE_COLS;      // two accumulators, and the scales
     static constexpr int TMEM_COLS = COLS <= 256 ? 256 : 512;
-    static constexpr int BARS = 2 * STAGES + 4;
-    static constexpr int SMEM = STAGES * STAGE + 1024 + 8 * BARS + 16 + 4 * (MAX_GROUPS + 1);
+    static constexpr int BARS = 2 * STAGES + 2 * SLOTS + 4;
+    static constexpr int SMEM = STAGES * STAGE + SLOTS * SLOT + 1024 + 8 * BARS + 16 + 4 * (MAX_GROUPS + 1);
     static_assert(STAGE % 1024 == 0 && COLS <= 512 && SMEM <= 232448 - 64, "");
-    static_assert(BN * BP * 4 <= STAGES * STAGE, "the partial tile of a split takes the place of the stages");
-    // instruction descriptor: E2M1 x E2M1, both K-major, one power of two (UE8M0) for 32, N = BN, M = 128, K = 64
-    static constexpr uint32_t IDESC = (1u << 7) | (1u << 10) | ((uint32_t)(BN >> 3) << 17) | (1u << 23) | (1u << 27);
+    static_assert(FORM != SPLIT || BN * BP * 4 <= STAGES * STAGE, "the partial tile of a split takes the place of the stages");
+    // instruction descriptor: E2M1 x E2M1, both K-major, one power of two (UE8M0) for 32, N = BN, M = rows of P, K = 64
+    static constexpr uint32_t IDESC = (1u << 7) | (1u << 10) | ((uint32_t)(BN >> 3) << 17) | (1u << 23) | ((uint32_t)(P_TILE >> 7) << 27);
 };
 
+template <bool PAIRED>
 __device__ __forceinline__ void mma_mx4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %6, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
-        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate) : "memory");
+    if constexpr (PAIRED)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+            ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate) : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+            ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate) : "memory");
 }
-// 512 bytes of scales (32 x 16) to four columns of tensor memory, the same in each quarter of the lanes
+// 512 bytes of scales (32 x 16) to four columns of tensor memory, the same in each quarter of the lanes (in a pair: in both CTAs, each
+// from its own shared memory)
+template <bool PAIRED>
 __device__ __forceinline__ void copy_scales(uint32_t tmem, uint32_t smem) {
     const uint64_t desc = (uint64_t)((smem & 0x3FFFFu) >> 4) | (8ull << 32) | (1ull << 46);   // no swizzle, groups of 8 rows 128 bytes apart
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
+    if constexpr (PAIRED) asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
+    else asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
+}
+// everything issued so far, done: arrives on the barrier (in a pair: on the barriers of both CTAs at this offset)
+template <bool PAIRED>
+__device__ __forceinline__ void commit(uint32_t bar) {
+    if constexpr (PAIRED)
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3) : "memory");
+    else mma_commit(bar);
+}
+
+// The value of lane 0 in all lanes: the compiler then keeps it, and what is computed from it, in the registers that a warp shares,
+// where tcgen05 and TMA instructions take their operands from.
+__device__ __forceinline__ int uniform(int x) { return __shfl_sync(~0u, x, 0); }
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return __shfl_sync(~0u, x, 0); }
+
+// the first n (0 < n < 16) bytes of v, zeros behind them
+__device__ __forceinline__ uint4 first_bytes(uint4 v, int n) {
+    auto keep = [&](uint32_t x, int from) { return n >= from + 4 ? x : n <= from ? 0u : x & ((1u << (8 * (n - from))) - 1u); };
+    return make_uint4(keep(v.x, 0), keep(v.y, 4), keep(v.z, 8), keep(v.w, 12));
 }
 
 // what a work item is
 struct Tile {
-    int group, tp, q0, q1;   // group, tile of P, rows [q0, q1) of Q (at most BN)
+    int group;
+    int p0, p1, q0, q1;      // rows of P and of Q: from the first, and where they end (this group's, not the tile's)
     int k0, k1;              // range along k
     int s0, s1;              // stages [s0, s1) of 256 that cover it (or this CTA's share of them)
 };
@@ -94,29 +139,28 @@ __device__ __forceinline__ void segment(const Params &p, int g, int limit, int &
     hi = min(max(__ldg(p.offsets + g + 1), lo), limit);
 }
 
-template <int BN> __device__ __forceinline__ int tiles_of(int rows) { return (rows + BN - 1) / BN; }
-
-// item w -> tile; `cum` has the running number of tiles of Q (BY_ROWS). Bands of `band` tiles of P are walked tile of Q by tile of Q,
+// item w -> tile; `cum` has the running number of token tiles (BY_ROWS). Bands of `band` tiles of P are walked tile of Q by tile of Q,
 // so that the CTAs at work at one time share both operands' panels in L2.
-template <int BN>
+template <class S>
 __device__ __forceinline__ Tile decode(const Params &p, const int *cum, int w) {
     Tile t;
-    int tq, tiles_q, q_lo = 0, q_hi = p.rows_q, idx;
+    const int nw = (p.weights + S::WEIGHTS - 1) / S::WEIGHTS;
+    int nt, lo = 0, hi = p.tokens, idx;
     t.k0 = 0;
     t.k1 = p.K;
     if (p.mode == BY_ROWS) {
-        int lo = 0, hi = p.groups;   // the last group whose first item is not behind w
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (cum[mid] * p.tiles_p <= w) lo = mid; else hi = mid;
+        int a = 0, b = p.groups;   // the last group whose first item is not behind w
+        while (b - a > 1) {
+            const int mid = (a + b) >> 1;
+            if (cum[mid] * nw <= w) a = mid; else b = mid;
         }
-        t.group = lo;
-        idx = w - cum[lo] * p.tiles_p;
-        tiles_q = cum[lo + 1] - cum[lo];
-        segment(p, lo, p.rows_q, q_lo, q_hi);
+        t.group = a;
+        idx = w - cum[a] * nw;
+        nt = cum[a + 1] - cum[a];
+        segment(p, a, p.tokens, lo, hi);
     } else {
-        tiles_q = tiles_of<BN>(p.rows_q);
-        const int per_group = tiles_q * p.tiles_p;
+        nt = (p.tokens + S::TOKENS - 1) / S::TOKENS;
+        const int per_group = nt * nw;
         t.group = w / per_group;
         idx = w - t.group * per_group;
         if (p.mode == ALONG_K) {
@@ -125,61 +169,92 @@ __device__ __forceinline__ Tile decode(const Params &p, const int *cum, int w) {
             t.k1 &= ~(UK - 1);
         }
     }
-    const int span = p.band * tiles_q, b = idx / span, first = b * p.band, rows = min(p.band, p.tiles_p - first), within = idx - b * span;
-    t.tp = first + within % rows;
-    tq = within / rows;
-    t.q0 = q_lo + tq * BN;
-    t.q1 = min(q_hi, t.q0 + BN);
+    const int np = S::wide ? nt : nw, nq = S::wide ? nw : nt;
+    const int span = p.band * nq, b = idx / span, first = b * p.band, rows = min(p.band, np - first), within = idx - b * span;
+    const int tp = first + within % rows, tq = within / rows;
+    t.p0 = (S::wide ? lo : 0) + tp * S::P_TILE;
+    t.p1 = S::wide ? hi : p.weights;
+    t.q0 = (S::wide ? 0 : lo) + tq * (S::wide ? S::WEIGHTS : S::TOKENS);
+    t.q1 = S::wide ? p.weights : hi;
     t.s0 = t.k0 / BK;
     t.s1 = t.k1 > t.k0 ? (t.k1 + BK - 1) / BK : t.s0;
     return t;
 }
 
-// 32 columns of a tile: lane = row of P, v[c] = column c
+// 32 columns of a tile, v[c] = column j + c of the lane's row i. NARROW: Y's rows are the columns j, a warp stores 32 lanes side by
+// side; WIDE: Y's row is i, a lane stores 16-byte pieces where they are whole and aligned.
 template <class T>
-__device__ __forceinline__ void store_columns(T *C, long long ldc, const uint32_t (&v)[32], int i, int rows_p, int j, int j1) {
-    if (i >= rows_p) return;
-    T *dst = C + (size_t)j * ldc + i;
+__device__ __forceinline__ void store_narrow(T *Y, long long ldy, const uint32_t (&v)[32], int i, int i1, int j, int j1) {
+    if (i >= i1) return;
+    T *dst = Y + (size_t)j * ldy + i;
 #pragma unroll
     for (int c = 0; c < 32; c++)
-        if (j + c < j1) dst[(size_t)c * ldc] = from_f32<T>(__uint_as_float(v[c]));
+        if (j + c < j1) dst[(size_t)c * ldy] = from_f32<T>(__uint_as_float(v[c]));
+}
+template <class T>
+__device__ __forceinline__ void store_wide(T *Y, long long ldy, const uint32_t (&v)[32], int i, int i1, int j, int j1) {
+    if (i >= i1 || j >= j1) return;
+    T *dst = Y + (size_t)i * ldy + j;
+    if (j + 32 <= j1 && !(reinterpret_cast<uintptr_t>(dst) & 15)) {
+        constexpr int N = Vec16<T>::N;
+#pragma unroll
+        for (int c = 0; c < 32; c += N) *reinterpret_cast<uint4 *>(dst + c) = Vec16<T>::pack(reinterpret_cast<const float *>(&v[c]));
+    } else {
+#pragma unroll
+        for (int c = 0; c < 32; c++)
+            if (j + c < j1) dst[c] = from_f32<T>(__uint_as_float(v[c]));
+    }
 }
 
-template <int BN, class T, bool SPLIT>
+template <int FORM, int BN, class T>
 __global__ void __launch_bounds__(THREADS, 1) mx4_gemm(const __grid_constant__ CUtensorMap mapP, const __grid_constant__ CUtensorMap mapQ,
                                                        const Params p) {
-    using S = Shape<BN>;
+    using S = Shape<FORM, BN>;
+    constexpr bool pair = S::pair;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t *const base_ptr = smem_raw + (base - smem_u32(smem_raw));
-    const uint32_t bars = base + S::STAGES * S::STAGE;
-    auto full_bar = [&](int s) { return bars + 8u * s; };
-    auto empty_bar = [&](int s) { return bars + 8u * (S::STAGES + s); };
-    auto accfull_bar = [&](int a) { return bars + 8u * (2 * S::STAGES + a); };
-    auto accempty_bar = [&](int a) { return bars + 8u * (2 * S::STAGES + 2 + a); };
+    const uint32_t slots = base + S::STAGES * S::STAGE, bars = slots + S::SLOTS * S::SLOT;
+    auto full_bar = [&](int s) { return bars + 8u * s; };                                        // codes are there, and the scales in tensor memory (in a pair: both CTAs', at the leader)
+    auto empty_bar = [&](int s) { return bars + 8u * (S::STAGES + s); };                         // the stage has been used up
+    auto turned_bar = [&](int s) { return bars + 8u * (2 * S::STAGES + s); };                    // a slot's scales are turned (in a pair: both CTAs', at the leader)
+    auto slot_bar = [&](int s) { return bars + 8u * (2 * S::STAGES + S::SLOTS + s); };           // the slot has been used up
+    auto accfull_bar = [&](int a) { return bars + 8u * (2 * S::STAGES + 2 * S::SLOTS + a); };
+    auto accempty_bar = [&](int a) { return bars + 8u * (2 * S::STAGES + 2 * S::SLOTS + 2 + a); };
     const uint32_t tmem_slot = bars + 8u * S::BARS;
-    int *const cum = reinterpret_cast<int *>(base_ptr + S::STAGES * S::STAGE + 8 * S::BARS + 16);
+    int *const cum = reinterpret_cast<int *>(base_ptr + S::STAGES * S::STAGE + S::SLOTS * S::SLOT + 8 * S::BARS + 16);
     __shared__ int abort_flag;
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
+    uint32_t rank = 0, ranks = 1;
+    if constexpr (FORM == SPLIT || pair) {
+        rank = uniform(cluster_rank());
+        asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks));
+    }
     if (threadIdx.x == 0) {
         abort_flag = 0;
-        for (int s = 0; s < S::STAGES; s++) { mbar_init(full_bar(s), 2); mbar_init(empty_bar(s), 1); }   // full: the TMA's bytes and a scale warp
-        for (int a = 0; a < 2; a++) { mbar_init(accfull_bar(a), 1); mbar_init(accempty_bar(a), 4); }
+        for (int s = 0; s < S::STAGES; s++) { mbar_init(full_bar(s), 2); mbar_init(empty_bar(s), 1); }
+        for (int s = 0; s < S::SLOTS; s++) { mbar_init(turned_bar(s), pair ? 2 : 1); mbar_init(slot_bar(s), 1); }
+        for (int a = 0; a < 2; a++) { mbar_init(accfull_bar(a), 1); mbar_init(accempty_bar(a), pair ? 8 : 4); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tmem_slot), "r"((uint32_t)S::TMEM_COLS) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        if constexpr (pair) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tmem_slot), "r"((uint32_t)S::TMEM_COLS) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tmem_slot), "r"((uint32_t)S::TMEM_COLS) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        }
     }
-    if (warp == 2 && p.mode == BY_ROWS) {   // running number of tiles of Q over the groups
+    if (warp == 2 && p.mode == BY_ROWS) {   // running number of token tiles over the groups
         int run = 0;
         for (int g0 = 0; g0 < p.groups; g0 += 32) {
             int n = 0;
             if (g0 + lane < p.groups) {
                 int lo, hi;
-                segment(p, g0 + lane, p.rows_q, lo, hi);
-                n = tiles_of<BN>(hi - lo);
+                segment(p, g0 + lane, p.tokens, lo, hi);
+                n = (hi - lo + S::TOKENS - 1) / S::TOKENS;
             }
             int inc = n;
 #pragma unroll
@@ -194,152 +269,201 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm(const __grid_constant__ C
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
+    if constexpr (pair) cluster_sync_all();   // the peer's barriers exist before anything arrives on them
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     uint32_t tmem_base;
     asm volatile("ld.shared.b32 %0, [%1];" : "=r"(tmem_base) : "r"(tmem_slot) : "memory");
+    tmem_base = uniform(tmem_base);
     const uint32_t tmem_scales = tmem_base + 2 * BN;
 
-    const int total = p.mode == BY_ROWS ? cum[p.groups] * p.tiles_p : tiles_of<BN>(p.rows_q) * p.tiles_p * (p.mode == ALONG_K ? p.groups : 1);
-    uint32_t rank = 0, ranks = 1;
+    const int nt = p.mode == BY_ROWS ? cum[p.groups] : (p.tokens + S::TOKENS - 1) / S::TOKENS * (p.mode == ALONG_K ? p.groups : 1);
+    const int total = uniform(nt) * ((p.weights + S::WEIGHTS - 1) / S::WEIGHTS);
     int first = blockIdx.x, step = gridDim.x;
-    if constexpr (SPLIT) {   // one tile to a cluster; this CTA takes its share of the stages
-        rank = cluster_rank();
-        asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks));
+    if constexpr (FORM == SPLIT) {   // one tile to a cluster; this CTA takes its share of the stages
         first = blockIdx.x / ranks;
         step = 1 << 30;
     }
+    if constexpr (pair) {
+        first = blockIdx.x >> 1;
+        step = gridDim.x >> 1;
+    }
     auto tile_at = [&](int w) {
-        Tile t = decode<BN>(p, cum, w);
-        if constexpr (SPLIT) {
+        Tile t = decode<S>(p, cum, w);
+        if constexpr (FORM == SPLIT) {
             const int n = t.s1 - t.s0, s0 = t.s0;
             t.s0 = s0 + (int)((long long)n * rank / ranks);
             t.s1 = s0 + (int)((long long)n * (rank + 1) / ranks);
         }
+        t.group = uniform(t.group);
+        t.p0 = uniform(t.p0); t.p1 = uniform(t.p1);
+        t.q0 = uniform(t.q0); t.q1 = uniform(t.q1);
+        t.k0 = uniform(t.k0); t.k1 = uniform(t.k1);
+        t.s0 = uniform(t.s0); t.s1 = uniform(t.s1);
         return t;
     };
+    auto new_slot = [](const Tile &t, int kb) { return kb == t.s0 || !(kb & 1); };   // a slot holds an even stage and the odd one behind it
     volatile int *abortp = &abort_flag;
-    uint32_t issued = 0;   // stages the producer has filled
+    uint32_t it = 0, sl = 0;   // running stage and slot (of the role that counts them)
 
     if (warp == 0) {
-        if (lane == 0) {
-            uint32_t it = 0;
-            for (int w = first; w < total && !*abortp; w += step) {
-                const Tile t = tile_at(w);
-                for (int kb = t.s0; kb < t.s1; kb++, it++) {
-                    const int s = it % S::STAGES;
-                    if (!mbar_wait(empty_bar(s), ((it / S::STAGES) & 1u) ^ 1u, abortp, 0x110)) break;
-                    mbar_expect_tx(full_bar(s), S::P_BYTES + S::Q_BYTES);
-                    const uint32_t at = base + s * S::STAGE;
-                    tma_load_3d(at, &mapP, kb * BKB, t.tp * BP, p.mode == BY_ROWS ? t.group : 0, full_bar(s));
-                    tma_load_3d(at + S::P_BYTES, &mapQ, kb * BKB, t.q0, 0, full_bar(s));
-                    issued = it + 1;
+        for (int w = first; w < total && !__any_sync(~0u, *abortp); w += step) {
+            const Tile t = tile_at(w);
+            const int zp = !S::wide && p.mode == BY_ROWS ? t.group : 0, zq = S::wide && p.mode == BY_ROWS ? t.group : 0;
+            const int p0 = t.p0 + (pair ? (int)rank * BP : 0), q0 = t.q0 + (pair ? (int)rank * S::Q_ROWS : 0);
+            for (int kb = t.s0; kb < t.s1; kb++, it++) {
+                const int s = it % S::STAGES;
+                if (!warp_wait(empty_bar(s), ((it / S::STAGES) & 1u) ^ 1u, abortp, 0x111)) break;
+                const uint32_t at = base + s * S::STAGE;
+                if (elect_one()) {
+                    if constexpr (pair) {
+                        const uint32_t lead = map_to_cta(full_bar(s), 0);
+                        if (rank == 0) mbar_expect_tx(full_bar(s), 2 * S::STAGE);   // both CTAs' bytes arrive here
+                        tma_load_3d_pair(at, &mapP, kb * BKB, p0, zp, lead);
+                        tma_load_3d_pair(at + S::P_BYTES, &mapQ, kb * BKB, q0, zq, lead);
+                    } else {
+                        mbar_expect_tx(full_bar(s), S::STAGE);
+                        tma_load_3d(at, &mapP, kb * BKB, p0, zp, full_bar(s));
+                        tma_load_3d(at + S::P_BYTES, &mapQ, kb * BKB, q0, zq, full_bar(s));
+                    }
                 }
+                __syncwarp();
             }
         }
     } else if (warp == 1) {
-        if (lane == 0) {
-            uint32_t it = 0, n = 0;
-            for (int w = first; w < total && !*abortp; w += step, n++) {
+        if (!pair || rank == 0) {
+            uint32_t n = 0;
+            for (int w = first; w < total && !__any_sync(~0u, *abortp); w += step, n++) {
                 const Tile t = tile_at(w);
                 const uint32_t acc = n & 1u;
-                if (!mbar_wait(accempty_bar(acc), ((n >> 1) & 1u) ^ 1u, abortp, 0x120)) break;
+                if (!warp_wait(accempty_bar(acc), ((n >> 1) & 1u) ^ 1u, abortp, 0x120)) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint32_t d = tmem_base + acc * BN;
                 bool ok = true;
                 uint32_t accumulate = 0;
                 for (int kb = t.s0; kb < t.s1; kb++, it++) {
                     const int s = it % S::STAGES;
-                    if (!mbar_wait(full_bar(s), (it / S::STAGES) & 1u, abortp, 0x130)) { ok = false; break; }
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const uint32_t at = base + s * S::STAGE, sp = at + S::P_BYTES + S::Q_BYTES, sq = sp + S::SP_BYTES;
-                    const uint32_t tp = tmem_scales + s * S::SCALE_COLS, tq = tp + 8;
-#pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        copy_scales(tp + 4 * h, sp + 512 * h);
-#pragma unroll
-                        for (int c = 0; c < S::Q_TILES; c++) copy_scales(tq + 4 * (h * S::Q_TILES + c), sq + 512 * (h * S::Q_TILES + c));
-                    }
+                    const uint32_t at = base + s * S::STAGE, tp = tmem_scales + s * S::SCALE_COLS, tq = tp + 8;
                     const uint64_t da = smem_desc(at), db = smem_desc(at + S::P_BYTES);
-                    const int k_lo = (t.k0 - kb * BK) / UK, k_hi = (t.k1 - kb * BK + UK - 1) / UK;   // the instructions of this stage that are in range
+                    const int k_lo = max(0, (t.k0 - kb * BK) / UK), k_hi = (t.k1 - kb * BK + UK - 1) / UK;   // the instructions of this stage that are in range
+                    if (!(ok = warp_wait(full_bar(s), (it / S::STAGES) & 1u, abortp, 0x130))) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    if (elect_one()) {
 #pragma unroll
-                    for (int k = 0; k < BK / UK; k++) {
-                        if (k < k_lo || k >= k_hi) continue;
-                        const uint32_t id = S::IDESC | ((k & 1u) ? (2u << 4) | (2u << 29) : 0u);      // which two of a word's four scales
-                        mma_mx4(d, da + 2u * k, db + 2u * k, id, tp + 4 * (k >> 1), tq + 4 * (k >> 1) * S::Q_TILES, accumulate);
-                        accumulate = 1;
+                        for (int k = 0; k < BK / UK; k++) {
+                            if (k < k_lo || k >= k_hi) continue;
+                            const uint32_t id = S::IDESC | ((k & 1u) ? (2u << 4) | (2u << 29) : 0u);      // which two of a word's four scales
+                            mma_mx4<pair>(d, da + 2u * k, db + 2u * k, id, tp + 4 * (k >> 1), tq + 4 * (k >> 1) * S::Q_TILES, accumulate | (uint32_t)(k > k_lo));
+                        }
+                        commit<pair>(empty_bar(s));
                     }
-                    mma_commit(empty_bar(s));
+                    __syncwarp();
+                    accumulate = 1;
                 }
                 if (!ok) break;
-                mma_commit(accfull_bar(acc));
+                if (elect_one()) commit<pair>(accfull_bar(acc));
+                __syncwarp();
             }
         }
-    } else if (warp < 4) {
-        const uint32_t own = warp & 1u;   // this warp takes the stages of its parity
-        const int blocks = (p.K + 31) / 32;
-        uint32_t it = 0;
-        for (int w = first; w < total && !*abortp; w += step) {
-            const Tile t = tile_at(w);
-            const uint8_t *rows_p = p.sp + (p.mode == BY_ROWS ? (size_t)t.group * p.plane_sp : 0);
-            bool ok = true;
-            for (int kb = t.s0; kb < t.s1; kb++, it++) {
-                if ((it & 1u) != own) continue;
-                const int s = it % S::STAGES;
-                constexpr int TILES = 1 + S::Q_TILES;
-                uint2 v[TILES][4];
-                // scales behind the last block of a row, and of rows that are not there, become 1: their codes are zero or unused
-                const int left = blocks - kb * 8;
+    } else if (warp == 2) {
+        if (!pair || rank == 0) {
+            sl = ~0u;
+            for (int w = first; w < total && !__any_sync(~0u, *abortp); w += step) {
+                const Tile t = tile_at(w);
+                for (int kb = t.s0; kb < t.s1; kb++, it++) {
+                    if (new_slot(t, kb)) {
+                        sl++;
+                        bool ok;
+                        if constexpr (pair) ok = __all_sync(~0u, mbar_wait_acquire_cluster(turned_bar(sl % S::SLOTS), (sl / S::SLOTS) & 1u, abortp, 0x131));
+                        else ok = warp_wait(turned_bar(sl % S::SLOTS), (sl / S::SLOTS) & 1u, abortp, 0x131);
+                        if (!ok) break;
+                    }
+                    const int s = it % S::STAGES, r = sl % S::SLOTS;
+                    const uint32_t tiles = slots + r * S::SLOT + 1024 * (kb & 1), q_tiles = slots + r * S::SLOT + 2048 + 1024 * S::Q_TILES * (kb & 1);
+                    const uint32_t tp = tmem_scales + s * S::SCALE_COLS, tq = tp + 8;
+                    const bool slot_done = kb + 1 == t.s1 || (kb & 1);
+                    if (!warp_wait(empty_bar(s), ((it / S::STAGES) & 1u) ^ 1u, abortp, 0x132)) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    if (elect_one()) {
 #pragma unroll
-                for (int c = 0; c < TILES; c++)
+                        for (int h = 0; h < 2; h++) {
+                            copy_scales<pair>(tp + 4 * h, tiles + 512 * h);
+#pragma unroll
+                            for (int c = 0; c < S::Q_TILES; c++) copy_scales<pair>(tq + 4 * (h * S::Q_TILES + c), q_tiles + 512 * (h * S::Q_TILES + c));
+                        }
+                        if constexpr (pair) mma_commit_pair(full_bar(s));
+                        else mma_commit(full_bar(s));
+                        if (slot_done) commit<pair>(slot_bar(r));
+                    }
+                    __syncwarp();
+                }
+            }
+        }
+    } else if (warp < 4 || warp >= 8) {
+        // Of TURNERS warps, in turns of a slot: each has its slot's loads in flight while the others' slots are used.
+        const uint32_t own = warp < 4 ? 0 : warp - 7;
+        const int blocks = (p.K + 31) / 32;
+        sl = 0;
+        for (int w = first; w < total && !__any_sync(~0u, *abortp); w += step) {
+            const Tile t = tile_at(w);
+            const int p0 = t.p0 + (pair ? (int)rank * BP : 0);
+            const uint8_t *sp = p.sp + (size_t)t.group * p.plane_sp, *sq = p.sq + (size_t)t.group * p.plane_sq;
+            bool ok = true;
+            for (int kb = t.s0; kb < t.s1; kb = (kb | 1) + 1, sl++) {
+                if (sl % TURNERS != own) continue;
+                const int r = sl % S::SLOTS, at = (kb >> 1) * 16, left = blocks - at;
+                uint4 v[1 + S::Q_TILES][4];
+#pragma unroll
+                for (int c = 0; c < 1 + S::Q_TILES; c++)   // P's tile, then Q's
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
-                        const int r = lane + 32 * i;
-                        v[c][i] = make_uint2(0x7f7f7f7fu, 0x7f7f7f7fu);
+                        const int row = i * 32 + lane;
+                        v[c][i] = make_uint4(0, 0, 0, 0);   // 2^-127: rows that are not there
                         if (c == 0) {
-                            if (t.tp * BP + r < p.rows_p) v[c][i] = __ldg(reinterpret_cast<const uint2 *>(rows_p + (size_t)(t.tp * BP + r) * p.ldsp + (size_t)kb * 8));
+                            if (p0 + row < t.p1) v[c][i] = __ldg(reinterpret_cast<const uint4 *>(sp + (size_t)(p0 + row) * p.ldsp + at));
                         } else {
-                            const int q = t.q0 + (c - 1) * 128 + r;
-                            if (q < t.q1) v[c][i] = __ldg(reinterpret_cast<const uint2 *>(p.sq + (size_t)q * p.ldsq + (size_t)kb * 8));
+                            const int q = (c - 1) * 128 + row;
+                            if (q < BN && t.q0 + q < t.q1) v[c][i] = __ldg(reinterpret_cast<const uint4 *>(sq + (size_t)(t.q0 + q) * p.ldsq + at));
                         }
                     }
-                if (left < 8) {
-                    const uint32_t keep0 = left >= 4 ? ~0u : (1u << (8 * left)) - 1u, keep1 = left >= 4 ? (1u << (8 * (left - 4))) - 1u : 0u;
+                if (left < 16) {   // bytes behind the last block may hold anything: their codes are zero, their scales become it
 #pragma unroll
-                    for (int c = 0; c < TILES; c++)
+                    for (int c = 0; c < 1 + S::Q_TILES; c++)
 #pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            v[c][i].x = (v[c][i].x & keep0) | (0x7f7f7f7fu & ~keep0);
-                            v[c][i].y = (v[c][i].y & keep1) | (0x7f7f7f7fu & ~keep1);
-                        }
+                        for (int i = 0; i < 4; i++) v[c][i] = first_bytes(v[c][i], left);
                 }
-                if (!__all_sync(~0u, mbar_wait(empty_bar(s), ((it / S::STAGES) & 1u) ^ 1u, abortp, 0x140))) { ok = false; break; }
-                uint8_t *sp = base_ptr + s * S::STAGE + S::P_BYTES + S::Q_BYTES;
+                if (!warp_wait(slot_bar(r), ((sl / S::SLOTS) & 1u) ^ 1u, abortp, 0x140)) { ok = false; break; }
+                uint8_t *slot = base_ptr + S::STAGES * S::STAGE + r * S::SLOT + 16 * lane;
 #pragma unroll
-                for (int c = 0; c < TILES; c++) {
-                    // tile of the first four blocks, then of the last four; Q's tiles of one half lie side by side
-                    uint8_t *lo = c == 0 ? sp : sp + S::SP_BYTES + 512 * (c - 1), *hi = c == 0 ? sp + 512 : lo + 512 * S::Q_TILES;
-                    *reinterpret_cast<uint4 *>(lo + 16 * lane) = make_uint4(v[c][0].x, v[c][1].x, v[c][2].x, v[c][3].x);
-                    *reinterpret_cast<uint4 *>(hi + 16 * lane) = make_uint4(v[c][0].y, v[c][1].y, v[c][2].y, v[c][3].y);
+                for (int c = 0; c < 1 + S::Q_TILES; c++) {
+                    uint8_t *dst = slot + (c == 0 ? 0 : 2048 + 512 * (c - 1));
+                    const int pitch = c == 0 ? 512 : 512 * S::Q_TILES;   // to the tile of the next word
+                    *reinterpret_cast<uint4 *>(dst) = make_uint4(v[c][0].x, v[c][1].x, v[c][2].x, v[c][3].x);
+                    *reinterpret_cast<uint4 *>(dst + pitch) = make_uint4(v[c][0].y, v[c][1].y, v[c][2].y, v[c][3].y);
+                    *reinterpret_cast<uint4 *>(dst + 2 * pitch) = make_uint4(v[c][0].z, v[c][1].z, v[c][2].z, v[c][3].z);
+                    *reinterpret_cast<uint4 *>(dst + 3 * pitch) = make_uint4(v[c][0].w, v[c][1].w, v[c][2].w, v[c][3].w);
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the tensor core reads these through the async proxy
                 __syncwarp();
-                if (lane == 0) mbar_arrive(full_bar(s));
+                if (lane == 0) {
+                    if (pair && rank) mbar_arrive_release_cluster(map_to_cta(turned_bar(r), 0));
+                    else mbar_arrive(turned_bar(r));
+                }
             }
             if (!ok) break;
         }
     } else {
         const int quarter = warp & 3;
         uint32_t n = 0;
-        for (int w = first; w < total && !*abortp; w += step, n++) {
+        for (int w = first; w < total && !__any_sync(~0u, *abortp); w += step, n++) {
             const Tile t = tile_at(w);
             const uint32_t acc = n & 1u;
-            if (!__all_sync(~0u, mbar_wait(accfull_bar(acc), (n >> 1) & 1u, abortp, 0x150))) break;
+            if (!warp_wait(accfull_bar(acc), (n >> 1) & 1u, abortp, 0x150)) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * BN;
             const bool some = t.s1 > t.s0;   // no stage: nothing was accumulated, the tile is zero
-            const int i = t.tp * BP + quarter * 32 + lane;
-            if constexpr (!SPLIT) {
-                T *C = reinterpret_cast<T *>(p.C) + (p.mode == ALONG_K ? (size_t)t.group * p.plane_c : 0);
+            const int i = t.p0 + (pair ? (int)rank * BP : 0) + quarter * 32 + lane;
+            if constexpr (FORM != SPLIT) {
+                T *Y = reinterpret_cast<T *>(p.Y) + (p.mode == ALONG_K ? (size_t)t.group * p.plane_y : 0);
 #pragma unroll 1
                 for (int c = 0; c < BN; c += 32) {
                     if (t.q0 + c >= t.q1) break;
@@ -350,7 +474,9 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm(const __grid_constant__ C
 #pragma unroll
                         for (int e = 0; e < 32; e++) v[e] = 0;
                     }
-                    store_columns<T>(C, p.ldc, v, i, p.rows_p, t.q0 + c, t.q1);
+                    const int j1 = min(t.q1, t.q0 + BN);   // a tile of 16 columns: the other 16 are not its own
+                    if constexpr (S::wide) store_wide<T>(Y, p.ldy, v, i, t.p1, t.q0 + c, j1);
+                    else store_narrow<T>(Y, p.ldy, v, i, t.p1, t.q0 + c, j1);
                 }
             } else {   // the partial tile, [column][row of P], over the stages that this CTA has used up
                 float *part = reinterpret_cast<float *>(base_ptr);
@@ -366,28 +492,31 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm(const __grid_constant__ C
             }
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
-            if (lane == 0) mbar_arrive(accempty_bar(acc));
+            if (lane == 0) {
+                if constexpr (pair) mbar_arrive_cluster(map_to_cta(accempty_bar(acc), 0));
+                else mbar_arrive(accempty_bar(acc));
+            }
         }
     }
 
     __syncwarp();
-    if constexpr (SPLIT) {
+    if constexpr (FORM == SPLIT) {
         // every CTA of the cluster adds its share of the columns over the ranks, in their order: the same sum on every run
         __syncthreads();
         cluster_sync_all();
         if (first < total) {
-            const Tile t = decode<BN>(p, cum, first);
-            T *C = reinterpret_cast<T *>(p.C) + (p.mode == ALONG_K ? (size_t)t.group * p.plane_c : 0);
-            const int r = threadIdx.x & (BP - 1), i = t.tp * BP + r;
-            const int n = t.q1 - t.q0, c0 = (int)((long long)n * rank / ranks), c1 = (int)((long long)n * (rank + 1) / ranks);
-            for (int c = c0 + (threadIdx.x >> 7); c < c1; c += THREADS / BP) {
+            const Tile t = decode<S>(p, cum, first);
+            T *Y = reinterpret_cast<T *>(p.Y) + (p.mode == ALONG_K ? (size_t)t.group * p.plane_y : 0);
+            const int r = threadIdx.x & (BP - 1), i = t.p0 + r;
+            const int n = min(BN, t.q1 - t.q0), c0 = (int)((long long)n * rank / ranks), c1 = (int)((long long)n * (rank + 1) / ranks);
+            for (int c = c0 + (threadIdx.x >> 7); c < c1 && threadIdx.x < 2 * BP; c += 2) {
                 float sum = 0.f;
                 for (uint32_t q = 0; q < ranks; q++) {
                     float x;
                     asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(map_to_cta(base + 4u * (c * BP + r), q)) : "memory");
                     sum += x;
                 }
-                if (i < p.rows_p) C[(size_t)(t.q0 + c) * p.ldc + i] = from_f32<T>(sum);
+                if (i < t.p1) Y[(size_t)(t.q0 + c) * p.ldy + i] = from_f32<T>(sum);
             }
         }
         cluster_sync_all();   // nobody leaves while a peer still reads its partial tile
@@ -396,14 +525,17 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm(const __grid_constant__ C
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     if (abort_flag && warp == 0 && lane == 0) {   // copies in flight land before this CTA's shared memory is given back
-        for (uint32_t it = issued > S::STAGES ? issued - S::STAGES : 0; it < issued; it++) {
-            int ignore = 0;
-            const unsigned long long until = now_ns() + 100000000ull;
-            while (!mbar_try(full_bar(it % S::STAGES), (it / S::STAGES) & 1u) && !ignore) ignore = now_ns() > until;
-        }
+        const unsigned long long until = now_ns() + 200000000ull;
+        for (uint32_t k = it > S::STAGES ? it - S::STAGES : 0; k < it && !pair; k++)
+            while (!mbar_try(full_bar(k % S::STAGES), (k / S::STAGES) & 1u) && now_ns() < until) {}
+        while (now_ns() < until) {}
     }
     __syncthreads();
-    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"((uint32_t)S::TMEM_COLS) : "memory");
+    if constexpr (pair) cluster_sync_all();   // nobody leaves while the peer can still signal into its shared memory
+    if (warp == 1) {
+        if constexpr (pair) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"((uint32_t)S::TMEM_COLS) : "memory");
+        else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"((uint32_t)S::TMEM_COLS) : "memory");
+    }
     if (threadIdx.x == 0 && abort_flag) {
         atomicCAS(p.status, 0, abort_flag);
         if (blockIdx.x < 63) p.status[1 + blockIdx.x] = abort_flag;
@@ -412,39 +544,82 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm(const __grid_constant__ C
 
 // ---- host ----
 
-// {bytes along k, row, plane}; 128 bytes of `box_rows` rows to a copy
+// {bytes along k, row, plane} of codes, in boxes of 128 bytes (256 values) by `box_rows` rows, swizzled
 cudaError_t make_map(CUtensorMap *map, const uint8_t *ptr, int K, int rows, int planes, long long ld, size_t plane, int box_rows) {
     EncodeTiledFn enc = encode_fn();
     if (!enc) return cudaErrorNotSupported;
-    const cuuint64_t dims[3] = {(cuuint64_t)((K + 31) / 32 * 16), (cuuint64_t)rows, (cuuint64_t)planes};
+    const cuuint64_t dims[3] = {(cuuint64_t)(((long long)K + 31) / 32 * 16), (cuuint64_t)rows, (cuuint64_t)planes};
     const cuuint64_t strides[2] = {(cuuint64_t)ld, (cuuint64_t)(planes > 1 ? plane : (size_t)ld * rows)};
     const cuuint32_t box[3] = {(cuuint32_t)BKB, (cuuint32_t)box_rows, 1};
     const cuuint32_t estr[3] = {1, 1, 1};
-    const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<uint8_t *>(ptr), dims, strides, box, estr,
-                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+    const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<uint8_t *>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
-template <int BN, class T, bool SPLIT>
-cudaError_t launch(const CUtensorMap &mapP, const CUtensorMap &mapQ, const Params &p, int grid, int split, cudaStream_t st) {
+// what a form of the kernel does with a product: how many tiles, in how many CTAs
+struct Work { long long most, expected; };   // token tiles times weight tiles: at most, and with even segments
+Work work_of(const Mx4Product &g, int tokens, int weights) {
+    const long long nw = (g.weights + weights - 1) / weights;
+    if (g.mode != BY_ROWS) {
+        const long long n = (long long)((g.tokens + tokens - 1) / tokens) * (g.mode == ALONG_K ? g.groups : 1) * nw;
+        return {n, n};
+    }
+    const long long some = g.groups < g.tokens ? g.groups : g.tokens, each = (g.tokens + g.groups - 1) / g.groups;   // groups with rows, rows of one
+    return {(some + g.tokens / tokens) * nw, some * ((each + tokens - 1) / tokens) * nw};
+}
+
+template <int FORM, int BN, class T>
+cudaError_t launch(const Mx4Product &g, Params p, int sms, int split, cudaStream_t st) {
+    using S = Shape<FORM, BN>;
     static PerDevice pd;
-    cudaError_t e = pd.once([] { return cudaFuncSetAttribute(mx4_gemm<BN, T, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<BN>::SMEM); });
+    cudaError_t e = pd.once([] { return cudaFuncSetAttribute(mx4_gemm<FORM, BN, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM); });
     if (e) return e;
+    const Work w = work_of(g, S::TOKENS, S::WEIGHTS);
+    if (w.most > 0x0fffffffLL) return cudaErrorInvalidValue;
+    const int planes = g.mode == BY_ROWS ? g.groups : 1;
+    CUtensorMap x, w4;
+    if ((e = make_map(&x, g.x, g.K, g.tokens, 1, g.ldx, 0, S::wide ? BP : S::Q_ROWS))) return e;
+    if ((e = make_map(&w4, g.w, g.K, g.weights, planes, g.ldw, g.plane_w, S::wide ? S::Q_ROWS : BP))) return e;
+    const size_t plane = planes > 1 ? g.plane_ws : 0;
+    p.sp = S::wide ? g.xs : g.ws; p.ldsp = S::wide ? g.ldxs : g.ldws; p.plane_sp = S::wide ? 0 : plane;
+    p.sq = S::wide ? g.ws : g.xs; p.ldsq = S::wide ? g.ldws : g.ldxs; p.plane_sq = S::wide ? plane : 0;
+    const int per = FORM == SPLIT ? split : FORM == PAIR ? 2 : 1;   // CTAs to a cluster
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(grid);
     cfg.blockDim = dim3(THREADS);
-    cfg.dynamicSmemBytes = Shape<BN>::SMEM;
+    cfg.dynamicSmemBytes = S::SMEM;
     cfg.stream = st;
     cudaLaunchAttribute at[1];
-    if (SPLIT) {
+    if (per > 1) {
         at[0].id = cudaLaunchAttributeClusterDimension;
-        at[0].val.clusterDim.x = split;
+        at[0].val.clusterDim.x = per;
         at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
         cfg.attrs = at;
         cfg.numAttrs = 1;
     }
-    return cudaLaunchKernelEx(&cfg, mx4_gemm<BN, T, SPLIT>, mapP, mapQ, p);
+    // A persistent grid must be resident as a whole: a pair that started behind another would find its share of the tiles still to do.
+    // Not every SM has a neighbour to pair with (74 pairs were asked for, and the product took twice its time).
+    long long clusters = w.most;
+    if (FORM != SPLIT) {
+        long long room = sms;
+        if (FORM == PAIR) {
+            static int pairs[64] = {};
+            int dev = 0;
+            if ((e = cudaGetDevice(&dev))) return e;
+            int &n = pairs[dev & 63];
+            if (!n) {
+                cfg.gridDim = dim3((unsigned)(sms & ~1));
+                int found = 0;
+                if (cudaOccupancyMaxActiveClusters(&found, mx4_gemm<FORM, BN, T>, &cfg) != cudaSuccess || found <= 0) { cudaGetLastError(); found = sms / 2; }
+                n = found;
+            }
+            room = n;
+        }
+        if (clusters > room) clusters = room;
+    }
+    cfg.gridDim = dim3((unsigned)(clusters * per));
+    return cudaLaunchKernelEx(&cfg, mx4_gemm<FORM, BN, T>, S::wide ? x : w4, S::wide ? w4 : x, p);
 }
 
 }  // namespace m4
@@ -454,63 +629,46 @@ cudaError_t mx4_product(const Mx4Product &g, int *status, cudaStream_t st) {
     Params p{};
     p.mode = g.mode;
     p.groups = g.groups;
-    p.rows_p = g.rows_p;
-    p.rows_q = g.rows_q;
+    p.tokens = g.tokens;
+    p.weights = g.weights;
     p.K = g.K;
-    p.tiles_p = (g.rows_p + BP - 1) / BP;
     p.band = 16;
     p.offsets = g.offsets;
-    p.sp = g.sp; p.ldsp = g.ldsp; p.plane_sp = g.plane_sp;
-    p.sq = g.sq; p.ldsq = g.ldsq;
-    p.C = g.C; p.ldc = g.ldc; p.plane_c = g.plane_c;
+    p.Y = g.y; p.ldy = g.ldy; p.plane_y = g.plane_y;
     p.status = status;
     int dev, sms;
     cudaError_t e = cudaGetDevice(&dev);
     if (!e) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
     if (e) return e;
 
-    // the width of a tile: the rows of Q that a group has (on average, by rows), rounded up to what there is
-    const int per_group = g.mode == BY_ROWS ? (g.rows_q + g.groups - 1) / g.groups : g.rows_q;
-    const int bn = per_group <= 16 ? 16 : per_group <= 32 ? 32 : per_group <= 64 ? 64 : per_group <= 512 ? 128 : 192;
-    // tiles of Q: exact, or (by rows) the most that there can be and the number to be expected of even segments
-    long long most, expected;
-    if (g.mode == BY_ROWS) {
-        most = (long long)(g.groups < g.rows_q ? g.groups : g.rows_q) + g.rows_q / bn;
-        expected = (long long)(g.groups < g.rows_q ? g.groups : g.rows_q) * ((per_group + bn - 1) / bn);
-    } else {
-        most = expected = (long long)((g.rows_q + bn - 1) / bn) * (g.mode == ALONG_K ? g.groups : 1);
-    }
-    most *= p.tiles_p;
-    expected *= p.tiles_p;
-    if (most > 0x3fffffffLL / 8) return cudaErrorInvalidValue;
-    // few tiles: split k, while every CTA keeps at least four stages
+    const int each = g.mode == BY_ROWS ? (g.tokens + g.groups - 1) / g.groups : g.tokens;   // tokens of a group
     const int stages = (g.K + BK - 1) / BK;
-    int split = 1;
-    if (bn <= 128 && g.mode != ALONG_K)
-        while (split < 8 && expected * split * 2 <= sms && stages / (split * 2) >= 4) split *= 2;
-
-    CUtensorMap mapP, mapQ;
-    if ((e = make_map(&mapP, g.p, g.K, g.rows_p, g.mode == BY_ROWS ? g.groups : 1, g.ldp, g.plane_p, BP))) return e;
-    if ((e = make_map(&mapQ, g.q, g.K, g.rows_q, 1, g.ldq, 0, bn))) return e;
-    const int grid = split > 1 ? (int)most * split : (int)(most < sms ? most : sms);
-    e = cudaErrorInvalidValue;
-    with_type(g.type, [&](auto t) {
-        using T = decltype(t);
-        auto go = [&](auto width) {
-            constexpr int BN = decltype(width)::value;
-            if constexpr (BN <= 128) {
-                if (split > 1) { e = launch<BN, T, true>(mapP, mapQ, p, grid, split, st); return; }
-            }
-            e = launch<BN, T, false>(mapP, mapQ, p, grid, 1, st);
+    auto run = [&](auto form, auto width, int split) {
+        with_type(g.type, [&](auto t) { e = launch<decltype(form)::value, decltype(width)::value, decltype(t)>(g, p, sms, split, st); });
+    };
+#define M4_FORM(F) std::integral_constant<int, F>()
+    // many tokens to a group, and at least half a tile for every SM: tokens as lanes; a pair of CTAs where there is enough for all pairs
+    if (each > 128 && work_of(g, 2 * BP, 192).expected >= sms / 2 && (g.mode != BY_ROWS || each >= 1024)) run(M4_FORM(PAIR), M4_FORM(192), 1);
+    else if (each > 128 && work_of(g, BP, 192).expected * 2 >= sms) run(M4_FORM(WIDE), M4_FORM(192), 1);
+    else {
+        // few: weights as lanes; few tiles as well: k split, while every CTA keeps at least four stages
+        const int bn = each <= 16 ? 16 : each <= 32 ? 32 : each <= 64 ? 64 : 128;
+        const long long tiles = work_of(g, bn, BP).expected;
+        int split = 1;
+        if (g.mode != ALONG_K)
+            while (split < 8 && tiles * split * 2 <= sms && stages / (split * 2) >= 4) split *= 2;
+        auto narrow = [&](auto width) {
+            if (split > 1) run(M4_FORM(SPLIT), width, split);
+            else run(M4_FORM(NARROW), width, 1);
         };
         switch (bn) {
-        case 16: go(std::integral_constant<int, 16>()); break;
-        case 32: go(std::integral_constant<int, 32>()); break;
-        case 64: go(std::integral_constant<int, 64>()); break;
-        case 128: go(std::integral_constant<int, 128>()); break;
-        default: go(std::integral_constant<int, 192>()); break;
+        case 16: narrow(M4_FORM(16)); break;
+        case 32: narrow(M4_FORM(32)); break;
+        case 64: narrow(M4_FORM(64)); break;
+        default: narrow(M4_FORM(128)); break;
         }
-    });
+    }
+#undef M4_FORM
     return e;
 }
 

@@ -57,16 +57,23 @@ cudaError_t mx4_quantize_cols(const void *X, int type, int nvec, int len, long l
                               size_t plane_s, cudaStream_t st);
 cudaError_t mx4_dequantize(const uint8_t *codes, long long ldq, const uint8_t *scales, long long lds, int nvec, int len, void *Y, int type,
                            long long ldy, cudaStream_t st);
-// products of it (mx4_gemm.cu): C[g][j][i] = sum_k P[g][i][k] Q[j][k]; mode 0 dense, 1 segments of the rows of Q, 2 segments of k
+// products of it (mx4_gemm.cu): y[t][n] = sum_k x[t][k] w[n][k]; mode 0 dense, 1 segments of the rows of x with a w each, 2 segments of k
 struct Mx4Product {
-    int mode, groups, rows_p, rows_q, K, type;
+    int mode, groups, tokens, weights, K, type;
     const int *offsets;
-    const uint8_t *p, *sp, *q, *sq;
-    long long ldp, ldsp, ldq, ldsq;
-    size_t plane_p, plane_sp;
-    void *C;
-    long long ldc;
-    size_t plane_c;
+    const uint8_t *x;
+    long long ldx;
+    const uint8_t *xs;
+    long long ldxs;
+    const uint8_t *w;
+    long long ldw;
+    size_t plane_w;
+    const uint8_t *ws;
+    long long ldws;
+    size_t plane_ws;
+    void *y;
+    long long ldy;
+    size_t plane_y;
 };
 cudaError_t mx4_product(const Mx4Product &g, int *status, cudaStream_t st);
 

@@ -73,7 +73,7 @@ def _codes(q, role, dims, device=None):
     if q.codes.shape[:-1] != q.scales.shape[:-1]:
         raise ValueError(f"{role}: codes {tuple(q.codes.shape)} and scales {tuple(q.scales.shape)} are of different vectors")
     blocks = -(-q.length // 32)
-    if q.codes.shape[-1] < 16 * blocks or q.scales.shape[-1] < blocks:
+    if q.codes.shape[-1] < 16 * blocks or q.scales.shape[-1] < -(-blocks // 16) * 16:
         raise ValueError(f"{role}: rows of {q.codes.shape[-1]} and {q.scales.shape[-1]} bytes do not hold {q.length} values")
     if q.scales.device != q.codes.device or (device is not None and q.codes.device != device):
         raise ValueError(f"{role} must be on one device with the other operands")

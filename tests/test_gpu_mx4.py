@@ -142,7 +142,8 @@ def test_dequantize_every_code_and_scale(dtype):
 
 @pytest.mark.parametrize("shape", [(1, 1, 1), (1, 128, 32), (1, 2048, 4096), (2, 130, 33), (15, 127, 64), (16, 129, 65), (17, 256, 255), (31, 64, 256), (33, 300, 257),
                                    (64, 128, 2085), (65, 1, 511), (128, 400, 512), (129, 257, 1000), (300, 70, 1537), (512, 384, 96), (513, 640, 288),
-                                   (700, 130, 2049), (3, 640, 16384)])
+                                   (700, 130, 2049), (3, 640, 16384), (150, 9500, 96), (300, 6000, 500), (129, 7200, 1100), (1100, 3070, 300), (2060, 1550, 1025),
+                                   (513, 5000, 64)])
 def test_product(shape):
     m, n, k = shape
     mx4 = _mx4()
@@ -187,9 +188,9 @@ def test_product_pitches_and_out():
 
     def spread(q):
         c = torch.full((q.codes.shape[0], 224), 0xFF, dtype=torch.uint8, device="cuda")
-        s = torch.full((q.codes.shape[0], 24), 0xFF, dtype=torch.uint8, device="cuda")
-        c[:, 16: 16 + q.codes.shape[1]], s[:, 8: 8 + 10] = q.codes, q.scales[:, :10]
-        return mx4.Mx4(c[:, 16: 16 + q.codes.shape[1]], s[:, 8:], k)
+        s = torch.full((q.codes.shape[0], 32), 0xFF, dtype=torch.uint8, device="cuda")
+        c[:, 16: 16 + q.codes.shape[1]], s[:, 16: 16 + 10] = q.codes, q.scales[:, :10]
+        return mx4.Mx4(c[:, 16: 16 + q.codes.shape[1]], s[:, 16:], k)
 
     out = torch.full((m + 1, n + 9), 3.0, dtype=torch.bfloat16, device="cuda")
     want = mx4.matmul(x, w)
@@ -218,22 +219,23 @@ def test_grouped_product(offsets, k):
     _status()
 
 
-def test_grouped_product_many_groups_and_wide_segments():
+@pytest.mark.parametrize("groups,r,n", [(1024, 500, 130), (3, 2000, 130), (40, 900, 130), (64, 2100, 130), (4, 1600, 3100), (5, 900, 2000), (2, 2500, 6000), (1, 300, 6000)])
+def test_grouped_product_many_groups_and_wide_segments(groups, r, n):
     mx4 = _mx4()
-    k, n = 96, 130
-    for groups, r in ((1024, 500), (3, 2000), (40, 900), (64, 2100)):
-        g = torch.Generator().manual_seed(groups)
-        cuts = torch.sort(torch.randint(0, r + 1, (groups - 1,), generator=g)).values
-        offsets = torch.cat([torch.tensor([0]), cuts, torch.tensor([r])]).to(torch.int32)
-        x = _packed(r, k, 13)
-        w = mx4.quantize(_random(groups * n, k, 14).reshape(groups, n, k).cuda())
-        y = mx4.grouped_matmul(x, w, offsets.cuda(), torch.bfloat16)
-        xs, ws = ref.of(x), ref.of(w)
-        which = torch.searchsorted(offsets[1:].contiguous(), torch.arange(r, dtype=torch.int32), right=True)
-        exact = torch.einsum("rk,rnk->rn", xs, ws[which])
-        size = torch.einsum("rk,rnk->rn", xs.abs(), ws[which].abs())
-        bound = k * 2.0 ** -23 * size + 2.0 ** -8 * exact.abs() + 1e-30
-        assert bool(((y.cpu().double() - exact).abs() <= bound).all()), (groups, r)
+    k = 96
+    g = torch.Generator().manual_seed(groups)
+    cuts = torch.sort(torch.randint(0, r + 1, (groups - 1,), generator=g)).values
+    offsets = [0] + cuts.tolist() + [r]
+    x = _packed(r, k, 13)
+    w = mx4.quantize(_random(groups * n, k, 14).reshape(groups, n, k).cuda())
+    out = torch.full((r + 2, n), 7.0, dtype=torch.bfloat16, device="cuda")
+    mx4.grouped_matmul(x, w, torch.tensor(offsets, dtype=torch.int32, device="cuda"), torch.bfloat16, out=out[1: r + 1])
+    assert bool((out[[0, r + 1]] == 7).all())
+    xs, ws = ref.of(x), ref.of(w)
+    for i in range(groups):
+        if offsets[i + 1] > offsets[i]:
+            _check_product(out[1 + offsets[i]: 1 + offsets[i + 1]], xs[offsets[i]: offsets[i + 1]], ws[i], torch.bfloat16)
+    _status()
 
 
 def test_grouped_product_takes_any_offsets_without_leaving_its_arrays():
@@ -267,6 +269,22 @@ def test_segment_product(offsets):
     a.scales[:, lo // 32: hi // 32] = 255
     y2 = mx4.segment_matmul(a, b, torch.tensor(offsets, dtype=torch.int32, device="cuda"), torch.float32)
     assert torch.equal(y2[:3], y[:3])
+    _status()
+
+
+@pytest.mark.parametrize("m,n,groups", [(200, 400, 16), (600, 1000, 16), (300, 100, 64), (40, 900, 32)])
+def test_segment_product_of_many(m, n, groups):
+    mx4 = _mx4()
+    g = torch.Generator().manual_seed(m)
+    lengths = torch.randint(0, 12, (groups,), generator=g) * 64
+    offsets = [0] + lengths.cumsum(0).tolist()
+    r = max(64, offsets[-1])
+    a, b = _packed(m, r, 19), _packed(n, r, 20)
+    y = mx4.segment_matmul(a, b, torch.tensor(offsets, dtype=torch.int32, device="cuda"), torch.bfloat16)
+    av, bv = ref.of(a), ref.of(b)
+    for i in range(groups):
+        lo, hi = offsets[i], offsets[i + 1]
+        _check_product(y[i], av[:, lo:hi], bv[:, lo:hi], torch.bfloat16)
     _status()
 
 

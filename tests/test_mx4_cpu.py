@@ -11,37 +11,37 @@ ARG, SIZE = 10001, 10006
 
 
 def _quantize(X=P, type=0, nvec=4, len=64, ldx=64, by_rows=1, rule=0, slots=None, per=0, sources=0, planes=1, plane_x=0, codes=P, ldq=32, plane_q=0,
-              scales=P, lds=8, plane_s=0):
+              scales=P, lds=16, plane_s=0):
     return lib.ozb_mx4_quantize(X, type, nvec, len, ldx, by_rows, rule, slots, per, sources, planes, plane_x, codes, ldq, plane_q, scales, lds, plane_s, None)
 
 
 @pytest.mark.parametrize("bad", [dict(X=None), dict(type=3), dict(type=-1), dict(nvec=0), dict(len=0), dict(len=-1), dict(len=2 ** 31 - 1), dict(ldx=63),
                                  dict(by_rows=0, ldx=3), dict(rule=2), dict(codes=None), dict(codes=ctypes.c_void_p(4104)), dict(ldq=24), dict(ldq=16),
-                                 dict(scales=None), dict(scales=ctypes.c_void_p(4100)), dict(lds=4), dict(lds=0), dict(slots=P), dict(slots=P, per=1),
-                                 dict(slots=P, per=1, sources=4, planes=2), dict(planes=0), dict(planes=2, plane_q=8), dict(planes=2, plane_q=16, plane_s=4),
+                                 dict(scales=None), dict(scales=ctypes.c_void_p(4104)), dict(lds=8), dict(lds=0), dict(slots=P), dict(slots=P, per=1),
+                                 dict(slots=P, per=1, sources=4, planes=2), dict(planes=0), dict(planes=2, plane_q=8), dict(planes=2, plane_q=16, plane_s=8),
                                  dict(X=ctypes.c_void_p(4098)), dict(X=ctypes.c_void_p(4097), type=1)])
 def test_quantize(bad):
     assert _quantize(**bad) == ARG
 
 
 def test_dequantize():
-    call = lambda **b: lib.ozb_mx4_dequantize(*{**dict(codes=P, ldq=32, scales=P, lds=8, nvec=4, len=64, Y=P, type=1, ldy=64), **b}.values(), None)  # noqa: E731
+    call = lambda **b: lib.ozb_mx4_dequantize(*{**dict(codes=P, ldq=32, scales=P, lds=16, nvec=4, len=64, Y=P, type=1, ldy=64), **b}.values(), None)  # noqa: E731
     for bad in (dict(codes=None), dict(scales=None), dict(Y=None), dict(nvec=0), dict(len=0), dict(len=65), dict(ldy=63), dict(type=4), dict(Y=ctypes.c_void_p(4097))):
         assert call(**bad) == ARG, bad
 
 
 def test_products():
-    dense = dict(M=4, N=4, K=64, X=P, ldx=32, Xs=P, ldxs=8, W=P, ldw=32, Ws=P, ldws=8, Y=P, type=0, ldy=4)
+    dense = dict(M=4, N=4, K=64, X=P, ldx=32, Xs=P, ldxs=16, W=P, ldw=32, Ws=P, ldws=16, Y=P, type=0, ldy=4)
     call = lambda **b: lib.ozb_mx4_gemm(*{**dense, **b}.values(), None)  # noqa: E731
     for bad in (dict(M=0), dict(N=0), dict(K=0), dict(K=65), dict(K=2 ** 31 - 1), dict(X=None), dict(Xs=None), dict(W=None), dict(Ws=None), dict(Y=None),
-                dict(ldx=16), dict(ldxs=4), dict(ldy=3), dict(type=3), dict(Y=ctypes.c_void_p(4098)), dict(W=ctypes.c_void_p(4104)), dict(M=-5)):
+                dict(ldx=16), dict(ldxs=8), dict(ldy=3), dict(type=3), dict(Y=ctypes.c_void_p(4098)), dict(W=ctypes.c_void_p(4104)), dict(M=-5)):
         assert call(**bad) == ARG, bad
-    grouped = dict(groups=2, R=4, N=4, K=64, offsets=P, X=P, ldx=32, Xs=P, ldxs=8, W=P, ldw=32, plane_w=128, Ws=P, ldws=8, plane_ws=32, Y=P, type=0, ldy=4)
+    grouped = dict(groups=2, R=4, N=4, K=64, offsets=P, X=P, ldx=32, Xs=P, ldxs=16, W=P, ldw=32, plane_w=128, Ws=P, ldws=16, plane_ws=32, Y=P, type=0, ldy=4)
     call = lambda **b: lib.ozb_mx4_gemm_grouped(*{**grouped, **b}.values(), None)  # noqa: E731
-    for bad in (dict(groups=0), dict(R=0), dict(N=0), dict(K=0), dict(offsets=None), dict(offsets=ctypes.c_void_p(4098)), dict(plane_w=8), dict(plane_ws=4), dict(ldy=3)):
+    for bad in (dict(groups=0), dict(R=0), dict(N=0), dict(K=0), dict(offsets=None), dict(offsets=ctypes.c_void_p(4098)), dict(plane_w=8), dict(plane_ws=8), dict(ldy=3)):
         assert call(**bad) == ARG, bad
     assert call(groups=1025) == SIZE
-    segments = dict(groups=2, M=4, N=4, R=64, offsets=P, A=P, lda=32, As=P, ldas=8, B=P, ldb=32, Bs=P, ldbs=8, Y=P, type=0, ldy=4, plane_y=16)
+    segments = dict(groups=2, M=4, N=4, R=64, offsets=P, A=P, lda=32, As=P, ldas=16, B=P, ldb=32, Bs=P, ldbs=16, Y=P, type=0, ldy=4, plane_y=16)
     call = lambda **b: lib.ozb_mx4_gemm_segments(*{**segments, **b}.values(), None)  # noqa: E731
     for bad in (dict(groups=0), dict(M=0), dict(N=0), dict(R=0), dict(R=65), dict(offsets=None), dict(As=None), dict(ldb=8)):
         assert call(**bad) == ARG, bad
