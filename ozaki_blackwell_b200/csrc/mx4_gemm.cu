@@ -12,7 +12,7 @@
 // values (128 bytes) of k make a stage, 512 (16 scale bytes) a scale slot.
 //   warp 0     producer: one thread, TMA of both operands' codes (128-byte swizzle) into a ring of stages. What lies outside a matrix
 //              comes as zero codes.
-//   warps 3, 8, 9  scales, in turns of a slot: a row's 16 bytes are four words, one to 128 values of k; the instruction wants, for a
+//   warps 3, 8 .. 10  scales, in turns of a slot: a row's 16 bytes are four words, one to 128 values of k; the instruction wants, for a
 //              word, 128 rows as 32 x 16 bytes (row r at 16 (r % 32) + 4 (r / 32)). A lane reads the rows l, l + 32, l + 64, l + 96
 //              and writes the 4 x 4 words turned: four 16-byte loads and stores for 128 rows by 512 values, without bank conflicts.
 //   warp 2     one thread; tcgen05.cp of a stage's turned scales into tensor memory, its completion counted by the stage's barrier
@@ -42,7 +42,7 @@ namespace m4 {
 constexpr int BP = 128;            // rows of P to a CTA
 constexpr int BK = 256, BKB = 128; // k of a stage, in values and in bytes
 constexpr int UK = 64;             // k of one tcgen05.mma kind::mxf4
-constexpr int THREADS = 320, TURNERS = 3;
+constexpr int TURNERS = 4, THREADS = 256 + 32 * (TURNERS - 1);
 constexpr int MAX_GROUPS = 1024;
 
 enum { DENSE = 0, BY_ROWS = 1, ALONG_K = 2 };
@@ -72,7 +72,9 @@ template <int FORM, int BN> struct Shape {
     static constexpr int SLOT = 4 * 512 * (1 + Q_TILES);           // turned scales of 512 values of k: four words of P's tile, then of Q's
     static constexpr int SCALE_COLS = 8 + 8 * Q_TILES;             // tensor-memory columns of a stage's scales
     static constexpr int STAGES = pair ? 5 : BN <= 32 ? 8 : BN <= 64 ? 7 : BN <= 128 ? 5 : 4;
-    static constexpr int SLOTS = TURNERS;                          // a slot is always the same warp's
+    // A multiple of the turning warps, so that a slot is always the same warp's: a warp that came to a slot before another had seen the
+    // slot's last use would take the parity of the use before that for its own.
+    static constexpr int SLOTS = 2 * TURNERS;
     static constexpr int COLS = 2 * BN + STAGES * SCALE_COLS;      // two accumulators, and the scales
     static constexpr int TMEM_COLS = COLS <= 256 ? 256 : 512;
     static constexpr int BARS = 2 * STAGES + 2 * SLOTS + 4;
@@ -301,7 +303,6 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm(const __grid_constant__ C
         t.s0 = uniform(t.s0); t.s1 = uniform(t.s1);
         return t;
     };
-    auto new_slot = [](const Tile &t, int kb) { return kb == t.s0 || !(kb & 1); };   // a slot holds an even stage and the odd one behind it
     volatile int *abortp = &abort_flag;
     uint32_t it = 0, sl = 0;   // running stage and slot (of the role that counts them)
 
@@ -340,24 +341,43 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm(const __grid_constant__ C
                 const uint32_t d = tmem_base + acc * BN;
                 bool ok = true;
                 uint32_t accumulate = 0;
-                for (int kb = t.s0; kb < t.s1; kb++, it++) {
-                    const int s = it % S::STAGES;
+                // a stage's instructions [k_lo, k_hi) of four, and its release
+                auto issue = [&](int s, int k_lo, int k_hi) {
                     const uint32_t at = base + s * S::STAGE, tp = tmem_scales + s * S::SCALE_COLS, tq = tp + 8;
                     const uint64_t da = smem_desc(at), db = smem_desc(at + S::P_BYTES);
-                    const int k_lo = max(0, (t.k0 - kb * BK) / UK), k_hi = (t.k1 - kb * BK + UK - 1) / UK;   // the instructions of this stage that are in range
-                    if (!(ok = warp_wait(full_bar(s), (it / S::STAGES) & 1u, abortp, 0x130))) break;
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    if (elect_one()) {
 #pragma unroll
-                        for (int k = 0; k < BK / UK; k++) {
-                            if (k < k_lo || k >= k_hi) continue;
-                            const uint32_t id = S::IDESC | ((k & 1u) ? (2u << 4) | (2u << 29) : 0u);      // which two of a word's four scales
-                            mma_mx4<pair>(d, da + 2u * k, db + 2u * k, id, tp + 4 * (k >> 1), tq + 4 * (k >> 1) * S::Q_TILES, accumulate | (uint32_t)(k > k_lo));
+                    for (int k = 0; k < BK / UK; k++) {
+                        if (k < k_lo || k >= k_hi) continue;
+                        const uint32_t id = S::IDESC | ((k & 1u) ? (2u << 4) | (2u << 29) : 0u);      // which two of a word's four scales
+                        mma_mx4<pair>(d, da + 2u * k, db + 2u * k, id, tp + 4 * (k >> 1), tq + 4 * (k >> 1) * S::Q_TILES, accumulate);
+                        accumulate = 1;
+                    }
+                    commit<pair>(empty_bar(s));
+                };
+                const int whole0 = (t.k0 + BK - 1) / BK, whole1 = t.k1 / BK;   // stages all of whose instructions are in range
+                for (int kb = t.s0; kb < t.s1;) {
+                    const int s = it % S::STAGES;
+                    const uint32_t parity = (it / S::STAGES) & 1u;
+                    if (kb >= whole0 && kb + 2 <= whole1 && kb + 2 <= t.s1) {   // two at a time: a wait costs as much as two instructions
+                        const int s2 = (it + 1) % S::STAGES;
+                        if (!(ok = warp_wait2(full_bar(s), parity, full_bar(s2), ((it + 1) / S::STAGES) & 1u, abortp, 0x130))) break;
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                        if (elect_one()) {
+                            issue(s, 0, 4);
+                            issue(s2, 0, 4);
                         }
-                        commit<pair>(empty_bar(s));
+                        accumulate = 1;
+                        kb += 2;
+                        it += 2;
+                    } else {
+                        if (!(ok = warp_wait(full_bar(s), parity, abortp, 0x130))) break;
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                        if (elect_one()) issue(s, max(0, (t.k0 - kb * BK) / UK), (t.k1 - kb * BK + UK - 1) / UK);
+                        accumulate = 1;
+                        kb++;
+                        it++;
                     }
                     __syncwarp();
-                    accumulate = 1;
                 }
                 if (!ok) break;
                 if (elect_one()) commit<pair>(accfull_bar(acc));
@@ -366,51 +386,56 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm(const __grid_constant__ C
         }
     } else if (warp == 2) {
         if (!pair || rank == 0) {
-            sl = ~0u;
             for (int w = first; w < total && !__any_sync(~0u, *abortp); w += step) {
                 const Tile t = tile_at(w);
-                for (int kb = t.s0; kb < t.s1; kb++, it++) {
-                    if (new_slot(t, kb)) {
-                        sl++;
-                        bool ok;
-                        if constexpr (pair) ok = __all_sync(~0u, mbar_wait_acquire_cluster(turned_bar(sl % S::SLOTS), (sl / S::SLOTS) & 1u, abortp, 0x131));
-                        else ok = warp_wait(turned_bar(sl % S::SLOTS), (sl / S::SLOTS) & 1u, abortp, 0x131);
-                        if (!ok) break;
-                    }
-                    const int s = it % S::STAGES, r = sl % S::SLOTS;
-                    const uint32_t tiles = slots + r * S::SLOT + 1024 * (kb & 1), q_tiles = slots + r * S::SLOT + 2048 + 1024 * S::Q_TILES * (kb & 1);
-                    const uint32_t tp = tmem_scales + s * S::SCALE_COLS, tq = tp + 8;
-                    const bool slot_done = kb + 1 == t.s1 || (kb & 1);
-                    if (!warp_wait(empty_bar(s), ((it / S::STAGES) & 1u) ^ 1u, abortp, 0x132)) break;
+                bool ok = true;
+                for (int kb = t.s0; kb < t.s1; sl++) {
+                    const int r = sl % S::SLOTS, s = it % S::STAGES, s2 = (it + 1) % S::STAGES;
+                    const bool both = !(kb & 1) && kb + 1 < t.s1;   // the slot's two stages, or its first or second alone
+                    const uint32_t parity = ((it / S::STAGES) & 1u) ^ 1u, parity2 = (((it + 1) / S::STAGES) & 1u) ^ 1u;
+                    if constexpr (pair) ok = __all_sync(~0u, mbar_wait_acquire_cluster(turned_bar(r), (sl / S::SLOTS) & 1u, abortp, 0x131));
+                    else ok = warp_wait(turned_bar(r), (sl / S::SLOTS) & 1u, abortp, 0x131);
+                    if (ok) ok = both ? warp_wait2(empty_bar(s), parity, empty_bar(s2), parity2, abortp, 0x132) : warp_wait(empty_bar(s), parity, abortp, 0x132);
+                    if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    if (elect_one()) {
+                    const uint32_t words = slots + r * S::SLOT;
+                    auto copy = [&](int s, int half) {   // the two words of a stage
+                        const uint32_t tp = tmem_scales + s * S::SCALE_COLS, tq = tp + 8;
 #pragma unroll
                         for (int h = 0; h < 2; h++) {
-                            copy_scales<pair>(tp + 4 * h, tiles + 512 * h);
+                            copy_scales<pair>(tp + 4 * h, words + 512 * (2 * half + h));
 #pragma unroll
-                            for (int c = 0; c < S::Q_TILES; c++) copy_scales<pair>(tq + 4 * (h * S::Q_TILES + c), q_tiles + 512 * (h * S::Q_TILES + c));
+                            for (int c = 0; c < S::Q_TILES; c++) copy_scales<pair>(tq + 4 * (h * S::Q_TILES + c), words + 2048 + 512 * ((2 * half + h) * S::Q_TILES + c));
                         }
                         if constexpr (pair) mma_commit_pair(full_bar(s));
                         else mma_commit(full_bar(s));
-                        if (slot_done) commit<pair>(slot_bar(r));
+                    };
+                    if (elect_one()) {
+                        if (both) {
+                            copy(s, 0);
+                            copy(s2, 1);
+                        } else copy(s, kb & 1);
+                        commit<pair>(slot_bar(r));
                     }
                     __syncwarp();
+                    kb += both ? 2 : 1;
+                    it += both ? 2 : 1;
                 }
+                if (!ok) break;
             }
         }
     } else if (warp < 4 || warp >= 8) {
-        // Of TURNERS warps, in turns of a slot: each has its slot's loads in flight while the others' slots are used.
+        // of TURNERS warps, in turns of a slot: while one waits for its slot's bytes, the others do theirs
         const uint32_t own = warp < 4 ? 0 : warp - 7;
         const int blocks = (p.K + 31) / 32;
-        sl = 0;
         for (int w = first; w < total && !__any_sync(~0u, *abortp); w += step) {
             const Tile t = tile_at(w);
             const int p0 = t.p0 + (pair ? (int)rank * BP : 0);
-            const uint8_t *sp = p.sp + (size_t)t.group * p.plane_sp, *sq = p.sq + (size_t)t.group * p.plane_sq;
             bool ok = true;
             for (int kb = t.s0; kb < t.s1; kb = (kb | 1) + 1, sl++) {
                 if (sl % TURNERS != own) continue;
-                const int r = sl % S::SLOTS, at = (kb >> 1) * 16, left = blocks - at;
+                const int r = sl % S::SLOTS, byte = (kb >> 1) * 16, left = blocks - byte;
+                const uint8_t *sp = p.sp + (size_t)t.group * p.plane_sp + byte, *sq = p.sq + (size_t)t.group * p.plane_sq + byte;
                 uint4 v[1 + S::Q_TILES][4];
 #pragma unroll
                 for (int c = 0; c < 1 + S::Q_TILES; c++)   // P's tile, then Q's
@@ -419,10 +444,10 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm(const __grid_constant__ C
                         const int row = i * 32 + lane;
                         v[c][i] = make_uint4(0, 0, 0, 0);   // 2^-127: rows that are not there
                         if (c == 0) {
-                            if (p0 + row < t.p1) v[c][i] = __ldg(reinterpret_cast<const uint4 *>(sp + (size_t)(p0 + row) * p.ldsp + at));
+                            if (p0 + row < t.p1) v[c][i] = __ldg(reinterpret_cast<const uint4 *>(sp + (size_t)(p0 + row) * p.ldsp));
                         } else {
                             const int q = (c - 1) * 128 + row;
-                            if (q < BN && t.q0 + q < t.q1) v[c][i] = __ldg(reinterpret_cast<const uint4 *>(sq + (size_t)(t.q0 + q) * p.ldsq + at));
+                            if (q < BN && t.q0 + q < t.q1) v[c][i] = __ldg(reinterpret_cast<const uint4 *>(sq + (size_t)(t.q0 + q) * p.ldsq));
                         }
                     }
                 if (left < 16) {   // bytes behind the last block may hold anything: their codes are zero, their scales become it
@@ -444,8 +469,10 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm(const __grid_constant__ C
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the tensor core reads these through the async proxy
                 __syncwarp();
+                // In a pair the leader's thread starts the copies of both CTAs. What the peer wrote is read by its own tensor core, behind the
+                // fence above, so a plain remote arrive passes it on; a release at cluster scope holds the warp for 1800 cycles.
                 if (lane == 0) {
-                    if (pair && rank) mbar_arrive_release_cluster(map_to_cta(turned_bar(r), 0));
+                    if (pair && rank) mbar_arrive_cluster(map_to_cta(turned_bar(r), 0));
                     else mbar_arrive(turned_bar(r));
                 }
             }

@@ -65,6 +65,12 @@ __device__ __forceinline__ bool elect_one() {
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int *abort_flag, int who) {
     return __all_sync(~0u, mbar_wait(bar, parity, abort_flag, who));
 }
+// ... for two barriers at once
+__device__ __forceinline__ bool warp_wait2(uint32_t bar0, uint32_t parity0, uint32_t bar1, uint32_t parity1, volatile int *abort_flag, int who) {
+    const bool first = mbar_try(bar0, parity0), second = mbar_try(bar1, parity1);   // in flight together
+    if (__all_sync(~0u, first && second)) return true;
+    return warp_wait(bar0, parity0, abort_flag, who) && warp_wait(bar1, parity1, abort_flag, who);
+}
 
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap *map, int c0, int c1, int c2, uint32_t bar) {
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
