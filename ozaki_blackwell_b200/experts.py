@@ -16,7 +16,7 @@ import torch
 
 from . import mx4
 from ._lib import lib as _lib
-from .mx4 import _call, _dense, _pitch, _result, _same_device, _type
+from .mx4 import _call, _pitch, _result, _routed, _type
 
 __all__ = ["Routing", "sort", "gather", "combine", "combine_grad", "matmul", "matmul_grad"]
 
@@ -30,20 +30,11 @@ class Routing(NamedTuple):
     align: int = 0
 
 
-def _routing(r, device):
-    for name, t in (("offsets", r.offsets), ("rows", r.rows), ("slots", r.slots)):
-        if t.dtype != torch.int32 or not t.is_contiguous() or t.device != device:
-            raise ValueError(f"routing.{name} must be contiguous int32 on {device}")
-    if r.rows.dim() != 2:
-        raise ValueError("routing.rows has a row for each token")
-    return r.rows.shape
-
-
-def _weights(weights, shape, device):
+def _weights(weights, shape, index):
     if weights is None:
         return None
-    if weights.dtype != torch.float32 or tuple(weights.shape) != tuple(shape) or not weights.is_contiguous() or weights.device != device:
-        raise ValueError(f"weights must be contiguous float32 {tuple(shape)} on {device}")
+    if weights.dtype is not torch.float32 or weights.shape != shape or not weights.is_contiguous() or weights.get_device() != index:
+        raise ValueError(f"weights must be contiguous float32 {tuple(shape)} on cuda:{index}")
     return weights.data_ptr()
 
 
@@ -57,50 +48,48 @@ def sort(ids, experts, align=1):
     if size < 0:
         raise ValueError(f"cannot sort {tokens} x {top} slots over {experts} experts in segments of {align}: sizes are positive, at most 1024 experts, align at most 256")
     need = _lib.ozb_expert_sort_scratch(tokens, top, experts)
-    # one allocation: offsets, rows, slots and the counts of the chunks
+    # one allocation: slots, rows, offsets and the counts of the chunks
     n = tokens * top
-    buf = torch.empty(experts + 1 + n + size + need // 4, dtype=torch.int32, device=ids.device)
-    offsets, rows, slots = buf[: experts + 1], buf[experts + 1 : experts + 1 + n], buf[experts + 1 + n : experts + 1 + n + size]
+    buf = ids.new_empty(size + n + experts + 1 + need // 4, dtype=torch.int32)
     at = buf.data_ptr()
-    _call(ids.device, _lib.ozb_expert_sort, tokens, top, experts, ids.data_ptr(), ids.element_size(), align, size, at, at + 4 * (experts + 1),
-          at + 4 * (experts + 1 + n), at + 4 * (experts + 1 + n + size), need)
-    return Routing(offsets, rows.view(tokens, top), slots, align)
+    _call(ids.get_device(), _lib.ozb_expert_sort, tokens, top, experts, ids.data_ptr(), ids.element_size(), align, size, at + 4 * (size + n), at + 4 * size, at,
+          at + 4 * (size + n + experts + 1), need)
+    return Routing(buf[size + n : size + n + experts + 1], buf[size : size + n].view(tokens, top), buf[:size], align)
 
 
 def gather(x, routing, out=None):
     """The rows of x [T, h] in the order of their experts, [R, h]; zeros where a row has no slot."""
-    _dense(x, "x")
-    tokens, top = _routing(routing, x.device)
+    ldx, index = _pitch(x, "x"), x.get_device()
+    tokens, top = _routed(routing, index)
     if x.shape[0] != tokens:
         raise ValueError(f"x has {x.shape[0]} rows, the routing {tokens} tokens")
-    y = _result(out, (routing.slots.numel(), x.shape[1]), x.dtype, x.device)
-    _call(x.device, _lib.ozb_expert_gather, y.shape[0], y.shape[1], x.data_ptr(), _type(x.dtype), _pitch(x), tokens, routing.slots.data_ptr(), top,
-          y.data_ptr(), _pitch(y))
+    kind, r, h = _type(x.dtype), routing.slots.shape[0], x.shape[1]
+    y, ldy = _result(x, out, (r, h), x.dtype)
+    _call(index, _lib.ozb_expert_gather, r, h, x.data_ptr(), kind, ldx, tokens, routing.slots.data_ptr(), top, y.data_ptr(), ldy)
     return y
 
 
 def combine(z, routing, weights=None, out=None):
     """y[t] = sum over j of weights[t, j] z[rows[t, j]] (weights None: 1), in FP32, rounded once to z's type."""
-    _dense(z, "z")
-    tokens, top = _routing(routing, z.device)
-    y = _result(out, (tokens, z.shape[1]), z.dtype, z.device)
-    _call(z.device, _lib.ozb_expert_combine, tokens, top, z.shape[1], z.data_ptr(), _type(z.dtype), z.shape[0], _pitch(z), routing.rows.data_ptr(),
-          _weights(weights, (tokens, top), z.device), y.data_ptr(), _pitch(y))
+    ldz, index = _pitch(z, "z"), z.get_device()
+    tokens, top = _routed(routing, index)
+    kind, (r, h), w = _type(z.dtype), z.shape, _weights(weights, routing.rows.shape, index)
+    y, ldy = _result(z, out, (tokens, h), z.dtype)
+    _call(index, _lib.ozb_expert_combine, tokens, top, h, z.data_ptr(), kind, r, ldz, routing.rows.data_ptr(), w, y.data_ptr(), ldy)
     return y
 
 
 def combine_grad(dy, z, routing, weights=None):
     """(dz, dweights) of combine(z, routing, weights) for a gradient dy [T, h] of z's type; dz is zero where a row has no slot."""
-    _dense(dy, "dy")
-    _dense(z, "z")
-    _same_device(z.device, dy=dy)
-    tokens, top = _routing(routing, z.device)
-    if dy.dtype != z.dtype or tuple(dy.shape) != (tokens, z.shape[1]) or z.shape[0] != routing.slots.numel():
-        raise ValueError(f"dy {tuple(dy.shape)} of {dy.dtype} and z {tuple(z.shape)} of {z.dtype} do not fit a routing of {tokens} tokens and {routing.slots.numel()} rows")
-    dz = torch.empty(z.shape, dtype=z.dtype, device=z.device)
-    dweights = torch.empty((tokens, top), dtype=torch.float32, device=z.device)
-    _call(z.device, _lib.ozb_expert_combine_grad, tokens, top, z.shape[1], dy.data_ptr(), _type(z.dtype), _pitch(dy), z.data_ptr(), _pitch(z), z.shape[0],
-          routing.rows.data_ptr(), routing.slots.data_ptr(), _weights(weights, (tokens, top), z.device), dz.data_ptr(), _pitch(dz), dweights.data_ptr())
+    lddy, ldz, index = _pitch(dy, "dy"), _pitch(z, "z"), z.get_device()
+    tokens, top = _routed(routing, index)
+    r, h = z.shape
+    if dy.dtype is not z.dtype or dy.shape != (tokens, h) or r != routing.slots.shape[0] or dy.get_device() != index:
+        raise ValueError(f"dy {tuple(dy.shape)} of {dy.dtype} and z {tuple(z.shape)} of {z.dtype} do not fit a routing of {tokens} tokens and {routing.slots.shape[0]} rows")
+    kind, w = _type(z.dtype), _weights(weights, routing.rows.shape, index)
+    dz, dweights = z.new_empty((r, h)), z.new_empty((tokens, top), dtype=torch.float32)
+    _call(index, _lib.ozb_expert_combine_grad, tokens, top, h, dy.data_ptr(), kind, lddy, z.data_ptr(), ldz, r, routing.rows.data_ptr(),
+          routing.slots.data_ptr(), w, dz.data_ptr(), h, dweights.data_ptr())
     return dz, dweights
 
 
@@ -108,7 +97,7 @@ def matmul(x, w, ids, weights=None, keep=False):
     """y[t] = sum over j of weights[t, j] W[ids[t, j]] x[t]: tokens sorted by expert, rounded to the 4-bit format as they are gathered, one
     product for all experts, and the rows added up by token. w: Mx4 stack [experts, n, ...] with blocks along the rows of x.
     keep: returns (y, z, routing) for matmul_grad, with segments padded to 64."""
-    _dense(x, "x")
+    _pitch(x, "x")
     r = sort(ids, w.codes.shape[0], 64 if keep else 1)
     z = mx4.grouped_matmul(mx4.quantize(x, routing=r), w, r.offsets, x.dtype)
     y = combine(z, r, weights)

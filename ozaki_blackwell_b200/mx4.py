@@ -18,6 +18,9 @@ import torch
 from . import OzakiError
 from ._lib import lib as _lib
 
+_current_device = torch.cuda.current_device
+_raw_stream = torch._C._cuda_getCurrentRawStream   # the number behind torch.cuda.current_stream(index), without making the object
+
 __all__ = ["Mx4", "quantize", "dequantize", "matmul", "grouped_matmul", "segment_matmul"]
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
@@ -38,67 +41,72 @@ def _type(dtype):
         raise TypeError(f"float32, bfloat16 or float16 are supported, not {dtype}") from None
 
 
-def _call(device, entry, *args):
-    """One call of the library on the current stream of `device`."""
-    if device.index == torch.cuda.current_device():
-        status = entry(*args, torch.cuda.current_stream().cuda_stream)
+def _call(index, entry, *args):
+    """One call of the library on the current stream of device `index`."""
+    if index == _current_device():
+        status = entry(*args, _raw_stream(index))
     else:
-        with torch.cuda.device(device):
-            status = entry(*args, torch.cuda.current_stream().cuda_stream)
+        with torch.cuda.device(index):
+            status = entry(*args, _raw_stream(index))
     if status:
         raise OzakiError(status)
 
 
-def _dense(x, role, dims=2):
-    """Checks that x is a matrix (or a stack of them) on a GPU whose rows are contiguous."""
+def _pitch(x, role, dims=2):
+    """Checks that x is a matrix (or a stack of them) on a GPU whose rows are contiguous; elements from one row to the next (a single row
+    has any stride)."""
+    shape, stride = x.shape, x.stride()
+    if len(shape) != dims:
+        raise ValueError(f"{role} must have {dims} dimensions, not {len(shape)}")
     if not x.is_cuda:
         raise TypeError(f"{role} must be on a GPU")
-    if x.dim() != dims:
-        raise ValueError(f"{role} must have {dims} dimensions, not {x.dim()}")
-    if x.stride(-1) != 1 and x.shape[-1] != 1:
+    if stride[-1] != 1 and shape[-1] != 1:
         raise ValueError(f"the rows of {role} must be contiguous; make it contiguous first")
-    return x
+    return stride[-2] if shape[-2] > 1 else max(stride[-2], shape[-1])
 
 
-def _pitch(x):
-    """Elements from one row to the next (a single row has any stride)."""
-    return x.stride(-2) if x.shape[-2] > 1 else max(x.stride(-2), x.shape[-1])
+def _codes(q, role, dims, index):
+    """Pointers and pitches of an Mx4 on device `index`: codes, ldq, scales, lds."""
+    codes, scales, length = q
+    blocks = (length + 31) >> 5
+    ldq, lds = _pitch(codes, role, dims), _pitch(scales, role, dims)
+    have, bytes_ = codes.shape, scales.shape
+    if codes.dtype is not torch.uint8 or scales.dtype is not torch.uint8:
+        raise TypeError(f"{role}: codes and scales are uint8, not {codes.dtype} and {scales.dtype}")
+    if have[:-1] != bytes_[:-1]:
+        raise ValueError(f"{role}: codes {tuple(have)} and scales {tuple(bytes_)} are of different vectors")
+    if have[-1] < 16 * blocks or bytes_[-1] < (blocks + 15) & ~15:
+        raise ValueError(f"{role}: rows of {have[-1]} and {bytes_[-1]} bytes do not hold {length} values")
+    if codes.get_device() != index or scales.get_device() != index:
+        raise ValueError(f"{role} must be on cuda:{index} with the other operands")
+    return codes.data_ptr(), ldq, scales.data_ptr(), lds
 
 
-def _codes(q, role, dims, device=None):
-    for t in (q.codes, q.scales):
-        if t.dtype != torch.uint8:
-            raise TypeError(f"{role}: codes and scales are uint8, not {t.dtype}")
-        _dense(t, role, dims)
-    if q.codes.shape[:-1] != q.scales.shape[:-1]:
-        raise ValueError(f"{role}: codes {tuple(q.codes.shape)} and scales {tuple(q.scales.shape)} are of different vectors")
-    blocks = -(-q.length // 32)
-    if q.codes.shape[-1] < 16 * blocks or q.scales.shape[-1] < -(-blocks // 16) * 16:
-        raise ValueError(f"{role}: rows of {q.codes.shape[-1]} and {q.scales.shape[-1]} bytes do not hold {q.length} values")
-    if q.scales.device != q.codes.device or (device is not None and q.codes.device != device):
-        raise ValueError(f"{role} must be on one device with the other operands")
-    return q.codes.data_ptr(), _pitch(q.codes), q.scales.data_ptr(), _pitch(q.scales)
-
-
-def _same_device(device, **tensors):
-    for name, t in tensors.items():
-        if t is not None and t.device != device:
-            raise ValueError(f"{name} must be on {device}, not {t.device}")
-
-
-def _result(out, shape, dtype, device):
+def _result(like, out, shape, dtype, dims=2):
+    """out, checked, or a new tensor on the device of `like`; and the pitch of its rows."""
     if out is None:
-        return torch.empty(shape, dtype=dtype, device=device)
-    if tuple(out.shape) != tuple(shape) or out.dtype != dtype or out.device != device:
-        raise ValueError(f"out= must be {tuple(shape)} of {dtype} on {device}")
-    return _dense(out, "out", len(shape))
+        return like.new_empty(shape, dtype=dtype), shape[-1]
+    if tuple(out.shape) != tuple(shape) or out.dtype != dtype or out.device != like.device:
+        raise ValueError(f"out= must be {tuple(shape)} of {dtype} on {like.device}")
+    return out, _pitch(out, "out", dims)
 
 
-def _offsets(offsets, device):
-    if offsets.dtype != torch.int32 or offsets.dim() != 1 or not offsets.is_contiguous() or offsets.numel() < 2:
+def _offsets(offsets, index):
+    if offsets.dtype is not torch.int32 or offsets.dim() != 1 or not offsets.is_contiguous() or offsets.shape[0] < 2:
         raise ValueError("offsets must be a contiguous int32 vector of at least two numbers")
-    _same_device(device, offsets=offsets)
-    return offsets.numel() - 1
+    if offsets.get_device() != index:
+        raise ValueError(f"offsets must be on cuda:{index}, not {offsets.device}")
+    return offsets.shape[0] - 1
+
+
+def _routed(r, index):
+    """Checks a Routing (of experts.sort) on device `index`; (tokens, top)."""
+    for name, t in (("offsets", r.offsets), ("rows", r.rows), ("slots", r.slots)):
+        if t.dtype is not torch.int32 or not t.is_contiguous() or t.get_device() != index:
+            raise ValueError(f"routing.{name} must be contiguous int32 on cuda:{index}")
+    if r.rows.dim() != 2:
+        raise ValueError("routing.rows has a row for each token")
+    return r.rows.shape
 
 
 def quantize(x, dim=-1, rule="floor", routing=None):
@@ -107,34 +115,40 @@ def quantize(x, dim=-1, rule="floor", routing=None):
     `routing` (of experts.sort) takes the rows of a matrix x in the order of their experts first, zeros where there is none."""
     if dim not in (-1, -2) or rule not in _RULES:
         raise ValueError(f"dim is -1 or -2 and rule one of {sorted(_RULES)}")
-    kind = _type(x.dtype)
-    if x.dim() not in (2, 3):
-        raise ValueError(f"x must be a matrix or a stack of matrices, not {x.dim()}-dimensional")
-    _dense(x, "x", x.dim())
-    rows, cols = x.shape[-2:]
-    slots = per = None
+    kind, shape = _type(x.dtype), x.shape
+    dims = len(shape)
+    if dims not in (2, 3):
+        raise ValueError(f"x must be a matrix or a stack of matrices, not {dims}-dimensional")
+    ldx, index = _pitch(x, "x", dims), x.get_device()
+    rows, cols = sources, _ = shape[-2:]
+    slots, per = None, 0
     if routing is not None:
-        if x.dim() != 2 or rows != routing.rows.shape[0]:
+        if dims != 2 or rows != routing.rows.shape[0]:
             raise ValueError("routing= takes a matrix with a row for each token")
-        _same_device(x.device, routing=routing.slots)
-        slots, per, rows = routing.slots.data_ptr(), routing.rows.shape[1], routing.slots.numel()
+        _, per = _routed(routing, index)
+        slots, rows = routing.slots.data_ptr(), routing.slots.shape[0]
     vectors, length = (rows, cols) if dim == -1 else (cols, rows)
-    blocks = -(-length // 32)
-    lead = tuple(x.shape[:-2])
-    codes = torch.empty((*lead, vectors, 16 * blocks), dtype=torch.uint8, device=x.device)
-    scales = torch.empty((*lead, vectors, -(-blocks // 16) * 16), dtype=torch.uint8, device=x.device)
-    planes = x.shape[0] if lead else 1
-    _call(x.device, _lib.ozb_mx4_quantize, x.data_ptr(), kind, vectors, length, _pitch(x), 1 if dim == -1 else 0, _RULES[rule], slots, per or 0,
-          x.shape[-2], planes, x.stride(0) if lead else 0, codes.data_ptr(), codes.shape[-1], codes.stride(0), scales.data_ptr(), scales.shape[-1],
-          scales.stride(0))
+    blocks = (length + 31) >> 5
+    ldq, lds = 16 * blocks, (blocks + 15) & ~15
+    if dims == 2:
+        codes, scales = x.new_empty((vectors, ldq), dtype=torch.uint8), x.new_empty((vectors, lds), dtype=torch.uint8)
+        planes = 1, 0, 0, 0
+    else:
+        codes, scales = x.new_empty((shape[0], vectors, ldq), dtype=torch.uint8), x.new_empty((shape[0], vectors, lds), dtype=torch.uint8)
+        planes = shape[0], x.stride(0), vectors * ldq, vectors * lds
+    _call(index, _lib.ozb_mx4_quantize, x.data_ptr(), kind, vectors, length, ldx, dim == -1, _RULES[rule], slots, per, sources, planes[0], planes[1],
+          codes.data_ptr(), ldq, planes[2], scales.data_ptr(), lds, planes[3])
     return Mx4(codes, scales, length)
 
 
 def dequantize(q, dtype=torch.float32, out=None):
     """The values of an Mx4 of vectors, [n, length] of `dtype` (exact in float32 and bfloat16)."""
-    codes, ldq, scales, lds = _codes(q, "q", 2)
-    y = _result(out, (q.codes.shape[0], q.length), dtype, q.codes.device)
-    _call(y.device, _lib.ozb_mx4_dequantize, codes, ldq, scales, lds, y.shape[0], q.length, y.data_ptr(), _type(dtype), _pitch(y))
+    like = q.codes
+    index = like.get_device()
+    codes, ldq, scales, lds = _codes(q, "q", 2, index)
+    n, length = like.shape[0], q.length
+    y, ldy = _result(like, out, (n, length), dtype)
+    _call(index, _lib.ozb_mx4_dequantize, codes, ldq, scales, lds, n, length, y.data_ptr(), _type(dtype), ldy)
     return y
 
 
@@ -146,32 +160,40 @@ def _common_length(a, b):
 
 def matmul(x, w, dtype=torch.bfloat16, out=None):
     """Y = X W^T, [rows of x, rows of w] of `dtype`: summed in FP32, rounded once."""
-    k, device = _common_length(x, w), x.codes.device
-    left, right = _codes(x, "x", 2), _codes(w, "w", 2, device)
-    y = _result(out, (x.codes.shape[0], w.codes.shape[0]), dtype, device)
-    _call(device, _lib.ozb_mx4_gemm, y.shape[0], y.shape[1], k, *left, *right, y.data_ptr(), _type(dtype), _pitch(y))
+    k, like = _common_length(x, w), x.codes
+    index = like.get_device()
+    left, right = _codes(x, "x", 2, index), _codes(w, "w", 2, index)
+    m, n = like.shape[0], w.codes.shape[0]
+    kind = _type(dtype)
+    y, ldy = _result(like, out, (m, n), dtype)
+    _call(index, _lib.ozb_mx4_gemm, m, n, k, *left, *right, y.data_ptr(), kind, ldy)
     return y
 
 
 def grouped_matmul(x, w, offsets, dtype=torch.bfloat16, out=None):
     """Rows offsets[g] .. offsets[g + 1] - 1 of X times W[g]^T for each g; w is a stack [groups, n, ...], offsets int32 on the device
     (groups + 1 numbers that do not decrease). Rows outside of the segments are not written."""
-    k, device, groups = _common_length(x, w), x.codes.device, w.codes.shape[0]
-    if _offsets(offsets, device) != groups:
+    k, like = _common_length(x, w), x.codes
+    index = like.get_device()
+    left, (wc, ldw, ws, ldws) = _codes(x, "x", 2, index), _codes(w, "w", 3, index)
+    groups, n = w.codes.shape[:2]
+    if _offsets(offsets, index) != groups:
         raise ValueError(f"{groups} groups need {groups + 1} offsets")
-    left, (wc, ldw, ws, ldws) = _codes(x, "x", 2), _codes(w, "w", 3, device)
-    y = _result(out, (x.codes.shape[0], w.codes.shape[1]), dtype, device)
-    _call(device, _lib.ozb_mx4_gemm_grouped, groups, y.shape[0], y.shape[1], k, offsets.data_ptr(), *left, wc, ldw, w.codes.stride(0), ws, ldws,
-          w.scales.stride(0), y.data_ptr(), _type(dtype), _pitch(y))
+    kind = _type(dtype)
+    y, ldy = _result(like, out, (like.shape[0], n), dtype)
+    _call(index, _lib.ozb_mx4_gemm_grouped, groups, like.shape[0], n, k, offsets.data_ptr(), *left, wc, ldw, w.codes.stride(0), ws, ldws, w.scales.stride(0),
+          y.data_ptr(), kind, ldy)
     return y
 
 
 def segment_matmul(a, b, offsets, dtype=torch.bfloat16, out=None):
     """Y[g] = A[:, offsets[g] : offsets[g + 1]] B[:, the same]^T, [groups, rows of a, rows of b]; the offsets are multiples of 64."""
-    r, device = _common_length(a, b), a.codes.device
-    groups = _offsets(offsets, device)
-    left, right = _codes(a, "a", 2), _codes(b, "b", 2, device)
-    y = _result(out, (groups, a.codes.shape[0], b.codes.shape[0]), dtype, device)
-    _call(device, _lib.ozb_mx4_gemm_segments, groups, y.shape[1], y.shape[2], r, offsets.data_ptr(), *left, *right, y.data_ptr(), _type(dtype), _pitch(y),
-          y.stride(0))
+    r, like = _common_length(a, b), a.codes
+    index = like.get_device()
+    groups = _offsets(offsets, index)
+    left, right = _codes(a, "a", 2, index), _codes(b, "b", 2, index)
+    m, n = like.shape[0], b.codes.shape[0]
+    kind = _type(dtype)
+    y, ldy = _result(like, out, (groups, m, n), dtype, 3)
+    _call(index, _lib.ozb_mx4_gemm_segments, groups, m, n, r, offsets.data_ptr(), *left, *right, y.data_ptr(), kind, ldy, y.stride(0))
     return y
