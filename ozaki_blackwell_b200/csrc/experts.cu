@@ -8,6 +8,7 @@
 //     its gradient  dz[r] = w[s] dy[s / top],  dw[s] = <dy[s / top], z[row_of[s]]>
 // and the gradient of gather is combine without weights. An index that is out of range counts as none: nothing is read or
 // written outside the arrays, whatever they hold.
+#include <type_traits>
 #include "oz_common.cuh"
 #include "oz_kernels.h"
 #include "oz_types.cuh"
@@ -17,7 +18,7 @@ namespace ozk {
 namespace {
 
 constexpr int MAX_EXPERTS = 1024;
-constexpr int CHUNK = 2048, SORT_THREADS = 256, SORT_WARPS = 8, PER_WARP = CHUNK / SORT_WARPS, ROUNDS = PER_WARP / 32;
+constexpr int CHUNK = 1024, SORT_THREADS = 256, SORT_WARPS = 8, PER_WARP = CHUNK / SORT_WARPS, ROUNDS = PER_WARP / 32;
 
 // the expert of slot s, or `experts` for a dropped one
 __device__ __forceinline__ int key_of(const void *ids, int id_bytes, int experts, int s) {
@@ -25,16 +26,28 @@ __device__ __forceinline__ int key_of(const void *ids, int id_bytes, int experts
     return id >= 0 && id < experts ? (int)id : experts;
 }
 
-// A warp owns PER_WARP consecutive slots of the chunk and takes them 32 at a time in their order: lanes with the same expert find each
-// other by a vote, the first of them adds their number to the warp's count, and a lane's rank is the count before plus the peers
-// below it. rank[i]: the rank of the i-th round's slot among the warp's slots of its expert; count[e]: the warp's total.
-__device__ __forceinline__ void rank_slots(const void *ids, int id_bytes, int experts, int slots, int first, int *count, int (&key)[ROUNDS], int (&rank)[ROUNDS]) {
-    const int lane = threadIdx.x & 31;
+struct SortShared {
+    int count[SORT_WARPS][MAX_EXPERTS];
+    int total[MAX_EXPERTS], before[MAX_EXPERTS];
+    int warp_sum[SORT_WARPS];
+};
+
+// Ranks of a chunk's slots among its slots of the same expert, in their order. A warp owns PER_WARP consecutive slots and takes them 32
+// at a time: lanes with the same expert find each other by a vote, the last of them adds their number to the warp's count, and a
+// lane's rank is the count before plus the peers below it; then the counts of the warps before are added. total[e]: the chunk's.
+__device__ __forceinline__ void rank_slots(SortShared &sh, const void *ids, int id_bytes, int experts, int slots, int first, int (&key)[ROUNDS], int (&rank)[ROUNDS]) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    for (int w = 0; w < SORT_WARPS; w++)
+        for (int e = threadIdx.x; e < experts; e += SORT_THREADS) sh.count[w][e] = 0;
+    first += warp * PER_WARP;
 #pragma unroll
     for (int i = 0; i < ROUNDS; i++) {
         const int s = first + i * 32 + lane;
         key[i] = s < slots ? key_of(ids, id_bytes, experts, s) : experts;
+        rank[i] = 0;
     }
+    __syncthreads();
+    int *count = sh.count[warp];
 #pragma unroll
     for (int i = 0; i < ROUNDS; i++) {
         if (first + i * 32 >= slots) break;   // the same for the whole warp
@@ -42,65 +55,34 @@ __device__ __forceinline__ void rank_slots(const void *ids, int id_bytes, int ex
         const int before = key[i] < experts ? count[key[i]] : 0;
         rank[i] = before + __popc(peers & ((1u << lane) - 1u));
         __syncwarp();
-        if (key[i] < experts && (peers >> lane) == 1u) count[key[i]] = before + __popc(peers);   // the highest of the peers
+        if (key[i] < experts && (peers >> lane) == 1u) count[key[i]] = before + __popc(peers);
         __syncwarp();
     }
-}
-
-// Two kernels where there is more than one chunk: the first counts each chunk's slots by expert (and clears slot_of), the second
-// adds up the counts of all chunks -- of every chunk for the segments' lengths, of the chunks before its own for where its slots
-// go -- and writes both maps. With one chunk the second does it all. Every count is an integer sum: the order is exact and the same
-// on every run.
-__global__ void __launch_bounds__(SORT_THREADS) sort_count(const void *ids, int id_bytes, int experts, int slots, int R, int *slot_of, int *counts) {
-    __shared__ int count[SORT_WARPS][MAX_EXPERTS];
-    const int warp = threadIdx.x >> 5;
-    for (int e = threadIdx.x; e < experts * SORT_WARPS; e += SORT_THREADS) count[e / experts][e % experts] = 0;
-    for (long long r = (long long)blockIdx.x * SORT_THREADS + threadIdx.x; r < R; r += (long long)gridDim.x * SORT_THREADS) slot_of[r] = -1;
-    __syncthreads();
-    int key[ROUNDS], rank[ROUNDS];
-    rank_slots(ids, id_bytes, experts, slots, blockIdx.x * CHUNK + warp * PER_WARP, count[warp], key, rank);
     __syncthreads();
     for (int e = threadIdx.x; e < experts; e += SORT_THREADS) {
         int n = 0;
 #pragma unroll
-        for (int w = 0; w < SORT_WARPS; w++) n += count[w][e];
-        counts[(size_t)blockIdx.x * experts + e] = n;
+        for (int w = 0; w < SORT_WARPS; w++) {
+            const int c = sh.count[w][e];
+            sh.count[w][e] = n;
+            n += c;
+        }
+        sh.total[e] = n;
+        sh.before[e] = 0;
     }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < ROUNDS; i++)
+        if (key[i] < experts) rank[i] += count[key[i]];
 }
 
-__global__ void __launch_bounds__(SORT_THREADS) sort_place(const void *ids, int id_bytes, int experts, int slots, int align, int R, int *offsets,
-                                                           int *row_of, int *slot_of, const int *counts) {
-    __shared__ int count[SORT_WARPS][MAX_EXPERTS];   // where the next slot of a warp for an expert goes, in the end
-    __shared__ int warp_sum[SORT_WARPS];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const bool alone = counts == nullptr;
-    for (int e = threadIdx.x; e < experts * SORT_WARPS; e += SORT_THREADS) count[e / experts][e % experts] = 0;
-    if (alone) for (int r = threadIdx.x; r < R; r += SORT_THREADS) slot_of[r] = -1;
-    __syncthreads();
-    const int first = blockIdx.x * CHUNK + warp * PER_WARP;
-    int key[ROUNDS], rank[ROUNDS];
-    rank_slots(ids, id_bytes, experts, slots, first, count[warp], key, rank);
-    __syncthreads();
-    // a thread takes up to four consecutive experts
-    constexpr int PER = MAX_EXPERTS / SORT_THREADS;
-    int before[PER], length[PER], sum = 0;
-#pragma unroll
-    for (int i = 0; i < PER; i++) {
-        const int e = threadIdx.x * PER + i;
-        before[i] = length[i] = 0;
-        if (e >= experts) continue;
-        if (alone) {
-#pragma unroll
-            for (int w = 0; w < SORT_WARPS; w++) length[i] += count[w][e];
-        } else {
-            for (int b = 0; b < (int)gridDim.x; b++) {
-                const int n = __ldg(counts + (size_t)b * experts + e);
-                if (b < (int)blockIdx.x) before[i] += n;
-                length[i] += n;
-            }
-        }
-        length[i] = (length[i] + align - 1) / align * align;
-        sum += length[i];
+// Where each segment begins, from the padded totals: total[e] becomes it, `offsets` is written if it is not null.
+__device__ __forceinline__ void place_segments(SortShared &sh, int experts, int align, int *offsets) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, per = (experts + SORT_THREADS - 1) / SORT_THREADS;   // consecutive experts to a thread
+    int sum = 0;
+    for (int i = 0; i < per; i++) {
+        const int e = threadIdx.x * per + i;
+        if (e < experts) sum += (sh.total[e] + align - 1) / align * align;
     }
     int inc = sum;
 #pragma unroll
@@ -108,35 +90,88 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_place(const void *ids, int 
         const int o = __shfl_up_sync(~0u, inc, d);
         if (lane >= d) inc += o;
     }
-    if (lane == 31) warp_sum[warp] = inc;
+    if (lane == 31) sh.warp_sum[warp] = inc;
     __syncthreads();
     int at = inc - sum;
-    for (int w = 0; w < warp; w++) at += warp_sum[w];
-#pragma unroll
-    for (int i = 0; i < PER; i++) {
-        const int e = threadIdx.x * PER + i;
-        if (e >= experts) continue;
-        if (blockIdx.x == 0) offsets[e] = at;
-        int next = at + before[i];
-#pragma unroll
-        for (int w = 0; w < SORT_WARPS; w++) {
-            const int n = count[w][e];
-            count[w][e] = next;
-            next += n;
-        }
-        at += length[i];
-        if (blockIdx.x == 0 && e == experts - 1) offsets[experts] = at;
+    for (int w = 0; w < warp; w++) at += sh.warp_sum[w];
+    for (int i = 0; i < per; i++) {
+        const int e = threadIdx.x * per + i;
+        if (e >= experts) break;
+        const int n = (sh.total[e] + align - 1) / align * align;
+        sh.total[e] = at;
+        if (offsets) offsets[e] = at;
+        at += n;
+        if (offsets && e == experts - 1) offsets[experts] = at;
     }
     __syncthreads();
+}
+
+// Up to CHUNK slots: one block does it all. More: sort_count ranks the slots of each chunk (row_of holds the ranks meanwhile), counts
+// them by expert and clears slot_of; sort_place adds up the counts -- of all chunks for the segments' lengths, of the chunks before its
+// own for where its slots go -- and writes both maps. All counts are whole numbers: the order is the same on every run.
+__global__ void __launch_bounds__(SORT_THREADS) sort_one(const void *ids, int id_bytes, int experts, int slots, int align, int R, int *offsets, int *row_of, int *slot_of) {
+    __shared__ SortShared sh;
+    for (int r = threadIdx.x; r < R; r += SORT_THREADS) slot_of[r] = -1;
+    int key[ROUNDS], rank[ROUNDS];
+    rank_slots(sh, ids, id_bytes, experts, slots, 0, key, rank);
+    place_segments(sh, experts, align, offsets);
 #pragma unroll
     for (int i = 0; i < ROUNDS; i++) {
-        const int s = first + i * 32 + lane;
+        const int s = (threadIdx.x >> 5) * PER_WARP + i * 32 + (threadIdx.x & 31);
         if (s >= slots) continue;
-        int row = -1;
-        if (key[i] < experts) {
-            row = count[warp][key[i]] + rank[i];
-            if (row < R) slot_of[row] = s;   // always: the caller's R holds every padded segment
+        const int row = key[i] < experts ? sh.total[key[i]] + rank[i] : -1;
+        if (row >= 0) slot_of[row] = s;
+        row_of[s] = row;
+    }
+}
+
+__global__ void __launch_bounds__(SORT_THREADS) sort_count(const void *ids, int id_bytes, int experts, int slots, int R, int *row_of, int *slot_of, int *counts) {
+    __shared__ SortShared sh;
+    for (long long r = (long long)blockIdx.x * SORT_THREADS + threadIdx.x; r < R; r += (long long)gridDim.x * SORT_THREADS) slot_of[r] = -1;
+    int key[ROUNDS], rank[ROUNDS];
+    rank_slots(sh, ids, id_bytes, experts, slots, blockIdx.x * CHUNK, key, rank);
+#pragma unroll
+    for (int i = 0; i < ROUNDS; i++) {
+        const int s = blockIdx.x * CHUNK + (threadIdx.x >> 5) * PER_WARP + i * 32 + (threadIdx.x & 31);
+        if (s < slots) row_of[s] = rank[i];
+    }
+    for (int e = threadIdx.x; e < experts; e += SORT_THREADS) counts[(size_t)blockIdx.x * experts + e] = sh.total[e];
+}
+
+__global__ void __launch_bounds__(SORT_THREADS) sort_place(const void *ids, int id_bytes, int experts, int slots, int align, int R, int *offsets,
+                                                           int *row_of, int *slot_of, const int *counts) {
+    __shared__ SortShared sh;
+    int rank[CHUNK / SORT_THREADS], key[CHUNK / SORT_THREADS];
+#pragma unroll
+    for (int i = 0; i < CHUNK / SORT_THREADS; i++) {
+        const int s = blockIdx.x * CHUNK + i * SORT_THREADS + threadIdx.x;
+        key[i] = s < slots ? key_of(ids, id_bytes, experts, s) : experts;
+        rank[i] = s < slots ? row_of[s] : 0;
+    }
+    for (int e = threadIdx.x; e < experts; e += SORT_THREADS) sh.total[e] = sh.before[e] = 0;
+    __syncthreads();
+    // all chunks' counts, eight loads in flight to a thread
+    const int n = gridDim.x * experts, own = blockIdx.x * experts;
+    for (int i0 = threadIdx.x; i0 < n; i0 += 8 * SORT_THREADS) {
+        int c[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) c[k] = i0 + k * SORT_THREADS < n ? __ldg(counts + i0 + k * SORT_THREADS) : 0;
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            const int i = i0 + k * SORT_THREADS;
+            if (!c[k]) continue;
+            atomicAdd(&sh.total[i % experts], c[k]);
+            if (i < own) atomicAdd(&sh.before[i % experts], c[k]);
         }
+    }
+    __syncthreads();
+    place_segments(sh, experts, align, blockIdx.x == 0 ? offsets : nullptr);
+#pragma unroll
+    for (int i = 0; i < CHUNK / SORT_THREADS; i++) {
+        const int s = blockIdx.x * CHUNK + i * SORT_THREADS + threadIdx.x;
+        if (s >= slots) continue;
+        const int row = key[i] < experts ? sh.total[key[i]] + sh.before[key[i]] + rank[i] : -1;
+        if (row >= 0) slot_of[row] = s;
         row_of[s] = row;
     }
 }
@@ -158,12 +193,13 @@ __global__ void __launch_bounds__(256) gather_rows(const E *X, long long pitch_x
         }
 #pragma unroll
         for (int i = 0; i < DEPTH; i++)
-            if (c0 + 32 * i < n) Y[(size_t)r * pitch_y + c0 + 32 * i] = v[i];
+            if (c0 + 32 * i < n) __stcs(Y + (size_t)r * pitch_y + c0 + 32 * i, v[i]);   // written once: the tokens' rows stay in L2 instead
     }
 }
 
-// A lane holds 16 bytes' worth of columns of one token and adds the token's rows in the order of j.
-template <class T, bool VEC>
+// A lane holds 16 bytes' worth of columns of one token and adds the token's rows in the order of j, U at a time: U loads are in flight,
+// made whether the slot has a row or not (from row 0 if not), since loads under a condition each would wait for one another.
+template <class T, bool VEC, int U>
 __global__ void __launch_bounds__(256) combine_rows(const T *Z, long long ldz, int R, const int *row_of, const float *weights, int tokens, int top, int H,
                                                     T *Y, long long ldy) {
     constexpr int N = Vec16<T>::N;
@@ -172,20 +208,36 @@ __global__ void __launch_bounds__(256) combine_rows(const T *Z, long long ldz, i
     for (long long w = (long long)blockIdx.x * 256 + threadIdx.x; w < total; w += (long long)gridDim.x * 256) {
         const int t = (int)(w / cols), c = (int)(w - (long long)t * cols) * N;
         float sum[N] = {};
-#pragma unroll 4
-        for (int j = 0; j < top; j++) {
-            const long long s = (long long)t * top + j;
-            const int r = __ldg(row_of + s);
-            if (r < 0 || r >= R) continue;
-            const float f = weights ? __ldg(weights + s) : 1.f;
-            const T *z = Z + (size_t)r * ldz + c;
-            float v[N];
-            if (VEC && c + N <= H) Vec16<T>::unpack(__ldg(reinterpret_cast<const uint4 *>(z)), v);
-            else
+        for (int j0 = 0; j0 < top; j0 += U) {
+            int r[U];
+            float f[U];
 #pragma unroll
-                for (int i = 0; i < N; i++) v[i] = c + i < H ? to_f32<T>(z[i]) : 0.f;
+            for (int u = 0; u < U; u++) {
+                const long long s = (long long)t * top + min(j0 + u, top - 1);
+                r[u] = j0 + u < top ? __ldg(row_of + s) : -1;
+                f[u] = weights ? __ldg(weights + s) : 1.f;
+                if (r[u] >= R) r[u] = -1;
+            }
+            if (VEC && c + N <= H) {
+                uint4 q[U];
 #pragma unroll
-            for (int i = 0; i < N; i++) sum[i] = fmaf(f, v[i], sum[i]);
+                for (int u = 0; u < U; u++) q[u] = __ldcs(reinterpret_cast<const uint4 *>(Z + (size_t)max(r[u], 0) * ldz + c));
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    float v[N];
+                    Vec16<T>::unpack(q[u], v);
+                    if (r[u] >= 0)
+#pragma unroll
+                        for (int i = 0; i < N; i++) sum[i] = fmaf(f[u], v[i], sum[i]);
+                }
+            } else {
+#pragma unroll
+                for (int u = 0; u < U; u++)
+                    if (r[u] >= 0)
+#pragma unroll
+                        for (int i = 0; i < N; i++)
+                            if (c + i < H) sum[i] = fmaf(f[u], to_f32<T>(Z[(size_t)r[u] * ldz + c + i]), sum[i]);
+            }
         }
         T *y = Y + (size_t)t * ldy + c;
         if (VEC && c + N <= H) *reinterpret_cast<uint4 *>(y) = Vec16<T>::pack(sum);
@@ -208,38 +260,55 @@ __global__ void __launch_bounds__(256) combine_grad_rows(const T *dY, long long 
     }
     for (long long r = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); r < R; r += (long long)gridDim.x * 8) {
         const int s = __ldg(slot_of + r);
-        const bool there = s >= 0 && s < slots;
-        const float f = !there ? 0.f : weights ? __ldg(weights + s) : 1.f;
-        const T *dy = dY + (size_t)(there ? s / top : 0) * lddy, *z = Z + (size_t)r * ldz;
         T *dz = dZ + (size_t)r * lddz;
-        float dot = 0.f;
-#pragma unroll 2
-        for (int c = lane * N; c < H; c += 32 * N) {
-            float a[N] = {}, b[N] = {};
-            if (VEC && c + N <= H) {
-                if (there) {
-                    Vec16<T>::unpack(__ldg(reinterpret_cast<const uint4 *>(dy + c)), a);
-                    Vec16<T>::unpack(__ldg(reinterpret_cast<const uint4 *>(z + c)), b);
-                }
-            } else if (there) {
+        constexpr int U = 4;   // pieces of both rows in flight
+        if (s < 0 || s >= slots) {
+            for (int c = lane * N; c < H; c += 32 * N) {
+                if (VEC && c + N <= H) *reinterpret_cast<uint4 *>(dz + c) = make_uint4(0, 0, 0, 0);
+                else
 #pragma unroll
-                for (int i = 0; i < N; i++)
-                    if (c + i < H) { a[i] = to_f32<T>(dy[c + i]); b[i] = to_f32<T>(z[c + i]); }
+                    for (int i = 0; i < N; i++)
+                        if (c + i < H) dz[c + i] = from_f32<T>(0.f);
             }
+            continue;
+        }
+        const float f = weights ? __ldg(weights + s) : 1.f;
+        const T *dy = dY + (size_t)(s / top) * lddy, *z = Z + (size_t)r * ldz;
+        float dot = 0.f;
+        auto use = [&](float (&a)[N], const float (&b)[N]) {
 #pragma unroll
             for (int i = 0; i < N; i++) {
                 dot = fmaf(a[i], b[i], dot);
-                a[i] = there ? f * a[i] : 0.f;
+                a[i] *= f;
             }
-            if (VEC && c + N <= H) *reinterpret_cast<uint4 *>(dz + c) = Vec16<T>::pack(a);
-            else
+        };
+        int c0 = 0;
+        if constexpr (VEC) {
+            for (; c0 + U * 32 * N <= H; c0 += U * 32 * N) {
+                uint4 qa[U], qb[U];
 #pragma unroll
-                for (int i = 0; i < N; i++)
-                    if (c + i < H) dz[c + i] = from_f32<T>(a[i]);
+                for (int u = 0; u < U; u++) {
+                    qa[u] = __ldg(reinterpret_cast<const uint4 *>(dy + c0 + (u * 32 + lane) * N));
+                    qb[u] = __ldcs(reinterpret_cast<const uint4 *>(z + c0 + (u * 32 + lane) * N));
+                }
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    float a[N], b[N];
+                    Vec16<T>::unpack(qa[u], a);
+                    Vec16<T>::unpack(qb[u], b);
+                    use(a, b);
+                    __stcs(reinterpret_cast<uint4 *>(dz + c0 + (u * 32 + lane) * N), Vec16<T>::pack(a));
+                }
+            }
+        }
+        for (int c = c0 + lane; c < H; c += 32) {   // what is left, or rows that do not start on 16 bytes: single columns
+            const float a = to_f32<T>(dy[c]);
+            dot = fmaf(a, to_f32<T>(z[c]), dot);
+            dz[c] = from_f32<T>(f * a);
         }
 #pragma unroll
         for (int d = 16; d; d >>= 1) dot += __shfl_xor_sync(~0u, dot, d);
-        if (lane == 0 && there) dW[s] = dot;
+        if (lane == 0) dW[s] = dot;
     }
 }
 
@@ -255,9 +324,13 @@ size_t expert_sort_scratch(int slots, int experts) {
 cudaError_t expert_sort(int slots, int experts, const void *ids, int id_bytes, int align, int R, int *offsets, int *rows, int *slot_of, void *scratch,
                         cudaStream_t st) {
     const int chunks = (slots + CHUNK - 1) / CHUNK;
-    int *counts = chunks > 1 ? static_cast<int *>(scratch) : nullptr;
-    if (counts) sort_count<<<chunks, SORT_THREADS, 0, st>>>(ids, id_bytes, experts, slots, R, slot_of, counts);
-    sort_place<<<chunks, SORT_THREADS, 0, st>>>(ids, id_bytes, experts, slots, align, R, offsets, rows, slot_of, counts);
+    if (chunks == 1) {
+        sort_one<<<1, SORT_THREADS, 0, st>>>(ids, id_bytes, experts, slots, align, R, offsets, rows, slot_of);
+    } else {
+        int *counts = static_cast<int *>(scratch);
+        sort_count<<<chunks, SORT_THREADS, 0, st>>>(ids, id_bytes, experts, slots, R, rows, slot_of, counts);
+        sort_place<<<chunks, SORT_THREADS, 0, st>>>(ids, id_bytes, experts, slots, align, R, offsets, rows, slot_of, counts);
+    }
     return cudaGetLastError();
 }
 
@@ -283,8 +356,14 @@ cudaError_t expert_combine(int T, int top, int H, const void *Z, int type, int R
     const int grid = grid_of(((long long)T * ((H + n - 1) / n) + 255) / 256);
     with_type(type, [&](auto t) {
         using E = decltype(t);
-        if (vec) combine_rows<E, true><<<grid, 256, 0, st>>>((const E *)Z, ldz, R, rows, weights, T, top, H, (E *)Y, ldy);
-        else combine_rows<E, false><<<grid, 256, 0, st>>>((const E *)Z, ldz, R, rows, weights, T, top, H, (E *)Y, ldy);
+        auto go = [&](auto many) {
+            constexpr int U = decltype(many)::value;
+            if (vec) combine_rows<E, true, U><<<grid, 256, 0, st>>>((const E *)Z, ldz, R, rows, weights, T, top, H, (E *)Y, ldy);
+            else combine_rows<E, false, U><<<grid, 256, 0, st>>>((const E *)Z, ldz, R, rows, weights, T, top, H, (E *)Y, ldy);
+        };
+        if (top <= 2) go(std::integral_constant<int, 2>());
+        else if (top <= 4) go(std::integral_constant<int, 4>());
+        else go(std::integral_constant<int, 8>());
     });
     return cudaGetLastError();
 }

@@ -73,6 +73,7 @@ template <class T, bool VEC>
 __global__ void __launch_bounds__(256) mx4_rows(const T *X, int nvec, int len, long long ldx, size_t plane_x, int planes, int rule,
                                                 const int *slots, int per, int sources, uint8_t *codes, long long ldq, size_t plane_q,
                                                 uint8_t *scales, long long lds, size_t plane_s) {
+    __shared__ float turn[8][32 * 17];
     const int lane = threadIdx.x & 31;
     const int pieces = (len + 511) / 512;
     const long long total = (long long)planes * nvec * pieces;
@@ -81,23 +82,33 @@ __global__ void __launch_bounds__(256) mx4_rows(const T *X, int nvec, int len, l
         const int i0 = (int)(w - vec * pieces) * 512 + lane * 16;
         const int z = (int)(vec / nvec), r = (int)(vec - (long long)z * nvec);
         const long long src = source_row(slots, per, sources, r);
+        const int at = i0 - lane * 16;
         float v[16];
-        if (src < 0 || i0 >= len) {
+        if (VEC && at + 512 <= len) {
+            constexpr int N = Vec16<T>::N;
+            uint4 q[16 / N] = {};
+            if (src >= 0) {
+                const uint4 *x = reinterpret_cast<const uint4 *>(X + (size_t)z * plane_x + (size_t)src * ldx + i0);
 #pragma unroll
-            for (int i = 0; i < 16; i++) v[i] = 0.f;
-        } else {
-            const T *x = X + (size_t)z * plane_x + (size_t)src * ldx + i0;
-            if (VEC && i0 + 16 <= len) {
-                constexpr int N = Vec16<T>::N;
-                uint4 q[16 / N];
-#pragma unroll
-                for (int i = 0; i < 16 / N; i++) q[i] = __ldg(reinterpret_cast<const uint4 *>(x) + i);
-#pragma unroll
-                for (int i = 0; i < 16 / N; i++) Vec16<T>::unpack(q[i], v + i * N);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 16; i++) v[i] = i0 + i < len ? to_f32<T>(x[i]) : 0.f;
+                for (int i = 0; i < 16 / N; i++) q[i] = __ldg(x + i);
             }
+#pragma unroll
+            for (int i = 0; i < 16 / N; i++) Vec16<T>::unpack(q[i], v + i * N);
+        } else {   // rows that do not start on 16 bytes, and ends: lanes load side by side, and turn the values through shared memory
+            float *mine = turn[threadIdx.x >> 5];
+            const T *x = X + (size_t)z * plane_x + (size_t)max(src, 0ll) * ldx + at;
+            T raw[16];
+#pragma unroll
+            for (int i = 0; i < 16; i++) raw[i] = x[min(i * 32 + lane, len - 1 - at)];
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                const int e = i * 32 + lane;
+                mine[e + (e >> 4)] = src >= 0 && at + e < len ? to_f32<T>(raw[i]) : 0.f;
+            }
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 16; i++) v[i] = mine[lane * 17 + i];
+            __syncwarp();
         }
         uint32_t m = 0;
 #pragma unroll
@@ -106,9 +117,10 @@ __global__ void __launch_bounds__(256) mx4_rows(const T *X, int nvec, int len, l
         const uint32_t byte = scale_byte(m, rule);
         const float inv = inverse_scale(byte);
 #pragma unroll
-        for (int i = 0; i < 16; i++) v[i] = byte == 255 ? 0.f : v[i] * inv;
+        for (int i = 0; i < 16; i++) v[i] *= inv;
         if ((i0 & ~31) < len) {   // the block exists: its codes are written whole, zeros behind the last value
-            *reinterpret_cast<uint2 *>(codes + (size_t)z * plane_q + (size_t)r * ldq + (i0 >> 1)) = make_uint2(codes_of(v), codes_of(v + 8));
+            const uint32_t number = byte == 255 ? 0u : ~0u;
+            *reinterpret_cast<uint2 *>(codes + (size_t)z * plane_q + (size_t)r * ldq + (i0 >> 1)) = make_uint2(codes_of(v) & number, codes_of(v + 8) & number);
             if (!(lane & 1)) scales[(size_t)z * plane_s + (size_t)r * lds + (i0 >> 5)] = (uint8_t)byte;
         }
     }
@@ -134,37 +146,33 @@ __global__ void __launch_bounds__(256) mx4_cols(const T *X, int nvec, int len, l
     X += (size_t)z * plane_x;
     codes += (size_t)z * plane_q;
     scales += (size_t)z * plane_s;
-    float v[2][32];
-    long long mine = -1;
-    if (k0 + lane < len) mine = source_row(slots, per, sources, k0 + lane);
+    struct alignas(2 * sizeof(T)) Pair { T a, b; };
+    Pair v[32];
+    // Every load is made, from a place that exists, and what was not there is cleared behind them: under a condition each they would
+    // wait for one another (a tile took the latency of 32 loads, 40 us where 8 are enough).
+    const long long mine = k0 + lane < len ? source_row(slots, per, sources, k0 + lane) : -1;
 #pragma unroll
     for (int i = 0; i < 32; i++) {
-        const long long src = __shfl_sync(~0u, mine, i);
-        v[0][i] = v[1][i] = 0.f;
-        if (src >= 0 && c < nvec) {
-            const T *x = X + (size_t)src * ldx + c;
-            if (VEC && c + 1 < nvec) {
-                struct alignas(2 * sizeof(T)) Pair { T a, b; };
-                const Pair p = *reinterpret_cast<const Pair *>(x);
-                v[0][i] = to_f32<T>(p.a);
-                v[1][i] = to_f32<T>(p.b);
-            } else {
-                v[0][i] = to_f32<T>(x[0]);
-                if (c + 1 < nvec) v[1][i] = to_f32<T>(x[1]);
-            }
-        }
+        const T *x = X + (size_t)max(__shfl_sync(~0u, mine, i), 0ll) * ldx;
+        if constexpr (VEC) v[i] = *reinterpret_cast<const Pair *>(x + (c < nvec ? c : 0));   // an even number of columns
+        else v[i].a = x[min(c, nvec - 1)], v[i].b = x[min(c + 1, nvec - 1)];
     }
+    const uint32_t rows = __ballot_sync(~0u, mine >= 0);
 #pragma unroll
     for (int h = 0; h < 2; h++) {
+        float f[32];
         uint32_t m = 0;
 #pragma unroll
-        for (int i = 0; i < 32; i++) m = max(m, magnitude(v[h][i]));
-        const uint32_t byte = scale_byte(m, rule);
+        for (int i = 0; i < 32; i++) {
+            f[i] = rows >> i & 1 ? to_f32<T>(h ? v[i].b : v[i].a) : 0.f;
+            m = max(m, magnitude(f[i]));
+        }
+        const uint32_t byte = scale_byte(m, rule), number = byte == 255 ? 0u : ~0u;
         const float inv = inverse_scale(byte);
 #pragma unroll
-        for (int i = 0; i < 32; i++) v[h][i] = byte == 255 ? 0.f : v[h][i] * inv;
+        for (int i = 0; i < 32; i++) f[i] *= inv;
         *reinterpret_cast<uint4 *>(tile + (2 * lane + h) * CT_PITCH + warp * 16) =
-            make_uint4(codes_of(v[h]), codes_of(v[h] + 8), codes_of(v[h] + 16), codes_of(v[h] + 24));
+            make_uint4(codes_of(f) & number, codes_of(f + 8) & number, codes_of(f + 16) & number, codes_of(f + 24) & number);
         stile[(2 * lane + h) * 8 + warp] = (uint8_t)byte;
     }
     __syncthreads();
@@ -187,29 +195,38 @@ __global__ void __launch_bounds__(256) mx4_cols(const T *X, int nvec, int len, l
 template <class T, bool VEC>
 __global__ void __launch_bounds__(256) mx4_values(const uint8_t *codes, long long ldq, const uint8_t *scales, long long lds, int nvec, int len,
                                                   T *Y, long long ldy) {
+    __shared__ float turn[8][32 * 17];
     const int lane = threadIdx.x & 31;
     const int pieces = (len + 511) / 512;
     const long long total = (long long)nvec * pieces;
     for (long long w = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); w < total; w += (long long)gridDim.x * 8) {
         const long long r = w / pieces;
-        const int i0 = (int)(w - r * pieces) * 512 + lane * 16;
-        if (i0 >= len) continue;
-        const uint2 q = __ldg(reinterpret_cast<const uint2 *>(codes + (size_t)r * ldq + (i0 >> 1)));
-        const float s = scale_of(__ldg(scales + (size_t)r * lds + (i0 >> 5)));
+        const int at = (int)(w - r * pieces) * 512, i0 = at + lane * 16;
+        T *y = Y + (size_t)r * ldy;
         float v[16];
-        values_of(q.x, v);
-        values_of(q.y, v + 8);
+        if (i0 < len) {
+            const uint2 q = __ldg(reinterpret_cast<const uint2 *>(codes + (size_t)r * ldq + (i0 >> 1)));
+            const float s = scale_of(__ldg(scales + (size_t)r * lds + (i0 >> 5)));
+            values_of(q.x, v);
+            values_of(q.y, v + 8);
 #pragma unroll
-        for (int i = 0; i < 16; i++) v[i] *= s;
-        T *y = Y + (size_t)r * ldy + i0;
-        if (VEC && i0 + 16 <= len) {
+            for (int i = 0; i < 16; i++) v[i] *= s;
+        }
+        if (VEC && at + 512 <= len) {
             constexpr int N = Vec16<T>::N;
 #pragma unroll
-            for (int i = 0; i < 16 / N; i++) *(reinterpret_cast<uint4 *>(y) + i) = Vec16<T>::pack(v + i * N);
-        } else {
+            for (int i = 0; i < 16 / N; i++) *(reinterpret_cast<uint4 *>(y + i0) + i) = Vec16<T>::pack(v + i * N);
+        } else {   // rows that do not start on 16 bytes, and ends: through shared memory, so that lanes store side by side
+            float *mine = turn[threadIdx.x >> 5];
 #pragma unroll
-            for (int i = 0; i < 16; i++)
-                if (i0 + i < len) y[i] = from_f32<T>(v[i]);
+            for (int i = 0; i < 16; i++) mine[lane * 17 + i] = v[i];
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                const int e = i * 32 + lane;
+                if (at + e < len) y[at + e] = from_f32<T>(mine[e + (e >> 4)]);
+            }
+            __syncwarp();
         }
     }
 }
@@ -239,7 +256,7 @@ cudaError_t mx4_quantize_cols(const void *X, int type, int nvec, int len, long l
                               int per, int sources, uint8_t *codes, long long ldq, size_t plane_q, uint8_t *scales, long long lds,
                               size_t plane_s, cudaStream_t st) {
     const int size = type_size(type);
-    const bool vec = !(reinterpret_cast<uintptr_t>(X) % (2 * size)) && !(ldx & 1) && !(plane_x & 1);
+    const bool vec = !(reinterpret_cast<uintptr_t>(X) % (2 * size)) && !((ldx | nvec) & 1) && !(plane_x & 1);
     const int col_tiles = (nvec + CT_COLS - 1) / CT_COLS, row_tiles = (len + CT_ROWS - 1) / CT_ROWS;
     const long long grid = (long long)col_tiles * row_tiles * planes;
     if (grid > 0x7fffffffLL) return cudaErrorInvalidValue;

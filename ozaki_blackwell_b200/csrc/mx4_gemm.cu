@@ -78,7 +78,8 @@ template <int FORM, int BN> struct Shape {
     static constexpr int COLS = 2 * BN + STAGES * SCALE_COLS;      // two accumulators, and the scales
     static constexpr int TMEM_COLS = COLS <= 256 ? 256 : 512;
     static constexpr int BARS = 2 * STAGES + 2 * SLOTS + 4;
-    static constexpr int SMEM = STAGES * STAGE + SLOTS * SLOT + 1024 + 8 * BARS + 16 + 4 * (MAX_GROUPS + 1);
+    static constexpr int TURN = wide ? 4 * 32 * (64 + 16) : 0;     // what the epilogue's warps turn their tiles through
+    static constexpr int SMEM = STAGES * STAGE + SLOTS * SLOT + TURN + 1024 + 8 * BARS + 16 + 4 * (MAX_GROUPS + 1);
     static_assert(STAGE % 1024 == 0 && COLS <= 512 && SMEM <= 232448 - 64, "");
     static_assert(FORM != SPLIT || BN * BP * 4 <= STAGES * STAGE, "the partial tile of a split takes the place of the stages");
     // instruction descriptor: E2M1 x E2M1, both K-major, one power of two (UE8M0) for 32, N = BN, M = rows of P, K = 64
@@ -183,8 +184,7 @@ __device__ __forceinline__ Tile decode(const Params &p, const int *cum, int w) {
     return t;
 }
 
-// 32 columns of a tile, v[c] = column j + c of the lane's row i. NARROW: Y's rows are the columns j, a warp stores 32 lanes side by
-// side; WIDE: Y's row is i, a lane stores 16-byte pieces where they are whole and aligned.
+// 32 columns of a tile, v[c] = column j + c of the lane's row. NARROW: Y's rows are the columns j, a warp stores 32 lanes side by side.
 template <class T>
 __device__ __forceinline__ void store_narrow(T *Y, long long ldy, const uint32_t (&v)[32], int i, int i1, int j, int j1) {
     if (i >= i1) return;
@@ -193,15 +193,30 @@ __device__ __forceinline__ void store_narrow(T *Y, long long ldy, const uint32_t
     for (int c = 0; c < 32; c++)
         if (j + c < j1) dst[(size_t)c * ldy] = from_f32<T>(__uint_as_float(v[c]));
 }
+// WIDE: Y's row is the lane's. Whole pieces turn through the warp's shared memory, so that four lanes store 64 contiguous bytes of a row
+// (whole sectors; a lane's own 16-byte stores to 32 rows at a time took the L2 twice as long). Columns at the edge, or rows that do not
+// start on 16 bytes, are stored one by one.
+constexpr int TURN_PITCH = 64 + 16, TURN_BYTES = 32 * TURN_PITCH;
 template <class T>
-__device__ __forceinline__ void store_wide(T *Y, long long ldy, const uint32_t (&v)[32], int i, int i1, int j, int j1) {
-    if (i >= i1 || j >= j1) return;
-    T *dst = Y + (size_t)i * ldy + j;
-    if (j + 32 <= j1 && !(reinterpret_cast<uintptr_t>(dst) & 15)) {
-        constexpr int N = Vec16<T>::N;
+__device__ __forceinline__ void store_wide(T *Y, long long ldy, const uint32_t (&v)[32], int i0, int lane, int i1, int j, int j1, uint8_t *turn) {
+    if (j >= j1) return;
+    constexpr int N = Vec16<T>::N, COLS = 4 * N;   // columns to 16 and to 64 bytes
+    if (j + 32 <= j1 && !((reinterpret_cast<uintptr_t>(Y + j) | (uintptr_t)(ldy * (long long)sizeof(T))) & 15)) {
 #pragma unroll
-        for (int c = 0; c < 32; c += N) *reinterpret_cast<uint4 *>(dst + c) = Vec16<T>::pack(reinterpret_cast<const float *>(&v[c]));
-    } else {
+        for (int h = 0; h < 32; h += COLS) {
+#pragma unroll
+            for (int c = 0; c < 4; c++) *reinterpret_cast<uint4 *>(turn + lane * TURN_PITCH + 16 * c) = Vec16<T>::pack(reinterpret_cast<const float *>(&v[h + c * N]));
+            __syncwarp();
+#pragma unroll
+            for (int r = 0; r < 32; r += 8) {
+                const int row = r + (lane >> 2);
+                const uint4 q = *reinterpret_cast<const uint4 *>(turn + row * TURN_PITCH + 16 * (lane & 3));
+                if (i0 + row < i1) *reinterpret_cast<uint4 *>(Y + (size_t)(i0 + row) * ldy + j + h + (lane & 3) * N) = q;
+            }
+            __syncwarp();
+        }
+    } else if (i0 + lane < i1) {
+        T *dst = Y + (size_t)(i0 + lane) * ldy + j;
 #pragma unroll
         for (int c = 0; c < 32; c++)
             if (j + c < j1) dst[c] = from_f32<T>(__uint_as_float(v[c]));
@@ -216,7 +231,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm(const __grid_constant__ C
     extern __shared__ uint8_t smem_raw[];
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t *const base_ptr = smem_raw + (base - smem_u32(smem_raw));
-    const uint32_t slots = base + S::STAGES * S::STAGE, bars = slots + S::SLOTS * S::SLOT;
+    const uint32_t slots = base + S::STAGES * S::STAGE, bars = slots + S::SLOTS * S::SLOT + S::TURN;
     auto full_bar = [&](int s) { return bars + 8u * s; };                                        // codes are there, and the scales in tensor memory (in a pair: both CTAs', at the leader)
     auto empty_bar = [&](int s) { return bars + 8u * (S::STAGES + s); };                         // the stage has been used up
     auto turned_bar = [&](int s) { return bars + 8u * (2 * S::STAGES + s); };                    // a slot's scales are turned (in a pair: both CTAs', at the leader)
@@ -224,7 +239,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm(const __grid_constant__ C
     auto accfull_bar = [&](int a) { return bars + 8u * (2 * S::STAGES + 2 * S::SLOTS + a); };
     auto accempty_bar = [&](int a) { return bars + 8u * (2 * S::STAGES + 2 * S::SLOTS + 2 + a); };
     const uint32_t tmem_slot = bars + 8u * S::BARS;
-    int *const cum = reinterpret_cast<int *>(base_ptr + S::STAGES * S::STAGE + S::SLOTS * S::SLOT + 8 * S::BARS + 16);
+    int *const cum = reinterpret_cast<int *>(base_ptr + S::STAGES * S::STAGE + S::SLOTS * S::SLOT + S::TURN + 8 * S::BARS + 16);
     __shared__ int abort_flag;
 
     const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
@@ -488,7 +503,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm(const __grid_constant__ C
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * BN;
             const bool some = t.s1 > t.s0;   // no stage: nothing was accumulated, the tile is zero
-            const int i = t.p0 + (pair ? (int)rank * BP : 0) + quarter * 32 + lane;
+            const int i0 = t.p0 + (pair ? (int)rank * BP : 0) + quarter * 32;   // the warp's first row of P
             if constexpr (FORM != SPLIT) {
                 T *Y = reinterpret_cast<T *>(p.Y) + (p.mode == ALONG_K ? (size_t)t.group * p.plane_y : 0);
 #pragma unroll 1
@@ -502,8 +517,8 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm(const __grid_constant__ C
                         for (int e = 0; e < 32; e++) v[e] = 0;
                     }
                     const int j1 = min(t.q1, t.q0 + BN);   // a tile of 16 columns: the other 16 are not its own
-                    if constexpr (S::wide) store_wide<T>(Y, p.ldy, v, i, t.p1, t.q0 + c, j1);
-                    else store_narrow<T>(Y, p.ldy, v, i, t.p1, t.q0 + c, j1);
+                    if constexpr (S::wide) store_wide<T>(Y, p.ldy, v, i0, lane, t.p1, t.q0 + c, j1, base_ptr + S::STAGES * S::STAGE + S::SLOTS * S::SLOT + quarter * TURN_BYTES);
+                    else store_narrow<T>(Y, p.ldy, v, i0 + lane, t.p1, t.q0 + c, j1);
                 }
             } else {   // the partial tile, [column][row of P], over the stages that this CTA has used up
                 float *part = reinterpret_cast<float *>(base_ptr);

@@ -54,7 +54,7 @@ def test_sort():
     assert lib.ozb_expert_sort_rows(1, 2, 100, 8) == 16                           # two slots touch two experts at most
     for bad in ((0, 1, 1, 1), (1, 0, 1, 1), (1, 1, 0, 1), (1, 1, 1025, 1), (1, 1, 1, 0), (1, 1, 1, 257), (2 ** 20, 2 ** 12, 1, 1)):
         assert lib.ozb_expert_sort_rows(*bad) == -ARG, bad
-    assert lib.ozb_expert_sort_scratch(1, 8, 64) == 0 and lib.ozb_expert_sort_scratch(2049, 1, 64) == 2 * 64 * 4
+    assert lib.ozb_expert_sort_scratch(128, 8, 64) == 0 and lib.ozb_expert_sort_scratch(1025, 1, 64) == 2 * 64 * 4
     base = dict(T=3, top=2, experts=4, ids=P, id_bytes=4, align=1, R=6, offsets=P, rows=P, slots=P, scratch=None, bytes=0)
     call = lambda **b: lib.ozb_expert_sort(*{**base, **b}.values(), None)  # noqa: E731
     for bad in (dict(T=0), dict(top=0), dict(experts=0), dict(ids=None), dict(id_bytes=2), dict(align=0), dict(align=257), dict(R=5), dict(align=64), dict(offsets=None),
