@@ -261,8 +261,10 @@ long long ozb_expert_sort_rows(int T, int top, int experts, int align);
 size_t ozb_expert_sort_scratch(int T, int top, int experts);
 int ozb_expert_sort(int T, int top, int experts, const void *ids, int id_bytes, int align, int R, int *offsets, int *rows, int *slots, void *scratch,
                     size_t scratch_bytes, void *stream);
-/* Y[r] = X[slots[r] / top] (T x H to R x H), zeros where there is no slot. Its gradient is ozb_expert_combine without weights. */
-int ozb_expert_gather(int R, int H, const void *X, int type, long long ldx, int T, const int *slots, int top, void *Y, long long ldy, void *stream);
+/* Y[rows[t][j]] = X[t] (T x H to R x H), zeros in the rows whose slots[r] is none: `rows` and `slots` are each other's inverse, as
+ * ozb_expert_sort makes them. The gradient is ozb_expert_combine without weights. */
+int ozb_expert_gather(int T, int top, int H, const void *X, int type, long long ldx, int R, const int *rows, const int *slots, void *Y,
+                      long long ldy, void *stream);
 /* Y[t] = sum over j of weights[t][j] Z[rows[t][j]] (weights NULL: 1), in FP32 in the order of j; dropped slots count nothing. */
 int ozb_expert_combine(int T, int top, int H, const void *Z, int type, int R, long long ldz, const int *rows, const float *weights, void *Y,
                        long long ldy, void *stream);

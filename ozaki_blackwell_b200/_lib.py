@@ -73,7 +73,7 @@ lib.ozb_expert_sort_rows.argtypes = [_i] * 4
 lib.ozb_expert_sort_scratch.restype = _sz
 lib.ozb_expert_sort_scratch.argtypes = [_i] * 3
 lib.ozb_expert_sort.argtypes = [_i] * 3 + [_p, _i, _i, _i, _p, _p, _p, _p, _sz, _p]
-lib.ozb_expert_gather.argtypes = [_i, _i, _p, _i, _ll, _i, _p, _i, _p, _ll, _p]
+lib.ozb_expert_gather.argtypes = [_i] * 3 + [_p, _i, _ll, _i, _p, _p, _p, _ll, _p]
 lib.ozb_expert_combine.argtypes = [_i] * 3 + [_p, _i, _i, _ll, _p, _p, _p, _ll, _p]
 lib.ozb_expert_combine_grad.argtypes = [_i] * 3 + [_p, _i, _ll, _p, _ll, _i, _p, _p, _p, _p, _ll, _p, _p]
 lib.ozb_int8_peak.argtypes = [_i, _i, ctypes.POINTER(ctypes.c_float), ctypes.POINTER(ctypes.c_double)]

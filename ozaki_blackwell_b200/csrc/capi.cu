@@ -937,12 +937,13 @@ OZB_API int ozb_expert_sort(int T, int top, int experts, const void *ids, int id
     if (int e = check_device()) return e;
     return (int)expert_sort(T * top, experts, ids, id_bytes, align, R, offsets, rows, slots, scratch, (cudaStream_t)stream);
 }
-OZB_API int ozb_expert_gather(int R, int H, const void *X, int type, long long ldx, int T, const int *slots, int top, void *Y, long long ldy, void *stream) {
-    if (R <= 0 || H <= 0 || H > MAX_LEN || bad_slots(T, top) || !X || !Y || !slots || X == Y || bad_type(type) || off_type(X, type) || off_type(Y, type) ||
-        off(slots, 4) || ldx < H || ldy < H)
+OZB_API int ozb_expert_gather(int T, int top, int H, const void *X, int type, long long ldx, int R, const int *rows, const int *slots, void *Y,
+                              long long ldy, void *stream) {
+    if (R <= 0 || H <= 0 || H > MAX_LEN || bad_slots(T, top) || !X || !Y || !rows || !slots || X == Y || bad_type(type) || off_type(X, type) ||
+        off_type(Y, type) || off(rows, 4) || off(slots, 4) || ldx < H || ldy < H)
         return OZB_EARG;
     if (int e = check_device()) return e;
-    return (int)expert_gather(R, H, X, type, ldx, T, slots, top, Y, ldy, (cudaStream_t)stream);
+    return (int)expert_gather(T, top, H, X, type, ldx, R, rows, slots, Y, ldy, (cudaStream_t)stream);
 }
 OZB_API int ozb_expert_combine(int T, int top, int H, const void *Z, int type, int R, long long ldz, const int *rows, const float *weights, void *Y,
                                long long ldy, void *stream) {

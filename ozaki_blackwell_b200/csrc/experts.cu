@@ -3,7 +3,7 @@
 // A token t of T goes to `top` experts; slot s = t * top + j is its j-th choice, ids[s] the expert (any number outside 0 .. E-1: the
 // slot is dropped). sort puts the slots in the order of their experts, stable, each expert's segment padded to a multiple of
 // `align` rows: row_of[s] and its inverse slot_of[r] (-1: none). With them
-//     gather        xs[r] = x[slot_of[r] / top]                      (zeros where there is no slot)
+//     gather        xs[row_of[t, j]] = x[t]                          (zeros where there is no slot)
 //     combine       y[t] = sum_j w[t, j] z[row_of[t, j]]             (in FP32, in the order of j)
 //     its gradient  dz[r] = w[s] dy[s / top],  dw[s] = <dy[s / top], z[row_of[s]]>
 // and the gradient of gather is combine without weights. An index that is out of range counts as none: nothing is read or
@@ -151,17 +151,20 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_place(const void *ids, int 
     for (int e = threadIdx.x; e < experts; e += SORT_THREADS) sh.total[e] = sh.before[e] = 0;
     __syncthreads();
     // all chunks' counts, eight loads in flight to a thread
-    const int n = gridDim.x * experts, own = blockIdx.x * experts;
+    const int n = gridDim.x * experts, own = blockIdx.x * experts, step = SORT_THREADS % experts;
+    int e = threadIdx.x % experts;
     for (int i0 = threadIdx.x; i0 < n; i0 += 8 * SORT_THREADS) {
         int c[8];
 #pragma unroll
         for (int k = 0; k < 8; k++) c[k] = i0 + k * SORT_THREADS < n ? __ldg(counts + i0 + k * SORT_THREADS) : 0;
 #pragma unroll
         for (int k = 0; k < 8; k++) {
-            const int i = i0 + k * SORT_THREADS;
-            if (!c[k]) continue;
-            atomicAdd(&sh.total[i % experts], c[k]);
-            if (i < own) atomicAdd(&sh.before[i % experts], c[k]);
+            if (c[k]) {
+                atomicAdd(&sh.total[e], c[k]);
+                if (i0 + k * SORT_THREADS < own) atomicAdd(&sh.before[e], c[k]);
+            }
+            e += step;
+            if (e >= experts) e -= experts;
         }
     }
     __syncthreads();
@@ -176,24 +179,35 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_place(const void *ids, int 
     }
 }
 
-// Rows move as they are: 16 bytes to a lane and load, four loads in flight, or single elements where rows do not start on 16 bytes.
+// A warp reads a piece of a token's row once and writes it to the rows of all its slots; other warps clear the rows without a slot. Rows
+// move as they are: 16 bytes to a lane and load, four loads in flight, or single elements where rows do not start on 16 bytes. (Row by
+// row, the tokens were read again from HBM for most of their slots: 824 MB for 605 at 16384 x 8 rows of 4 KB.)
 template <class E>
-__global__ void __launch_bounds__(256) gather_rows(const E *X, long long pitch_x, const int *slot_of, int top, int T, int R, int n, E *Y, long long pitch_y) {
+__global__ void __launch_bounds__(256) gather_rows(const E *X, long long pitch_x, const int *row_of, const int *slot_of, int top, int T, int R, int n, E *Y,
+                                                   long long pitch_y) {
     constexpr int DEPTH = 4;
     const int lane = threadIdx.x & 31, pieces = (n + 32 * DEPTH - 1) / (32 * DEPTH);
-    const long long total = (long long)R * pieces;
+    const long long total = ((long long)T + R) * pieces, slots = (long long)T * top;
     for (long long w = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); w < total; w += (long long)gridDim.x * 8) {
-        const int r = (int)(w / pieces), c0 = (int)(w - (long long)r * pieces) * 32 * DEPTH + lane;
-        const int s = __ldg(slot_of + r), t = s >= 0 ? s / top : -1;
-        E v[DEPTH];
+        const long long job = w / pieces;
+        const int c0 = (int)(w - job * pieces) * 32 * DEPTH + lane;
+        auto write = [&](long long r, const E (&v)[DEPTH]) {
 #pragma unroll
-        for (int i = 0; i < DEPTH; i++) {
-            v[i] = E();
-            if (t >= 0 && t < T && c0 + 32 * i < n) v[i] = __ldg(X + (size_t)t * pitch_x + c0 + 32 * i);
+            for (int i = 0; i < DEPTH; i++)
+                if (c0 + 32 * i < n) __stcs(Y + r * pitch_y + c0 + 32 * i, v[i]);
+        };
+        E v[DEPTH] = {};
+        if (job < T) {
+#pragma unroll
+            for (int i = 0; i < DEPTH; i++) v[i] = __ldg(X + job * pitch_x + min(c0 + 32 * i, n - 1));
+            for (int j = 0; j < top; j++) {
+                const int r = __ldg(row_of + job * top + j);
+                if (r >= 0 && r < R) write(r, v);
+            }
+        } else {
+            const int s = __ldg(slot_of + (job - T));
+            if (s < 0 || s >= slots) write(job - T, v);
         }
-#pragma unroll
-        for (int i = 0; i < DEPTH; i++)
-            if (c0 + 32 * i < n) __stcs(Y + (size_t)r * pitch_y + c0 + 32 * i, v[i]);   // written once: the tokens' rows stay in L2 instead
     }
 }
 
@@ -301,6 +315,15 @@ __global__ void __launch_bounds__(256) combine_grad_rows(const T *dY, long long 
                 }
             }
         }
+        if constexpr (VEC) {
+            for (; c0 + 32 * N <= H; c0 += 32 * N) {
+                float a[N], b[N];
+                Vec16<T>::unpack(__ldg(reinterpret_cast<const uint4 *>(dy + c0 + lane * N)), a);
+                Vec16<T>::unpack(__ldcs(reinterpret_cast<const uint4 *>(z + c0 + lane * N)), b);
+                use(a, b);
+                __stcs(reinterpret_cast<uint4 *>(dz + c0 + lane * N), Vec16<T>::pack(a));
+            }
+        }
         for (int c = c0 + lane; c < H; c += 32) {   // what is left, or rows that do not start on 16 bytes: single columns
             const float a = to_f32<T>(dy[c]);
             dot = fmaf(a, to_f32<T>(z[c]), dot);
@@ -334,17 +357,17 @@ cudaError_t expert_sort(int slots, int experts, const void *ids, int id_bytes, i
     return cudaGetLastError();
 }
 
-cudaError_t expert_gather(int R, int H, const void *X, int type, long long ldx, int T, const int *slots, int top, void *Y, long long ldy,
-                          cudaStream_t st) {
+cudaError_t expert_gather(int T, int top, int H, const void *X, int type, long long ldx, int R, const int *rows, const int *slots, void *Y,
+                          long long ldy, cudaStream_t st) {
     const int size = type_size(type);
-    auto grid = [&](int n) { return grid_of(((long long)R * ((n + 127) / 128) + 7) / 8); };
+    auto grid = [&](int n) { return grid_of((((long long)T + R) * ((n + 127) / 128) + 7) / 8); };
     if (aligned(X, ldx, size) && aligned(Y, ldy, size) && !((long long)H * size & 15)) {
         const int n = H * size / 16;
-        gather_rows<uint4><<<grid(n), 256, 0, st>>>((const uint4 *)X, ldx * size / 16, slots, top, T, R, n, (uint4 *)Y, ldy * size / 16);
+        gather_rows<uint4><<<grid(n), 256, 0, st>>>((const uint4 *)X, ldx * size / 16, rows, slots, top, T, R, n, (uint4 *)Y, ldy * size / 16);
     } else if (size == 4) {
-        gather_rows<uint32_t><<<grid(H), 256, 0, st>>>((const uint32_t *)X, ldx, slots, top, T, R, H, (uint32_t *)Y, ldy);
+        gather_rows<uint32_t><<<grid(H), 256, 0, st>>>((const uint32_t *)X, ldx, rows, slots, top, T, R, H, (uint32_t *)Y, ldy);
     } else {
-        gather_rows<uint16_t><<<grid(H), 256, 0, st>>>((const uint16_t *)X, ldx, slots, top, T, R, H, (uint16_t *)Y, ldy);
+        gather_rows<uint16_t><<<grid(H), 256, 0, st>>>((const uint16_t *)X, ldx, rows, slots, top, T, R, H, (uint16_t *)Y, ldy);
     }
     return cudaGetLastError();
 }

@@ -67,61 +67,89 @@ __device__ __forceinline__ long long source_row(const int *slots, int per, int s
     return row < sources ? row : -1;
 }
 
+// The largest magnitude of 16 values held in 16-byte words, as the bits of a float: two 16-bit values at a time (a magnitude's bits
+// order like the number, infinities and NaN above all).
+template <class T> __device__ __forceinline__ uint32_t magnitude_of(const uint4 *q) {
+    const uint32_t *w = reinterpret_cast<const uint32_t *>(q);
+    uint32_t m = 0;
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < 16; i++) m = max(m, w[i] & 0x7fffffffu);
+        return m;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) m = __vmaxu2(m, w[i] & 0x7fff7fffu);
+        m = max(m & 0xffffu, m >> 16);
+        return magnitude(to_f32<T>(reinterpret_cast<const T *>(&m)[0]));
+    }
+}
+
 // Blocks along the rows of X. A lane holds 16 values, two lanes a block; a warp takes 512 values of one row, so that its loads are
-// 512 or 1024 bytes in a piece and its stores 256. Bound by HBM: the codes leave as 8-byte words, the scales as bytes.
+// 512 or 1024 bytes in a piece and its stores 256. `share` warps (a power of two) work on one row. The kernel is nearer to the limit
+// of instruction issue than to HBM's, so magnitudes are compared and values scaled two at a time.
 template <class T, bool VEC>
 __global__ void __launch_bounds__(256) mx4_rows(const T *X, int nvec, int len, long long ldx, size_t plane_x, int planes, int rule,
                                                 const int *slots, int per, int sources, uint8_t *codes, long long ldq, size_t plane_q,
-                                                uint8_t *scales, long long lds, size_t plane_s) {
-    __shared__ float turn[8][32 * 17];
-    const int lane = threadIdx.x & 31;
-    const int pieces = (len + 511) / 512;
-    const long long total = (long long)planes * nvec * pieces;
-    for (long long w = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); w < total; w += (long long)gridDim.x * 8) {
-        const long long vec = w / pieces;
-        const int i0 = (int)(w - vec * pieces) * 512 + lane * 16;
-        const int z = (int)(vec / nvec), r = (int)(vec - (long long)z * nvec);
-        const long long src = source_row(slots, per, sources, r);
-        const int at = i0 - lane * 16;
-        float v[16];
-        if (VEC && at + 512 <= len) {
-            constexpr int N = Vec16<T>::N;
-            uint4 q[16 / N] = {};
-            if (src >= 0) {
-                const uint4 *x = reinterpret_cast<const uint4 *>(X + (size_t)z * plane_x + (size_t)src * ldx + i0);
+                                                uint8_t *scales, long long lds, size_t plane_s, int share_log) {
+    __shared__ float turn[VEC ? 1 : 8][32 * 17];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = warp & ((1 << share_log) - 1);
+    const long long total = (long long)planes * nvec;
+    for (long long vec = ((long long)blockIdx.x << (3 - share_log)) + (warp >> share_log); vec < total; vec += (long long)gridDim.x << (3 - share_log)) {
+        const long long z = planes > 1 ? vec / nvec : 0, r = vec - z * nvec;
+        const long long src = source_row(slots, per, sources, (int)r);
+        const T *x = X + z * plane_x + max(src, 0ll) * ldx;
+        uint8_t *c = codes + z * plane_q + r * ldq, *s = scales + z * plane_s + r * lds;
+        for (int at = part * 512; at < len; at += 512 << share_log) {
+            const int i0 = at + lane * 16;
+            float v[16];
+            uint32_t m;
+            if constexpr (VEC) {   // rows start on 16 bytes; a piece that does not exist is zero, the last one may be cut
+                constexpr int N = Vec16<T>::N;
+                uint4 q[16 / N] = {};
+                if (src >= 0) {
 #pragma unroll
-                for (int i = 0; i < 16 / N; i++) q[i] = __ldg(x + i);
+                    for (int i = 0; i < 16 / N; i++) {
+                        const int e = i0 + i * N;
+                        if (e + N <= len) q[i] = __ldg(reinterpret_cast<const uint4 *>(x + e));
+                        else if (e < len)
+                            for (int k = 0; e + k < len; k++) reinterpret_cast<T *>(&q[i])[k] = x[e + k];
+                    }
+                }
+                m = magnitude_of<T>(q);
+#pragma unroll
+                for (int i = 0; i < 16 / N; i++) Vec16<T>::unpack(q[i], v + i * N);
+            } else {   // lanes load side by side, and turn the values through shared memory
+                float *mine = turn[warp];
+                T raw[16];
+#pragma unroll
+                for (int i = 0; i < 16; i++) raw[i] = x[min(at + i * 32 + lane, len - 1)];
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    const int e = i * 32 + lane;
+                    mine[e + (e >> 4)] = src >= 0 && at + e < len ? to_f32<T>(raw[i]) : 0.f;
+                }
+                __syncwarp();
+                m = 0;
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    v[i] = mine[lane * 17 + i];
+                    m = max(m, magnitude(v[i]));
+                }
+                __syncwarp();
             }
+            m = max(m, __shfl_xor_sync(~0u, m, 1));
+            const uint32_t byte = scale_byte(m, rule), number = byte == 255 ? 0u : ~0u;
+            const float2 inv = make_float2(inverse_scale(byte), inverse_scale(byte));
 #pragma unroll
-            for (int i = 0; i < 16 / N; i++) Vec16<T>::unpack(q[i], v + i * N);
-        } else {   // rows that do not start on 16 bytes, and ends: lanes load side by side, and turn the values through shared memory
-            float *mine = turn[threadIdx.x >> 5];
-            const T *x = X + (size_t)z * plane_x + (size_t)max(src, 0ll) * ldx + at;
-            T raw[16];
-#pragma unroll
-            for (int i = 0; i < 16; i++) raw[i] = x[min(i * 32 + lane, len - 1 - at)];
-#pragma unroll
-            for (int i = 0; i < 16; i++) {
-                const int e = i * 32 + lane;
-                mine[e + (e >> 4)] = src >= 0 && at + e < len ? to_f32<T>(raw[i]) : 0.f;
+            for (int i = 0; i < 16; i += 2) {
+                const float2 f = __fmul2_rn(make_float2(v[i], v[i + 1]), inv);
+                v[i] = f.x;
+                v[i + 1] = f.y;
             }
-            __syncwarp();
-#pragma unroll
-            for (int i = 0; i < 16; i++) v[i] = mine[lane * 17 + i];
-            __syncwarp();
-        }
-        uint32_t m = 0;
-#pragma unroll
-        for (int i = 0; i < 16; i++) m = max(m, magnitude(v[i]));
-        m = max(m, __shfl_xor_sync(~0u, m, 1));
-        const uint32_t byte = scale_byte(m, rule);
-        const float inv = inverse_scale(byte);
-#pragma unroll
-        for (int i = 0; i < 16; i++) v[i] *= inv;
-        if ((i0 & ~31) < len) {   // the block exists: its codes are written whole, zeros behind the last value
-            const uint32_t number = byte == 255 ? 0u : ~0u;
-            *reinterpret_cast<uint2 *>(codes + (size_t)z * plane_q + (size_t)r * ldq + (i0 >> 1)) = make_uint2(codes_of(v) & number, codes_of(v + 8) & number);
-            if (!(lane & 1)) scales[(size_t)z * plane_s + (size_t)r * lds + (i0 >> 5)] = (uint8_t)byte;
+            if ((i0 & ~31) < len) {   // the block exists: its codes are written whole, zeros behind the last value
+                *reinterpret_cast<uint2 *>(c + (i0 >> 1)) = make_uint2(codes_of(v) & number, codes_of(v + 8) & number);
+                if (!(lane & 1)) s[i0 >> 5] = (uint8_t)byte;
+            }
         }
     }
 }
@@ -243,11 +271,13 @@ cudaError_t mx4_quantize_rows(const void *X, int type, int nvec, int len, long l
                               size_t plane_s, cudaStream_t st) {
     const int size = type_size(type);
     const bool vec = !(reinterpret_cast<uintptr_t>(X) & 15) && !(ldx * size & 15) && !(plane_x * size & 15);
-    const int grid = warp_grid((long long)planes * nvec * ((len + 511) / 512));
+    int share_log = 0;   // warps to a row: as many as it has pieces, up to eight
+    while (share_log < 3 && (512 << share_log) < len) share_log++;
+    const int grid = warp_grid(((long long)planes * nvec) << share_log);
     with_type(type, [&](auto t) {
         using T = decltype(t);
-        if (vec) mx4_rows<T, true><<<grid, 256, 0, st>>>((const T *)X, nvec, len, ldx, plane_x, planes, rule, slots, per, sources, codes, ldq, plane_q, scales, lds, plane_s);
-        else mx4_rows<T, false><<<grid, 256, 0, st>>>((const T *)X, nvec, len, ldx, plane_x, planes, rule, slots, per, sources, codes, ldq, plane_q, scales, lds, plane_s);
+        if (vec) mx4_rows<T, true><<<grid, 256, 0, st>>>((const T *)X, nvec, len, ldx, plane_x, planes, rule, slots, per, sources, codes, ldq, plane_q, scales, lds, plane_s, share_log);
+        else mx4_rows<T, false><<<grid, 256, 0, st>>>((const T *)X, nvec, len, ldx, plane_x, planes, rule, slots, per, sources, codes, ldq, plane_q, scales, lds, plane_s, share_log);
     });
     return cudaGetLastError();
 }

@@ -17,7 +17,8 @@
 //              and writes the 4 x 4 words turned: four 16-byte loads and stores for 128 rows by 512 values, without bank conflicts.
 //   warp 2     one thread; tcgen05.cp of a stage's turned scales into tensor memory, its completion counted by the stage's barrier
 //   warp 1     issuer: one thread; four tcgen05.mma kind::mxf4 (K = 64) to a stage
-//   warps 4-7  epilogue: tensor memory to registers to global memory, while the next tile accumulates
+//   warps 4-7, 12-15  epilogue: tensor memory to registers to global memory, 32 columns at a time in turns, while the next tile
+//              accumulates
 // An instruction of tcgen05 takes 20 to 60 cycles to issue, whatever it does; with the four to six copies of a stage's scales in
 // the thread that issues its four products the tensor pipe waited, so the copies have a thread of their own. Bringing the scale
 // bytes by TMA was slower: boxes 16 bytes wide cost the TMA unit as much for a row as the 128 bytes of its codes (900 cycles a slot).
@@ -42,7 +43,7 @@ namespace m4 {
 constexpr int BP = 128;            // rows of P to a CTA
 constexpr int BK = 256, BKB = 128; // k of a stage, in values and in bytes
 constexpr int UK = 64;             // k of one tcgen05.mma kind::mxf4
-constexpr int TURNERS = 4, THREADS = 256 + 32 * (TURNERS - 1);
+constexpr int TURNERS = 4, THREADS = 512;   // warp 11 is idle: the epilogue's second four must be warps 0 .. 3 modulo 4
 constexpr int MAX_GROUPS = 1024;
 
 enum { DENSE = 0, BY_ROWS = 1, ALONG_K = 2 };
@@ -74,11 +75,11 @@ template <int FORM, int BN> struct Shape {
     static constexpr int STAGES = pair ? 5 : BN <= 32 ? 8 : BN <= 64 ? 7 : BN <= 128 ? 5 : 4;
     // A multiple of the turning warps, so that a slot is always the same warp's: a warp that came to a slot before another had seen the
     // slot's last use would take the parity of the use before that for its own.
-    static constexpr int SLOTS = 2 * TURNERS;
+    static constexpr int SLOTS = FORM == WIDE ? TURNERS : 2 * TURNERS;
     static constexpr int COLS = 2 * BN + STAGES * SCALE_COLS;      // two accumulators, and the scales
     static constexpr int TMEM_COLS = COLS <= 256 ? 256 : 512;
     static constexpr int BARS = 2 * STAGES + 2 * SLOTS + 4;
-    static constexpr int TURN = wide ? 4 * 32 * (64 + 16) : 0;     // what the epilogue's warps turn their tiles through
+    static constexpr int TURN = wide ? 8 * 32 * (64 + 16) : 0;     // what the epilogue's warps turn their tiles through
     static constexpr int SMEM = STAGES * STAGE + SLOTS * SLOT + TURN + 1024 + 8 * BARS + 16 + 4 * (MAX_GROUPS + 1);
     static_assert(STAGE % 1024 == 0 && COLS <= 512 && SMEM <= 232448 - 64, "");
     static_assert(FORM != SPLIT || BN * BP * 4 <= STAGES * STAGE, "the partial tile of a split takes the place of the stages");
@@ -252,7 +253,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm(const __grid_constant__ C
         abort_flag = 0;
         for (int s = 0; s < S::STAGES; s++) { mbar_init(full_bar(s), 2); mbar_init(empty_bar(s), 1); }
         for (int s = 0; s < S::SLOTS; s++) { mbar_init(turned_bar(s), pair ? 2 : 1); mbar_init(slot_bar(s), 1); }
-        for (int a = 0; a < 2; a++) { mbar_init(accfull_bar(a), 1); mbar_init(accempty_bar(a), pair ? 8 : 4); }
+        for (int a = 0; a < 2; a++) { mbar_init(accfull_bar(a), 1); mbar_init(accempty_bar(a), pair ? 16 : 8); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
@@ -439,9 +440,9 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm(const __grid_constant__ C
                 if (!ok) break;
             }
         }
-    } else if (warp < 4 || warp >= 8) {
+    } else if (warp == 3 || (warp >= 8 && warp < 7 + TURNERS)) {
         // of TURNERS warps, in turns of a slot: while one waits for its slot's bytes, the others do theirs
-        const uint32_t own = warp < 4 ? 0 : warp - 7;
+        const uint32_t own = warp == 3 ? 0 : warp - 7;
         const int blocks = (p.K + 31) / 32;
         for (int w = first; w < total && !__any_sync(~0u, *abortp); w += step) {
             const Tile t = tile_at(w);
@@ -493,8 +494,8 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm(const __grid_constant__ C
             }
             if (!ok) break;
         }
-    } else {
-        const int quarter = warp & 3;
+    } else if (warp != 11) {
+        const int quarter = warp & 3, half = warp >= 12;   // lanes 32 quarter .. +31, every other 32 columns
         uint32_t n = 0;
         for (int w = first; w < total && !__any_sync(~0u, *abortp); w += step, n++) {
             const Tile t = tile_at(w);
@@ -507,7 +508,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm(const __grid_constant__ C
             if constexpr (FORM != SPLIT) {
                 T *Y = reinterpret_cast<T *>(p.Y) + (p.mode == ALONG_K ? (size_t)t.group * p.plane_y : 0);
 #pragma unroll 1
-                for (int c = 0; c < BN; c += 32) {
+                for (int c = 32 * half; c < BN; c += 64) {
                     if (t.q0 + c >= t.q1) break;
                     uint32_t v[32];
                     tmem_ld32(taddr + c, v);
@@ -517,13 +518,13 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm(const __grid_constant__ C
                         for (int e = 0; e < 32; e++) v[e] = 0;
                     }
                     const int j1 = min(t.q1, t.q0 + BN);   // a tile of 16 columns: the other 16 are not its own
-                    if constexpr (S::wide) store_wide<T>(Y, p.ldy, v, i0, lane, t.p1, t.q0 + c, j1, base_ptr + S::STAGES * S::STAGE + S::SLOTS * S::SLOT + quarter * TURN_BYTES);
+                    if constexpr (S::wide) store_wide<T>(Y, p.ldy, v, i0, lane, t.p1, t.q0 + c, j1, base_ptr + S::STAGES * S::STAGE + S::SLOTS * S::SLOT + (quarter + 4 * half) * TURN_BYTES);
                     else store_narrow<T>(Y, p.ldy, v, i0 + lane, t.p1, t.q0 + c, j1);
                 }
             } else {   // the partial tile, [column][row of P], over the stages that this CTA has used up
                 float *part = reinterpret_cast<float *>(base_ptr);
 #pragma unroll 1
-                for (int c = 0; c < BN; c += 32) {
+                for (int c = 32 * half; c < BN; c += 64) {
                     uint32_t v[32];
                     tmem_ld32(taddr + c, v);
                     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
@@ -551,7 +552,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm(const __grid_constant__ C
             T *Y = reinterpret_cast<T *>(p.Y) + (p.mode == ALONG_K ? (size_t)t.group * p.plane_y : 0);
             const int r = threadIdx.x & (BP - 1), i = t.p0 + r;
             const int n = min(BN, t.q1 - t.q0), c0 = (int)((long long)n * rank / ranks), c1 = (int)((long long)n * (rank + 1) / ranks);
-            for (int c = c0 + (threadIdx.x >> 7); c < c1 && threadIdx.x < 2 * BP; c += 2) {
+            for (int c = c0 + (threadIdx.x >> 7); c < c1; c += THREADS / BP) {
                 float sum = 0.f;
                 for (uint32_t q = 0; q < ranks; q++) {
                     float x;

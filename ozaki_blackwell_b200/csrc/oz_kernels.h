@@ -81,8 +81,8 @@ cudaError_t mx4_product(const Mx4Product &g, int *status, cudaStream_t st);
 size_t expert_sort_scratch(int slots, int experts);
 cudaError_t expert_sort(int slots, int experts, const void *ids, int id_bytes, int align, int R, int *offsets, int *rows, int *slot_of, void *scratch,
                         cudaStream_t st);
-cudaError_t expert_gather(int R, int H, const void *X, int type, long long ldx, int T, const int *slots, int top, void *Y, long long ldy,
-                          cudaStream_t st);
+cudaError_t expert_gather(int T, int top, int H, const void *X, int type, long long ldx, int R, const int *rows, const int *slots, void *Y,
+                          long long ldy, cudaStream_t st);
 cudaError_t expert_combine(int T, int top, int H, const void *Z, int type, int R, long long ldz, const int *rows, const float *weights, void *Y,
                            long long ldy, cudaStream_t st);
 cudaError_t expert_combine_grad(int T, int top, int H, const void *dY, int type, long long lddy, const void *Z, long long ldz, int R, const int *rows,

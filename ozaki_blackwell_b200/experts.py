@@ -65,7 +65,7 @@ def gather(x, routing, out=None):
         raise ValueError(f"x has {x.shape[0]} rows, the routing {tokens} tokens")
     kind, r, h = _type(x.dtype), routing.slots.shape[0], x.shape[1]
     y, ldy = _result(x, out, (r, h), x.dtype)
-    _call(index, _lib.ozb_expert_gather, r, h, x.data_ptr(), kind, ldx, tokens, routing.slots.data_ptr(), top, y.data_ptr(), ldy)
+    _call(index, _lib.ozb_expert_gather, tokens, top, h, x.data_ptr(), kind, ldx, r, routing.rows.data_ptr(), routing.slots.data_ptr(), y.data_ptr(), ldy)
     return y
 
 

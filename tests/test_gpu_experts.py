@@ -128,16 +128,17 @@ def test_indices_out_of_range_are_none():
     ex = _experts()
     tokens, top, h = 6, 2, 72
     z, dy = torch.randn(5, h, device="cuda"), torch.randn(tokens, h, device="cuda")
-    rows = torch.tensor([[0, 5], [-3, 2 ** 31 - 1], [4, 1], [-2 ** 31, 9], [2, 3], [6, -1]], dtype=torch.int32, device="cuda")
+    rows = torch.tensor([[0, 5], [-3, 2 ** 31 - 1], [-1, 1], [-2 ** 31, 9], [-1, 2 ** 30], [6, -1]], dtype=torch.int32, device="cuda")
     slots = torch.tensor([0, 5, 12, 2 ** 31 - 1, -2 ** 31], dtype=torch.int32, device="cuda")
     r = ex.Routing(torch.zeros(2, dtype=torch.int32, device="cuda"), rows, slots)
     y = ex.combine(z, r)
-    assert torch.equal(y[0], z[0]) and torch.equal(y[2], z[4] + z[1]) and bool((y[[1, 3, 5]] == 0).all())
-    x = ex.gather(dy, r)
-    assert torch.equal(x[0], dy[0]) and torch.equal(x[1], dy[2]) and bool((x[2:] == 0).all())
+    assert torch.equal(y[0], z[0]) and torch.equal(y[2], z[1]) and bool((y[[1, 3, 4, 5]] == 0).all())
+    guard = torch.full((7, h), 5.0, device="cuda")
+    x = ex.gather(dy, r, out=guard[1:6])
+    assert torch.equal(x[0], dy[0]) and torch.equal(x[1], dy[2]) and bool((x[2:] == 0).all()) and bool((guard[[0, 6]] == 5).all())
     dz, dw = ex.combine_grad(dy, z, r)
     assert torch.equal(dz[0], dy[0]) and torch.equal(dz[1], dy[2]) and bool((dz[2:] == 0).all())
-    assert bool((dw[[0, 1, 3, 5], [1, 0, 1, 0]] == 0).all())
+    assert bool((dw[[0, 1, 3, 4, 5], [1, 0, 1, 0, 0]] == 0).all())
 
 
 def _layer(x, w, ids, weights, z_type):

@@ -64,9 +64,9 @@ def test_sort():
 
 
 def test_rows():
-    base = dict(R=6, H=8, X=P, type=0, ldx=8, T=3, slots=P, top=2, Y=ctypes.c_void_p(8192), ldy=8)
+    base = dict(T=3, top=2, H=8, X=P, type=0, ldx=8, R=6, rows=P, slots=P, Y=ctypes.c_void_p(8192), ldy=8)
     call = lambda **b: lib.ozb_expert_gather(*{**base, **b}.values(), None)  # noqa: E731
-    for bad in (dict(R=0), dict(H=0), dict(X=None), dict(type=5), dict(ldx=7), dict(T=0), dict(slots=None), dict(top=0), dict(Y=None), dict(Y=P), dict(ldy=7)):
+    for bad in (dict(R=0), dict(H=0), dict(X=None), dict(type=5), dict(ldx=7), dict(T=0), dict(rows=None), dict(slots=None), dict(top=0), dict(Y=None), dict(Y=P), dict(ldy=7)):
         assert call(**bad) == ARG, bad
     base = dict(T=3, top=2, H=8, Z=P, type=0, R=6, ldz=8, rows=P, weights=None, Y=ctypes.c_void_p(8192), ldy=8)
     call = lambda **b: lib.ozb_expert_combine(*{**base, **b}.values(), None)  # noqa: E731
