@@ -228,12 +228,12 @@ enum { OZB_F32 = 0, OZB_BF16 = 1, OZB_F16 = 2 };
  * ozb_mx4_quantize: `nvec` vectors of `len` values of X to that format, nearest code, ties to the even one. by_rows = 1: the rows of
  * X (pitch ldx); by_rows = 0: the columns of a row-major len x nvec X, which come out as rows. rule 0: the block's scale is
  * 2^(floor(log2 amax) - 2), values above 6 of it saturate; rule 1: the smallest power of two with amax <= 6 of it. Scales stay
- * within 2^-127 .. 2^127. A block that holds an infinity or a NaN gets s = 255 and codes 0. `slots` (may be NULL) takes the
- * rows of X through the map of ozb_expert_sort: row r of the matrix that is quantised is row slots[r] / per of X, or zeros where
- * slots[r] is negative or the row is not below `sources`. planes > 1 (without slots): that many matrices, plane_x elements,
+ * within 2^-127 .. 2^127. A block that holds an infinity or a NaN gets s = 255 and codes 0. `rows` and `slots` (both
+ * NULL, or the maps of ozb_expert_sort for `tokens` tokens of `top` slots) put the rows of X (tokens x ..) in the order of their
+ * experts first, as ozb_expert_gather does: nvec (by_rows = 1) or len (by_rows = 0) is then the number of sorted rows. planes > 1 (without the maps): that many matrices, plane_x elements,
  * plane_q and plane_s bytes apart (multiples of 16). The gradient is passed through (straight-through), no call needed. */
-int ozb_mx4_quantize(const void *X, int type, int nvec, int len, long long ldx, int by_rows, int rule, const int *slots, int per, int sources,
-                     int planes, size_t plane_x, uint8_t *codes, long long ldq, size_t plane_q, uint8_t *scales, long long lds,
+int ozb_mx4_quantize(const void *X, int type, int nvec, int len, long long ldx, int by_rows, int rule, const int *rows, const int *slots, int top,
+                     int tokens, int planes, size_t plane_x, uint8_t *codes, long long ldq, size_t plane_q, uint8_t *scales, long long lds,
                      size_t plane_s, void *stream);
 /* the values that codes and scales stand for, rounded to `type` (exact in FP32 and BF16); NaN for a block with s = 255 */
 int ozb_mx4_dequantize(const uint8_t *codes, long long ldq, const uint8_t *scales, long long lds, int nvec, int len, void *Y, int type,

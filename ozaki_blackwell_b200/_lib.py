@@ -63,7 +63,7 @@ lib.ozb_gemm_i8_mod.argtypes = [_p, _p, _p, _i, _i, _i, _i, _ll, _ll, _ll, _sz, 
 lib.ozb_gemm_i8_mod_beside.argtypes = [_p, _p, _p, _i, _i, _i, _i, _ll, _ll, _ll, _sz, _sz, _sz, _i, _i, _p, _p]
 lib.ozb_crt_i32.argtypes = [_i, _p, _sz, _i, _i, _ll, _p, _p, _p, _ll, _p]
 lib.ozb_crt_i8.argtypes = [_i, _p, _sz, _i, _i, _ll, _p, _p, _p, _ll, _p]
-lib.ozb_mx4_quantize.argtypes = [_p, _i, _i, _i, _ll, _i, _i, _p, _i, _i, _i, _sz, _p, _ll, _sz, _p, _ll, _sz, _p]
+lib.ozb_mx4_quantize.argtypes = [_p, _i, _i, _i, _ll, _i, _i, _p, _p, _i, _i, _i, _sz, _p, _ll, _sz, _p, _ll, _sz, _p]
 lib.ozb_mx4_dequantize.argtypes = [_p, _ll, _p, _ll, _i, _i, _p, _i, _ll, _p]
 lib.ozb_mx4_gemm.argtypes = [_i] * 3 + [_p, _ll] * 4 + [_p, _i, _ll, _p]
 lib.ozb_mx4_gemm_grouped.argtypes = [_i] * 4 + [_p] + [_p, _ll] * 2 + [_p, _ll, _sz] * 2 + [_p, _i, _ll, _p]

@@ -440,6 +440,7 @@ bool bad_mx4(const void *codes, long long ldq, const void *scales, long long lds
            lds < ((long long)len + 31) / 32;
 }
 constexpr int MAX_LEN = 0x7fffffff - 1023;   // lengths are rounded up in 32 bits
+bool bad_slots(int T, int top) { return T <= 0 || top <= 0 || (long long)T * top > MAX_LEN; }
 bool bad_type(int type) { return type < OZB_F32 || type > OZB_F16; }
 bool off_type(const void *p, int type) { return off(p, type == OZB_F32 ? 4 : 2); }
 }  // namespace
@@ -859,18 +860,20 @@ OZB_API int ozb_bf16_fp8_gemm(int M, int N, int K, const void *X, const void *W,
 }
 
 // ---- microscaled 4-bit format -------------------------------------------------------------------------------------
-OZB_API int ozb_mx4_quantize(const void *X, int type, int nvec, int len, long long ldx, int by_rows, int rule, const int *slots, int per, int sources,
-                             int planes, size_t plane_x, uint8_t *codes, long long ldq, size_t plane_q, uint8_t *scales, long long lds,
+OZB_API int ozb_mx4_quantize(const void *X, int type, int nvec, int len, long long ldx, int by_rows, int rule, const int *rows, const int *slots, int top,
+                             int tokens, int planes, size_t plane_x, uint8_t *codes, long long ldq, size_t plane_q, uint8_t *scales, long long lds,
                              size_t plane_s, void *stream) {
     if (nvec <= 0 || len <= 0 || len > MAX_LEN || nvec > MAX_LEN || planes <= 0 || !X || bad_type(type) || off_type(X, type) || (rule != 0 && rule != 1) ||
         ldx < (by_rows ? len : nvec) || bad_mx4(codes, ldq, scales, lds, len))
         return OZB_EARG;
-    if (slots && (per <= 0 || sources <= 0 || planes > 1 || off(slots, 4))) return OZB_EARG;
+    if (!rows != !slots) return OZB_EARG;
+    if (slots && (bad_slots(tokens, top) || planes > 1 || off(slots, 4) || off(rows, 4))) return OZB_EARG;
     if (planes > 1 && ((plane_q & 15) || (plane_s & 15))) return OZB_EARG;
     if (int e = check_device()) return e;
     if (planes == 1) plane_x = plane_q = plane_s = 0;
-    return (int)(by_rows ? mx4_quantize_rows : mx4_quantize_cols)(X, type, nvec, len, ldx, plane_x, planes, rule, slots, per, sources, codes, ldq,
-                                                                 plane_q, scales, lds, plane_s, (cudaStream_t)stream);
+    const int e = (int)(by_rows ? mx4_quantize_rows : mx4_quantize_cols)(X, type, nvec, len, ldx, plane_x, planes, rule, rows, slots, top, tokens, codes, ldq,
+                                                                        plane_q, scales, lds, plane_s, (cudaStream_t)stream);
+    return e == (int)cudaErrorInvalidValue ? OZB_ESIZE : e;
 }
 OZB_API int ozb_mx4_dequantize(const uint8_t *codes, long long ldq, const uint8_t *scales, long long lds, int nvec, int len, void *Y, int type,
                                long long ldy, void *stream) {
@@ -915,7 +918,6 @@ OZB_API int ozb_mx4_gemm_segments(int groups, int M, int N, int R, const int *of
 static long long sorted_rows(long long slots, int experts, int align) {   // the most rows that the padded segments take
     return (slots + (slots < experts ? slots : experts) * (align - 1)) / align * align;
 }
-static bool bad_slots(int T, int top) { return T <= 0 || top <= 0 || (long long)T * top > MAX_LEN; }
 OZB_API long long ozb_expert_sort_rows(int T, int top, int experts, int align) {
     if (bad_slots(T, top) || experts <= 0 || experts > 1024 || align <= 0 || align > 256) return -OZB_EARG;
     return sorted_rows((long long)T * top, experts, align);

@@ -179,34 +179,40 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_place(const void *ids, int 
     }
 }
 
-// A warp reads a piece of a token's row once and writes it to the rows of all its slots; other warps clear the rows without a slot. Rows
-// move as they are: 16 bytes to a lane and load, four loads in flight, or single elements where rows do not start on 16 bytes. (Row by
-// row, the tokens were read again from HBM for most of their slots: 824 MB for 605 at 16384 x 8 rows of 4 KB.)
+// A warp reads a piece of a token's row once and writes it to the rows of all its slots; then it looks through 32 rows at a time for those
+// without a slot and clears them. Rows move as they are: 16 bytes to a lane and load, four loads in flight, or single elements where
+// rows do not start on 16 bytes. (Row by row, the tokens were read again from HBM for most of their slots: 824 MB for 605 at
+// 16384 x 8 rows of 4 KB.)
 template <class E>
 __global__ void __launch_bounds__(256) gather_rows(const E *X, long long pitch_x, const int *row_of, const int *slot_of, int top, int T, int R, int n, E *Y,
                                                    long long pitch_y) {
-    constexpr int DEPTH = 4;
-    const int lane = threadIdx.x & 31, pieces = (n + 32 * DEPTH - 1) / (32 * DEPTH);
-    const long long total = ((long long)T + R) * pieces, slots = (long long)T * top;
-    for (long long w = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); w < total; w += (long long)gridDim.x * 8) {
-        const long long job = w / pieces;
-        const int c0 = (int)(w - job * pieces) * 32 * DEPTH + lane;
-        auto write = [&](long long r, const E (&v)[DEPTH]) {
+    constexpr int DEPTH = 4, PIECE = 32 * DEPTH;
+    const int lane = threadIdx.x & 31, pieces = (n + PIECE - 1) / PIECE;
+    const long long warp = (long long)blockIdx.x * 8 + (threadIdx.x >> 5), warps = (long long)gridDim.x * 8, slots = (long long)T * top;
+    auto write = [&](long long r, int c0, const E (&v)[DEPTH]) {
 #pragma unroll
-            for (int i = 0; i < DEPTH; i++)
-                if (c0 + 32 * i < n) __stcs(Y + r * pitch_y + c0 + 32 * i, v[i]);
-        };
-        E v[DEPTH] = {};
-        if (job < T) {
+        for (int i = 0; i < DEPTH; i++)
+            if (c0 + 32 * i < n) __stcs(Y + r * pitch_y + c0 + 32 * i, v[i]);
+    };
+    for (long long w = warp; w < (long long)T * pieces; w += warps) {
+        const long long t = w / pieces;
+        const int c0 = (int)(w - t * pieces) * PIECE + lane;
+        E v[DEPTH];
 #pragma unroll
-            for (int i = 0; i < DEPTH; i++) v[i] = __ldg(X + job * pitch_x + min(c0 + 32 * i, n - 1));
-            for (int j = 0; j < top; j++) {
-                const int r = __ldg(row_of + job * top + j);
-                if (r >= 0 && r < R) write(r, v);
-            }
-        } else {
-            const int s = __ldg(slot_of + (job - T));
-            if (s < 0 || s >= slots) write(job - T, v);
+        for (int i = 0; i < DEPTH; i++) v[i] = __ldg(X + t * pitch_x + min(c0 + 32 * i, n - 1));
+        for (int j = 0; j < top; j++) {
+            const int r = __ldg(row_of + t * top + j);
+            if (r >= 0 && r < R) write(r, c0, v);
+        }
+    }
+    for (long long r0 = warp * 32; r0 < R; r0 += warps * 32) {
+        const int s = r0 + lane < R ? __ldg(slot_of + r0 + lane) : 0;
+        uint32_t none = __ballot_sync(~0u, s < 0 || s >= slots);
+        const E zero[DEPTH] = {};
+        while (none) {
+            const int i = __ffs(none) - 1;
+            none &= none - 1;
+            for (int c0 = lane; c0 < n; c0 += PIECE) write(r0 + i, c0, zero);
         }
     }
 }
@@ -360,7 +366,7 @@ cudaError_t expert_sort(int slots, int experts, const void *ids, int id_bytes, i
 cudaError_t expert_gather(int T, int top, int H, const void *X, int type, long long ldx, int R, const int *rows, const int *slots, void *Y,
                           long long ldy, cudaStream_t st) {
     const int size = type_size(type);
-    auto grid = [&](int n) { return grid_of((((long long)T + R) * ((n + 127) / 128) + 7) / 8); };
+    auto grid = [&](int n) { return grid_of(((long long)T * ((n + 127) / 128) + R / 32 + 7) / 8); };
     if (aligned(X, ldx, size) && aligned(Y, ldy, size) && !((long long)H * size & 15)) {
         const int n = H * size / 16;
         gather_rows<uint4><<<grid(n), 256, 0, st>>>((const uint4 *)X, ldx * size / 16, rows, slots, top, T, R, n, (uint4 *)Y, ldy * size / 16);

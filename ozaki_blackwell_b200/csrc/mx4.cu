@@ -8,6 +8,7 @@
 // stored as the byte e + 127, clamped at 0 (an empty block, or values below 2^-125); 255 marks a block that holds an infinity or a
 // NaN. x 2^-e is exact: it is below 8, and what falls below 2^-126 is rounded to the code of 0 either way. The rounding itself is
 // the hardware's conversion (cvt.rn.satfinite.e2m1x2.f32).
+#include <type_traits>
 #include "oz_common.cuh"
 #include "oz_kernels.h"
 #include "oz_types.cuh"
@@ -26,6 +27,16 @@ __device__ __forceinline__ uint32_t codes_of(const float *v) {
         "cvt.rn.satfinite.e2m1x2.f32 b3, %8, %7;\n\t"
         "mov.b32 %0, {b0, b1, b2, b3};\n\t}"
         : "=r"(r) : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
+    return r;
+}
+__device__ __forceinline__ uint32_t codes_of4(const float *v) {   // four
+    uint32_t r;
+    asm("{\n\t.reg .b8 b0, b1, z;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b1, %4, %3;\n\t"
+        "cvt.u8.u32 z, 0;\n\t"
+        "mov.b32 %0, {b0, b1, z, z};\n\t}"
+        : "=r"(r) : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]));
     return r;
 }
 // eight codes -> eight values
@@ -67,88 +78,100 @@ __device__ __forceinline__ long long source_row(const int *slots, int per, int s
     return row < sources ? row : -1;
 }
 
-// The largest magnitude of 16 values held in 16-byte words, as the bits of a float: two 16-bit values at a time (a magnitude's bits
-// order like the number, infinities and NaN above all).
-template <class T> __device__ __forceinline__ uint32_t magnitude_of(const uint4 *q) {
-    const uint32_t *w = reinterpret_cast<const uint32_t *>(q);
-    uint32_t m = 0;
-    if constexpr (sizeof(T) == 4) {
-#pragma unroll
-        for (int i = 0; i < 16; i++) m = max(m, w[i] & 0x7fffffffu);
-        return m;
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; i++) m = __vmaxu2(m, w[i] & 0x7fff7fffu);
+// The largest magnitude of the values in a 16-byte word, as the bits of a float: two 16-bit values at a time (a magnitude's bits order
+// like the number, infinities and NaN above all).
+template <class T> __device__ __forceinline__ uint32_t magnitude_of(const uint4 &q) {
+    if constexpr (sizeof(T) == 4) return max(max(q.x & 0x7fffffffu, q.y & 0x7fffffffu), max(q.z & 0x7fffffffu, q.w & 0x7fffffffu));
+    else {
+        constexpr uint32_t M = 0x7fff7fffu;
+        uint32_t m = __vmaxu2(__vmaxu2(q.x & M, q.y & M), __vmaxu2(q.z & M, q.w & M));
         m = max(m & 0xffffu, m >> 16);
         return magnitude(to_f32<T>(reinterpret_cast<const T *>(&m)[0]));
     }
 }
 
-// Blocks along the rows of X. A lane holds 16 values, two lanes a block; a warp takes 512 values of one row, so that its loads are
-// 512 or 1024 bytes in a piece and its stores 256. `share` warps (a power of two) work on one row. The kernel is nearer to the limit
-// of instruction issue than to HBM's, so magnitudes are compared and values scaled two at a time.
-template <class T, bool VEC>
+// Blocks along the rows of X. A lane holds 16 bytes of values, 4 or 8 lanes a block; a warp's load is 512 contiguous bytes and UNITS of
+// them are in flight. Bound by HBM, and near the limit of instruction issue, so magnitudes are compared and values scaled two at a
+// time. (With 32 or 64 contiguous bytes to a lane the loads touched two or four times the lines: 81 us for 16384 x 7168 BF16.)
+// ROUTED: the warp's row is a token, rounded once and written to the rows of all its slots; then rows without a slot are looked for,
+// 32 at a time, and become zeros.
+constexpr int UNITS = 4;
+template <class T, bool VEC, bool ROUTED>
 __global__ void __launch_bounds__(256) mx4_rows(const T *X, int nvec, int len, long long ldx, size_t plane_x, int planes, int rule,
-                                                const int *slots, int per, int sources, uint8_t *codes, long long ldq, size_t plane_q,
-                                                uint8_t *scales, long long lds, size_t plane_s, int share_log) {
-    __shared__ float turn[VEC ? 1 : 8][32 * 17];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = warp & ((1 << share_log) - 1);
-    const long long total = (long long)planes * nvec;
-    for (long long vec = ((long long)blockIdx.x << (3 - share_log)) + (warp >> share_log); vec < total; vec += (long long)gridDim.x << (3 - share_log)) {
+                                                const int *row_of, const int *slot_of, int top, int tokens, uint8_t *codes, long long ldq,
+                                                size_t plane_q, uint8_t *scales, long long lds, size_t plane_s) {
+    constexpr int N = Vec16<T>::N, LOAD = 32 * N, SHARE = 32 / N;   // values of a lane, of a load of the warp; lanes of a block
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint32_t units = (len + LOAD * UNITS - 1) / (LOAD * UNITS);
+    const long long total = (long long)(ROUTED ? tokens : (long long)planes * nvec) * units;
+    for (long long w = (long long)blockIdx.x * 8 + warp; w < total; w += (long long)gridDim.x * 8) {
+        const long long vec = total < 0x80000000ll ? (long long)((uint32_t)w / units) : w / units;
         const long long z = planes > 1 ? vec / nvec : 0, r = vec - z * nvec;
-        const long long src = source_row(slots, per, sources, (int)r);
-        const T *x = X + z * plane_x + max(src, 0ll) * ldx;
-        uint8_t *c = codes + z * plane_q + r * ldq, *s = scales + z * plane_s + r * lds;
-        for (int at = part * 512; at < len; at += 512 << share_log) {
-            const int i0 = at + lane * 16;
-            float v[16];
-            uint32_t m;
-            if constexpr (VEC) {   // rows start on 16 bytes; a piece that does not exist is zero, the last one may be cut
-                constexpr int N = Vec16<T>::N;
-                uint4 q[16 / N] = {};
-                if (src >= 0) {
+        const int at = (int)(w - vec * units) * LOAD * UNITS + lane * N;   // the lane's first value
+        const T *x = X + z * plane_x + r * ldx;
+        uint4 q[UNITS];
+        if constexpr (VEC) {   // rows start on 16 bytes and end on them; loads behind the end are made at the end, and cleared
 #pragma unroll
-                    for (int i = 0; i < 16 / N; i++) {
-                        const int e = i0 + i * N;
-                        if (e + N <= len) q[i] = __ldg(reinterpret_cast<const uint4 *>(x + e));
-                        else if (e < len)
-                            for (int k = 0; e + k < len; k++) reinterpret_cast<T *>(&q[i])[k] = x[e + k];
-                    }
-                }
-                m = magnitude_of<T>(q);
+            for (int u = 0; u < UNITS; u++) q[u] = __ldg(reinterpret_cast<const uint4 *>(x + min(at + u * LOAD, len - N)));
 #pragma unroll
-                for (int i = 0; i < 16 / N; i++) Vec16<T>::unpack(q[i], v + i * N);
-            } else {   // lanes load side by side, and turn the values through shared memory
-                float *mine = turn[warp];
-                T raw[16];
+            for (int u = 0; u < UNITS; u++)
+                if (at + u * LOAD >= len) q[u] = make_uint4(0, 0, 0, 0);
+        } else {   // value by value, zeros behind the last
 #pragma unroll
-                for (int i = 0; i < 16; i++) raw[i] = x[min(at + i * 32 + lane, len - 1)];
+            for (int u = 0; u < UNITS; u++) {
+                T *v = reinterpret_cast<T *>(&q[u]);
 #pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    const int e = i * 32 + lane;
-                    mine[e + (e >> 4)] = src >= 0 && at + e < len ? to_f32<T>(raw[i]) : 0.f;
-                }
-                __syncwarp();
-                m = 0;
+                for (int i = 0; i < N; i++) v[i] = x[min(at + u * LOAD + i, len - 1)];
 #pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    v[i] = mine[lane * 17 + i];
-                    m = max(m, magnitude(v[i]));
-                }
-                __syncwarp();
+                for (int i = 0; i < N; i++)
+                    if (at + u * LOAD + i >= len) v[i] = from_f32<T>(0.f);
             }
-            m = max(m, __shfl_xor_sync(~0u, m, 1));
-            const uint32_t byte = scale_byte(m, rule), number = byte == 255 ? 0u : ~0u;
-            const float2 inv = make_float2(inverse_scale(byte), inverse_scale(byte));
+        }
 #pragma unroll
-            for (int i = 0; i < 16; i += 2) {
+        for (int u = 0; u < UNITS; u++) {
+            const int e = at + u * LOAD;
+            if (e - lane * N >= len) break;   // the same for the whole warp
+            uint32_t m = magnitude_of<T>(q[u]);
+#pragma unroll
+            for (int d = 1; d < SHARE; d <<= 1) m = max(m, __shfl_xor_sync(~0u, m, d));
+            const uint32_t byte = scale_byte(m, rule);
+            const float2 inv = make_float2(inverse_scale(byte), inverse_scale(byte));
+            float v[8] = {};
+            Vec16<T>::unpack(q[u], v);
+#pragma unroll
+            for (int i = 0; i < N; i += 2) {
                 const float2 f = __fmul2_rn(make_float2(v[i], v[i + 1]), inv);
                 v[i] = f.x;
                 v[i + 1] = f.y;
             }
-            if ((i0 & ~31) < len) {   // the block exists: its codes are written whole, zeros behind the last value
-                *reinterpret_cast<uint2 *>(c + (i0 >> 1)) = make_uint2(codes_of(v) & number, codes_of(v + 8) & number);
-                if (!(lane & 1)) s[i0 >> 5] = (uint8_t)byte;
+            const uint32_t c = byte == 255 ? 0u : N == 8 ? codes_of(v) : codes_of4(v);
+            auto write = [&](uint8_t *codes_row, uint8_t *scales_row) {   // a block is written whole, zeros behind the last value
+                if ((e & ~31) >= len) return;
+                if constexpr (N == 8) *reinterpret_cast<uint32_t *>(codes_row + (e >> 1)) = c;
+                else *reinterpret_cast<uint16_t *>(codes_row + (e >> 1)) = (uint16_t)c;
+                if (lane % SHARE == 0) scales_row[e >> 5] = (uint8_t)byte;
+            };
+            if constexpr (ROUTED) {
+                for (int j = 0; j < top; j++) {
+                    const int row = __ldg(row_of + r * top + j);
+                    if (row >= 0 && row < nvec) write(codes + (size_t)row * ldq, scales + (size_t)row * lds);
+                }
+            } else write(codes + z * plane_q + r * ldq, scales + z * plane_s + r * lds);
+        }
+    }
+    if constexpr (ROUTED) {
+        const long long slots = (long long)tokens * top;
+        const int blocks = (len + 31) / 32;
+        for (long long r0 = ((long long)blockIdx.x * 8 + warp) * 32; r0 < nvec; r0 += (long long)gridDim.x * 256) {
+            const int s = r0 + lane < nvec ? __ldg(slot_of + r0 + lane) : 0;
+            uint32_t none = __ballot_sync(~0u, s < 0 || s >= slots);
+            while (none) {
+                const long long r = r0 + __ffs(none) - 1;
+                none &= none - 1;
+                for (int b = lane; b < blocks; b += 32) {
+                    *reinterpret_cast<uint4 *>(codes + r * ldq + b * 16) = make_uint4(0, 0, 0, 0);
+                    scales[r * lds + b] = 0;
+                }
             }
         }
     }
@@ -218,33 +241,52 @@ __global__ void __launch_bounds__(256) mx4_cols(const T *X, int nvec, int len, l
     }
 }
 
-// Codes and scales back to values: a lane takes half a block (8 bytes of codes), a warp 512 values of one vector. Every product of a
-// code's value and a power of two is exact in FP32; T rounds it once (FP16 may overflow or lose small values, BF16 does not lose any).
+// Codes and scales back to values. Every product of a code's value and a power of two is exact in FP32 (or an infinity); T rounds it
+// once (FP16 may overflow or lose small values, BF16 does not lose any). Where rows start and end on 16 bytes a lane stores 16 bytes
+// beside its neighbours', four of them from loads in flight together; else a warp turns 512 values through shared memory, so that
+// single values are stored side by side.
 template <class T, bool VEC>
 __global__ void __launch_bounds__(256) mx4_values(const uint8_t *codes, long long ldq, const uint8_t *scales, long long lds, int nvec, int len,
                                                   T *Y, long long ldy) {
-    __shared__ float turn[8][32 * 17];
+    __shared__ float turn[VEC ? 1 : 8][32 * 17];
+    constexpr int N = Vec16<T>::N, LOAD = VEC ? 32 * N : 512, PIECE = VEC ? LOAD * UNITS : LOAD;
     const int lane = threadIdx.x & 31;
-    const int pieces = (len + 511) / 512;
+    const uint32_t pieces = (len + PIECE - 1) / PIECE;
     const long long total = (long long)nvec * pieces;
     for (long long w = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); w < total; w += (long long)gridDim.x * 8) {
-        const long long r = w / pieces;
-        const int at = (int)(w - r * pieces) * 512, i0 = at + lane * 16;
-        T *y = Y + (size_t)r * ldy;
-        float v[16];
-        if (i0 < len) {
-            const uint2 q = __ldg(reinterpret_cast<const uint2 *>(codes + (size_t)r * ldq + (i0 >> 1)));
-            const float s = scale_of(__ldg(scales + (size_t)r * lds + (i0 >> 5)));
-            values_of(q.x, v);
-            values_of(q.y, v + 8);
+        const long long r = total < 0x80000000ll ? (long long)((uint32_t)w / pieces) : w / pieces;
+        const int at = (int)(w - r * pieces) * PIECE;
+        T *y = Y + r * ldy;
+        const uint8_t *c = codes + r * ldq, *s = scales + r * lds;
+        if constexpr (VEC) {
+            uint32_t q[UNITS];
+            uint8_t b[UNITS];
 #pragma unroll
-            for (int i = 0; i < 16; i++) v[i] *= s;
-        }
-        if (VEC && at + 512 <= len) {
-            constexpr int N = Vec16<T>::N;
+            for (int u = 0; u < UNITS; u++) {
+                const int e = min(at + u * LOAD + lane * N, len - N);
+                q[u] = N == 8 ? __ldg(reinterpret_cast<const uint32_t *>(c + (e >> 1))) : __ldg(reinterpret_cast<const uint16_t *>(c + (e >> 1)));
+                b[u] = __ldg(s + (e >> 5));
+            }
 #pragma unroll
-            for (int i = 0; i < 16 / N; i++) *(reinterpret_cast<uint4 *>(y + i0) + i) = Vec16<T>::pack(v + i * N);
-        } else {   // rows that do not start on 16 bytes, and ends: through shared memory, so that lanes store side by side
+            for (int u = 0; u < UNITS; u++) {
+                const int e = at + u * LOAD + lane * N;
+                float v[8];
+                values_of(q[u], v);
+#pragma unroll
+                for (int i = 0; i < N; i++) v[i] *= scale_of(b[u]);
+                if (e < len) *reinterpret_cast<uint4 *>(y + e) = Vec16<T>::pack(v);
+            }
+        } else {
+            const int i0 = at + lane * 16;
+            float v[16];
+            if (i0 < len) {
+                const uint2 q = __ldg(reinterpret_cast<const uint2 *>(c + (i0 >> 1)));
+                const float scale = scale_of(__ldg(s + (i0 >> 5)));
+                values_of(q.x, v);
+                values_of(q.y, v + 8);
+#pragma unroll
+                for (int i = 0; i < 16; i++) v[i] *= scale;
+            }
             float *mine = turn[threadIdx.x >> 5];
 #pragma unroll
             for (int i = 0; i < 16; i++) mine[lane * 17 + i] = v[i];
@@ -266,24 +308,30 @@ int warp_grid(long long warps) {   // eight warps to a block, at most 2^20 block
 
 }  // namespace
 
-cudaError_t mx4_quantize_rows(const void *X, int type, int nvec, int len, long long ldx, size_t plane_x, int planes, int rule, const int *slots,
-                              int per, int sources, uint8_t *codes, long long ldq, size_t plane_q, uint8_t *scales, long long lds,
+cudaError_t mx4_quantize_rows(const void *X, int type, int nvec, int len, long long ldx, size_t plane_x, int planes, int rule, const int *rows,
+                              const int *slots, int top, int tokens, uint8_t *codes, long long ldq, size_t plane_q, uint8_t *scales, long long lds,
                               size_t plane_s, cudaStream_t st) {
     const int size = type_size(type);
-    const bool vec = !(reinterpret_cast<uintptr_t>(X) & 15) && !(ldx * size & 15) && !(plane_x * size & 15);
-    int share_log = 0;   // warps to a row: as many as it has pieces, up to eight
-    while (share_log < 3 && (512 << share_log) < len) share_log++;
-    const int grid = warp_grid(((long long)planes * nvec) << share_log);
+    const bool vec = !(reinterpret_cast<uintptr_t>(X) & 15) && !(ldx * size & 15) && !(plane_x * size & 15) && !((long long)len * size & 15);
+    const long long vectors = slots ? tokens : (long long)planes * nvec;
+    const int unit = 512 / size * UNITS;   // values that a warp takes at a time
+    const int grid = warp_grid(vectors * ((len + unit - 1) / unit) + (slots ? nvec / 32 : 0));
     with_type(type, [&](auto t) {
         using T = decltype(t);
-        if (vec) mx4_rows<T, true><<<grid, 256, 0, st>>>((const T *)X, nvec, len, ldx, plane_x, planes, rule, slots, per, sources, codes, ldq, plane_q, scales, lds, plane_s, share_log);
-        else mx4_rows<T, false><<<grid, 256, 0, st>>>((const T *)X, nvec, len, ldx, plane_x, planes, rule, slots, per, sources, codes, ldq, plane_q, scales, lds, plane_s, share_log);
+        auto go = [&](auto vec_, auto routed_) {
+            mx4_rows<T, decltype(vec_)::value, decltype(routed_)::value><<<grid, 256, 0, st>>>((const T *)X, nvec, len, ldx, plane_x, planes, rule, rows, slots, top,
+                                                                                               tokens, codes, ldq, plane_q, scales, lds, plane_s);
+        };
+        if (vec && slots) go(std::true_type(), std::true_type());
+        else if (vec) go(std::true_type(), std::false_type());
+        else if (slots) go(std::false_type(), std::true_type());
+        else go(std::false_type(), std::false_type());
     });
     return cudaGetLastError();
 }
 
-cudaError_t mx4_quantize_cols(const void *X, int type, int nvec, int len, long long ldx, size_t plane_x, int planes, int rule, const int *slots,
-                              int per, int sources, uint8_t *codes, long long ldq, size_t plane_q, uint8_t *scales, long long lds,
+cudaError_t mx4_quantize_cols(const void *X, int type, int nvec, int len, long long ldx, size_t plane_x, int planes, int rule, const int *,
+                              const int *slots, int top, int tokens, uint8_t *codes, long long ldq, size_t plane_q, uint8_t *scales, long long lds,
                               size_t plane_s, cudaStream_t st) {
     const int size = type_size(type);
     const bool vec = !(reinterpret_cast<uintptr_t>(X) % (2 * size)) && !((ldx | nvec) & 1) && !(plane_x & 1);
@@ -292,8 +340,8 @@ cudaError_t mx4_quantize_cols(const void *X, int type, int nvec, int len, long l
     if (grid > 0x7fffffffLL) return cudaErrorInvalidValue;
     with_type(type, [&](auto t) {
         using T = decltype(t);
-        if (vec) mx4_cols<T, true><<<(int)grid, 256, 0, st>>>((const T *)X, nvec, len, ldx, plane_x, rule, slots, per, sources, codes, ldq, plane_q, scales, lds, plane_s, col_tiles, row_tiles);
-        else mx4_cols<T, false><<<(int)grid, 256, 0, st>>>((const T *)X, nvec, len, ldx, plane_x, rule, slots, per, sources, codes, ldq, plane_q, scales, lds, plane_s, col_tiles, row_tiles);
+        if (vec) mx4_cols<T, true><<<(int)grid, 256, 0, st>>>((const T *)X, nvec, len, ldx, plane_x, rule, slots, top, tokens, codes, ldq, plane_q, scales, lds, plane_s, col_tiles, row_tiles);
+        else mx4_cols<T, false><<<(int)grid, 256, 0, st>>>((const T *)X, nvec, len, ldx, plane_x, rule, slots, top, tokens, codes, ldq, plane_q, scales, lds, plane_s, col_tiles, row_tiles);
     });
     return cudaGetLastError();
 }
@@ -301,8 +349,9 @@ cudaError_t mx4_quantize_cols(const void *X, int type, int nvec, int len, long l
 cudaError_t mx4_dequantize(const uint8_t *codes, long long ldq, const uint8_t *scales, long long lds, int nvec, int len, void *Y, int type,
                            long long ldy, cudaStream_t st) {
     const int size = type_size(type);
-    const bool vec = !(reinterpret_cast<uintptr_t>(Y) & 15) && !(ldy * size & 15);
-    const int grid = warp_grid((long long)nvec * ((len + 511) / 512));
+    const bool vec = !(reinterpret_cast<uintptr_t>(Y) & 15) && !(ldy * size & 15) && !((long long)len * size & 15);
+    const int piece = vec ? 512 / size * UNITS : 512;   // values that a warp takes at a time
+    const int grid = warp_grid((long long)nvec * ((len + piece - 1) / piece));
     with_type(type, [&](auto t) {
         using T = decltype(t);
         if (vec) mx4_values<T, true><<<grid, 256, 0, st>>>(codes, ldq, scales, lds, nvec, len, (T *)Y, ldy);

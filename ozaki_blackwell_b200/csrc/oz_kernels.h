@@ -49,11 +49,11 @@ void exact_f8_release();
 
 
 // microscaled 4-bit format (mx4.cu): element types 0 FP32, 1 BF16, 2 FP16
-cudaError_t mx4_quantize_rows(const void *X, int type, int nvec, int len, long long ldx, size_t plane_x, int planes, int rule, const int *slots,
-                              int per, int sources, uint8_t *codes, long long ldq, size_t plane_q, uint8_t *scales, long long lds,
+cudaError_t mx4_quantize_rows(const void *X, int type, int nvec, int len, long long ldx, size_t plane_x, int planes, int rule, const int *rows,
+                              const int *slots, int top, int tokens, uint8_t *codes, long long ldq, size_t plane_q, uint8_t *scales, long long lds,
                               size_t plane_s, cudaStream_t st);
-cudaError_t mx4_quantize_cols(const void *X, int type, int nvec, int len, long long ldx, size_t plane_x, int planes, int rule, const int *slots,
-                              int per, int sources, uint8_t *codes, long long ldq, size_t plane_q, uint8_t *scales, long long lds,
+cudaError_t mx4_quantize_cols(const void *X, int type, int nvec, int len, long long ldx, size_t plane_x, int planes, int rule, const int *rows,
+                              const int *slots, int top, int tokens, uint8_t *codes, long long ldq, size_t plane_q, uint8_t *scales, long long lds,
                               size_t plane_s, cudaStream_t st);
 cudaError_t mx4_dequantize(const uint8_t *codes, long long ldq, const uint8_t *scales, long long lds, int nvec, int len, void *Y, int type,
                            long long ldy, cudaStream_t st);

@@ -120,13 +120,13 @@ def quantize(x, dim=-1, rule="floor", routing=None):
     if dims not in (2, 3):
         raise ValueError(f"x must be a matrix or a stack of matrices, not {dims}-dimensional")
     ldx, index = _pitch(x, "x", dims), x.get_device()
-    rows, cols = sources, _ = shape[-2:]
-    slots, per = None, 0
+    rows, cols = shape[-2:]
+    maps = None, None, 0, 0
     if routing is not None:
         if dims != 2 or rows != routing.rows.shape[0]:
             raise ValueError("routing= takes a matrix with a row for each token")
-        _, per = _routed(routing, index)
-        slots, rows = routing.slots.data_ptr(), routing.slots.shape[0]
+        tokens, top = _routed(routing, index)
+        maps, rows = (routing.rows.data_ptr(), routing.slots.data_ptr(), top, tokens), routing.slots.shape[0]
     vectors, length = (rows, cols) if dim == -1 else (cols, rows)
     blocks = (length + 31) >> 5
     ldq, lds = 16 * blocks, (blocks + 15) & ~15
@@ -136,7 +136,7 @@ def quantize(x, dim=-1, rule="floor", routing=None):
     else:
         codes, scales = x.new_empty((shape[0], vectors, ldq), dtype=torch.uint8), x.new_empty((shape[0], vectors, lds), dtype=torch.uint8)
         planes = shape[0], x.stride(0), vectors * ldq, vectors * lds
-    _call(index, _lib.ozb_mx4_quantize, x.data_ptr(), kind, vectors, length, ldx, dim == -1, _RULES[rule], slots, per, sources, planes[0], planes[1],
+    _call(index, _lib.ozb_mx4_quantize, x.data_ptr(), kind, vectors, length, ldx, dim == -1, _RULES[rule], *maps, planes[0], planes[1],
           codes.data_ptr(), ldq, planes[2], scales.data_ptr(), lds, planes[3])
     return Mx4(codes, scales, length)
 

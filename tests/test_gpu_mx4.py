@@ -105,7 +105,7 @@ def test_nothing_is_written_behind_the_blocks():
     for by_rows, nvec, length in ((1, 5, 40), (0, 40, 5)):
         codes = torch.full((nvec + 1, 64), 0xAB, dtype=torch.uint8, device="cuda")
         scales = torch.full((nvec + 1, 16), 0xCD, dtype=torch.uint8, device="cuda")
-        assert lib.ozb_mx4_quantize(x.data_ptr(), 0, nvec, length, 40, by_rows, 0, None, 0, 0, 1, 0, codes.data_ptr(), 64, 0, scales.data_ptr(), 16, 0, None) == 0
+        assert lib.ozb_mx4_quantize(x.data_ptr(), 0, nvec, length, 40, by_rows, 0, None, None, 0, 0, 1, 0, codes.data_ptr(), 64, 0, scales.data_ptr(), 16, 0, None) == 0
         torch.cuda.synchronize()
         blocks = -(-length // 32)
         assert bool((codes[nvec] == 0xAB).all()) and bool((codes[:, 16 * blocks:] == 0xAB).all())
@@ -113,15 +113,31 @@ def test_nothing_is_written_behind_the_blocks():
 
 
 @pytest.mark.parametrize("dim", [-1, -2])
-def test_quantize_of_routed_rows(dim):
+@pytest.mark.parametrize("h,dtype", [(130, torch.float32), (1600, torch.bfloat16), (33, torch.float16)])
+def test_quantize_of_routed_rows(dim, h, dtype):
     from ozaki_blackwell_b200 import experts
     mx4 = _mx4()
-    x = _random(9, 130, 8).cuda()
-    slots = torch.tensor([4, -1, 0, 17, 17, 18, 2 ** 30, -2 ** 31, 8] * 5, dtype=torch.int32, device="cuda")   # two slots to a token
-    r = experts.Routing(torch.zeros(2, dtype=torch.int32, device="cuda"), torch.zeros(9, 2, dtype=torch.int32, device="cuda"), slots)
-    row = [2, None, 0, 8, 8, None, None, None, 4] * 5
-    rows = torch.stack([x[i].cpu() if i is not None else torch.zeros(130) for i in row])
-    got, want = ref.unpack(mx4.quantize(x, dim, routing=r)), ref.quantize(rows if dim == -1 else rows.t())
+    tokens, top = 90, 3
+    x = _random(tokens, h, 8).to(dtype).cuda()
+    g = torch.Generator().manual_seed(h)
+    r = experts.sort(torch.randint(-1, 5, (tokens, top), generator=g).cuda(), 5, 64)
+    for src in (x, _random(tokens, h + 9, 8).to(dtype).cuda()[:, 3: 3 + h]):
+        rows = experts.gather(src, r).cpu()
+        got, want = ref.unpack(mx4.quantize(src, dim, "ceil", routing=r)), ref.quantize(rows if dim == -1 else rows.t(), "ceil")
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("dim", [-1, -2])
+def test_quantize_takes_any_routing_without_leaving_its_arrays(dim):
+    from ozaki_blackwell_b200 import experts
+    mx4 = _mx4()
+    x = _random(3, 64, 9).cuda()
+    rows = torch.tensor([[0, 5], [-3, 2 ** 31 - 1], [-1, 1]], dtype=torch.int32, device="cuda")
+    slots = torch.tensor([0, 5, 6, 2 ** 31 - 1, -2 ** 31], dtype=torch.int32, device="cuda")
+    r = experts.Routing(torch.zeros(2, dtype=torch.int32, device="cuda"), rows, slots)
+    want = torch.zeros(5, 64)
+    want[0], want[1] = x[0].cpu(), x[2].cpu()
+    got, want = ref.unpack(mx4.quantize(x, dim, routing=r)), ref.quantize(want if dim == -1 else want.t())
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
 
 

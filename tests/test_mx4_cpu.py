@@ -10,15 +10,15 @@ P = ctypes.c_void_p(4096)          # never dereferenced: every call below is ref
 ARG, SIZE = 10001, 10006
 
 
-def _quantize(X=P, type=0, nvec=4, len=64, ldx=64, by_rows=1, rule=0, slots=None, per=0, sources=0, planes=1, plane_x=0, codes=P, ldq=32, plane_q=0,
+def _quantize(X=P, type=0, nvec=4, len=64, ldx=64, by_rows=1, rule=0, rows=None, slots=None, top=0, tokens=0, planes=1, plane_x=0, codes=P, ldq=32, plane_q=0,
               scales=P, lds=16, plane_s=0):
-    return lib.ozb_mx4_quantize(X, type, nvec, len, ldx, by_rows, rule, slots, per, sources, planes, plane_x, codes, ldq, plane_q, scales, lds, plane_s, None)
+    return lib.ozb_mx4_quantize(X, type, nvec, len, ldx, by_rows, rule, rows, slots, top, tokens, planes, plane_x, codes, ldq, plane_q, scales, lds, plane_s, None)
 
 
 @pytest.mark.parametrize("bad", [dict(X=None), dict(type=3), dict(type=-1), dict(nvec=0), dict(len=0), dict(len=-1), dict(len=2 ** 31 - 1), dict(ldx=63),
                                  dict(by_rows=0, ldx=3), dict(rule=2), dict(codes=None), dict(codes=ctypes.c_void_p(4104)), dict(ldq=24), dict(ldq=16),
-                                 dict(scales=None), dict(scales=ctypes.c_void_p(4104)), dict(lds=8), dict(lds=0), dict(slots=P), dict(slots=P, per=1),
-                                 dict(slots=P, per=1, sources=4, planes=2), dict(planes=0), dict(planes=2, plane_q=8), dict(planes=2, plane_q=16, plane_s=8),
+                                 dict(scales=None), dict(scales=ctypes.c_void_p(4104)), dict(lds=8), dict(lds=0), dict(slots=P), dict(rows=P),
+                                 dict(rows=P, slots=P, top=1), dict(rows=P, slots=P, tokens=4), dict(rows=P, slots=P, top=1, tokens=4, planes=2), dict(planes=0), dict(planes=2, plane_q=8), dict(planes=2, plane_q=16, plane_s=8),
                                  dict(X=ctypes.c_void_p(4098)), dict(X=ctypes.c_void_p(4097), type=1)])
 def test_quantize(bad):
     assert _quantize(**bad) == ARG
