@@ -39,21 +39,24 @@ __device__ __forceinline__ uint32_t codes_of4(const float *v) {   // four
         : "=r"(r) : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]));
     return r;
 }
-// eight codes -> eight values
-__device__ __forceinline__ void values_of(uint32_t c, float *v) {
-    uint32_t h[4];
-    asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
-        "mov.b32 {b0, b1, b2, b3}, %4;\n\t"
-        "cvt.rn.f16x2.e2m1x2 %0, b0;\n\t"
-        "cvt.rn.f16x2.e2m1x2 %1, b1;\n\t"
-        "cvt.rn.f16x2.e2m1x2 %2, b2;\n\t"
-        "cvt.rn.f16x2.e2m1x2 %3, b3;\n\t}"
-        : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3]) : "r"(c));
+// two codes (a byte) -> two values
+__device__ __forceinline__ float2 pair_of(uint32_t byte) {
+    uint32_t h;
+    asm("{\n\t.reg .b8 b;\n\t"
+        "cvt.u8.u32 b, %1;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %0, b;\n\t}"
+        : "=r"(h) : "r"(byte));
+    __half2 p;
+    memcpy(&p, &h, 4);
+    return __half22float2(p);
+}
+// N codes -> N values
+template <int N> __device__ __forceinline__ void values_of(uint32_t c, float *v) {
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&h[i]));
-        v[2 * i] = f.x;
-        v[2 * i + 1] = f.y;
+    for (int i = 0; i < N; i += 2) {
+        const float2 f = pair_of(c >> (4 * i) & 0xffu);
+        v[i] = f.x;
+        v[i + 1] = f.y;
     }
 }
 // the block's scale byte from the bits of its largest magnitude (0 .. 255)
@@ -86,7 +89,9 @@ template <class T> __device__ __forceinline__ uint32_t magnitude_of(const uint4 
         constexpr uint32_t M = 0x7fff7fffu;
         uint32_t m = __vmaxu2(__vmaxu2(q.x & M, q.y & M), __vmaxu2(q.z & M, q.w & M));
         m = max(m & 0xffffu, m >> 16);
-        return magnitude(to_f32<T>(reinterpret_cast<const T *>(&m)[0]));
+        T t;
+        memcpy(&t, &m, sizeof t);
+        return magnitude(to_f32<T>(t));
     }
 }
 
@@ -119,12 +124,13 @@ __global__ void __launch_bounds__(256) mx4_rows(const T *X, int nvec, int len, l
         } else {   // value by value, zeros behind the last
 #pragma unroll
             for (int u = 0; u < UNITS; u++) {
-                T *v = reinterpret_cast<T *>(&q[u]);
+                T v[N];
 #pragma unroll
                 for (int i = 0; i < N; i++) v[i] = x[min(at + u * LOAD + i, len - 1)];
 #pragma unroll
                 for (int i = 0; i < N; i++)
                     if (at + u * LOAD + i >= len) v[i] = from_f32<T>(0.f);
+                memcpy(&q[u], v, 16);
             }
         }
 #pragma unroll
@@ -264,14 +270,15 @@ __global__ void __launch_bounds__(256) mx4_values(const uint8_t *codes, long lon
 #pragma unroll
             for (int u = 0; u < UNITS; u++) {
                 const int e = min(at + u * LOAD + lane * N, len - N);
-                q[u] = N == 8 ? __ldg(reinterpret_cast<const uint32_t *>(c + (e >> 1))) : __ldg(reinterpret_cast<const uint16_t *>(c + (e >> 1)));
+                // four codes: the half of an aligned word that holds them
+                q[u] = __ldg(reinterpret_cast<const uint32_t *>(c + ((e >> 1) & ~3))) >> (N == 8 ? 0 : 4 * (e & 4));
                 b[u] = __ldg(s + (e >> 5));
             }
 #pragma unroll
             for (int u = 0; u < UNITS; u++) {
                 const int e = at + u * LOAD + lane * N;
-                float v[8];
-                values_of(q[u], v);
+                float v[N];
+                values_of<N>(q[u], v);
 #pragma unroll
                 for (int i = 0; i < N; i++) v[i] *= scale_of(b[u]);
                 if (e < len) *reinterpret_cast<uint4 *>(y + e) = Vec16<T>::pack(v);
@@ -282,8 +289,8 @@ __global__ void __launch_bounds__(256) mx4_values(const uint8_t *codes, long lon
             if (i0 < len) {
                 const uint2 q = __ldg(reinterpret_cast<const uint2 *>(c + (i0 >> 1)));
                 const float scale = scale_of(__ldg(s + (i0 >> 5)));
-                values_of(q.x, v);
-                values_of(q.y, v + 8);
+                values_of<8>(q.x, v);
+                values_of<8>(q.y, v + 8);
 #pragma unroll
                 for (int i = 0; i < 16; i++) v[i] *= scale;
             }

@@ -206,7 +206,12 @@ __device__ __forceinline__ void store_wide(T *Y, long long ldy, const uint32_t (
 #pragma unroll
         for (int h = 0; h < 32; h += COLS) {
 #pragma unroll
-            for (int c = 0; c < 4; c++) *reinterpret_cast<uint4 *>(turn + lane * TURN_PITCH + 16 * c) = Vec16<T>::pack(reinterpret_cast<const float *>(&v[h + c * N]));
+            for (int c = 0; c < 4; c++) {
+                float f[N];
+#pragma unroll
+                for (int e = 0; e < N; e++) f[e] = __uint_as_float(v[h + c * N + e]);
+                *reinterpret_cast<uint4 *>(turn + lane * TURN_PITCH + 16 * c) = Vec16<T>::pack(f);
+            }
             __syncwarp();
 #pragma unroll
             for (int r = 0; r < 32; r += 8) {

@@ -1,6 +1,7 @@
 // oz_types.cuh -- the element types of the low-bit and expert operators (OZB_F32, OZB_BF16, OZB_F16 of ozb.h) on the device.
 #pragma once
 #include <cstdint>
+#include <cstring>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -20,16 +21,18 @@ template <> __device__ __forceinline__ __half from_f32<__half>(float x) { return
 // 16 bytes of T as floats and back
 template <class T> struct Vec16 {
     static constexpr int N = 16 / (int)sizeof(T);
-    static __device__ __forceinline__ void unpack(uint4 q, float *f) {
-        const T *t = reinterpret_cast<const T *>(&q);
+    static __device__ __forceinline__ void unpack(const uint4 &q, float *f) {
+        T t[N];
+        memcpy(t, &q, 16);
 #pragma unroll
         for (int i = 0; i < N; i++) f[i] = to_f32<T>(t[i]);
     }
     static __device__ __forceinline__ uint4 pack(const float *f) {
-        uint4 q;
-        T *t = reinterpret_cast<T *>(&q);
+        T t[N];
 #pragma unroll
         for (int i = 0; i < N; i++) t[i] = from_f32<T>(f[i]);
+        uint4 q;
+        memcpy(&q, t, 16);
         return q;
     }
 };
