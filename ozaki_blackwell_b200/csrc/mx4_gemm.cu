@@ -45,6 +45,7 @@ constexpr int BK = 256, BKB = 128; // k of a stage, in values and in bytes
 constexpr int UK = 64;             // k of one tcgen05.mma kind::mxf4
 constexpr int TURNERS = 4, THREADS = 512;   // warp 11 is idle: the epilogue's second four must be warps 0 .. 3 modulo 4
 constexpr int MAX_GROUPS = 1024;
+constexpr int AHEAD = 64;          // tiles of a CTA that are worked out before it starts
 
 enum { DENSE = 0, BY_ROWS = 1, ALONG_K = 2 };
 enum { NARROW = 0, SPLIT = 1, WIDE = 2, PAIR = 3 };
@@ -80,7 +81,7 @@ template <int FORM, int BN> struct Shape {
     static constexpr int TMEM_COLS = COLS <= 256 ? 256 : 512;
     static constexpr int BARS = 2 * STAGES + 2 * SLOTS + 4;
     static constexpr int TURN = wide ? 8 * 32 * (64 + 16) : 0;     // what the epilogue's warps turn their tiles through
-    static constexpr int SMEM = STAGES * STAGE + SLOTS * SLOT + TURN + 1024 + 8 * BARS + 16 + 4 * (MAX_GROUPS + 1);
+    static constexpr int SMEM = STAGES * STAGE + SLOTS * SLOT + TURN + 1024 + 8 * BARS + 16 + 4 * (MAX_GROUPS + 4) + AHEAD * 32;
     static_assert(STAGE % 1024 == 0 && COLS <= 512 && SMEM <= 232448 - 64, "");
     static_assert(FORM != SPLIT || BN * BP * 4 <= STAGES * STAGE, "the partial tile of a split takes the place of the stages");
     // instruction descriptor: E2M1 x E2M1, both K-major, one power of two (UE8M0) for 32, N = BN, M = rows of P, K = 64
@@ -180,8 +181,6 @@ __device__ __forceinline__ Tile decode(const Params &p, const int *cum, int w) {
     t.p1 = S::wide ? hi : p.weights;
     t.q0 = (S::wide ? 0 : lo) + tq * (S::wide ? S::WEIGHTS : S::TOKENS);
     t.q1 = S::wide ? p.weights : hi;
-    t.s0 = t.k0 / BK;
-    t.s1 = t.k1 > t.k0 ? (t.k1 + BK - 1) / BK : t.s0;
     return t;
 }
 
@@ -246,6 +245,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm(const __grid_constant__ C
     auto accempty_bar = [&](int a) { return bars + 8u * (2 * S::STAGES + 2 * S::SLOTS + 2 + a); };
     const uint32_t tmem_slot = bars + 8u * S::BARS;
     int *const cum = reinterpret_cast<int *>(base_ptr + S::STAGES * S::STAGE + S::SLOTS * S::SLOT + S::TURN + 8 * S::BARS + 16);
+    int4 *const ahead = reinterpret_cast<int4 *>(cum + MAX_GROUPS + 4);   // [AHEAD][2]
     __shared__ int abort_flag;
 
     const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
@@ -310,8 +310,23 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm(const __grid_constant__ C
         first = blockIdx.x >> 1;
         step = gridDim.x >> 1;
     }
-    auto tile_at = [&](int w) {
-        Tile t = decode<S>(p, cum, w);
+    // A tile takes divisions and looks at the offsets: 900 cycles, as much as a short tile's products. The first AHEAD tiles of this CTA
+    // are worked out by a thread each; the roles then read them.
+    for (int n = threadIdx.x; n < AHEAD && n * (long long)step + first < total; n += THREADS) {
+        const Tile t = decode<S>(p, cum, first + n * step);
+        ahead[2 * n] = make_int4(t.group, t.p0, t.p1, t.q0);
+        ahead[2 * n + 1] = make_int4(t.q1, t.k0, t.k1, 0);
+    }
+    __syncthreads();
+    auto tile_at = [&](int w, uint32_t n) {   // the n-th tile of this CTA, item w
+        Tile t;
+        if (n < AHEAD) {
+            const int4 a = ahead[2 * n], b = ahead[2 * n + 1];
+            t.group = a.x; t.p0 = a.y; t.p1 = a.z; t.q0 = a.w;
+            t.q1 = b.x; t.k0 = b.y; t.k1 = b.z;
+        } else t = decode<S>(p, cum, w);
+        t.s0 = t.k0 / BK;
+        t.s1 = t.k1 > t.k0 ? (t.k1 + BK - 1) / BK : t.s0;
         if constexpr (FORM == SPLIT) {
             const int n = t.s1 - t.s0, s0 = t.s0;
             t.s0 = s0 + (int)((long long)n * rank / ranks);
@@ -328,8 +343,9 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm(const __grid_constant__ C
     uint32_t it = 0, sl = 0;   // running stage and slot (of the role that counts them)
 
     if (warp == 0) {
-        for (int w = first; w < total && !__any_sync(~0u, *abortp); w += step) {
-            const Tile t = tile_at(w);
+        uint32_t n = 0;
+        for (int w = first; w < total && !__any_sync(~0u, *abortp); w += step, n++) {
+            const Tile t = tile_at(w, n);
             const int zp = !S::wide && p.mode == BY_ROWS ? t.group : 0, zq = S::wide && p.mode == BY_ROWS ? t.group : 0;
             const int p0 = t.p0 + (pair ? (int)rank * BP : 0), q0 = t.q0 + (pair ? (int)rank * S::Q_ROWS : 0);
             for (int kb = t.s0; kb < t.s1; kb++, it++) {
@@ -355,7 +371,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm(const __grid_constant__ C
         if (!pair || rank == 0) {
             uint32_t n = 0;
             for (int w = first; w < total && !__any_sync(~0u, *abortp); w += step, n++) {
-                const Tile t = tile_at(w);
+                const Tile t = tile_at(w, n);
                 const uint32_t acc = n & 1u;
                 if (!warp_wait(accempty_bar(acc), ((n >> 1) & 1u) ^ 1u, abortp, 0x120)) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -407,8 +423,9 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm(const __grid_constant__ C
         }
     } else if (warp == 2) {
         if (!pair || rank == 0) {
-            for (int w = first; w < total && !__any_sync(~0u, *abortp); w += step) {
-                const Tile t = tile_at(w);
+            uint32_t n = 0;
+            for (int w = first; w < total && !__any_sync(~0u, *abortp); w += step, n++) {
+                const Tile t = tile_at(w, n);
                 bool ok = true;
                 for (int kb = t.s0; kb < t.s1; sl++) {
                     const int r = sl % S::SLOTS, s = it % S::STAGES, s2 = (it + 1) % S::STAGES;
@@ -449,8 +466,9 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm(const __grid_constant__ C
         // of TURNERS warps, in turns of a slot: while one waits for its slot's bytes, the others do theirs
         const uint32_t own = warp == 3 ? 0 : warp - 7;
         const int blocks = (p.K + 31) / 32;
-        for (int w = first; w < total && !__any_sync(~0u, *abortp); w += step) {
-            const Tile t = tile_at(w);
+        uint32_t n = 0;
+        for (int w = first; w < total && !__any_sync(~0u, *abortp); w += step, n++) {
+            const Tile t = tile_at(w, n);
             const int p0 = t.p0 + (pair ? (int)rank * BP : 0);
             bool ok = true;
             for (int kb = t.s0; kb < t.s1; kb = (kb | 1) + 1, sl++) {
@@ -503,7 +521,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm(const __grid_constant__ C
         const int quarter = warp & 3, half = warp >= 12;   // lanes 32 quarter .. +31, every other 32 columns
         uint32_t n = 0;
         for (int w = first; w < total && !__any_sync(~0u, *abortp); w += step, n++) {
-            const Tile t = tile_at(w);
+            const Tile t = tile_at(w, n);
             const uint32_t acc = n & 1u;
             if (!warp_wait(accfull_bar(acc), (n >> 1) & 1u, abortp, 0x150)) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
