@@ -272,6 +272,25 @@ int ozb_expert_combine(int T, int top, int H, const void *Z, int type, int R, lo
  * Z[rows[s]]> (0 for a dropped slot). dZ is neither dY nor Z. */
 int ozb_expert_combine_grad(int T, int top, int H, const void *dY, int type, long long lddy, const void *Z, long long ldz, int R, const int *rows,
                             const int *slots, const float *weights, void *dZ, long long lddz, float *dweights, void *stream);
+/* The experts' layer in one call: Y[t] = sum over j of weights[t][j] W[ids[t][j]] X[t] with X (T x K) rounded to the 4-bit format
+ * (rule 0) and W [experts] of N x K in it, blocks along K: ozb_expert_sort, ozb_mx4_quantize, ozb_mx4_gemm_grouped and
+ * ozb_expert_combine on one stream. Z (R x N, the rows before they are added up) and the maps may be NULL, or given to be kept for the
+ * gradients, which need align = 64; R is ozb_expert_sort_rows(T, top, experts, align). `work`: ozb_expert_mx4_work bytes on the
+ * device, 16-byte aligned (0: the sizes are refused). */
+size_t ozb_expert_mx4_work(int T, int top, int experts, int N, int K, int type, int align);
+int ozb_expert_mx4(int T, int top, int experts, int N, int K, const void *X, int type, long long ldx, const void *ids, int id_bytes,
+                   const float *weights, const uint8_t *W, long long ldw, size_t plane_w, const uint8_t *Ws, long long ldws, size_t plane_ws,
+                   int align, int *offsets, int *rows, int *slots, void *Z, long long ldz, void *Y, long long ldy, void *work, size_t work_bytes,
+                   void *stream);
+/* Its gradients for dY (T x N): dX (T x K), dweights [T][top], and dW [experts] of N x K (plane_dw elements from one to the next), all
+ * but dweights of `type`. Wt: the weights with blocks along N, [experts] of K x N; Z and the maps as ozb_expert_mx4 left them (segments
+ * padded to 64). dZ = ozb_expert_combine_grad is rounded to `type`, then to the 4-bit format by rows for dX and by columns, as X, for
+ * dW; the gradient passes through the roundings. `work`: ozb_expert_mx4_grad_work bytes, 16-byte aligned. */
+size_t ozb_expert_mx4_grad_work(int R, int N, int K, int type);
+int ozb_expert_mx4_grad(int T, int top, int experts, int N, int K, int R, const void *dY, int type, long long lddy, const void *X, long long ldx,
+                        const void *Z, long long ldz, const uint8_t *Wt, long long ldwt, size_t plane_wt, const uint8_t *Wts, long long ldwts,
+                        size_t plane_wts, const int *offsets, const int *rows, const int *slots, const float *weights, void *dX, long long lddx,
+                        float *dweights, void *dW, long long lddw, size_t plane_dw, void *work, size_t work_bytes, void *stream);
 
 /* The four stages on caller-owned device buffers (what bench/phases.cu launches one by one). Asynchronous.
  * Pitches: ld of int8 planes in bytes and a multiple of 16; `plane` = distance between planes in elements. */

@@ -76,6 +76,12 @@ lib.ozb_expert_sort.argtypes = [_i] * 3 + [_p, _i, _i, _i, _p, _p, _p, _p, _sz, 
 lib.ozb_expert_gather.argtypes = [_i] * 3 + [_p, _i, _ll, _i, _p, _p, _p, _ll, _p]
 lib.ozb_expert_combine.argtypes = [_i] * 3 + [_p, _i, _i, _ll, _p, _p, _p, _ll, _p]
 lib.ozb_expert_combine_grad.argtypes = [_i] * 3 + [_p, _i, _ll, _p, _ll, _i, _p, _p, _p, _p, _ll, _p, _p]
+lib.ozb_expert_mx4_work.restype = _sz
+lib.ozb_expert_mx4_work.argtypes = [_i] * 7
+lib.ozb_expert_mx4.argtypes = [_i] * 5 + [_p, _i, _ll, _p, _i, _p] + [_p, _ll, _sz] * 2 + [_i, _p, _p, _p, _p, _ll, _p, _ll, _p, _sz, _p]
+lib.ozb_expert_mx4_grad_work.restype = _sz
+lib.ozb_expert_mx4_grad_work.argtypes = [_i] * 4
+lib.ozb_expert_mx4_grad.argtypes = [_i] * 6 + [_p, _i, _ll] + [_p, _ll] * 2 + [_p, _ll, _sz] * 2 + [_p] * 4 + [_p, _ll, _p, _p, _ll, _sz, _p, _sz, _p]
 lib.ozb_int8_peak.argtypes = [_i, _i, ctypes.POINTER(ctypes.c_float), ctypes.POINTER(ctypes.c_double)]
 lib.ozb_selftest_wait_expiry.argtypes = [_i]
 lib.ozb_dgemm_mg.argtypes = [_i] * 3 + [_p] * 3 + [_i] * 3
@@ -103,5 +109,6 @@ SYMBOLS = [
     "ozb_status", "ozb_int8_peak", "ozb_selftest_wait_expiry", "ozb_bounds_report", "ozb_selftest_bounds",
     "ozb_mx4_quantize", "ozb_mx4_dequantize", "ozb_mx4_gemm", "ozb_mx4_gemm_grouped", "ozb_mx4_gemm_segments",
     "ozb_expert_sort_rows", "ozb_expert_sort_scratch", "ozb_expert_sort", "ozb_expert_gather", "ozb_expert_combine", "ozb_expert_combine_grad",
+    "ozb_expert_mx4_work", "ozb_expert_mx4", "ozb_expert_mx4_grad_work", "ozb_expert_mx4_grad",
     "ozb_dgemm_mg", "ozb_mg_release", "ozb_mg_unique_id", "ozb_mg_create", "ozb_mg_destroy", "ozb_mg_dgemm", "ozb_mg_wait", "ozb_mg_info", "ozb_mg_schedule", "ozb_mg_schedule_pieces",
 ]

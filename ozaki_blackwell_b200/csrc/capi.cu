@@ -442,7 +442,8 @@ bool bad_mx4(const void *codes, long long ldq, const void *scales, long long lds
 constexpr int MAX_LEN = 0x7fffffff - 1023;   // lengths are rounded up in 32 bits
 bool bad_slots(int T, int top) { return T <= 0 || top <= 0 || (long long)T * top > MAX_LEN; }
 bool bad_type(int type) { return type < OZB_F32 || type > OZB_F16; }
-bool off_type(const void *p, int type) { return off(p, type == OZB_F32 ? 4 : 2); }
+int type_bytes(int type) { return type == OZB_F32 ? 4 : 2; }
+bool off_type(const void *p, int type) { return off(p, type_bytes(type)); }
 }  // namespace
 
 OZB_API const char *ozb_version(void) { return OZB_VERSION; }
@@ -963,6 +964,116 @@ OZB_API int ozb_expert_combine_grad(int T, int top, int H, const void *dY, int t
         return OZB_EARG;
     if (int e = check_device()) return e;
     return (int)expert_combine_grad(T, top, H, dY, type, lddy, Z, ldz, R, rows, slots, weights, dZ, lddz, dweights, (cudaStream_t)stream);
+}
+
+// ---- the experts' layer in one call --------------------------------------------------------------------------------
+namespace {
+struct Carve {   // pieces of a workspace, each on 256 bytes
+    char *base;
+    size_t at = 0;
+    template <class T> T *take(size_t n) {
+        T *p = base ? reinterpret_cast<T *>(base + at) : nullptr;
+        at += (n * sizeof(T) + 255) / 256 * 256;
+        return p;
+    }
+};
+struct Packed { uint8_t *codes, *scales; long long ldq, lds; };
+Packed take_packed(Carve &c, long long n, long long len) {
+    const long long blocks = (len + 31) / 32, ldq = 16 * blocks, lds = (blocks + 15) / 16 * 16;
+    Packed p{nullptr, nullptr, ldq, lds};
+    p.codes = c.take<uint8_t>((size_t)(n * ldq));
+    p.scales = c.take<uint8_t>((size_t)(n * lds));
+    return p;
+}
+struct Layer { int *offsets, *rows, *slots; void *counts; Packed x; char *z; size_t bytes; };
+Layer carve_layer(void *work, int T, int top, int experts, int N, int K, int type, long long R) {
+    Carve c{static_cast<char *>(work)};
+    Layer l{};
+    l.offsets = c.take<int>(experts + 1);
+    l.rows = c.take<int>((size_t)T * top);
+    l.slots = c.take<int>((size_t)R);
+    l.counts = c.take<char>(expert_sort_scratch(T * top, experts));
+    l.x = take_packed(c, R, K);
+    l.z = c.take<char>((size_t)R * N * type_bytes(type));
+    l.bytes = c.at;
+    return l;
+}
+struct Gradient { char *dz, *dxs; Packed rows, dzt, xt; size_t bytes; };
+Gradient carve_gradient(void *work, int N, int K, int type, long long R) {
+    Carve c{static_cast<char *>(work)};
+    Gradient g{};
+    g.dz = c.take<char>((size_t)R * N * type_bytes(type));
+    g.dxs = c.take<char>((size_t)R * K * type_bytes(type));
+    g.rows = take_packed(c, R, N);
+    g.dzt = take_packed(c, N, R);
+    g.xt = take_packed(c, K, R);
+    g.bytes = c.at;
+    return g;
+}
+bool bad_layer(int T, int top, int experts, int N, int K, int type) {
+    return bad_slots(T, top) || experts <= 0 || N <= 0 || K <= 0 || N > MAX_LEN || K > MAX_LEN || bad_type(type);
+}
+}  // namespace
+OZB_API size_t ozb_expert_mx4_work(int T, int top, int experts, int N, int K, int type, int align) {
+    if (bad_layer(T, top, experts, N, K, type) || experts > 1024 || align <= 0 || align > 256) return 0;
+    const long long R = sorted_rows((long long)T * top, experts, align);
+    return R > MAX_LEN ? 0 : carve_layer(nullptr, T, top, experts, N, K, type, R).bytes;
+}
+OZB_API int ozb_expert_mx4(int T, int top, int experts, int N, int K, const void *X, int type, long long ldx, const void *ids, int id_bytes,
+                           const float *weights, const uint8_t *W, long long ldw, size_t plane_w, const uint8_t *Ws, long long ldws, size_t plane_ws,
+                           int align, int *offsets, int *rows, int *slots, void *Z, long long ldz, void *Y, long long ldy, void *work, size_t work_bytes,
+                           void *stream) {
+    if (bad_layer(T, top, experts, N, K, type) || align <= 0 || align > 256 || !X || off_type(X, type) || ldx < K || (id_bytes != 4 && id_bytes != 8) || !ids ||
+        off(ids, id_bytes) || off(weights, 4) || bad_mx4(W, ldw, Ws, ldws, K) || (experts > 1 && ((plane_w & 15) || (plane_ws & 15))) || !Y || off_type(Y, type) ||
+        ldy < N || !work || off(work, 16) || (Z && (ldz < N || off_type(Z, type))) || off(offsets, 4) || off(rows, 4) || off(slots, 4) ||
+        !offsets != !rows || !rows != !slots)
+        return OZB_EARG;
+    const long long R = experts > 1024 ? 0 : sorted_rows((long long)T * top, experts, align);
+    if (experts > 1024 || R > MAX_LEN) return OZB_ESIZE;
+    if (work_bytes < carve_layer(nullptr, T, top, experts, N, K, type, R).bytes) return OZB_EARG;
+    if (int e = check_device()) return e;
+    int *status = status_word();
+    if (!status) return (int)cudaErrorMemoryAllocation;
+    Layer l = carve_layer(work, T, top, experts, N, K, type, R);
+    if (offsets) { l.offsets = offsets; l.rows = rows; l.slots = slots; }
+    if (!Z) { Z = l.z; ldz = N; }
+    cudaStream_t st = (cudaStream_t)stream;
+    cudaError_t e = expert_sort(T * top, experts, ids, id_bytes, align, (int)R, l.offsets, l.rows, l.slots, l.counts, st);
+    if (!e) e = mx4_quantize_rows(X, type, (int)R, K, ldx, 0, 1, 0, l.rows, l.slots, top, T, l.x.codes, l.x.ldq, 0, l.x.scales, l.x.lds, 0, st);
+    if (!e) e = mx4_product({1, experts, (int)R, N, K, type, l.offsets, l.x.codes, l.x.ldq, l.x.scales, l.x.lds, W, ldw, plane_w, Ws, ldws, plane_ws, Z, ldz, 0}, status, st);
+    if (!e) e = expert_combine(T, top, N, Z, type, (int)R, ldz, l.rows, weights, Y, ldy, st);
+    return e == cudaErrorInvalidValue ? OZB_ESIZE : (int)e;
+}
+OZB_API size_t ozb_expert_mx4_grad_work(int R, int N, int K, int type) {
+    if (R <= 0 || R > MAX_LEN || N <= 0 || K <= 0 || N > MAX_LEN || K > MAX_LEN || bad_type(type)) return 0;
+    return carve_gradient(nullptr, N, K, type, R).bytes;
+}
+OZB_API int ozb_expert_mx4_grad(int T, int top, int experts, int N, int K, int R, const void *dY, int type, long long lddy, const void *X, long long ldx,
+                                const void *Z, long long ldz, const uint8_t *Wt, long long ldwt, size_t plane_wt, const uint8_t *Wts, long long ldwts,
+                                size_t plane_wts, const int *offsets, const int *rows, const int *slots, const float *weights, void *dX, long long lddx,
+                                float *dweights, void *dW, long long lddw, size_t plane_dw, void *work, size_t work_bytes, void *stream) {
+    if (bad_layer(T, top, experts, N, K, type) || R <= 0 || R > MAX_LEN || !dY || !X || !Z || off_type(dY, type) || off_type(X, type) || off_type(Z, type) ||
+        lddy < N || ldx < K || ldz < N || bad_mx4(Wt, ldwt, Wts, ldwts, N) || (experts > 1 && ((plane_wt & 15) || (plane_wts & 15))) || !offsets || !rows ||
+        !slots || off(offsets, 4) || off(rows, 4) || off(slots, 4) || off(weights, 4) || !dX || off_type(dX, type) || lddx < K || !dweights || off(dweights, 4) ||
+        !dW || off_type(dW, type) || lddw < K || !work || off(work, 16))
+        return OZB_EARG;
+    if (experts > 1024) return OZB_ESIZE;
+    if (work_bytes < carve_gradient(nullptr, N, K, type, R).bytes) return OZB_EARG;
+    if (int e = check_device()) return e;
+    int *status = status_word();
+    if (!status) return (int)cudaErrorMemoryAllocation;
+    const Gradient g = carve_gradient(work, N, K, type, R);
+    cudaStream_t st = (cudaStream_t)stream;
+    cudaError_t e = expert_combine_grad(T, top, N, dY, type, lddy, Z, ldz, R, rows, slots, weights, g.dz, N, dweights, st);
+    if (!e) e = mx4_quantize_rows(g.dz, type, R, N, N, 0, 1, 0, nullptr, nullptr, 0, 0, g.rows.codes, g.rows.ldq, 0, g.rows.scales, g.rows.lds, 0, st);
+    if (!e) e = mx4_product({1, experts, R, K, N, type, offsets, g.rows.codes, g.rows.ldq, g.rows.scales, g.rows.lds, Wt, ldwt, plane_wt, Wts, ldwts, plane_wts,
+                             g.dxs, K, 0}, status, st);
+    if (!e) e = expert_combine(T, top, K, g.dxs, type, R, K, rows, nullptr, dX, lddx, st);
+    if (!e) e = mx4_quantize_cols(g.dz, type, N, R, N, 0, 1, 0, nullptr, nullptr, 0, 0, g.dzt.codes, g.dzt.ldq, 0, g.dzt.scales, g.dzt.lds, 0, st);
+    if (!e) e = mx4_quantize_cols(X, type, K, R, ldx, 0, 1, 0, rows, slots, top, T, g.xt.codes, g.xt.ldq, 0, g.xt.scales, g.xt.lds, 0, st);
+    if (!e) e = mx4_product({2, experts, N, K, R, type, offsets, g.dzt.codes, g.dzt.ldq, g.dzt.scales, g.dzt.lds, g.xt.codes, g.xt.ldq, 0, g.xt.scales, g.xt.lds, 0,
+                             dW, lddw, plane_dw}, status, st);
+    return e == cudaErrorInvalidValue ? OZB_ESIZE : (int)e;
 }
 OZB_API int ozb_int8_peak(int iters, int pair, float *ms, double *tops) {
     if (int e = check_args(1, 1, 1)) return e;

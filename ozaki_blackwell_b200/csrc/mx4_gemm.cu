@@ -216,7 +216,7 @@ __device__ __forceinline__ void store_wide(T *Y, long long ldy, const uint32_t (
             for (int r = 0; r < 32; r += 8) {
                 const int row = r + (lane >> 2);
                 const uint4 q = *reinterpret_cast<const uint4 *>(turn + row * TURN_PITCH + 16 * (lane & 3));
-                if (i0 + row < i1) *reinterpret_cast<uint4 *>(Y + (size_t)(i0 + row) * ldy + j + h + (lane & 3) * N) = q;
+                if (i0 + row < i1) __stcs(reinterpret_cast<uint4 *>(Y + (size_t)(i0 + row) * ldy + j + h + (lane & 3) * N), q);   // not read here again: the operands keep their place in L2
             }
             __syncwarp();
         }

@@ -14,9 +14,8 @@ from typing import NamedTuple
 
 import torch
 
-from . import mx4
 from ._lib import lib as _lib
-from .mx4 import _call, _pitch, _result, _routed, _type
+from .mx4 import _call, _codes, _pitch, _result, _routed, _type
 
 __all__ = ["Routing", "sort", "gather", "combine", "combine_grad", "matmul", "matmul_grad"]
 
@@ -95,22 +94,55 @@ def combine_grad(dy, z, routing, weights=None):
 
 def matmul(x, w, ids, weights=None, keep=False):
     """y[t] = sum over j of weights[t, j] W[ids[t, j]] x[t]: tokens sorted by expert, rounded to the 4-bit format as they are gathered, one
-    product for all experts, and the rows added up by token. w: Mx4 stack [experts, n, ...] with blocks along the rows of x.
-    keep: returns (y, z, routing) for matmul_grad, with segments padded to 64."""
-    _pitch(x, "x")
-    r = sort(ids, w.codes.shape[0], 64 if keep else 1)
-    z = mx4.grouped_matmul(mx4.quantize(x, routing=r), w, r.offsets, x.dtype)
-    y = combine(z, r, weights)
+    product for all experts, and the rows added up by token, in one call of the library. w: Mx4 stack [experts, n, ...] with blocks
+    along the rows of x. keep: returns (y, z, routing) for matmul_grad, with segments padded to 64."""
+    ldx, index = _pitch(x, "x"), x.get_device()
+    kind, (tokens, k) = _type(x.dtype), x.shape
+    if (ids.dtype is not torch.int32 and ids.dtype is not torch.int64) or ids.dim() != 2 or ids.shape[0] != tokens or not ids.is_contiguous() or ids.get_device() != index:
+        raise ValueError(f"ids must be a contiguous [{tokens}, top] matrix of int32 or int64 on cuda:{index}")
+    wc, ldw, ws, ldws = _codes(w, "w", 3, index)
+    if w.length != k:
+        raise ValueError(f"cannot multiply rows of {k} by vectors of {w.length}")
+    (experts, n), top = w.codes.shape[:2], ids.shape[1]
+    factors = _weights(weights, ids.shape, index)
+    align = 64 if keep else 1
+    need = _lib.ozb_expert_mx4_work(tokens, top, experts, n, k, kind, align)
+    if not need:
+        raise ValueError(f"cannot sort {tokens} x {top} slots over {experts} experts: sizes are positive, at most 1024 experts")
+    y, work = x.new_empty((tokens, n)), x.new_empty((need,), dtype=torch.uint8)
+    maps, z, r = (None, None, None, None), None, None
+    if keep:
+        size = _lib.ozb_expert_sort_rows(tokens, top, experts, align)
+        buf = ids.new_empty(size + tokens * top + experts + 1, dtype=torch.int32)
+        r = Routing(buf[size + tokens * top :], buf[size : size + tokens * top].view(tokens, top), buf[:size], align)
+        z = x.new_empty((size, n))
+        at = buf.data_ptr()
+        maps = at + 4 * (size + tokens * top), at + 4 * size, at, z.data_ptr()
+    _call(index, _lib.ozb_expert_mx4, tokens, top, experts, n, k, x.data_ptr(), kind, ldx, ids.data_ptr(), ids.element_size(), factors, wc, ldw,
+          w.codes.stride(0), ws, ldws, w.scales.stride(0), align, *maps, n, y.data_ptr(), n, work.data_ptr(), need)
     return (y, z, r) if keep else y
 
 
 def matmul_grad(dy, x, z, wt, routing, weights=None):
-    """The gradients of matmul(..., keep=True): (dx, dweights, dw) with dw [experts, n, k] of x's type. wt: the weights with blocks along n,
-    mx4.quantize(W, dim=-2), a stack [experts, k, ...]. Operands of the products are rounded to the 4-bit format, gradients pass
-    through that rounding."""
+    """The gradients of matmul(..., keep=True): (dx, dweights, dw) with dw [experts, n, k] of x's type, in one call of the library. wt: the
+    weights with blocks along n, mx4.quantize(W, dim=-2), a stack [experts, k, ...]. Operands of the products are rounded to the 4-bit
+    format, gradients pass through that rounding."""
     if routing.align % 64:
         raise ValueError(f"the segments are padded to {routing.align}: products along the tokens need multiples of 64 (matmul with keep=True)")
-    dz, dweights = combine_grad(dy, z, routing, weights)
-    dx = combine(mx4.grouped_matmul(mx4.quantize(dz), wt, routing.offsets, z.dtype), routing)
-    dw = mx4.segment_matmul(mx4.quantize(dz, dim=-2), mx4.quantize(x, dim=-2, routing=routing), routing.offsets, x.dtype)
+    lddy, ldx, ldz, index = _pitch(dy, "dy"), _pitch(x, "x"), _pitch(z, "z"), x.get_device()
+    tokens, top = _routed(routing, index)
+    kind, (r, n), k = _type(x.dtype), z.shape, x.shape[1]
+    wc, ldw, ws, ldws = _codes(wt, "wt", 3, index)
+    experts = wt.codes.shape[0]
+    if not dy.dtype is z.dtype is x.dtype or dy.shape != (tokens, n) or x.shape[0] != tokens or r != routing.slots.shape[0] or dy.get_device() != index or z.get_device() != index:
+        raise ValueError(f"dy {tuple(dy.shape)}, x {tuple(x.shape)} and z {tuple(z.shape)} do not fit a routing of {tokens} tokens and {routing.slots.shape[0]} rows, or differ in type")
+    if wt.length != n or wt.codes.shape[1] != k or routing.offsets.shape[0] != experts + 1:
+        raise ValueError(f"wt must be a stack of {routing.offsets.shape[0] - 1} matrices of {k} vectors of {n}")
+    factors = _weights(weights, routing.rows.shape, index)
+    need = _lib.ozb_expert_mx4_grad_work(r, n, k, kind)
+    dx, dweights = x.new_empty((tokens, k)), x.new_empty((tokens, top), dtype=torch.float32)
+    dw, work = x.new_empty((experts, n, k)), x.new_empty((need,), dtype=torch.uint8)
+    _call(index, _lib.ozb_expert_mx4_grad, tokens, top, experts, n, k, r, dy.data_ptr(), kind, lddy, x.data_ptr(), ldx, z.data_ptr(), ldz, wc, ldw,
+          wt.codes.stride(0), ws, ldws, wt.scales.stride(0), routing.offsets.data_ptr(), routing.rows.data_ptr(), routing.slots.data_ptr(), factors,
+          dx.data_ptr(), k, dweights.data_ptr(), dw.data_ptr(), k, n * k, work.data_ptr(), need)
     return dx, dweights, dw
