@@ -11,6 +11,7 @@
 #include <type_traits>
 #include "oz_common.cuh"
 #include "oz_kernels.h"
+#include "oz_launch.cuh"
 #include "oz_types.cuh"
 
 namespace ozk {
@@ -22,7 +23,7 @@ constexpr int CHUNK = 1024, SORT_THREADS = 256, SORT_WARPS = 8, PER_WARP = CHUNK
 
 // the expert of slot s, or `experts` for a dropped one
 __device__ __forceinline__ int key_of(const void *ids, int id_bytes, int experts, int s) {
-    const long long id = id_bytes == 8 ? __ldg(reinterpret_cast<const long long *>(ids) + s) : (long long)__ldg(reinterpret_cast<const int *>(ids) + s);
+    const long long id = id_bytes == 8 ? *(reinterpret_cast<const long long *>(ids) + s) : (long long)*(reinterpret_cast<const int *>(ids) + s);
     return id >= 0 && id < experts ? (int)id : experts;
 }
 
@@ -110,6 +111,7 @@ __device__ __forceinline__ void place_segments(SortShared &sh, int experts, int 
 // them by expert and clears slot_of; sort_place adds up the counts -- of all chunks for the segments' lengths, of the chunks before its
 // own for where its slots go -- and writes both maps. All counts are whole numbers: the order is the same on every run.
 __global__ void __launch_bounds__(SORT_THREADS) sort_one(const void *ids, int id_bytes, int experts, int slots, int align, int R, int *offsets, int *row_of, int *slot_of) {
+    behind_predecessors();
     __shared__ SortShared sh;
     for (int r = threadIdx.x; r < R; r += SORT_THREADS) slot_of[r] = -1;
     int key[ROUNDS], rank[ROUNDS];
@@ -126,6 +128,7 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_one(const void *ids, int id
 }
 
 __global__ void __launch_bounds__(SORT_THREADS) sort_count(const void *ids, int id_bytes, int experts, int slots, int R, int *row_of, int *slot_of, int *counts) {
+    behind_predecessors();
     __shared__ SortShared sh;
     for (long long r = (long long)blockIdx.x * SORT_THREADS + threadIdx.x; r < R; r += (long long)gridDim.x * SORT_THREADS) slot_of[r] = -1;
     int key[ROUNDS], rank[ROUNDS];
@@ -140,6 +143,7 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_count(const void *ids, int 
 
 __global__ void __launch_bounds__(SORT_THREADS) sort_place(const void *ids, int id_bytes, int experts, int slots, int align, int R, int *offsets,
                                                            int *row_of, int *slot_of, const int *counts) {
+    behind_predecessors();
     __shared__ SortShared sh;
     int rank[CHUNK / SORT_THREADS], key[CHUNK / SORT_THREADS];
 #pragma unroll
@@ -156,7 +160,7 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_place(const void *ids, int 
     for (int i0 = threadIdx.x; i0 < n; i0 += 8 * SORT_THREADS) {
         int c[8];
 #pragma unroll
-        for (int k = 0; k < 8; k++) c[k] = i0 + k * SORT_THREADS < n ? __ldg(counts + i0 + k * SORT_THREADS) : 0;
+        for (int k = 0; k < 8; k++) c[k] = i0 + k * SORT_THREADS < n ? counts[i0 + k * SORT_THREADS] : 0;
 #pragma unroll
         for (int k = 0; k < 8; k++) {
             if (c[k]) {
@@ -186,6 +190,7 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_place(const void *ids, int 
 template <class E>
 __global__ void __launch_bounds__(256) gather_rows(const E *X, long long pitch_x, const int *row_of, const int *slot_of, int top, int T, int R, int n, E *Y,
                                                    long long pitch_y) {
+    behind_predecessors();
     constexpr int DEPTH = 4, PIECE = 32 * DEPTH;
     const int lane = threadIdx.x & 31, pieces = (n + PIECE - 1) / PIECE;
     const long long warp = (long long)blockIdx.x * 8 + (threadIdx.x >> 5), warps = (long long)gridDim.x * 8, slots = (long long)T * top;
@@ -199,14 +204,14 @@ __global__ void __launch_bounds__(256) gather_rows(const E *X, long long pitch_x
         const int c0 = (int)(w - t * pieces) * PIECE + lane;
         E v[DEPTH];
 #pragma unroll
-        for (int i = 0; i < DEPTH; i++) v[i] = __ldg(X + t * pitch_x + min(c0 + 32 * i, n - 1));
+        for (int i = 0; i < DEPTH; i++) v[i] = X[t * pitch_x + min(c0 + 32 * i, n - 1)];
         for (int j = 0; j < top; j++) {
-            const int r = __ldg(row_of + t * top + j);
+            const int r = row_of[t * top + j];
             if (r >= 0 && r < R) write(r, c0, v);
         }
     }
     for (long long r0 = warp * 32; r0 < R; r0 += warps * 32) {
-        const int s = r0 + lane < R ? __ldg(slot_of + r0 + lane) : 0;
+        const int s = r0 + lane < R ? slot_of[r0 + lane] : 0;
         uint32_t none = __ballot_sync(~0u, s < 0 || s >= slots);
         const E zero[DEPTH] = {};
         while (none) {
@@ -222,6 +227,7 @@ __global__ void __launch_bounds__(256) gather_rows(const E *X, long long pitch_x
 template <class T, bool VEC, int U>
 __global__ void __launch_bounds__(256) combine_rows(const T *Z, long long ldz, int R, const int *row_of, const float *weights, int tokens, int top, int H,
                                                     T *Y, long long ldy) {
+    behind_predecessors();
     constexpr int N = Vec16<T>::N;
     const int cols = (H + N - 1) / N;
     const long long total = (long long)tokens * cols;
@@ -234,8 +240,8 @@ __global__ void __launch_bounds__(256) combine_rows(const T *Z, long long ldz, i
 #pragma unroll
             for (int u = 0; u < U; u++) {
                 const long long s = (long long)t * top + min(j0 + u, top - 1);
-                r[u] = j0 + u < top ? __ldg(row_of + s) : -1;
-                f[u] = weights ? __ldg(weights + s) : 1.f;
+                r[u] = j0 + u < top ? row_of[s] : -1;
+                f[u] = weights ? weights[s] : 1.f;
                 if (r[u] >= R) r[u] = -1;
             }
             if (VEC && c + N <= H) {
@@ -272,14 +278,15 @@ __global__ void __launch_bounds__(256) combine_rows(const T *Z, long long ldz, i
 template <class T, bool VEC>
 __global__ void __launch_bounds__(256) combine_grad_rows(const T *dY, long long lddy, const T *Z, long long ldz, int R, const int *row_of, const int *slot_of,
                                                          const float *weights, int slots, int top, int H, T *dZ, long long lddz, float *dW) {
+    behind_predecessors();
     constexpr int N = Vec16<T>::N;
     const int lane = threadIdx.x & 31;
     for (long long s = (long long)blockIdx.x * 256 + threadIdx.x; s < slots; s += (long long)gridDim.x * 256) {
-        const int r = __ldg(row_of + s);
+        const int r = row_of[s];
         if (r < 0 || r >= R) dW[s] = 0.f;   // a dropped slot
     }
     for (long long r = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); r < R; r += (long long)gridDim.x * 8) {
-        const int s = __ldg(slot_of + r);
+        const int s = slot_of[r];
         T *dz = dZ + (size_t)r * lddz;
         constexpr int U = 4;   // pieces of both rows in flight
         if (s < 0 || s >= slots) {
@@ -292,7 +299,7 @@ __global__ void __launch_bounds__(256) combine_grad_rows(const T *dY, long long 
             }
             continue;
         }
-        const float f = weights ? __ldg(weights + s) : 1.f;
+        const float f = weights ? weights[s] : 1.f;
         const T *dy = dY + (size_t)(s / top) * lddy, *z = Z + (size_t)r * ldz;
         float dot = 0.f;
         auto use = [&](float (&a)[N], const float (&b)[N]) {
@@ -308,7 +315,7 @@ __global__ void __launch_bounds__(256) combine_grad_rows(const T *dY, long long 
                 uint4 qa[U], qb[U];
 #pragma unroll
                 for (int u = 0; u < U; u++) {
-                    qa[u] = __ldg(reinterpret_cast<const uint4 *>(dy + c0 + (u * 32 + lane) * N));
+                    qa[u] = *reinterpret_cast<const uint4 *>(dy + c0 + (u * 32 + lane) * N);
                     qb[u] = __ldcs(reinterpret_cast<const uint4 *>(z + c0 + (u * 32 + lane) * N));
                 }
 #pragma unroll
@@ -324,7 +331,7 @@ __global__ void __launch_bounds__(256) combine_grad_rows(const T *dY, long long 
         if constexpr (VEC) {
             for (; c0 + 32 * N <= H; c0 += 32 * N) {
                 float a[N], b[N];
-                Vec16<T>::unpack(__ldg(reinterpret_cast<const uint4 *>(dy + c0 + lane * N)), a);
+                Vec16<T>::unpack(*reinterpret_cast<const uint4 *>(dy + c0 + lane * N), a);
                 Vec16<T>::unpack(__ldcs(reinterpret_cast<const uint4 *>(z + c0 + lane * N)), b);
                 use(a, b);
                 __stcs(reinterpret_cast<uint4 *>(dz + c0 + lane * N), Vec16<T>::pack(a));
@@ -354,13 +361,11 @@ cudaError_t expert_sort(int slots, int experts, const void *ids, int id_bytes, i
                         cudaStream_t st) {
     const int chunks = (slots + CHUNK - 1) / CHUNK;
     if (chunks == 1) {
-        sort_one<<<1, SORT_THREADS, 0, st>>>(ids, id_bytes, experts, slots, align, R, offsets, rows, slot_of);
-    } else {
-        int *counts = static_cast<int *>(scratch);
-        sort_count<<<chunks, SORT_THREADS, 0, st>>>(ids, id_bytes, experts, slots, R, rows, slot_of, counts);
-        sort_place<<<chunks, SORT_THREADS, 0, st>>>(ids, id_bytes, experts, slots, align, R, offsets, rows, slot_of, counts);
+        return launch_behind(sort_one, 1, SORT_THREADS, 0, 1, st, ids, id_bytes, experts, slots, align, R, offsets, rows, slot_of);
     }
-    return cudaGetLastError();
+    int *counts = static_cast<int *>(scratch);
+    if (cudaError_t e = launch_behind(sort_count, chunks, SORT_THREADS, 0, 1, st, ids, id_bytes, experts, slots, R, rows, slot_of, counts)) return e;
+    return launch_behind(sort_place, chunks, SORT_THREADS, 0, 1, st, ids, id_bytes, experts, slots, align, R, offsets, rows, slot_of, counts);
 }
 
 cudaError_t expert_gather(int T, int top, int H, const void *X, int type, long long ldx, int R, const int *rows, const int *slots, void *Y,
@@ -369,17 +374,16 @@ cudaError_t expert_gather(int T, int top, int H, const void *X, int type, long l
     auto grid = [&](int n) { return grid_of(((long long)T * ((n + 127) / 128) + R / 32 + 7) / 8); };
     if (aligned(X, ldx, size) && aligned(Y, ldy, size) && !((long long)H * size & 15)) {
         const int n = H * size / 16;
-        gather_rows<uint4><<<grid(n), 256, 0, st>>>((const uint4 *)X, ldx * size / 16, rows, slots, top, T, R, n, (uint4 *)Y, ldy * size / 16);
-    } else if (size == 4) {
-        gather_rows<uint32_t><<<grid(H), 256, 0, st>>>((const uint32_t *)X, ldx, rows, slots, top, T, R, H, (uint32_t *)Y, ldy);
-    } else {
-        gather_rows<uint16_t><<<grid(H), 256, 0, st>>>((const uint16_t *)X, ldx, rows, slots, top, T, R, H, (uint16_t *)Y, ldy);
+        return launch_behind(gather_rows<uint4>, grid(n), 256, 0, 1, st, (const uint4 *)X, ldx * size / 16, rows, slots, top, T, R, n, (uint4 *)Y, ldy * size / 16);
     }
-    return cudaGetLastError();
+    if (size == 4)
+        return launch_behind(gather_rows<uint32_t>, grid(H), 256, 0, 1, st, (const uint32_t *)X, ldx, rows, slots, top, T, R, H, (uint32_t *)Y, ldy);
+    return launch_behind(gather_rows<uint16_t>, grid(H), 256, 0, 1, st, (const uint16_t *)X, ldx, rows, slots, top, T, R, H, (uint16_t *)Y, ldy);
 }
 
 cudaError_t expert_combine(int T, int top, int H, const void *Z, int type, int R, long long ldz, const int *rows, const float *weights, void *Y,
                            long long ldy, cudaStream_t st) {
+    cudaError_t e = cudaErrorInvalidValue;
     const int size = type_size(type), n = 16 / size;
     const bool vec = aligned(Z, ldz, size) && aligned(Y, ldy, size);
     const int grid = grid_of(((long long)T * ((H + n - 1) / n) + 255) / 256);
@@ -387,27 +391,26 @@ cudaError_t expert_combine(int T, int top, int H, const void *Z, int type, int R
         using E = decltype(t);
         auto go = [&](auto many) {
             constexpr int U = decltype(many)::value;
-            if (vec) combine_rows<E, true, U><<<grid, 256, 0, st>>>((const E *)Z, ldz, R, rows, weights, T, top, H, (E *)Y, ldy);
-            else combine_rows<E, false, U><<<grid, 256, 0, st>>>((const E *)Z, ldz, R, rows, weights, T, top, H, (E *)Y, ldy);
+            e = launch_behind(vec ? combine_rows<E, true, U> : combine_rows<E, false, U>, grid, 256, 0, 1, st, (const E *)Z, ldz, R, rows, weights, T, top, H, (E *)Y, ldy);
         };
         if (top <= 2) go(std::integral_constant<int, 2>());
         else if (top <= 4) go(std::integral_constant<int, 4>());
         else go(std::integral_constant<int, 8>());
     });
-    return cudaGetLastError();
+    return e;
 }
 
 cudaError_t expert_combine_grad(int T, int top, int H, const void *dY, int type, long long lddy, const void *Z, long long ldz, int R, const int *rows,
                                 const int *slots, const float *weights, void *dZ, long long lddz, float *dweights, cudaStream_t st) {
+    cudaError_t e = cudaErrorInvalidValue;
     const int size = type_size(type);
     const bool vec = aligned(dY, lddy, size) && aligned(Z, ldz, size) && aligned(dZ, lddz, size);
     const int grid = grid_of(((long long)R + 7) / 8);
     with_type(type, [&](auto t) {
         using E = decltype(t);
-        if (vec) combine_grad_rows<E, true><<<grid, 256, 0, st>>>((const E *)dY, lddy, (const E *)Z, ldz, R, rows, slots, weights, T * top, top, H, (E *)dZ, lddz, dweights);
-        else combine_grad_rows<E, false><<<grid, 256, 0, st>>>((const E *)dY, lddy, (const E *)Z, ldz, R, rows, slots, weights, T * top, top, H, (E *)dZ, lddz, dweights);
+        e = launch_behind(vec ? combine_grad_rows<E, true> : combine_grad_rows<E, false>, grid, 256, 0, 1, st, (const E *)dY, lddy, (const E *)Z, ldz, R, rows, slots, weights, T * top, top, H, (E *)dZ, lddz, dweights);
     });
-    return cudaGetLastError();
+    return e;
 }
 
 }  // namespace ozk

@@ -11,6 +11,7 @@
 #include <type_traits>
 #include "oz_common.cuh"
 #include "oz_kernels.h"
+#include "oz_launch.cuh"
 #include "oz_types.cuh"
 
 namespace ozk {
@@ -75,7 +76,7 @@ __device__ __forceinline__ uint32_t magnitude(float x) { return __float_as_uint(
 // the row of X that vector or element r takes its values from; -1: none (zeros)
 __device__ __forceinline__ long long source_row(const int *slots, int per, int sources, int r) {
     if (!slots) return r;
-    const int s = __ldg(slots + r);
+    const int s = slots[r];
     if (s < 0) return -1;
     const int row = s / per;
     return row < sources ? row : -1;
@@ -101,29 +102,31 @@ template <class T> __device__ __forceinline__ uint32_t magnitude_of(const uint4 
 // ROUTED: the warp's row is a token, rounded once and written to the rows of all its slots; then rows without a slot are looked for,
 // 32 at a time, and become zeros.
 constexpr int UNITS = 4;
-template <class T, bool VEC, bool ROUTED>
+template <class T, bool VEC, bool ROUTED, int U>
 __global__ void __launch_bounds__(256) mx4_rows(const T *X, int nvec, int len, long long ldx, size_t plane_x, int planes, int rule,
                                                 const int *row_of, const int *slot_of, int top, int tokens, uint8_t *codes, long long ldq,
                                                 size_t plane_q, uint8_t *scales, long long lds, size_t plane_s) {
+    behind_predecessors();
     constexpr int N = Vec16<T>::N, LOAD = 32 * N, SHARE = 32 / N;   // values of a lane, of a load of the warp; lanes of a block
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const uint32_t units = (len + LOAD * UNITS - 1) / (LOAD * UNITS);
+    const uint32_t units = (len + LOAD * U - 1) / (LOAD * U);
     const long long total = (long long)(ROUTED ? tokens : (long long)planes * nvec) * units;
     for (long long w = (long long)blockIdx.x * 8 + warp; w < total; w += (long long)gridDim.x * 8) {
         const long long vec = total < 0x80000000ll ? (long long)((uint32_t)w / units) : w / units;
         const long long z = planes > 1 ? vec / nvec : 0, r = vec - z * nvec;
-        const int at = (int)(w - vec * units) * LOAD * UNITS + lane * N;   // the lane's first value
+        const int at = (int)(w - vec * units) * LOAD * U + lane * N;   // the lane's first value
         const T *x = X + z * plane_x + r * ldx;
-        uint4 q[UNITS];
+        uint4 q[U];
+        int mine = -1;   // ROUTED: 32 of the token's rows, a lane each
         if constexpr (VEC) {   // rows start on 16 bytes and end on them; loads behind the end are made at the end, and cleared
 #pragma unroll
-            for (int u = 0; u < UNITS; u++) q[u] = __ldg(reinterpret_cast<const uint4 *>(x + min(at + u * LOAD, len - N)));
+            for (int u = 0; u < U; u++) q[u] = *reinterpret_cast<const uint4 *>(x + min(at + u * LOAD, len - N));
 #pragma unroll
-            for (int u = 0; u < UNITS; u++)
+            for (int u = 0; u < U; u++)
                 if (at + u * LOAD >= len) q[u] = make_uint4(0, 0, 0, 0);
         } else {   // value by value, zeros behind the last
 #pragma unroll
-            for (int u = 0; u < UNITS; u++) {
+            for (int u = 0; u < U; u++) {
                 T v[N];
 #pragma unroll
                 for (int i = 0; i < N; i++) v[i] = x[min(at + u * LOAD + i, len - 1)];
@@ -134,7 +137,7 @@ __global__ void __launch_bounds__(256) mx4_rows(const T *X, int nvec, int len, l
             }
         }
 #pragma unroll
-        for (int u = 0; u < UNITS; u++) {
+        for (int u = 0; u < U; u++) {
             const int e = at + u * LOAD;
             if (e - lane * N >= len) break;   // the same for the whole warp
             uint32_t m = magnitude_of<T>(q[u]);
@@ -159,7 +162,8 @@ __global__ void __launch_bounds__(256) mx4_rows(const T *X, int nvec, int len, l
             };
             if constexpr (ROUTED) {
                 for (int j = 0; j < top; j++) {
-                    const int row = __ldg(row_of + r * top + j);
+                    if (j % 32 == 0) mine = j + lane < top ? row_of[r * top + j + lane] : -1;
+                    const int row = __shfl_sync(~0u, mine, j % 32);
                     if (row >= 0 && row < nvec) write(codes + (size_t)row * ldq, scales + (size_t)row * lds);
                 }
             } else write(codes + z * plane_q + r * ldq, scales + z * plane_s + r * lds);
@@ -169,7 +173,7 @@ __global__ void __launch_bounds__(256) mx4_rows(const T *X, int nvec, int len, l
         const long long slots = (long long)tokens * top;
         const int blocks = (len + 31) / 32;
         for (long long r0 = ((long long)blockIdx.x * 8 + warp) * 32; r0 < nvec; r0 += (long long)gridDim.x * 256) {
-            const int s = r0 + lane < nvec ? __ldg(slot_of + r0 + lane) : 0;
+            const int s = r0 + lane < nvec ? slot_of[r0 + lane] : 0;
             uint32_t none = __ballot_sync(~0u, s < 0 || s >= slots);
             while (none) {
                 const long long r = r0 + __ffs(none) - 1;
@@ -192,6 +196,7 @@ template <class T, bool VEC>
 __global__ void __launch_bounds__(256) mx4_cols(const T *X, int nvec, int len, long long ldx, size_t plane_x, int rule, const int *slots,
                                                 int per, int sources, uint8_t *codes, long long ldq, size_t plane_q, uint8_t *scales,
                                                 long long lds, size_t plane_s, int col_tiles, int row_tiles) {
+    behind_predecessors();
     __shared__ __align__(16) uint8_t tile[CT_COLS * CT_PITCH];
     __shared__ __align__(8) uint8_t stile[CT_COLS * 8];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -254,6 +259,7 @@ __global__ void __launch_bounds__(256) mx4_cols(const T *X, int nvec, int len, l
 template <class T, bool VEC>
 __global__ void __launch_bounds__(256) mx4_values(const uint8_t *codes, long long ldq, const uint8_t *scales, long long lds, int nvec, int len,
                                                   T *Y, long long ldy) {
+    behind_predecessors();
     __shared__ float turn[VEC ? 1 : 8][32 * 17];
     constexpr int N = Vec16<T>::N, LOAD = VEC ? 32 * N : 512, PIECE = VEC ? LOAD * UNITS : LOAD;
     const int lane = threadIdx.x & 31;
@@ -271,8 +277,8 @@ __global__ void __launch_bounds__(256) mx4_values(const uint8_t *codes, long lon
             for (int u = 0; u < UNITS; u++) {
                 const int e = min(at + u * LOAD + lane * N, len - N);
                 // four codes: the half of an aligned word that holds them
-                q[u] = __ldg(reinterpret_cast<const uint32_t *>(c + ((e >> 1) & ~3))) >> (N == 8 ? 0 : 4 * (e & 4));
-                b[u] = __ldg(s + (e >> 5));
+                q[u] = *reinterpret_cast<const uint32_t *>(c + ((e >> 1) & ~3)) >> (N == 8 ? 0 : 4 * (e & 4));
+                b[u] = s[e >> 5];
             }
 #pragma unroll
             for (int u = 0; u < UNITS; u++) {
@@ -287,8 +293,8 @@ __global__ void __launch_bounds__(256) mx4_values(const uint8_t *codes, long lon
             const int i0 = at + lane * 16;
             float v[16];
             if (i0 < len) {
-                const uint2 q = __ldg(reinterpret_cast<const uint2 *>(c + (i0 >> 1)));
-                const float scale = scale_of(__ldg(s + (i0 >> 5)));
+                const uint2 q = *reinterpret_cast<const uint2 *>(c + (i0 >> 1));
+                const float scale = scale_of(s[i0 >> 5]);
                 values_of<8>(q.x, v);
                 values_of<8>(q.y, v + 8);
 #pragma unroll
@@ -321,20 +327,27 @@ cudaError_t mx4_quantize_rows(const void *X, int type, int nvec, int len, long l
     const int size = type_size(type);
     const bool vec = !(reinterpret_cast<uintptr_t>(X) & 15) && !(ldx * size & 15) && !(plane_x * size & 15) && !((long long)len * size & 15);
     const long long vectors = slots ? tokens : (long long)planes * nvec;
-    const int unit = 512 / size * UNITS;   // values that a warp takes at a time
+    const int load = 512 / size;   // values that a warp loads at a time
+    const bool few = vectors * ((len + load - 1) / load) < 148 * 16;
+    const int unit = few ? load : load * UNITS;
     const int grid = warp_grid(vectors * ((len + unit - 1) / unit) + (slots ? nvec / 32 : 0));
+    cudaError_t e = cudaErrorInvalidValue;
     with_type(type, [&](auto t) {
         using T = decltype(t);
         auto go = [&](auto vec_, auto routed_) {
-            mx4_rows<T, decltype(vec_)::value, decltype(routed_)::value><<<grid, 256, 0, st>>>((const T *)X, nvec, len, ldx, plane_x, planes, rule, rows, slots, top,
-                                                                                               tokens, codes, ldq, plane_q, scales, lds, plane_s);
+            constexpr bool v = decltype(vec_)::value, r = decltype(routed_)::value;
+            // four loads in flight to a warp, or one where there are few: (16, 4096) values 2.4 and 1.9 us, (2048, 7168) 8.6 and 13.4
+            e = few ? launch_behind(mx4_rows<T, v, r, 1>, grid, 256, 0, 1, st, (const T *)X, nvec, len, ldx, plane_x, planes, rule, rows, slots, top, tokens, codes, ldq,
+                                    plane_q, scales, lds, plane_s)
+                    : launch_behind(mx4_rows<T, v, r, UNITS>, grid, 256, 0, 1, st, (const T *)X, nvec, len, ldx, plane_x, planes, rule, rows, slots, top, tokens, codes,
+                                    ldq, plane_q, scales, lds, plane_s);
         };
         if (vec && slots) go(std::true_type(), std::true_type());
         else if (vec) go(std::true_type(), std::false_type());
         else if (slots) go(std::false_type(), std::true_type());
         else go(std::false_type(), std::false_type());
     });
-    return cudaGetLastError();
+    return e;
 }
 
 cudaError_t mx4_quantize_cols(const void *X, int type, int nvec, int len, long long ldx, size_t plane_x, int planes, int rule, const int *,
@@ -345,26 +358,27 @@ cudaError_t mx4_quantize_cols(const void *X, int type, int nvec, int len, long l
     const int col_tiles = (nvec + CT_COLS - 1) / CT_COLS, row_tiles = (len + CT_ROWS - 1) / CT_ROWS;
     const long long grid = (long long)col_tiles * row_tiles * planes;
     if (grid > 0x7fffffffLL) return cudaErrorInvalidValue;
+    cudaError_t e = cudaErrorInvalidValue;
     with_type(type, [&](auto t) {
         using T = decltype(t);
-        if (vec) mx4_cols<T, true><<<(int)grid, 256, 0, st>>>((const T *)X, nvec, len, ldx, plane_x, rule, slots, top, tokens, codes, ldq, plane_q, scales, lds, plane_s, col_tiles, row_tiles);
-        else mx4_cols<T, false><<<(int)grid, 256, 0, st>>>((const T *)X, nvec, len, ldx, plane_x, rule, slots, top, tokens, codes, ldq, plane_q, scales, lds, plane_s, col_tiles, row_tiles);
+        e = launch_behind(vec ? mx4_cols<T, true> : mx4_cols<T, false>, (int)grid, 256, 0, 1, st, (const T *)X, nvec, len, ldx, plane_x, rule, slots, top, tokens, codes, ldq,
+                          plane_q, scales, lds, plane_s, col_tiles, row_tiles);
     });
-    return cudaGetLastError();
+    return e;
 }
 
 cudaError_t mx4_dequantize(const uint8_t *codes, long long ldq, const uint8_t *scales, long long lds, int nvec, int len, void *Y, int type,
                            long long ldy, cudaStream_t st) {
     const int size = type_size(type);
     const bool vec = !(reinterpret_cast<uintptr_t>(Y) & 15) && !(ldy * size & 15) && !((long long)len * size & 15);
+    cudaError_t e = cudaErrorInvalidValue;
     const int piece = vec ? 512 / size * UNITS : 512;   // values that a warp takes at a time
     const int grid = warp_grid((long long)nvec * ((len + piece - 1) / piece));
     with_type(type, [&](auto t) {
         using T = decltype(t);
-        if (vec) mx4_values<T, true><<<grid, 256, 0, st>>>(codes, ldq, scales, lds, nvec, len, (T *)Y, ldy);
-        else mx4_values<T, false><<<grid, 256, 0, st>>>(codes, ldq, scales, lds, nvec, len, (T *)Y, ldy);
+        e = launch_behind(vec ? mx4_values<T, true> : mx4_values<T, false>, grid, 256, 0, 1, st, codes, ldq, scales, lds, nvec, len, (T *)Y, ldy);
     });
-    return cudaGetLastError();
+    return e;
 }
 
 }  // namespace ozk

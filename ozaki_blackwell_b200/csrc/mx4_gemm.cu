@@ -34,6 +34,7 @@
 #include "oz_async.cuh"
 #include "oz_common.cuh"
 #include "oz_kernels.h"
+#include "oz_launch.cuh"
 #include "oz_types.cuh"
 
 namespace ozk {
@@ -140,8 +141,8 @@ struct Tile {
 
 // The range along k or of rows that `offsets` gives group g. Offsets that are out of order or out of range are cut to what is there.
 __device__ __forceinline__ void segment(const Params &p, int g, int limit, int &lo, int &hi) {
-    lo = min(max(__ldg(p.offsets + g), 0), limit);
-    hi = min(max(__ldg(p.offsets + g + 1), lo), limit);
+    lo = min(max(p.offsets[g], 0), limit);
+    hi = min(max(p.offsets[g + 1], lo), limit);
 }
 
 // item w -> tile; `cum` has the running number of token tiles (BY_ROWS). Bands of `band` tiles of P are walked tile of Q by tile of Q,
@@ -270,6 +271,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm(const __grid_constant__ C
             asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
         }
     }
+    behind_predecessors();
     if (warp == 2 && p.mode == BY_ROWS) {   // running number of token tiles over the groups
         int run = 0;
         for (int g0 = 0; g0 < p.groups; g0 += 32) {
@@ -483,10 +485,10 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm(const __grid_constant__ C
                         const int row = i * 32 + lane;
                         v[c][i] = make_uint4(0, 0, 0, 0);   // 2^-127: rows that are not there
                         if (c == 0) {
-                            if (p0 + row < t.p1) v[c][i] = __ldg(reinterpret_cast<const uint4 *>(sp + (size_t)(p0 + row) * p.ldsp));
+                            if (p0 + row < t.p1) v[c][i] = *reinterpret_cast<const uint4 *>(sp + (size_t)(p0 + row) * p.ldsp);
                         } else {
                             const int q = (c - 1) * 128 + row;
-                            if (q < BN && t.q0 + q < t.q1) v[c][i] = __ldg(reinterpret_cast<const uint4 *>(sq + (size_t)(t.q0 + q) * p.ldsq));
+                            if (q < BN && t.q0 + q < t.q1) v[c][i] = *reinterpret_cast<const uint4 *>(sq + (size_t)(t.q0 + q) * p.ldsq);
                         }
                     }
                 if (left < 16) {   // bytes behind the last block may hold anything: their codes are zero, their scales become it
@@ -652,18 +654,6 @@ cudaError_t launch(const Mx4Product &g, Params p, int sms, int split, cudaStream
     p.sp = S::wide ? g.xs : g.ws; p.ldsp = S::wide ? g.ldxs : g.ldws; p.plane_sp = S::wide ? 0 : plane;
     p.sq = S::wide ? g.ws : g.xs; p.ldsq = S::wide ? g.ldws : g.ldxs; p.plane_sq = S::wide ? plane : 0;
     const int per = FORM == SPLIT ? split : FORM == PAIR ? 2 : 1;   // CTAs to a cluster
-    cudaLaunchConfig_t cfg = {};
-    cfg.blockDim = dim3(THREADS);
-    cfg.dynamicSmemBytes = S::SMEM;
-    cfg.stream = st;
-    cudaLaunchAttribute at[1];
-    if (per > 1) {
-        at[0].id = cudaLaunchAttributeClusterDimension;
-        at[0].val.clusterDim.x = per;
-        at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-        cfg.attrs = at;
-        cfg.numAttrs = 1;
-    }
     // A persistent grid must be resident as a whole: a pair that started behind another would find its share of the tiles still to do.
     // Not every SM has a neighbour to pair with (74 pairs were asked for, and the product took twice its time).
     long long clusters = w.most;
@@ -675,7 +665,16 @@ cudaError_t launch(const Mx4Product &g, Params p, int sms, int split, cudaStream
             if ((e = cudaGetDevice(&dev))) return e;
             int &n = pairs[dev & 63];
             if (!n) {
+                cudaLaunchConfig_t cfg = {};
                 cfg.gridDim = dim3((unsigned)(sms & ~1));
+                cfg.blockDim = dim3(THREADS);
+                cfg.dynamicSmemBytes = S::SMEM;
+                cudaLaunchAttribute at[1];
+                at[0].id = cudaLaunchAttributeClusterDimension;
+                at[0].val.clusterDim.x = per;
+                at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+                cfg.attrs = at;
+                cfg.numAttrs = 1;
                 int found = 0;
                 if (cudaOccupancyMaxActiveClusters(&found, mx4_gemm<FORM, BN, T>, &cfg) != cudaSuccess || found <= 0) { cudaGetLastError(); found = sms / 2; }
                 n = found;
@@ -684,8 +683,7 @@ cudaError_t launch(const Mx4Product &g, Params p, int sms, int split, cudaStream
         }
         if (clusters > room) clusters = room;
     }
-    cfg.gridDim = dim3((unsigned)(clusters * per));
-    return cudaLaunchKernelEx(&cfg, mx4_gemm<FORM, BN, T>, S::wide ? x : w4, S::wide ? w4 : x, p);
+    return launch_behind(mx4_gemm<FORM, BN, T>, (int)(clusters * per), THREADS, S::SMEM, per, st, S::wide ? x : w4, S::wide ? w4 : x, p);
 }
 
 }  // namespace m4
