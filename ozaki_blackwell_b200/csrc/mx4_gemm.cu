@@ -46,7 +46,7 @@ constexpr int BK = 256, BKB = 128; // k of a stage, in values and in bytes
 constexpr int UK = 64;             // k of one tcgen05.mma kind::mxf4
 constexpr int TURNERS = 4, THREADS = 512;   // warp 11 is idle: the epilogue's second four must be warps 0 .. 3 modulo 4
 constexpr int MAX_GROUPS = 1024;
-constexpr int AHEAD = 64;          // tiles of a CTA that are worked out before it starts
+constexpr int AHEAD = 48;          // tiles of a CTA that are worked out before it starts
 
 enum { DENSE = 0, BY_ROWS = 1, ALONG_K = 2 };
 enum { NARROW = 0, SPLIT = 1, WIDE = 2, PAIR = 3 };
@@ -61,6 +61,7 @@ struct Params {
     size_t plane_sp, plane_sq;      // bytes between two groups' (0: shared)
     void *Y;
     long long ldy;
+    int whole_words;                // Y's rows start on 16 bytes: mapY is one of it
     size_t plane_y;                 // elements between the results of two groups (ALONG_K)
     int *status;
 };
@@ -78,10 +79,11 @@ template <int FORM, int BN> struct Shape {
     // A multiple of the turning warps, so that a slot is always the same warp's: a warp that came to a slot before another had seen the
     // slot's last use would take the parity of the use before that for its own.
     static constexpr int SLOTS = FORM == WIDE ? TURNERS : 2 * TURNERS;
+    static_assert(SLOT % 512 == 0, "the pieces behind the slots are swizzled");
     static constexpr int COLS = 2 * BN + STAGES * SCALE_COLS;      // two accumulators, and the scales
     static constexpr int TMEM_COLS = COLS <= 256 ? 256 : 512;
     static constexpr int BARS = 2 * STAGES + 2 * SLOTS + 4;
-    static constexpr int TURN = wide ? 8 * 32 * (64 + 16) : 0;     // what the epilogue's warps turn their tiles through
+    static constexpr int TURN = wide ? 8 * 2 * 2048 : 0;            // two pieces of 32 rows x 64 bytes to each warp of the epilogue
     static constexpr int SMEM = STAGES * STAGE + SLOTS * SLOT + TURN + 1024 + 8 * BARS + 16 + 4 * (MAX_GROUPS + 4) + AHEAD * 32;
     static_assert(STAGE % 1024 == 0 && COLS <= 512 && SMEM <= 232448 - 64, "");
     static_assert(FORM != SPLIT || BN * BP * 4 <= STAGES * STAGE, "the partial tile of a split takes the place of the stages");
@@ -185,53 +187,100 @@ __device__ __forceinline__ Tile decode(const Params &p, const int *cum, int w) {
     return t;
 }
 
-// 32 columns of a tile, v[c] = column j + c of the lane's row. NARROW: Y's rows are the columns j, a warp stores 32 lanes side by side.
+// 32 columns of a tile, v[c] = column j + c of the lane's row. NARROW: Y's rows are the columns j, a warp stores 32 lanes side by side;
+// 16-bit values change places with the neighbour lane's, so that one 4-byte store serves two rows of Y.
 template <class T>
-__device__ __forceinline__ void store_narrow(T *Y, long long ldy, const uint32_t (&v)[32], int i, int i1, int j, int j1) {
-    if (i >= i1) return;
-    T *dst = Y + (size_t)j * ldy + i;
+__device__ __forceinline__ void store_narrow(T *Y, long long ldy, const uint32_t (&v)[32], int i0, int lane, int i1, int j, int j1) {
+    T *dst = Y + (size_t)j * ldy + i0 + lane;
+    if constexpr (sizeof(T) == 2) {
+        if (i0 + 32 <= i1 && !((reinterpret_cast<uintptr_t>(Y) & 3) | (ldy & 1))) {
+            const bool odd = lane & 1;
+#pragma unroll
+            for (int c = 0; c < 32; c += 2) {
+                const uint32_t own = Vec16<T>::word(__uint_as_float(v[c]), __uint_as_float(v[c + 1])), other = __shfl_xor_sync(~0u, own, 1);
+                const uint32_t w = odd ? __byte_perm(other, own, 0x7632) : __byte_perm(own, other, 0x5410);   // row c of lanes l, l + 1; or row c + 1 of l - 1, l
+                if (j + c + odd < j1) *reinterpret_cast<uint32_t *>(dst + (size_t)(c + odd) * ldy - odd) = w;
+            }
+            return;
+        }
+    }
+    if (i0 + lane >= i1) return;
 #pragma unroll
     for (int c = 0; c < 32; c++)
         if (j + c < j1) dst[(size_t)c * ldy] = from_f32<T>(__uint_as_float(v[c]));
 }
-// WIDE: Y's row is the lane's. Whole pieces turn through the warp's shared memory, so that four lanes store 64 contiguous bytes of a row
-// (whole sectors; a lane's own 16-byte stores to 32 rows at a time took the L2 twice as long). Columns at the edge, or rows that do not
-// start on 16 bytes, are stored one by one.
-constexpr int TURN_PITCH = 64 + 16, TURN_BYTES = 32 * TURN_PITCH;
+// WIDE: Y's row is the lane's. Whole 64-byte pieces of 32 rows go to the warp's shared memory (16-byte words permuted by their row, as
+// the TMA unit's 64-byte swizzle has them, so that no two lanes meet in a bank) and from there by TMA, which takes them while the warp
+// goes on: with stores of its own the warp held its accumulator until the L2 had taken them (segments of 512 tokens: 39 us for 100
+// MB). Where the group's rows end inside the piece, four lanes store 64 contiguous bytes of each row that is there. Rows that do not
+// start on 16 bytes are stored value by value.
+struct Piece {
+    uint8_t *buffer;       // two of 2048 bytes
+    uint32_t used;         // pieces so far
+    uint64_t policy;       // Y is not read here: its lines are the first to leave the L2
+};
 template <class T>
-__device__ __forceinline__ void store_wide(T *Y, long long ldy, const uint32_t (&v)[32], int i0, int lane, int i1, int j, int j1, uint8_t *turn) {
-    if (j >= j1) return;
+__device__ __forceinline__ void store_wide(const CUtensorMap *map, bool whole_words, T *Y, long long ldy, const uint32_t (&v)[32], int i0, int lane, int i1, int j, int j1,
+                                           int group, Piece &piece) {
+    if (j >= j1 || i0 >= i1) return;
     constexpr int N = Vec16<T>::N, COLS = 4 * N;   // columns to 16 and to 64 bytes
-    if (j + 32 <= j1 && !((reinterpret_cast<uintptr_t>(Y + j) | (uintptr_t)(ldy * (long long)sizeof(T))) & 15)) {
+    if (!whole_words) {
+        if (i0 + lane < i1) {
+            T *dst = Y + (size_t)(i0 + lane) * ldy + j;
 #pragma unroll
-        for (int h = 0; h < 32; h += COLS) {
+            for (int c = 0; c < 32; c++)
+                if (j + c < j1) dst[c] = from_f32<T>(__uint_as_float(v[c]));
+        }
+        return;
+    }
 #pragma unroll
-            for (int c = 0; c < 4; c++) {
-                float f[N];
+    for (int h = 0; h < 32; h += COLS) {
+        if (j + h >= j1) break;
+        uint8_t *buf = piece.buffer + 2048 * (piece.used++ & 1);
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");   // the piece before the last has left its buffer
+        __syncwarp();
 #pragma unroll
-                for (int e = 0; e < N; e++) f[e] = __uint_as_float(v[h + c * N + e]);
-                *reinterpret_cast<uint4 *>(turn + lane * TURN_PITCH + 16 * c) = Vec16<T>::pack(f);
+        for (int c = 0; c < 4; c++) {
+            float f[N];
+#pragma unroll
+            for (int e = 0; e < N; e++) f[e] = __uint_as_float(v[h + c * N + e]);
+            *reinterpret_cast<uint4 *>(buf + lane * 64 + 16 * (c ^ (lane >> 1 & 3))) = Vec16<T>::pack(f);
+        }
+        if (i0 + 32 <= i1) {   // columns behind the last are cut by the tensor map
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) {
+                asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group.L2::cache_hint [%0, {%2, %3, %4}], [%1], %5;"
+                             ::"l"(map), "r"(smem_u32(buf)), "r"((j + h) * (int)sizeof(T)), "r"(i0), "r"(group), "l"(piece.policy) : "memory");
+                asm volatile("cp.async.bulk.commit_group;" ::: "memory");
             }
+        } else {
             __syncwarp();
 #pragma unroll
             for (int r = 0; r < 32; r += 8) {
-                const int row = r + (lane >> 2);
-                const uint4 q = *reinterpret_cast<const uint4 *>(turn + row * TURN_PITCH + 16 * (lane & 3));
-                if (i0 + row < i1) __stcs(reinterpret_cast<uint4 *>(Y + (size_t)(i0 + row) * ldy + j + h + (lane & 3) * N), q);   // not read here again: the operands keep their place in L2
+                const int row = r + (lane >> 2), c = lane & 3;
+                const uint4 q = *reinterpret_cast<const uint4 *>(buf + row * 64 + 16 * (c ^ (row >> 1 & 3)));
+                T *dst = Y + (size_t)(i0 + row) * ldy + j + h + c * N;
+                if (i0 + row < i1) {
+                    if (j + h + (c + 1) * N <= j1) __stcs(reinterpret_cast<uint4 *>(dst), q);
+                    else {
+                        float f[N];
+                        Vec16<T>::unpack(q, f);
+#pragma unroll
+                        for (int e = 0; e < N; e++)
+                            if (j + h + c * N + e < j1) dst[e] = from_f32<T>(f[e]);
+                    }
+                }
             }
+            if (lane == 0) asm volatile("cp.async.bulk.commit_group;" ::: "memory");   // an empty one, to keep the count
             __syncwarp();
         }
-    } else if (i0 + lane < i1) {
-        T *dst = Y + (size_t)(i0 + lane) * ldy + j;
-#pragma unroll
-        for (int c = 0; c < 32; c++)
-            if (j + c < j1) dst[c] = from_f32<T>(__uint_as_float(v[c]));
     }
 }
 
 template <int FORM, int BN, class T>
 __global__ void __launch_bounds__(THREADS, 1) mx4_gemm(const __grid_constant__ CUtensorMap mapP, const __grid_constant__ CUtensorMap mapQ,
-                                                       const Params p) {
+                                                       const __grid_constant__ CUtensorMap mapY, const Params p) {
     using S = Shape<FORM, BN>;
     constexpr bool pair = S::pair;
     extern __shared__ uint8_t smem_raw[];
@@ -521,6 +570,8 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm(const __grid_constant__ C
         }
     } else if (warp != 11) {
         const int quarter = warp & 3, half = warp >= 12;   // lanes 32 quarter .. +31, every other 32 columns
+        Piece piece = {base_ptr + S::STAGES * S::STAGE + S::SLOTS * S::SLOT + (quarter + 4 * half) * 4096, 0, 0};
+        asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(piece.policy));
         uint32_t n = 0;
         for (int w = first; w < total && !__any_sync(~0u, *abortp); w += step, n++) {
             const Tile t = tile_at(w, n);
@@ -543,8 +594,8 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm(const __grid_constant__ C
                         for (int e = 0; e < 32; e++) v[e] = 0;
                     }
                     const int j1 = min(t.q1, t.q0 + BN);   // a tile of 16 columns: the other 16 are not its own
-                    if constexpr (S::wide) store_wide<T>(Y, p.ldy, v, i0, lane, t.p1, t.q0 + c, j1, base_ptr + S::STAGES * S::STAGE + S::SLOTS * S::SLOT + (quarter + 4 * half) * TURN_BYTES);
-                    else store_narrow<T>(Y, p.ldy, v, i0 + lane, t.p1, t.q0 + c, j1);
+                    if constexpr (S::wide) store_wide<T>(&mapY, p.whole_words, Y, p.ldy, v, i0, lane, t.p1, t.q0 + c, j1, p.mode == ALONG_K ? t.group : 0, piece);
+                    else store_narrow<T>(Y, p.ldy, v, i0, lane, t.p1, t.q0 + c, j1);
                 }
             } else {   // the partial tile, [column][row of P], over the stages that this CTA has used up
                 float *part = reinterpret_cast<float *>(base_ptr);
@@ -565,6 +616,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm(const __grid_constant__ C
                 else mbar_arrive(accempty_bar(acc));
             }
         }
+        if (S::wide && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");   // every piece is in Y
     }
 
     __syncwarp();
@@ -638,6 +690,19 @@ Work work_of(const Mx4Product &g, int tokens, int weights) {
     return {(some + g.tokens / tokens) * nw, some * ((each + tokens - 1) / tokens) * nw};
 }
 
+// {bytes of a row, row, group} of Y, in boxes of 64 bytes by 32 rows
+cudaError_t make_map_y(CUtensorMap *map, void *y, long long bytes, int rows, int groups, long long ld, size_t plane) {
+    EncodeTiledFn enc = encode_fn();
+    if (!enc) return cudaErrorNotSupported;
+    const cuuint64_t dims[3] = {(cuuint64_t)bytes, (cuuint64_t)rows, (cuuint64_t)groups};
+    const cuuint64_t strides[2] = {(cuuint64_t)ld, (cuuint64_t)(groups > 1 ? plane : (size_t)ld * rows)};
+    const cuuint32_t box[3] = {64, 32, 1};
+    const cuuint32_t estr[3] = {1, 1, 1};
+    const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, y, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B,
+                           CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
 template <int FORM, int BN, class T>
 cudaError_t launch(const Mx4Product &g, Params p, int sms, int split, cudaStream_t st) {
     using S = Shape<FORM, BN>;
@@ -650,16 +715,20 @@ cudaError_t launch(const Mx4Product &g, Params p, int sms, int split, cudaStream
     CUtensorMap x, w4;
     if ((e = make_map(&x, g.x, g.K, g.tokens, 1, g.ldx, 0, S::wide ? BP : S::Q_ROWS))) return e;
     if ((e = make_map(&w4, g.w, g.K, g.weights, planes, g.ldw, g.plane_w, S::wide ? S::Q_ROWS : BP))) return e;
+    CUtensorMap y = x;
+    const int results = g.mode == ALONG_K ? g.groups : 1;
+    p.whole_words = S::wide && !(reinterpret_cast<uintptr_t>(g.y) & 15) && !(g.ldy * sizeof(T) & 15) && !(results > 1 && (g.plane_y * sizeof(T) & 15));
+    if (p.whole_words && (e = make_map_y(&y, g.y, (long long)g.weights * sizeof(T), g.tokens, results, g.ldy * sizeof(T), g.plane_y * sizeof(T)))) return e;
     const size_t plane = planes > 1 ? g.plane_ws : 0;
     p.sp = S::wide ? g.xs : g.ws; p.ldsp = S::wide ? g.ldxs : g.ldws; p.plane_sp = S::wide ? 0 : plane;
     p.sq = S::wide ? g.ws : g.xs; p.ldsq = S::wide ? g.ldws : g.ldxs; p.plane_sq = S::wide ? plane : 0;
-    const int per = FORM == SPLIT ? split : FORM == PAIR ? 2 : 1;   // CTAs to a cluster
+    const int per = FORM == SPLIT ? split : S::pair ? 2 : 1;   // CTAs to a cluster
     // A persistent grid must be resident as a whole: a pair that started behind another would find its share of the tiles still to do.
     // Not every SM has a neighbour to pair with (74 pairs were asked for, and the product took twice its time).
     long long clusters = w.most;
     if (FORM != SPLIT) {
         long long room = sms;
-        if (FORM == PAIR) {
+        if (S::pair) {
             static int pairs[64] = {};
             int dev = 0;
             if ((e = cudaGetDevice(&dev))) return e;
@@ -683,7 +752,7 @@ cudaError_t launch(const Mx4Product &g, Params p, int sms, int split, cudaStream
         }
         if (clusters > room) clusters = room;
     }
-    return launch_behind(mx4_gemm<FORM, BN, T>, (int)(clusters * per), THREADS, S::SMEM, per, st, S::wide ? x : w4, S::wide ? w4 : x, p);
+    return launch_behind(mx4_gemm<FORM, BN, T>, (int)(clusters * per), THREADS, S::SMEM, per, st, S::wide ? x : w4, S::wide ? w4 : x, y, p);
 }
 
 }  // namespace m4
@@ -712,7 +781,7 @@ cudaError_t mx4_product(const Mx4Product &g, int *status, cudaStream_t st) {
     };
 #define M4_FORM(F) std::integral_constant<int, F>()
     // many tokens to a group, and at least half a tile for every SM: tokens as lanes; a pair of CTAs where there is enough for all pairs
-    if (each > 128 && work_of(g, 2 * BP, 192).expected >= sms / 2 && (g.mode != BY_ROWS || each >= 1024)) run(M4_FORM(PAIR), M4_FORM(192), 1);
+    if (each > 128 && work_of(g, 2 * BP, 192).expected >= sms / 2 && (g.mode != BY_ROWS || each >= 512)) run(M4_FORM(PAIR), M4_FORM(192), 1);
     else if (each > 128 && work_of(g, BP, 192).expected * 2 >= sms) run(M4_FORM(WIDE), M4_FORM(192), 1);
     else {
         // few: weights as lanes; few tiles as well: k split, while every CTA keeps at least four stages
