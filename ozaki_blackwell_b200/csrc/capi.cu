@@ -451,10 +451,10 @@ OZB_API const char *ozb_version(void) { return OZB_VERSION; }
 OZB_API const char *ozb_error(int e) {
     switch (e) {
     case 0: return "ok";
-    case OZB_EARG: return "M, N and K must be positive";
+    case OZB_EARG: return "M, N and K must be positive, and every other argument there, aligned and in its range";
     case OZB_EK: return "K must be below 131072 (the int32 accumulators of the INT8 GEMMs)";
     case OZB_EARCH: return "this build runs on compute capability 10.x GPUs (B200, sm_100a: tcgen05 tensor cores) only";
-    case OZB_ETIMEOUT: return "a bounded wait inside the INT8 GEMM kernel expired; the result is not valid";
+    case OZB_ETIMEOUT: return "a bounded wait inside a GEMM kernel expired; the result is not valid";
     case OZB_ENOTBUILT: return "this entry point is exported for ABI compatibility but not built in this library";
     case OZB_ESIZE: return "a size exceeds the fixed limit of this entry point";
     case OZB_ECOMM: return "the exchange between GPUs failed or did not finish in time; the communicator was aborted";

@@ -19,7 +19,8 @@ namespace ozk {
 namespace {
 
 constexpr int MAX_EXPERTS = 1024;
-constexpr int CHUNK = 1024, SORT_THREADS = 256, SORT_WARPS = 8, PER_WARP = CHUNK / SORT_WARPS, ROUNDS = PER_WARP / 32;
+constexpr int FEW_CHUNKS = 256;   // up to here every block adds up all chunks' counts itself
+constexpr int CHUNK = 1024, SORT_THREADS = 256, SORT_WARPS = 8, PER_WARP = CHUNK / SORT_WARPS, ROUNDS = PER_WARP / 32, PLACE_THREADS = 1024;
 
 // the expert of slot s, or `experts` for a dropped one
 __device__ __forceinline__ int key_of(const void *ids, int id_bytes, int experts, int s) {
@@ -30,7 +31,7 @@ __device__ __forceinline__ int key_of(const void *ids, int id_bytes, int experts
 struct SortShared {
     int count[SORT_WARPS][MAX_EXPERTS];
     int total[MAX_EXPERTS], before[MAX_EXPERTS];
-    int warp_sum[SORT_WARPS];
+    int warp_sum[32];
 };
 
 // Ranks of a chunk's slots among its slots of the same expert, in their order. A warp owns PER_WARP consecutive slots and takes them 32
@@ -78,8 +79,9 @@ __device__ __forceinline__ void rank_slots(SortShared &sh, const void *ids, int 
 }
 
 // Where each segment begins, from the padded totals: total[e] becomes it, `offsets` is written if it is not null.
+template <int THREADS>
 __device__ __forceinline__ void place_segments(SortShared &sh, int experts, int align, int *offsets) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, per = (experts + SORT_THREADS - 1) / SORT_THREADS;   // consecutive experts to a thread
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, per = (experts + THREADS - 1) / THREADS;   // consecutive experts to a thread
     int sum = 0;
     for (int i = 0; i < per; i++) {
         const int e = threadIdx.x * per + i;
@@ -109,14 +111,16 @@ __device__ __forceinline__ void place_segments(SortShared &sh, int experts, int 
 
 // Up to CHUNK slots: one block does it all. More: sort_count ranks the slots of each chunk (row_of holds the ranks meanwhile), counts
 // them by expert and clears slot_of; sort_place adds up the counts -- of all chunks for the segments' lengths, of the chunks before its
-// own for where its slots go -- and writes both maps. All counts are whole numbers: the order is the same on every run.
+// own for where its slots go -- and writes both maps. With more than FEW_CHUNKS that would be the square of their number, so sort_scan
+// comes between, which turns the counts into running sums over the chunks. All counts are whole numbers: the order is the same on
+// every run.
 __global__ void __launch_bounds__(SORT_THREADS) sort_one(const void *ids, int id_bytes, int experts, int slots, int align, int R, int *offsets, int *row_of, int *slot_of) {
     behind_predecessors();
     __shared__ SortShared sh;
     for (int r = threadIdx.x; r < R; r += SORT_THREADS) slot_of[r] = -1;
     int key[ROUNDS], rank[ROUNDS];
     rank_slots(sh, ids, id_bytes, experts, slots, 0, key, rank);
-    place_segments(sh, experts, align, offsets);
+    place_segments<SORT_THREADS>(sh, experts, align, offsets);
 #pragma unroll
     for (int i = 0; i < ROUNDS; i++) {
         const int s = (threadIdx.x >> 5) * PER_WARP + i * 32 + (threadIdx.x & 31);
@@ -141,41 +145,75 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_count(const void *ids, int 
     for (int e = threadIdx.x; e < experts; e += SORT_THREADS) counts[(size_t)blockIdx.x * experts + e] = sh.total[e];
 }
 
-__global__ void __launch_bounds__(SORT_THREADS) sort_place(const void *ids, int id_bytes, int experts, int slots, int align, int R, int *offsets,
-                                                           int *row_of, int *slot_of, const int *counts) {
-    behind_predecessors();
-    __shared__ SortShared sh;
-    int rank[CHUNK / SORT_THREADS], key[CHUNK / SORT_THREADS];
-#pragma unroll
-    for (int i = 0; i < CHUNK / SORT_THREADS; i++) {
-        const int s = blockIdx.x * CHUNK + i * SORT_THREADS + threadIdx.x;
-        key[i] = s < slots ? key_of(ids, id_bytes, experts, s) : experts;
-        rank[i] = s < slots ? row_of[s] : 0;
-    }
-    for (int e = threadIdx.x; e < experts; e += SORT_THREADS) sh.total[e] = sh.before[e] = 0;
+// total[e] = all chunks' counts, before[e] = those of the chunks before this block's; eight loads in flight to a thread (of 1024: with 256 the 16384 counts of
+// 128 chunks by 128 experts took 8 us)
+__device__ __forceinline__ void add_counts(SortShared &sh, const int *counts, int experts) {
+    for (int e = threadIdx.x; e < experts; e += PLACE_THREADS) sh.total[e] = sh.before[e] = 0;
     __syncthreads();
-    // all chunks' counts, eight loads in flight to a thread
-    const int n = gridDim.x * experts, own = blockIdx.x * experts, step = SORT_THREADS % experts;
+    const int n = gridDim.x * experts, own = blockIdx.x * experts, step = PLACE_THREADS % experts;
     int e = threadIdx.x % experts;
-    for (int i0 = threadIdx.x; i0 < n; i0 += 8 * SORT_THREADS) {
+    for (int i0 = threadIdx.x; i0 < n; i0 += 8 * PLACE_THREADS) {
         int c[8];
 #pragma unroll
-        for (int k = 0; k < 8; k++) c[k] = i0 + k * SORT_THREADS < n ? counts[i0 + k * SORT_THREADS] : 0;
+        for (int k = 0; k < 8; k++) c[k] = i0 + k * PLACE_THREADS < n ? counts[i0 + k * PLACE_THREADS] : 0;
 #pragma unroll
         for (int k = 0; k < 8; k++) {
             if (c[k]) {
                 atomicAdd(&sh.total[e], c[k]);
-                if (i0 + k * SORT_THREADS < own) atomicAdd(&sh.before[e], c[k]);
+                if (i0 + k * PLACE_THREADS < own) atomicAdd(&sh.before[e], c[k]);
             }
             e += step;
             if (e >= experts) e -= experts;
         }
     }
     __syncthreads();
-    place_segments(sh, experts, align, blockIdx.x == 0 ? offsets : nullptr);
+}
+
+// counts[chunk][e] -> the sum over the chunks before it; totals[e]. A block has 32 experts, a warp a range of the chunks.
+__global__ void __launch_bounds__(1024) sort_scan(int *counts, int *totals, int chunks, int experts) {
+    behind_predecessors();
+    __shared__ int sums[32][32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, e = blockIdx.x * 32 + lane;
+    const int b0 = (int)((long long)chunks * warp / 32), b1 = (int)((long long)chunks * (warp + 1) / 32);
+    int sum = 0;
+    if (e < experts)
+#pragma unroll 8
+        for (int b = b0; b < b1; b++) sum += counts[(size_t)b * experts + e];
+    sums[warp][lane] = sum;
+    __syncthreads();
+    int run = 0;
+    for (int w = 0; w < warp; w++) run += sums[w][lane];
+    if (e >= experts) return;
+    if (warp == 31) totals[e] = run + sum;
+    for (int b = b0; b < b1; b++) {
+        const int n = counts[(size_t)b * experts + e];
+        counts[(size_t)b * experts + e] = run;
+        run += n;
+    }
+}
+
+__global__ void __launch_bounds__(PLACE_THREADS) sort_place(const void *ids, int id_bytes, int experts, int slots, int align, int R, int *offsets,
+                                                           int *row_of, int *slot_of, const int *counts, const int *totals) {
+    behind_predecessors();
+    __shared__ SortShared sh;
+    int rank[CHUNK / PLACE_THREADS], key[CHUNK / PLACE_THREADS];
 #pragma unroll
-    for (int i = 0; i < CHUNK / SORT_THREADS; i++) {
-        const int s = blockIdx.x * CHUNK + i * SORT_THREADS + threadIdx.x;
+    for (int i = 0; i < CHUNK / PLACE_THREADS; i++) {
+        const int s = blockIdx.x * CHUNK + i * PLACE_THREADS + threadIdx.x;
+        key[i] = s < slots ? key_of(ids, id_bytes, experts, s) : experts;
+        rank[i] = s < slots ? row_of[s] : 0;
+    }
+    if (totals) {   // the counts are running sums
+        for (int e = threadIdx.x; e < experts; e += PLACE_THREADS) {
+            sh.total[e] = totals[e];
+            sh.before[e] = counts[(size_t)blockIdx.x * experts + e];
+        }
+        __syncthreads();
+    } else add_counts(sh, counts, experts);
+    place_segments<PLACE_THREADS>(sh, experts, align, blockIdx.x == 0 ? offsets : nullptr);
+#pragma unroll
+    for (int i = 0; i < CHUNK / PLACE_THREADS; i++) {
+        const int s = blockIdx.x * CHUNK + i * PLACE_THREADS + threadIdx.x;
         if (s >= slots) continue;
         const int row = key[i] < experts ? sh.total[key[i]] + sh.before[key[i]] + rank[i] : -1;
         if (row >= 0) slot_of[row] = s;
@@ -354,7 +392,8 @@ bool aligned(const void *p, long long ld, int size) { return !(reinterpret_cast<
 }  // namespace
 
 size_t expert_sort_scratch(int slots, int experts) {
-    return slots > CHUNK ? (size_t)((slots + CHUNK - 1) / CHUNK) * experts * sizeof(int) : 0;
+    const size_t chunks = (slots + CHUNK - 1) / CHUNK;
+    return chunks > 1 ? (chunks + (chunks > FEW_CHUNKS)) * experts * sizeof(int) : 0;
 }
 
 cudaError_t expert_sort(int slots, int experts, const void *ids, int id_bytes, int align, int R, int *offsets, int *rows, int *slot_of, void *scratch,
@@ -365,7 +404,12 @@ cudaError_t expert_sort(int slots, int experts, const void *ids, int id_bytes, i
     }
     int *counts = static_cast<int *>(scratch);
     if (cudaError_t e = launch_behind(sort_count, chunks, SORT_THREADS, 0, 1, st, ids, id_bytes, experts, slots, R, rows, slot_of, counts)) return e;
-    return launch_behind(sort_place, chunks, SORT_THREADS, 0, 1, st, ids, id_bytes, experts, slots, align, R, offsets, rows, slot_of, counts);
+    int *totals = nullptr;
+    if (chunks > FEW_CHUNKS) {
+        totals = counts + (size_t)chunks * experts;
+        if (cudaError_t e = launch_behind(sort_scan, (experts + 31) / 32, 1024, 0, 1, st, counts, totals, chunks, experts)) return e;
+    }
+    return launch_behind(sort_place, chunks, PLACE_THREADS, 0, 1, st, ids, id_bytes, experts, slots, align, R, offsets, rows, slot_of, counts, totals);
 }
 
 cudaError_t expert_gather(int T, int top, int H, const void *X, int type, long long ldx, int R, const int *rows, const int *slots, void *Y,

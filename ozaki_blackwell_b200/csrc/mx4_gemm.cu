@@ -322,13 +322,14 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm(const __grid_constant__ C
     }
     behind_predecessors();
     if (warp == 2 && p.mode == BY_ROWS) {   // running number of token tiles over the groups
+        const int most = 0x3fffffff / ((p.weights + S::WEIGHTS - 1) / S::WEIGHTS);   // offsets out of order may name rows again and again
         int run = 0;
         for (int g0 = 0; g0 < p.groups; g0 += 32) {
             int n = 0;
             if (g0 + lane < p.groups) {
                 int lo, hi;
                 segment(p, g0 + lane, p.tokens, lo, hi);
-                n = (hi - lo + S::TOKENS - 1) / S::TOKENS;
+                n = min((hi - lo + S::TOKENS - 1) / S::TOKENS, most / 32);
             }
             int inc = n;
 #pragma unroll
@@ -336,8 +337,8 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm(const __grid_constant__ C
                 const int o = __shfl_up_sync(~0u, inc, d);
                 if (lane >= d) inc += o;
             }
-            if (g0 + lane < p.groups) cum[g0 + lane] = run + inc - n;
-            run += __shfl_sync(~0u, inc, 31);
+            if (g0 + lane < p.groups) cum[g0 + lane] = min(run + inc - n, most);
+            run = min(run + __shfl_sync(~0u, inc, 31), most);
         }
         if (lane == 0) cum[p.groups] = run;
     }
@@ -669,7 +670,7 @@ cudaError_t make_map(CUtensorMap *map, const uint8_t *ptr, int K, int rows, int 
     EncodeTiledFn enc = encode_fn();
     if (!enc) return cudaErrorNotSupported;
     const cuuint64_t dims[3] = {(cuuint64_t)(((long long)K + 31) / 32 * 16), (cuuint64_t)rows, (cuuint64_t)planes};
-    const cuuint64_t strides[2] = {(cuuint64_t)ld, (cuuint64_t)(planes > 1 ? plane : (size_t)ld * rows)};
+    const cuuint64_t strides[2] = {(cuuint64_t)ld, (cuuint64_t)(planes > 1 ? plane : (size_t)ld)};
     const cuuint32_t box[3] = {(cuuint32_t)BKB, (cuuint32_t)box_rows, 1};
     const cuuint32_t estr[3] = {1, 1, 1};
     const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<uint8_t *>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
@@ -695,7 +696,7 @@ cudaError_t make_map_y(CUtensorMap *map, void *y, long long bytes, int rows, int
     EncodeTiledFn enc = encode_fn();
     if (!enc) return cudaErrorNotSupported;
     const cuuint64_t dims[3] = {(cuuint64_t)bytes, (cuuint64_t)rows, (cuuint64_t)groups};
-    const cuuint64_t strides[2] = {(cuuint64_t)ld, (cuuint64_t)(groups > 1 ? plane : (size_t)ld * rows)};
+    const cuuint64_t strides[2] = {(cuuint64_t)ld, (cuuint64_t)(groups > 1 ? plane : (size_t)ld)};
     const cuuint32_t box[3] = {64, 32, 1};
     const cuuint32_t estr[3] = {1, 1, 1};
     const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, y, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B,

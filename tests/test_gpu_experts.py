@@ -56,6 +56,25 @@ def _fast_sort(ids, experts, align):
     return offsets, [offsets[e] + p if p >= 0 else -1 for e, p in zip(flat, place)]
 
 
+@pytest.mark.parametrize("slots,experts", [(256 * 1024, 40), (256 * 1024 + 1, 1024), (300000, 3), (3000001, 77)])
+def test_sort_of_many(slots, experts):
+    """Over 256 chunks of 1024 slots the counts go through a scan of their own."""
+    ids = _ids(slots, 1, experts, slots).cuda()
+    r = _experts().sort(ids, experts, 8)
+    flat = ids.reshape(-1).long()
+    key = torch.where((flat >= 0) & (flat < experts), flat, experts)
+    order = torch.sort(key, stable=True).indices
+    counts = torch.bincount(key, minlength=experts + 1)
+    offsets = torch.nn.functional.pad(((counts[:experts] + 7) // 8 * 8).cumsum(0), (1, 0))
+    place = offsets[key[order]] + torch.arange(slots, device="cuda") - (counts.cumsum(0) - counts)[key[order]]
+    rows = torch.full((slots,), -1, device="cuda").scatter(0, order, torch.where(key[order] < experts, place, -1))
+    assert torch.equal(r.offsets.long(), offsets) and torch.equal(r.rows.reshape(-1).long(), rows)
+    kept = rows >= 0
+    want = torch.full((r.slots.numel(),), -1, device="cuda")
+    want[rows[kept]] = torch.arange(slots, device="cuda")[kept]
+    assert torch.equal(r.slots.long(), want)
+
+
 @pytest.mark.parametrize("what", ["all dropped", "one expert", "every token the same expert twice"])
 def test_sort_extremes(what):
     tokens, top, experts = 700, 4, 33

@@ -328,12 +328,13 @@ def test_streams_and_graphs():
         assert torch.equal(y, want[i])
 
 
-def test_first_product_of_a_process_in_a_capture():
+@pytest.mark.parametrize("m,n", [(8, 8), (300, 6000), (1100, 3100)])
+def test_first_product_of_a_process_in_a_capture(m, n):
     import subprocess
     import sys
-    code = ("import torch; from ozaki_blackwell_b200 import mx4; x = torch.randn(8, 64, device='cuda'); g = torch.cuda.CUDAGraph()\n"
-            "with torch.cuda.graph(g):\n    q = mx4.quantize(x); y = mx4.matmul(q, q, torch.float32)\n"
-            "g.replay(); v = mx4.dequantize(q).double(); assert torch.allclose(y.double(), v @ v.t(), rtol=1e-5, atol=1e-4), (y, v @ v.t())")
+    code = (f"import torch; from ozaki_blackwell_b200 import mx4; x, w = torch.randn({m}, 64, device='cuda'), torch.randn({n}, 64, device='cuda'); g = torch.cuda.CUDAGraph()\n"
+            "with torch.cuda.graph(g):\n    q, p = mx4.quantize(x), mx4.quantize(w); y = mx4.matmul(q, p, torch.float32)\n"
+            "g.replay(); a, b = (mx4.dequantize(t).double() for t in (q, p)); assert torch.allclose(y.double(), a @ b.t(), rtol=1e-5, atol=1e-4)")
     out = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
     assert out.returncode == 0, out.stderr[-2000:]
 
