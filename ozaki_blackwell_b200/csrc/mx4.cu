@@ -188,65 +188,71 @@ __global__ void __launch_bounds__(256) mx4_rows(const T *X, int nvec, int len, l
 }
 
 // Blocks down the columns of a row-major X (len x nvec): vector c is column c, and comes out as a row. A block of threads takes 256
-// rows of 64 columns: warp w holds rows 32w .. 32w+31, two columns to a lane, in registers (32 independent loads of a pair in
-// flight to a lane), so that a lane has a whole block of each of its columns; the codes turn through shared memory into 128
-// contiguous bytes for each column.
-constexpr int CT_COLS = 64, CT_ROWS = 256, CT_PITCH = 128 + 16;
+// rows of 64 (FP32) or 128 columns: warp w holds rows 32w .. 32w+31, 8 bytes of columns to a lane (single columns are loaded one by
+// one where groups are not aligned, two to a lane), in registers, so that a lane has a
+// whole block of each of its columns and 32 loads of 256 contiguous bytes are in flight to a warp (with 4 bytes to a lane 16-bit
+// matrices came at 4.0 TB/s where FP32 ones reached 6.5). The codes turn through shared memory into 128 contiguous bytes for each
+// column.
+constexpr int CT_ROWS = 256, CT_PITCH = 128 + 16;
+template <class T, bool VEC> struct Columns { static constexpr int LANE = VEC ? 8 / (int)sizeof(T) : 2, TILE = 32 * LANE; };
 template <class T, bool VEC>
 __global__ void __launch_bounds__(256) mx4_cols(const T *X, int nvec, int len, long long ldx, size_t plane_x, int rule, const int *slots,
-                                                int per, int sources, uint8_t *codes, long long ldq, size_t plane_q, uint8_t *scales,
+                                                int top, int tokens, uint8_t *codes, long long ldq, size_t plane_q, uint8_t *scales,
                                                 long long lds, size_t plane_s, int col_tiles, int row_tiles) {
     behind_predecessors();
-    __shared__ __align__(16) uint8_t tile[CT_COLS * CT_PITCH];
-    __shared__ __align__(8) uint8_t stile[CT_COLS * 8];
+    constexpr int L = Columns<T, VEC>::LANE, TILE = Columns<T, VEC>::TILE;
+    __shared__ __align__(16) uint8_t tile[TILE * CT_PITCH];
+    __shared__ __align__(8) uint8_t stile[TILE * 8];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     long long b = blockIdx.x;
     const int ct = (int)(b % col_tiles);
     b /= col_tiles;
     const int rt = (int)(b % row_tiles), z = (int)(b / row_tiles);
-    const int c = ct * CT_COLS + 2 * lane, k0 = rt * CT_ROWS + warp * 32;
+    const int c = ct * TILE + L * lane, k0 = rt * CT_ROWS + warp * 32;
     X += (size_t)z * plane_x;
     codes += (size_t)z * plane_q;
     scales += (size_t)z * plane_s;
-    struct alignas(2 * sizeof(T)) Pair { T a, b; };
-    Pair v[32];
+    struct alignas(L * sizeof(T)) Group { T t[L]; };
+    Group v[32];
     // Every load is made, from a place that exists, and what was not there is cleared behind them: under a condition each they would
     // wait for one another (a tile took the latency of 32 loads, 40 us where 8 are enough).
-    const long long mine = k0 + lane < len ? source_row(slots, per, sources, k0 + lane) : -1;
+    const long long mine = k0 + lane < len ? source_row(slots, top, tokens, k0 + lane) : -1;
 #pragma unroll
     for (int i = 0; i < 32; i++) {
         const T *x = X + (size_t)max(__shfl_sync(~0u, mine, i), 0ll) * ldx;
-        if constexpr (VEC) v[i] = *reinterpret_cast<const Pair *>(x + (c < nvec ? c : 0));   // an even number of columns
-        else v[i].a = x[min(c, nvec - 1)], v[i].b = x[min(c + 1, nvec - 1)];
+        if constexpr (VEC) v[i] = *reinterpret_cast<const Group *>(x + (c < nvec ? c : 0));   // whole groups of columns
+        else
+#pragma unroll
+            for (int g = 0; g < L; g++) v[i].t[g] = x[min(c + g, nvec - 1)];
     }
     const uint32_t rows = __ballot_sync(~0u, mine >= 0);
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
+    for (int g = 0; g < L; g++) {
         float f[32];
         uint32_t m = 0;
 #pragma unroll
         for (int i = 0; i < 32; i++) {
-            f[i] = rows >> i & 1 ? to_f32<T>(h ? v[i].b : v[i].a) : 0.f;
+            f[i] = rows >> i & 1 ? to_f32<T>(v[i].t[g]) : 0.f;
             m = max(m, magnitude(f[i]));
         }
         const uint32_t byte = scale_byte(m, rule), number = byte == 255 ? 0u : ~0u;
         const float inv = inverse_scale(byte);
 #pragma unroll
         for (int i = 0; i < 32; i++) f[i] *= inv;
-        *reinterpret_cast<uint4 *>(tile + (2 * lane + h) * CT_PITCH + warp * 16) =
+        *reinterpret_cast<uint4 *>(tile + (L * lane + g) * CT_PITCH + warp * 16) =
             make_uint4(codes_of(f) & number, codes_of(f + 8) & number, codes_of(f + 16) & number, codes_of(f + 24) & number);
-        stile[(2 * lane + h) * 8 + warp] = (uint8_t)byte;
+        stile[(L * lane + g) * 8 + warp] = (uint8_t)byte;
     }
     __syncthreads();
     const int blocks = (len + 31) / 32, kb = rt * 8;   // blocks of a column, and this tile's first
 #pragma unroll
-    for (int i = 0; i < CT_COLS * 8 / 256; i++) {
-        const int col = i * 32 + (threadIdx.x >> 3), blk = threadIdx.x & 7, g = ct * CT_COLS + col;
+    for (int i = 0; i < TILE * 8 / 256; i++) {
+        const int col = i * 32 + (threadIdx.x >> 3), blk = threadIdx.x & 7, g = ct * TILE + col;
         if (g < nvec && kb + blk < blocks)
             *reinterpret_cast<uint4 *>(codes + (size_t)g * ldq + (size_t)(kb + blk) * 16) = *reinterpret_cast<const uint4 *>(tile + col * CT_PITCH + blk * 16);
     }
-    if (threadIdx.x < CT_COLS && ct * CT_COLS + (int)threadIdx.x < nvec) {
-        uint8_t *dst = scales + (size_t)(ct * CT_COLS + threadIdx.x) * lds + kb;
+    if (threadIdx.x < TILE && ct * TILE + (int)threadIdx.x < nvec) {
+        uint8_t *dst = scales + (size_t)(ct * TILE + threadIdx.x) * lds + kb;
         if (kb + 8 <= blocks) *reinterpret_cast<uint2 *>(dst) = *reinterpret_cast<const uint2 *>(stile + threadIdx.x * 8);
         else for (int i = 0; kb + i < blocks; i++) dst[i] = stile[threadIdx.x * 8 + i];
     }
@@ -354,8 +360,10 @@ cudaError_t mx4_quantize_cols(const void *X, int type, int nvec, int len, long l
                               const int *slots, int top, int tokens, uint8_t *codes, long long ldq, size_t plane_q, uint8_t *scales, long long lds,
                               size_t plane_s, cudaStream_t st) {
     const int size = type_size(type);
-    const bool vec = !(reinterpret_cast<uintptr_t>(X) % (2 * size)) && !((ldx | nvec) & 1) && !(plane_x & 1);
-    const int col_tiles = (nvec + CT_COLS - 1) / CT_COLS, row_tiles = (len + CT_ROWS - 1) / CT_ROWS;
+    const int group = 8 / size;
+    const bool vec = !(reinterpret_cast<uintptr_t>(X) & 7) && !((ldx | nvec) % group) && !(plane_x % group);
+    const int tile = 32 * (vec ? group : 2);   // columns of a block
+    const int col_tiles = (nvec + tile - 1) / tile, row_tiles = (len + CT_ROWS - 1) / CT_ROWS;
     const long long grid = (long long)col_tiles * row_tiles * planes;
     if (grid > 0x7fffffffLL) return cudaErrorInvalidValue;
     cudaError_t e = cudaErrorInvalidValue;
