@@ -24,7 +24,7 @@
 // bytes by TMA was slower: boxes 16 bytes wide cost the TMA unit as much for a row as the 128 bytes of its codes (900 cycles a slot).
 //
 // Few tokens (NARROW): P = weights, Q = tokens, BN = 16 .. 128 by the tokens there are, Y's columns are the lanes, so that a warp stores
-// contiguous columns of one token. With few tiles the k of a tile is split over a cluster of 2, 4 or 8 CTAs, whose partial tiles
+// contiguous columns of one token. With few tiles the k of a tile is split over a cluster of 2 or 4 CTAs, whose partial tiles
 // are added in a fixed order through distributed shared memory. Many tokens (WIDE): P = tokens, Q = weights, BN = 192, a lane stores
 // 32 columns of its token in 16-byte pieces; two accumulators of 192 columns leave 128 columns of tensor memory for scales. With
 // enough tiles a pair of CTAs (cta_group::2) shares a tile of 256 tokens: each loads its own 128 tokens and half of the weights'
@@ -631,12 +631,13 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm(const __grid_constant__ C
             const int r = threadIdx.x & (BP - 1), i = t.p0 + r;
             const int n = min(BN, t.q1 - t.q0), c0 = (int)((long long)n * rank / ranks), c1 = (int)((long long)n * (rank + 1) / ranks);
             for (int c = c0 + (threadIdx.x >> 7); c < c1; c += THREADS / BP) {
-                float sum = 0.f;
-                for (uint32_t q = 0; q < ranks; q++) {
-                    float x;
-                    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(map_to_cta(base + 4u * (c * BP + r), q)) : "memory");
-                    sum += x;
-                }
+                float x[4], sum = 0.f;
+#pragma unroll
+                for (uint32_t q = 0; q < 4; q++)   // all in flight; ranks beyond the cluster's read this CTA's and are not added
+                    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x[q]) : "r"(map_to_cta(base + 4u * (c * BP + r), q < ranks ? q : rank)));
+#pragma unroll
+                for (uint32_t q = 0; q < 4; q++)
+                    if (q < ranks) sum += x[q];
                 if (i < t.p1) Y[(size_t)(t.q0 + c) * p.ldy + i] = from_f32<T>(sum);
             }
         }
@@ -704,6 +705,31 @@ cudaError_t make_map_y(CUtensorMap *map, void *y, long long bytes, int rows, int
     return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
+// how many clusters of `per` CTAs of the kernel the device holds at once
+template <int FORM, int BN, class T>
+int room_for(int per, int sms) {
+    static int known[64][5] = {};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return sms / per;
+    int &n = known[dev & 63][per];
+    if (!n) {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)(sms / per * per));
+        cfg.blockDim = dim3(THREADS);
+        cfg.dynamicSmemBytes = Shape<FORM, BN>::SMEM;
+        cudaLaunchAttribute at[1];
+        at[0].id = cudaLaunchAttributeClusterDimension;
+        at[0].val.clusterDim.x = per;
+        at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+        cfg.attrs = at;
+        cfg.numAttrs = 1;
+        int found = 0;
+        if (cudaOccupancyMaxActiveClusters(&found, mx4_gemm<FORM, BN, T>, &cfg) != cudaSuccess || found <= 0) { cudaGetLastError(); found = sms / per / 2; }
+        n = found;
+    }
+    return n;
+}
+
 template <int FORM, int BN, class T>
 cudaError_t launch(const Mx4Product &g, Params p, int sms, int split, cudaStream_t st) {
     using S = Shape<FORM, BN>;
@@ -723,35 +749,19 @@ cudaError_t launch(const Mx4Product &g, Params p, int sms, int split, cudaStream
     const size_t plane = planes > 1 ? g.plane_ws : 0;
     p.sp = S::wide ? g.xs : g.ws; p.ldsp = S::wide ? g.ldxs : g.ldws; p.plane_sp = S::wide ? 0 : plane;
     p.sq = S::wide ? g.ws : g.xs; p.ldsq = S::wide ? g.ldws : g.ldxs; p.plane_sq = S::wide ? plane : 0;
-    const int per = FORM == SPLIT ? split : S::pair ? 2 : 1;   // CTAs to a cluster
-    // A persistent grid must be resident as a whole: a pair that started behind another would find its share of the tiles still to do.
-    // Not every SM has a neighbour to pair with (74 pairs were asked for, and the product took twice its time).
-    long long clusters = w.most;
-    if (FORM != SPLIT) {
-        long long room = sms;
-        if (S::pair) {
-            static int pairs[64] = {};
-            int dev = 0;
-            if ((e = cudaGetDevice(&dev))) return e;
-            int &n = pairs[dev & 63];
-            if (!n) {
-                cudaLaunchConfig_t cfg = {};
-                cfg.gridDim = dim3((unsigned)(sms & ~1));
-                cfg.blockDim = dim3(THREADS);
-                cfg.dynamicSmemBytes = S::SMEM;
-                cudaLaunchAttribute at[1];
-                at[0].id = cudaLaunchAttributeClusterDimension;
-                at[0].val.clusterDim.x = per;
-                at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-                cfg.attrs = at;
-                cfg.numAttrs = 1;
-                int found = 0;
-                if (cudaOccupancyMaxActiveClusters(&found, mx4_gemm<FORM, BN, T>, &cfg) != cudaSuccess || found <= 0) { cudaGetLastError(); found = sms / 2; }
-                n = found;
-            }
-            room = n;
-        }
-        if (clusters > room) clusters = room;
+    // CTAs to a cluster, and clusters. A grid that is not resident as a whole takes twice its time: a pair that started behind another
+    // would find its share of the tiles still to do. Not every SM has free neighbours, so the device is asked how many clusters there
+    // can be (16 clusters of 8 were too many, for one).
+    int per = 1;
+    long long clusters = w.most < sms ? w.most : sms;
+    if (FORM == PAIR) {
+        per = 2;
+        long long room = room_for<FORM, BN, T>(2, sms);
+        clusters = w.most < room ? w.most : room;
+    } else if (FORM == SPLIT) {
+        for (per = split; per > 1 && w.expected > room_for<FORM, BN, T>(per, sms); per /= 2) {}
+        clusters = w.most;
+        if (per == 1) return launch<NARROW, BN, T>(g, p, sms, 1, st);
     }
     return launch_behind(mx4_gemm<FORM, BN, T>, (int)(clusters * per), THREADS, S::SMEM, per, st, S::wide ? x : w4, S::wide ? w4 : x, y, p);
 }
@@ -786,11 +796,12 @@ cudaError_t mx4_product(const Mx4Product &g, int *status, cudaStream_t st) {
     else if (each > 128 && work_of(g, BP, 192).expected * 2 >= sms) run(M4_FORM(WIDE), M4_FORM(192), 1);
     else {
         // few: weights as lanes; few tiles as well: k split, while every CTA keeps at least four stages
-        const int bn = each <= 16 ? 16 : each <= 32 ? 32 : each <= 64 ? 64 : 128;
+        int bn = each <= 16 ? 16 : each <= 32 ? 32 : each <= 64 ? 64 : 128;
+        while (bn > 32 && work_of(g, bn, BP).expected * 2 <= sms) bn /= 2;   // narrower, if that fills more SMs: 333 x 1030 x 2085 10.8 us at 128, 5.4 at 32
         const long long tiles = work_of(g, bn, BP).expected;
-        int split = 1;
-        if (g.mode != ALONG_K)
-            while (split < 8 && tiles * split * 2 <= sms && stages / (split * 2) >= 4) split *= 2;
+        int split = 1;   // few tiles and a long k: the partial tiles cost about 2 us, 16 stages 3 (40 x 1024 x 8192: 8.8 us whole, 7.6 in four; 32 x 2048 x 2048: 4.9 and 6.9 in two)
+        if (g.mode != ALONG_K && stages >= 32)
+            while (split < 4 && tiles * split * 2 <= sms && stages / (split * 2) >= 8) split *= 2;
         auto narrow = [&](auto width) {
             if (split > 1) run(M4_FORM(SPLIT), width, split);
             else run(M4_FORM(NARROW), width, 1);

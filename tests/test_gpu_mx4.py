@@ -159,7 +159,7 @@ def test_dequantize_every_code_and_scale(dtype):
 @pytest.mark.parametrize("shape", [(1, 1, 1), (1, 128, 32), (1, 2048, 4096), (2, 130, 33), (15, 127, 64), (16, 129, 65), (17, 256, 255), (31, 64, 256), (33, 300, 257),
                                    (64, 128, 2085), (65, 1, 511), (128, 400, 512), (129, 257, 1000), (300, 70, 1537), (512, 384, 96), (513, 640, 288),
                                    (700, 130, 2049), (3, 640, 16384), (150, 9500, 96), (300, 6000, 500), (129, 7200, 1100), (1100, 3070, 300), (2060, 1550, 1025),
-                                   (513, 5000, 64)])
+                                   (513, 5000, 64), (40, 1024, 8192), (4, 300, 16400), (90, 500, 9000), (17, 130, 20000)])
 def test_product(shape):
     m, n, k = shape
     mx4 = _mx4()
