@@ -24,11 +24,16 @@
 // bytes by TMA was slower: boxes 16 bytes wide cost the TMA unit as much for a row as the 128 bytes of its codes (900 cycles a slot).
 //
 // Few tokens (NARROW): P = weights, Q = tokens, BN = 16 .. 128 by the tokens there are, Y's columns are the lanes, so that a warp stores
-// contiguous columns of one token. With few tiles the k of a tile is split over a cluster of 2 or 4 CTAs, whose partial tiles
-// are added in a fixed order through distributed shared memory. Many tokens (WIDE): P = tokens, Q = weights, BN = 192, a lane stores
-// 32 columns of its token in 16-byte pieces; two accumulators of 192 columns leave 128 columns of tensor memory for scales. With
-// enough tiles a pair of CTAs (cta_group::2) shares a tile of 256 tokens: each loads its own 128 tokens and half of the weights'
-// rows (a seventh of the bytes in shared memory for an operation less than a third), and turns its own and all the weights' scales.
+// contiguous columns of one token. With few tiles and a long k the k of a tile is split over a cluster of 2 or 4 CTAs (SPLIT), whose
+// partial tiles are added in a fixed order through distributed shared memory. Many tokens (WIDE): P = tokens, Q = weights, BN = 192;
+// two accumulators of 192 columns leave 128 columns of tensor memory for scales; tiles leave through shared memory and TMA. With
+// enough tiles two CTAs (cta_group::2) share a tile of 256 tokens (PAIR): each loads its own 128 tokens and half of the weights' rows,
+// and turns its own tokens' and all the weights' scales.
+//
+// What bounds it: for one token HBM (18432 x 7168 in 10.4 us, 6.7 TB/s with the weights partly in L2; 14.1 us from HBM); for many, what
+// the L2 delivers. At 2048 x 18432 x 7168 (107 us, 5040 TFLOP/s, 0.76 of four times the measured burst rate of BF16, 0.89 of four times
+// the sustained one) the CTAs fetch 1.2 GB of operands, 11 TB/s, and every other many-token shape comes to the same rate; the clock is
+// then at 1.5 GHz under the power limit. WIDE fetches 40 KB to a stage of 128 x 192, PAIR 56 KB to one of 256 x 192.
 // Every wait is bounded: on expiry the CTA raises the status word, stops, frees its tensor memory and returns.
 #include <type_traits>
 #include "oz_async.cuh"
@@ -791,27 +796,27 @@ cudaError_t mx4_product(const Mx4Product &g, int *status, cudaStream_t st) {
         with_type(g.type, [&](auto t) { e = launch<decltype(form)::value, decltype(width)::value, decltype(t)>(g, p, sms, split, st); });
     };
 #define M4_FORM(F) std::integral_constant<int, F>()
-    // many tokens to a group, and at least half a tile for every SM: tokens as lanes; a pair of CTAs where there is enough for all pairs
+    // Many tokens to a group: tokens as lanes, in pairs of CTAs where there are tiles for all of them (groups of fewer than 512 tokens
+    // fill too little of a pair's 256: 16 experts of 580, 21.6 us alone and 20.5 in pairs; 32 of 256, 50.5 and 53.4). Where 128 x 128
+    // tiles are one to an SM or fewer they are better: 256 x 8192 x 8192 15.8 us with tokens as lanes, 13.4 without.
     if (each > 128 && work_of(g, 2 * BP, 192).expected >= sms / 2 && (g.mode != BY_ROWS || each >= 512)) run(M4_FORM(PAIR), M4_FORM(192), 1);
-    else if (each > 128 && work_of(g, BP, 192).expected * 2 >= sms) run(M4_FORM(WIDE), M4_FORM(192), 1);
+    else if (each > 128 && work_of(g, 128, BP).expected > sms) run(M4_FORM(WIDE), M4_FORM(192), 1);
     else {
-        // few: weights as lanes; few tiles as well: k split, while every CTA keeps at least four stages
+        // Few tokens, or few tiles: weights as lanes; narrower tiles if that fills more SMs (333 x 1030 x 2085: 10.8 us at 128, 5.4 at 32).
         int bn = each <= 16 ? 16 : each <= 32 ? 32 : each <= 64 ? 64 : 128;
-        while (bn > 32 && work_of(g, bn, BP).expected * 2 <= sms) bn /= 2;   // narrower, if that fills more SMs: 333 x 1030 x 2085 10.8 us at 128, 5.4 at 32
+        while (bn > 32 && work_of(g, bn, BP).expected * 2 <= sms) bn /= 2;
+        // Still few, and a long k: in two or four. The partial tiles cost about 2 us, 16 stages 3 (40 x 1024 x 8192: 8.8 us whole, 7.6 in
+        // four; 32 x 2048 x 2048: 4.9 whole, 6.9 in two).
         const long long tiles = work_of(g, bn, BP).expected;
-        int split = 1;   // few tiles and a long k: the partial tiles cost about 2 us, 16 stages 3 (40 x 1024 x 8192: 8.8 us whole, 7.6 in four; 32 x 2048 x 2048: 4.9 and 6.9 in two)
-        if (g.mode != ALONG_K && stages >= 32)
+        int split = 1;
+        if (bn <= 32 && g.mode != ALONG_K && stages >= 32)
             while (split < 4 && tiles * split * 2 <= sms && stages / (split * 2) >= 8) split *= 2;
-        auto narrow = [&](auto width) {
-            if (split > 1) run(M4_FORM(SPLIT), width, split);
-            else run(M4_FORM(NARROW), width, 1);
-        };
-        switch (bn) {
-        case 16: narrow(M4_FORM(16)); break;
-        case 32: narrow(M4_FORM(32)); break;
-        case 64: narrow(M4_FORM(64)); break;
-        default: narrow(M4_FORM(128)); break;
-        }
+        if (bn == 16 && split > 1) run(M4_FORM(SPLIT), M4_FORM(16), split);
+        else if (bn == 32 && split > 1) run(M4_FORM(SPLIT), M4_FORM(32), split);
+        else if (bn == 16) run(M4_FORM(NARROW), M4_FORM(16), 1);
+        else if (bn == 32) run(M4_FORM(NARROW), M4_FORM(32), 1);
+        else if (bn == 64) run(M4_FORM(NARROW), M4_FORM(64), 1);
+        else run(M4_FORM(NARROW), M4_FORM(128), 1);
     }
 #undef M4_FORM
     return e;

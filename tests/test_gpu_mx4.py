@@ -288,7 +288,7 @@ def test_segment_product(offsets):
     _status()
 
 
-@pytest.mark.parametrize("m,n,groups", [(200, 400, 16), (600, 1000, 16), (300, 100, 64), (40, 900, 32)])
+@pytest.mark.parametrize("m,n,groups", [(200, 400, 16), (600, 1000, 16), (300, 100, 64), (40, 900, 32), (130, 400, 20)])
 def test_segment_product_of_many(m, n, groups):
     mx4 = _mx4()
     g = torch.Generator().manual_seed(m)
