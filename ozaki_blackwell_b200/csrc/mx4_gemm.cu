@@ -759,11 +759,11 @@ cudaError_t launch(const Mx4Product &g, Params p, int sms, int split, cudaStream
     // can be (16 clusters of 8 were too many, for one).
     int per = 1;
     long long clusters = w.most < sms ? w.most : sms;
-    if (FORM == PAIR) {
+    if constexpr (FORM == PAIR) {
         per = 2;
         long long room = room_for<FORM, BN, T>(2, sms);
         clusters = w.most < room ? w.most : room;
-    } else if (FORM == SPLIT) {
+    } else if constexpr (FORM == SPLIT) {
         for (per = split; per > 1 && w.expected > room_for<FORM, BN, T>(per, sms); per /= 2) {}
         clusters = w.most;
         if (per == 1) return launch<NARROW, BN, T>(g, p, sms, 1, st);
