@@ -12,7 +12,7 @@
 // values (128 bytes) of k make a stage, 512 (16 scale bytes) a scale slot.
 //   warp 0     producer: one thread, TMA of both operands' codes (128-byte swizzle) into a ring of stages. What lies outside a matrix
 //              comes as zero codes.
-//   warps 3, 8 .. 10  scales, in turns of a slot: a row's 16 bytes are four words, one to 128 values of k; the instruction wants, for a
+//   warps 3, 8 .. 10  scales, in turns of one or two slots: a row's 16 bytes are four words, one to 128 values of k; the instruction wants, for a
 //              word, 128 rows as 32 x 16 bytes (row r at 16 (r % 32) + 4 (r / 32)). A lane reads the rows l, l + 32, l + 64, l + 96
 //              and writes the 4 x 4 words turned: four 16-byte loads and stores for 128 rows by 512 values, without bank conflicts.
 //   warp 2     one thread; tcgen05.cp of a stage's turned scales into tensor memory, its completion counted by the stage's barrier
@@ -49,7 +49,7 @@ namespace m4 {
 constexpr int BP = 128;            // rows of P to a CTA
 constexpr int BK = 256, BKB = 128; // k of a stage, in values and in bytes
 constexpr int UK = 64;             // k of one tcgen05.mma kind::mxf4
-constexpr int TURNERS = 4, THREADS = 512;   // warp 11 is idle: the epilogue's second four must be warps 0 .. 3 modulo 4
+constexpr int THREADS = 512;       // warp 11 is idle: the epilogue's second four must be warps 0 .. 3 modulo 4
 constexpr int MAX_GROUPS = 1024;
 constexpr int AHEAD = 48;          // tiles of a CTA that are worked out before it starts
 
@@ -81,9 +81,9 @@ template <int FORM, int BN> struct Shape {
     static constexpr int SLOT = 4 * 512 * (1 + Q_TILES);           // turned scales of 512 values of k: four words of P's tile, then of Q's
     static constexpr int SCALE_COLS = 8 + 8 * Q_TILES;             // tensor-memory columns of a stage's scales
     static constexpr int STAGES = pair ? 5 : BN <= 32 ? 8 : BN <= 64 ? 7 : BN <= 128 ? 5 : 4;
-    // A multiple of the turning warps, so that a slot is always the same warp's: a warp that came to a slot before another had seen the
-    // slot's last use would take the parity of the use before that for its own.
-    static constexpr int SLOTS = FORM == WIDE ? TURNERS : 2 * TURNERS;
+    // Scale slots, two to a turning warp: a slot is always the same warp's. (A warp that came to a slot before another had seen the slot's
+    // last use would take the parity of the use before that for its own.) A warp turns HALVES slots at a time.
+    static constexpr int TURNERS = FORM == WIDE ? 2 : 4, SLOTS = 2 * TURNERS, HALVES = wide ? 2 : 1, WINDOW = 2 * HALVES;   // WINDOW: stages of a turn
     static_assert(SLOT % 512 == 0, "the pieces behind the slots are swizzled");
     static constexpr int COLS = 2 * BN + STAGES * SCALE_COLS;      // two accumulators, and the scales
     static constexpr int TMEM_COLS = COLS <= 256 ? 256 : 512;
@@ -484,43 +484,47 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm(const __grid_constant__ C
             for (int w = first; w < total && !__any_sync(~0u, *abortp); w += step, n++) {
                 const Tile t = tile_at(w, n);
                 bool ok = true;
-                for (int kb = t.s0; kb < t.s1; sl++) {
-                    const int r = sl % S::SLOTS, s = it % S::STAGES, s2 = (it + 1) % S::STAGES;
-                    const bool both = !(kb & 1) && kb + 1 < t.s1;   // the slot's two stages, or its first or second alone
-                    const uint32_t parity = ((it / S::STAGES) & 1u) ^ 1u, parity2 = (((it + 1) / S::STAGES) & 1u) ^ 1u;
-                    if constexpr (pair) ok = __all_sync(~0u, mbar_wait_acquire_cluster(turned_bar(r), (sl / S::SLOTS) & 1u, abortp, 0x131));
-                    else ok = warp_wait(turned_bar(r), (sl / S::SLOTS) & 1u, abortp, 0x131);
-                    if (ok) ok = both ? warp_wait2(empty_bar(s), parity, empty_bar(s2), parity2, abortp, 0x132) : warp_wait(empty_bar(s), parity, abortp, 0x132);
-                    if (!ok) break;
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const uint32_t words = slots + r * S::SLOT;
-                    auto copy = [&](int s, int half) {   // the two words of a stage
-                        const uint32_t tp = tmem_scales + s * S::SCALE_COLS, tq = tp + 8;
+                for (int at = t.s0 & ~(S::WINDOW - 1); at < t.s1 && ok; at += S::WINDOW)
+                    for (int half = 0; half < S::HALVES && ok; half++, sl++) {
+                        const int r = sl % S::SLOTS, s = it % S::STAGES, s2 = (it + 1) % S::STAGES;
+                        const int from = max(t.s0, at + 2 * half), count = min(t.s1, at + 2 * half + 2) - from;   // this slot's stages: two, one or none
+                        const uint32_t parity = ((it / S::STAGES) & 1u) ^ 1u, parity2 = (((it + 1) / S::STAGES) & 1u) ^ 1u;
+                        if constexpr (pair) ok = __all_sync(~0u, mbar_wait_acquire_cluster(turned_bar(r), (sl / S::SLOTS) & 1u, abortp, 0x131));
+                        else ok = warp_wait(turned_bar(r), (sl / S::SLOTS) & 1u, abortp, 0x131);
+                        if (ok && count > 1) ok = warp_wait2(empty_bar(s), parity, empty_bar(s2), parity2, abortp, 0x132);
+                        else if (ok && count > 0) ok = warp_wait(empty_bar(s), parity, abortp, 0x132);
+                        if (!ok) break;
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                        const uint32_t words = slots + r * S::SLOT;
+                        auto copy = [&](int s, int second) {   // the two words of a stage
+                            const uint32_t tp = tmem_scales + s * S::SCALE_COLS, tq = tp + 8;
 #pragma unroll
-                        for (int h = 0; h < 2; h++) {
-                            copy_scales<pair>(tp + 4 * h, words + 512 * (2 * half + h));
+                            for (int h = 0; h < 2; h++) {
+                                copy_scales<pair>(tp + 4 * h, words + 512 * (2 * second + h));
 #pragma unroll
-                            for (int c = 0; c < S::Q_TILES; c++) copy_scales<pair>(tq + 4 * (h * S::Q_TILES + c), words + 2048 + 512 * ((2 * half + h) * S::Q_TILES + c));
+                                for (int c = 0; c < S::Q_TILES; c++) copy_scales<pair>(tq + 4 * (h * S::Q_TILES + c), words + 2048 + 512 * ((2 * second + h) * S::Q_TILES + c));
+                            }
+                            if constexpr (pair) mma_commit_pair(full_bar(s));
+                            else mma_commit(full_bar(s));
+                        };
+                        if (elect_one()) {
+                            if (count > 1) {
+                                copy(s, 0);
+                                copy(s2, 1);
+                            } else if (count > 0) copy(s, from & 1);
+                            commit<pair>(slot_bar(r));
                         }
-                        if constexpr (pair) mma_commit_pair(full_bar(s));
-                        else mma_commit(full_bar(s));
-                    };
-                    if (elect_one()) {
-                        if (both) {
-                            copy(s, 0);
-                            copy(s2, 1);
-                        } else copy(s, kb & 1);
-                        commit<pair>(slot_bar(r));
+                        __syncwarp();
+                        it += max(count, 0);
                     }
-                    __syncwarp();
-                    kb += both ? 2 : 1;
-                    it += both ? 2 : 1;
-                }
                 if (!ok) break;
             }
         }
-    } else if (warp == 3 || (warp >= 8 && warp < 7 + TURNERS)) {
-        // of TURNERS warps, in turns of a slot: while one waits for its slot's bytes, the others do theirs
+    } else if (warp == 3 || (warp >= 8 && warp < 7 + S::TURNERS)) {
+        // Of TURNERS warps, in turns of a window: while one waits for its window's bytes, the others do theirs. Where many tiles share the
+        // L2 a window is two slots: a row's 32 bytes are one sector of the L2's and are asked for at once (slot by slot they were fetched
+        // twice, 15 % of all that the CTAs fetched: 2048 x 18432 x 7168 under the power limit 133 us, 125 so). For few tokens it is one,
+        // which is there sooner (64 x 4096 x 4096: 6.5 us, 7.3 with two).
         const uint32_t own = warp == 3 ? 0 : warp - 7;
         const int blocks = (p.K + 31) / 32;
         uint32_t n = 0;
@@ -528,53 +532,63 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm(const __grid_constant__ C
             const Tile t = tile_at(w, n);
             const int p0 = t.p0 + (pair ? (int)rank * BP : 0);
             bool ok = true;
-            for (int kb = t.s0; kb < t.s1; kb = (kb | 1) + 1, sl++) {
-                if (sl % TURNERS != own) continue;
-                const int r = sl % S::SLOTS, byte = (kb >> 1) * 16, left = blocks - byte;
+            for (int at = t.s0 & ~(S::WINDOW - 1); at < t.s1; at += S::WINDOW, sl += S::HALVES) {
+                if (sl / S::HALVES % S::TURNERS != own) continue;
+                const int r = sl % S::SLOTS, byte = at * 8, left = blocks - byte;
+                const uint32_t parity = ((sl / S::SLOTS) & 1u) ^ 1u;
                 const uint8_t *sp = p.sp + (size_t)t.group * p.plane_sp + byte, *sq = p.sq + (size_t)t.group * p.plane_sq + byte;
-                uint4 v[1 + S::Q_TILES][4];
-#pragma unroll
-                for (int c = 0; c < 1 + S::Q_TILES; c++)   // P's tile, then Q's
+                uint8_t *slot = base_ptr + S::STAGES * S::STAGE + r * S::SLOT + 16 * lane;
+                using Words = uint4[S::HALVES][4];
+                auto load = [&](Words &v, int c) {   // tile c: P's, then Q's
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
-                        const int row = i * 32 + lane;
-                        v[c][i] = make_uint4(0, 0, 0, 0);   // 2^-127: rows that are not there
-                        if (c == 0) {
-                            if (p0 + row < t.p1) v[c][i] = *reinterpret_cast<const uint4 *>(sp + (size_t)(p0 + row) * p.ldsp);
-                        } else {
-                            const int q = (c - 1) * 128 + row;
-                            if (q < BN && t.q0 + q < t.q1) v[c][i] = *reinterpret_cast<const uint4 *>(sq + (size_t)(t.q0 + q) * p.ldsq);
+                        const int row = i * 32 + lane, q = (c - 1) * 128 + row;
+                        const bool there = c == 0 ? p0 + row < t.p1 : q < BN && t.q0 + q < t.q1;
+                        const uint8_t *from = c == 0 ? sp + (size_t)(p0 + row) * p.ldsp : sq + (size_t)(t.q0 + q) * p.ldsq;
+#pragma unroll
+                        for (int h = 0; h < S::HALVES; h++) {
+                            v[h][i] = make_uint4(0, 0, 0, 0);   // 2^-127: rows that are not there, and words behind a row's last
+                            if (there && left > 16 * h) v[h][i] = *reinterpret_cast<const uint4 *>(from + 16 * h);
                         }
                     }
-                if (left < 16) {   // bytes behind the last block may hold anything: their codes are zero, their scales become it
-#pragma unroll
-                    for (int c = 0; c < 1 + S::Q_TILES; c++)
-#pragma unroll
-                        for (int i = 0; i < 4; i++) v[c][i] = first_bytes(v[c][i], left);
-                }
-                if (!warp_wait(slot_bar(r), ((sl / S::SLOTS) & 1u) ^ 1u, abortp, 0x140)) { ok = false; break; }
-                uint8_t *slot = base_ptr + S::STAGES * S::STAGE + r * S::SLOT + 16 * lane;
-#pragma unroll
-                for (int c = 0; c < 1 + S::Q_TILES; c++) {
-                    uint8_t *dst = slot + (c == 0 ? 0 : 2048 + 512 * (c - 1));
+                };
+                auto turn = [&](Words &v, int c) {
                     const int pitch = c == 0 ? 512 : 512 * S::Q_TILES;   // to the tile of the next word
-                    *reinterpret_cast<uint4 *>(dst) = make_uint4(v[c][0].x, v[c][1].x, v[c][2].x, v[c][3].x);
-                    *reinterpret_cast<uint4 *>(dst + pitch) = make_uint4(v[c][0].y, v[c][1].y, v[c][2].y, v[c][3].y);
-                    *reinterpret_cast<uint4 *>(dst + 2 * pitch) = make_uint4(v[c][0].z, v[c][1].z, v[c][2].z, v[c][3].z);
-                    *reinterpret_cast<uint4 *>(dst + 3 * pitch) = make_uint4(v[c][0].w, v[c][1].w, v[c][2].w, v[c][3].w);
-                }
+#pragma unroll
+                    for (int h = 0; h < S::HALVES; h++) {
+                        if (left < 16 * h + 16 && left > 16 * h) {   // bytes behind the last block may hold anything: their codes are zero, their scales become it
+#pragma unroll
+                            for (int i = 0; i < 4; i++) v[h][i] = first_bytes(v[h][i], left - 16 * h);
+                        }
+                        uint8_t *dst = slot + h * S::SLOT + (c == 0 ? 0 : 2048 + 512 * (c - 1));
+                        *reinterpret_cast<uint4 *>(dst) = make_uint4(v[h][0].x, v[h][1].x, v[h][2].x, v[h][3].x);
+                        *reinterpret_cast<uint4 *>(dst + pitch) = make_uint4(v[h][0].y, v[h][1].y, v[h][2].y, v[h][3].y);
+                        *reinterpret_cast<uint4 *>(dst + 2 * pitch) = make_uint4(v[h][0].z, v[h][1].z, v[h][2].z, v[h][3].z);
+                        *reinterpret_cast<uint4 *>(dst + 3 * pitch) = make_uint4(v[h][0].w, v[h][1].w, v[h][2].w, v[h][3].w);
+                    }
+                };
+                Words a, b;   // a third tile takes the first one's registers
+                load(a, 0);
+                load(b, 1);
+                ok = warp_wait(slot_bar(r), parity, abortp, 0x140);
+                if (S::HALVES == 2 && ok) ok = warp_wait(slot_bar(r + 1), parity, abortp, 0x140);
+                if (!ok) break;
+                turn(a, 0);
+                if constexpr (S::Q_TILES == 2) load(a, 2);
+                turn(b, 1);
+                if constexpr (S::Q_TILES == 2) turn(a, 2);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the tensor core reads these through the async proxy
                 __syncwarp();
                 // In a pair the leader's thread starts the copies of both CTAs. What the peer wrote is read by its own tensor core, behind the
                 // fence above, so a plain remote arrive passes it on; a release at cluster scope holds the warp for 1800 cycles.
-                if (lane == 0) {
-                    if (pair && rank) mbar_arrive_cluster(map_to_cta(turned_bar(r), 0));
-                    else mbar_arrive(turned_bar(r));
+                if (lane < S::HALVES) {
+                    if (pair && rank) mbar_arrive_cluster(map_to_cta(turned_bar(r + lane), 0));
+                    else mbar_arrive(turned_bar(r + lane));
                 }
             }
             if (!ok) break;
         }
-    } else if (warp != 11) {
+    } else if ((warp >= 4 && warp < 8) || warp >= 12) {
         const int quarter = warp & 3, half = warp >= 12;   // lanes 32 quarter .. +31, every other 32 columns
         Piece piece = {base_ptr + S::STAGES * S::STAGE + S::SLOTS * S::SLOT + (quarter + 4 * half) * 4096, 0, 0};
         asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(piece.policy));
