@@ -78,6 +78,33 @@ def test_rows():
         assert call(**bad) == ARG, bad
 
 
+def test_the_layer_in_one_call():
+    assert lib.ozb_expert_mx4_work(4, 2, 8, 64, 96, 1, 64) > 0 and lib.ozb_expert_mx4_grad_work(512, 64, 96, 1) > 0
+    for bad in ((0, 2, 8, 64, 96, 1, 1), (4, 0, 8, 64, 96, 1, 1), (4, 2, 0, 64, 96, 1, 1), (4, 2, 1025, 64, 96, 1, 1), (4, 2, 8, 0, 96, 1, 1), (4, 2, 8, 64, 0, 1, 1),
+                (4, 2, 8, 64, 96, 3, 1), (4, 2, 8, 64, 96, 1, 0), (4, 2, 8, 64, 96, 1, 257)):
+        assert lib.ozb_expert_mx4_work(*bad) == 0, bad
+    for bad in ((0, 64, 96, 1), (512, 0, 96, 1), (512, 64, 0, 1), (512, 64, 96, 5)):
+        assert lib.ozb_expert_mx4_grad_work(*bad) == 0, bad
+    need = lib.ozb_expert_mx4_work(3, 2, 4, 8, 64, 0, 64)
+    base = dict(T=3, top=2, experts=4, N=8, K=64, X=P, type=0, ldx=64, ids=P, id_bytes=4, weights=None, W=P, ldw=32, plane_w=256, Ws=P, ldws=16, plane_ws=128, align=64,
+                offsets=None, rows=None, slots=None, Z=None, ldz=0, Y=P, ldy=8, work=P, bytes=need)
+    call = lambda **b: lib.ozb_expert_mx4(*{**base, **b}.values(), None)  # noqa: E731
+    for bad in (dict(T=0), dict(top=0), dict(experts=0), dict(N=0), dict(K=0), dict(X=None), dict(type=7), dict(ldx=63), dict(ids=None), dict(id_bytes=1), dict(W=None), dict(ldw=16),
+                dict(plane_w=8), dict(plane_ws=8), dict(Ws=None), dict(ldws=8), dict(align=0), dict(align=300), dict(offsets=P), dict(rows=P, slots=P), dict(Z=P, ldz=7), dict(Y=None),
+                dict(ldy=7), dict(work=None), dict(bytes=need - 1), dict(work=ctypes.c_void_p(4100))):
+        assert call(**bad) == ARG, bad
+    assert call(experts=1025) == SIZE
+    need = lib.ozb_expert_mx4_grad_work(256, 8, 64, 0)
+    base = dict(T=3, top=2, experts=4, N=8, K=64, R=256, dY=P, type=0, lddy=8, X=P, ldx=64, Z=P, ldz=8, Wt=P, ldwt=16, plane_wt=1024, Wts=P, ldwts=16, plane_wts=1024, offsets=P, rows=P,
+                slots=P, weights=None, dX=P, lddx=64, dweights=P, dW=P, lddw=64, plane_dw=512, work=P, bytes=need)
+    call = lambda **b: lib.ozb_expert_mx4_grad(*{**base, **b}.values(), None)  # noqa: E731
+    for bad in (dict(T=0), dict(R=0), dict(N=0), dict(K=0), dict(dY=None), dict(X=None), dict(Z=None), dict(Wt=None), dict(Wts=None), dict(offsets=None), dict(rows=None), dict(slots=None),
+                dict(dX=None), dict(dweights=None), dict(dW=None), dict(lddy=7), dict(ldx=63), dict(ldz=7), dict(lddx=63), dict(lddw=63), dict(work=None), dict(bytes=need - 1), dict(type=9),
+                dict(plane_wt=8)):
+        assert call(**bad) == ARG, bad
+    assert call(experts=1025) == SIZE
+
+
 def test_host_tensors_are_refused():
     from ozaki_blackwell_b200 import experts, mx4
     x = torch.zeros(4, 64)
