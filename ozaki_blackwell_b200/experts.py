@@ -47,13 +47,11 @@ def sort(ids, experts, align=1):
     if size < 0:
         raise ValueError(f"cannot sort {tokens} x {top} slots over {experts} experts in segments of {align}: sizes are positive, at most 1024 experts, align at most 256")
     need = _lib.ozb_expert_sort_scratch(tokens, top, experts)
-    # one allocation: slots, rows, offsets and the counts of the chunks
-    n = tokens * top
-    buf = ids.new_empty(size + n + experts + 1 + need // 4, dtype=torch.int32)
-    at = buf.data_ptr()
-    _call(ids.get_device(), _lib.ozb_expert_sort, tokens, top, experts, ids.data_ptr(), ids.element_size(), align, size, at + 4 * (size + n), at + 4 * size, at,
-          at + 4 * (size + n + experts + 1), need)
-    return Routing(buf[size + n : size + n + experts + 1], buf[size : size + n].view(tokens, top), buf[:size], align)
+    offsets, rows, slots = ids.new_empty(experts + 1, dtype=torch.int32), ids.new_empty(tokens, top, dtype=torch.int32), ids.new_empty(size, dtype=torch.int32)
+    scratch = ids.new_empty(need, dtype=torch.uint8) if need else None
+    _call(ids.get_device(), _lib.ozb_expert_sort, tokens, top, experts, ids.data_ptr(), ids.element_size(), align, size, offsets.data_ptr(), rows.data_ptr(),
+          slots.data_ptr(), scratch.data_ptr() if need else None, need)
+    return Routing(offsets, rows, slots, align)
 
 
 def gather(x, routing, out=None):
@@ -86,7 +84,7 @@ def combine_grad(dy, z, routing, weights=None):
     if dy.dtype is not z.dtype or dy.shape != (tokens, h) or r != routing.slots.shape[0] or dy.get_device() != index:
         raise ValueError(f"dy {tuple(dy.shape)} of {dy.dtype} and z {tuple(z.shape)} of {z.dtype} do not fit a routing of {tokens} tokens and {routing.slots.shape[0]} rows")
     kind, w = _type(z.dtype), _weights(weights, routing.rows.shape, index)
-    dz, dweights = z.new_empty((r, h)), z.new_empty((tokens, top), dtype=torch.float32)
+    dz, dweights = z.new_empty(r, h), z.new_empty(tokens, top, dtype=torch.float32)
     _call(index, _lib.ozb_expert_combine_grad, tokens, top, h, dy.data_ptr(), kind, lddy, z.data_ptr(), ldz, r, routing.rows.data_ptr(),
           routing.slots.data_ptr(), w, dz.data_ptr(), h, dweights.data_ptr())
     return dz, dweights
@@ -109,15 +107,13 @@ def matmul(x, w, ids, weights=None, keep=False):
     need = _lib.ozb_expert_mx4_work(tokens, top, experts, n, k, kind, align)
     if not need:
         raise ValueError(f"cannot sort {tokens} x {top} slots over {experts} experts: sizes are positive, at most 1024 experts")
-    y, work = x.new_empty((tokens, n)), x.new_empty((need,), dtype=torch.uint8)
+    y, work = x.new_empty(tokens, n), x.new_empty(need, dtype=torch.uint8)
     maps, z, r = (None, None, None, None), None, None
     if keep:
         size = _lib.ozb_expert_sort_rows(tokens, top, experts, align)
-        buf = ids.new_empty(size + tokens * top + experts + 1, dtype=torch.int32)
-        r = Routing(buf[size + tokens * top :], buf[size : size + tokens * top].view(tokens, top), buf[:size], align)
-        z = x.new_empty((size, n))
-        at = buf.data_ptr()
-        maps = at + 4 * (size + tokens * top), at + 4 * size, at, z.data_ptr()
+        r = Routing(ids.new_empty(experts + 1, dtype=torch.int32), ids.new_empty(tokens, top, dtype=torch.int32), ids.new_empty(size, dtype=torch.int32), align)
+        z = x.new_empty(size, n)
+        maps = r.offsets.data_ptr(), r.rows.data_ptr(), r.slots.data_ptr(), z.data_ptr()
     _call(index, _lib.ozb_expert_mx4, tokens, top, experts, n, k, x.data_ptr(), kind, ldx, ids.data_ptr(), ids.element_size(), factors, wc, ldw,
           w.codes.stride(0), ws, ldws, w.scales.stride(0), align, *maps, n, y.data_ptr(), n, work.data_ptr(), need)
     return (y, z, r) if keep else y
@@ -140,8 +136,8 @@ def matmul_grad(dy, x, z, wt, routing, weights=None):
         raise ValueError(f"wt must be a stack of {routing.offsets.shape[0] - 1} matrices of {k} vectors of {n}")
     factors = _weights(weights, routing.rows.shape, index)
     need = _lib.ozb_expert_mx4_grad_work(r, n, k, kind)
-    dx, dweights = x.new_empty((tokens, k)), x.new_empty((tokens, top), dtype=torch.float32)
-    dw, work = x.new_empty((experts, n, k)), x.new_empty((need,), dtype=torch.uint8)
+    dx, dweights = x.new_empty(tokens, k), x.new_empty(tokens, top, dtype=torch.float32)
+    dw, work = x.new_empty(experts, n, k), x.new_empty(need, dtype=torch.uint8)
     _call(index, _lib.ozb_expert_mx4_grad, tokens, top, experts, n, k, r, dy.data_ptr(), kind, lddy, x.data_ptr(), ldx, z.data_ptr(), ldz, wc, ldw,
           wt.codes.stride(0), ws, ldws, wt.scales.stride(0), routing.offsets.data_ptr(), routing.rows.data_ptr(), routing.slots.data_ptr(), factors,
           dx.data_ptr(), k, dweights.data_ptr(), dw.data_ptr(), k, n * k, work.data_ptr(), need)

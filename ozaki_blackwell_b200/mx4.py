@@ -69,8 +69,12 @@ def _codes(q, role, dims, index):
     """Pointers and pitches of an Mx4 on device `index`: codes, ldq, scales, lds."""
     codes, scales, length = q
     blocks = (length + 31) >> 5
+    have, bytes_, at, steps = codes.shape, scales.shape, codes.stride(), scales.stride()
+    if (codes.dtype is torch.uint8 and scales.dtype is torch.uint8 and len(have) == dims and have[:-1] == bytes_[:-1] and have[-2] > 1 and at[-1] == 1 and steps[-1] == 1
+            and have[-1] >= 16 * blocks and bytes_[-1] >= (blocks + 15) & ~15 and codes.get_device() == index == scales.get_device() and index >= 0):
+        return codes.data_ptr(), at[-2], scales.data_ptr(), steps[-2]
+    # a single vector, whose pitch may be anything, or something to refuse
     ldq, lds = _pitch(codes, role, dims), _pitch(scales, role, dims)
-    have, bytes_ = codes.shape, scales.shape
     if codes.dtype is not torch.uint8 or scales.dtype is not torch.uint8:
         raise TypeError(f"{role}: codes and scales are uint8, not {codes.dtype} and {scales.dtype}")
     if have[:-1] != bytes_[:-1]:
@@ -85,7 +89,7 @@ def _codes(q, role, dims, index):
 def _result(like, out, shape, dtype, dims=2):
     """out, checked, or a new tensor on the device of `like`; and the pitch of its rows."""
     if out is None:
-        return like.new_empty(shape, dtype=dtype), shape[-1]
+        return like.new_empty(*shape, dtype=dtype), shape[-1]
     if tuple(out.shape) != tuple(shape) or out.dtype != dtype or out.device != like.device:
         raise ValueError(f"out= must be {tuple(shape)} of {dtype} on {like.device}")
     return out, _pitch(out, "out", dims)
@@ -131,10 +135,10 @@ def quantize(x, dim=-1, rule="floor", routing=None):
     blocks = (length + 31) >> 5
     ldq, lds = 16 * blocks, (blocks + 15) & ~15
     if dims == 2:
-        codes, scales = x.new_empty((vectors, ldq), dtype=torch.uint8), x.new_empty((vectors, lds), dtype=torch.uint8)
+        codes, scales = x.new_empty(vectors, ldq, dtype=torch.uint8), x.new_empty(vectors, lds, dtype=torch.uint8)
         planes = 1, 0, 0, 0
     else:
-        codes, scales = x.new_empty((shape[0], vectors, ldq), dtype=torch.uint8), x.new_empty((shape[0], vectors, lds), dtype=torch.uint8)
+        codes, scales = x.new_empty(shape[0], vectors, ldq, dtype=torch.uint8), x.new_empty(shape[0], vectors, lds, dtype=torch.uint8)
         planes = shape[0], x.stride(0), vectors * ldq, vectors * lds
     _call(index, _lib.ozb_mx4_quantize, x.data_ptr(), kind, vectors, length, ldx, dim == -1, _RULES[rule], *maps, planes[0], planes[1],
           codes.data_ptr(), ldq, planes[2], scales.data_ptr(), lds, planes[3])

@@ -318,6 +318,25 @@ def test_streams_and_graphs():
             got[i] = mx4.matmul(mx4.quantize(x), w)
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+    # a chain over two streams, each step behind an event of the other's last, on buffers that are written again and again
+    a, b = streams
+    buf, out, done = xs[0].clone(), torch.empty_like(want[0]), torch.cuda.Event()
+    torch.cuda.synchronize()
+    for i in list(range(4)) * 8:
+        with torch.cuda.stream(a):
+            a.wait_event(done)
+            buf.copy_(xs[i])
+            q = mx4.quantize(buf)
+            ready = torch.cuda.Event()
+            ready.record(a)
+        with torch.cuda.stream(b):
+            b.wait_event(ready)
+            mx4.matmul(q, w, out=out)
+            keep = out.clone()
+            done = torch.cuda.Event()
+            done.record(b)
+        b.synchronize()
+        assert torch.equal(keep, want[i])
     x = xs[0].clone()
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
