@@ -223,15 +223,17 @@ enum { OZB_F32 = 0, OZB_BF16 = 1, OZB_F16 = 2 };
  * 1.5, 2, 3, 4, 6) times the block's power of two 2^(s - 127), s one byte (255: the block is not a number). Row-major: row r of
  * the codes at codes + r * ldq (two codes to a byte, the earlier one in the low half), its scales at scales + r * lds (bytes,
  * one to a block). Both start on 16 bytes and have pitches that are multiples of 16; a row of codes has room for ceil(len / 32)
- * whole blocks, a row of scales for that many bytes rounded up to 16, and the codes behind `len` in the last one are 0.
+ * whole blocks, a row of scales for that many bytes rounded up to 16, and the codes behind `len` in the last one are 0. Where
+ * there are several matrices, a plane apart, the codes of one and what is written of it end before the next begins (a plane of 0 is
+ * refused).
  *
  * ozb_mx4_quantize: `nvec` vectors of `len` values of X to that format, nearest code, ties to the even one. by_rows = 1: the rows of
  * X (pitch ldx); by_rows = 0: the columns of a row-major len x nvec X, which come out as rows. rule 0: the block's scale is
  * 2^(floor(log2 amax) - 2), values above 6 of it saturate; rule 1: the smallest power of two with amax <= 6 of it. Scales stay
  * within 2^-127 .. 2^127. A block that holds an infinity or a NaN gets s = 255 and codes 0. `rows` and `slots` (both
  * NULL, or the maps of ozb_expert_sort for `tokens` tokens of `top` slots) put the rows of X (tokens x ..) in the order of their
- * experts first, as ozb_expert_gather does: nvec (by_rows = 1) or len (by_rows = 0) is then the number of sorted rows. planes > 1 (without the maps): that many matrices, plane_x elements,
- * plane_q and plane_s bytes apart (multiples of 16). The gradient is passed through (straight-through), no call needed. */
+ * experts first, as ozb_expert_gather does: nvec (by_rows = 1) or len (by_rows = 0) is then the number of sorted rows. planes > 1
+ * (without the maps): that many matrices, plane_x elements, plane_q and plane_s bytes apart (multiples of 16). The gradient is passed through (straight-through), no call needed. */
 int ozb_mx4_quantize(const void *X, int type, int nvec, int len, long long ldx, int by_rows, int rule, const int *rows, const int *slots, int top,
                      int tokens, int planes, size_t plane_x, uint8_t *codes, long long ldq, size_t plane_q, uint8_t *scales, long long lds,
                      size_t plane_s, void *stream);

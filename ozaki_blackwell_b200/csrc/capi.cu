@@ -434,10 +434,19 @@ int check_device() {
     return major != 10 ? OZB_EARCH : 0;
 }
 bool off(const void *p, unsigned to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) != 0; }   // not aligned
+long long code_bytes(int len) { return ((long long)len + 31) / 32 * 16; }
+long long scale_bytes(int len) { return ((long long)len + 31) / 32; }
 // a 4-bit operand: rows of `len` values, codes and scales
 bool bad_mx4(const void *codes, long long ldq, const void *scales, long long lds, int len) {
-    return !codes || !scales || off(codes, 16) || off(scales, 16) || (ldq & 15) || (lds & 15) || ldq < ((long long)len + 31) / 32 * 16 ||
-           lds < ((long long)len + 31) / 32;
+    return !codes || !scales || off(codes, 16) || off(scales, 16) || (ldq & 15) || (lds & 15) || ldq < code_bytes(len) || lds < scale_bytes(len);
+}
+// matrices of `rows` rows of `width` (elements or bytes) that lie in one another, n of them
+bool bad_planes(long long n, long long rows, long long ld, long long width, size_t plane) {
+    return n > 1 && (double)plane < (double)(rows - 1) * (double)ld + (double)width;   // no product of these overflows a double
+}
+// the codes of several groups' weights lie one after the other, as a tensor map has them; their scales are only read, from anywhere
+bool bad_stack(int n, int rows, int len, long long ld, size_t plane, size_t plane_s) {
+    return n > 1 && ((plane & 15) || (plane_s & 15) || bad_planes(n, rows, ld, code_bytes(len), plane));
 }
 constexpr int MAX_LEN = 0x7fffffff - 1023;   // lengths are rounded up in 32 bits
 bool bad_slots(int T, int top) { return T <= 0 || top <= 0 || (long long)T * top > MAX_LEN; }
@@ -869,7 +878,7 @@ OZB_API int ozb_mx4_quantize(const void *X, int type, int nvec, int len, long lo
         return OZB_EARG;
     if (!rows != !slots) return OZB_EARG;
     if (slots && (bad_slots(tokens, top) || planes > 1 || off(slots, 4) || off(rows, 4))) return OZB_EARG;
-    if (planes > 1 && ((plane_q & 15) || (plane_s & 15))) return OZB_EARG;
+    if (bad_stack(planes, nvec, len, ldq, plane_q, plane_s) || bad_planes(planes, nvec, lds, scale_bytes(len), plane_s)) return OZB_EARG;
     if (int e = check_device()) return e;
     if (planes == 1) plane_x = plane_q = plane_s = 0;
     const int e = (int)(by_rows ? mx4_quantize_rows : mx4_quantize_cols)(X, type, nvec, len, ldx, plane_x, planes, rule, rows, slots, top, tokens, codes, ldq,
@@ -900,7 +909,7 @@ OZB_API int ozb_mx4_gemm_grouped(int groups, int R, int N, int K, const int *off
                                  const uint8_t *W, long long ldw, size_t plane_w, const uint8_t *Ws, long long ldws, size_t plane_ws, void *Y, int type,
                                  long long ldy, void *stream) {
     if (groups <= 0 || R <= 0 || N <= 0 || K <= 0 || K > MAX_LEN || N > MAX_LEN || R > MAX_LEN || !offsets || off(offsets, 4) || bad_type(type) || !Y ||
-        off_type(Y, type) || ldy < N || bad_mx4(X, ldx, Xs, ldxs, K) || bad_mx4(W, ldw, Ws, ldws, K) || (groups > 1 && ((plane_w & 15) || (plane_ws & 15))))
+        off_type(Y, type) || ldy < N || bad_mx4(X, ldx, Xs, ldxs, K) || bad_mx4(W, ldw, Ws, ldws, K) || bad_stack(groups, N, K, ldw, plane_w, plane_ws))
         return OZB_EARG;
     if (groups > 1024) return OZB_ESIZE;
     return run_mx4({1, groups, R, N, K, type, offsets, X, ldx, Xs, ldxs, W, ldw, plane_w, Ws, ldws, plane_ws, Y, ldy, 0}, stream);
@@ -909,7 +918,7 @@ OZB_API int ozb_mx4_gemm_segments(int groups, int M, int N, int R, const int *of
                                   const uint8_t *B, long long ldb, const uint8_t *Bs, long long ldbs, void *Y, int type, long long ldy, size_t plane_y,
                                   void *stream) {
     if (groups <= 0 || M <= 0 || N <= 0 || R <= 0 || M > MAX_LEN || N > MAX_LEN || R > MAX_LEN || !offsets || off(offsets, 4) || bad_type(type) || !Y ||
-        off_type(Y, type) || ldy < N || bad_mx4(A, lda, As, ldas, R) || bad_mx4(B, ldb, Bs, ldbs, R))
+        off_type(Y, type) || ldy < N || bad_mx4(A, lda, As, ldas, R) || bad_mx4(B, ldb, Bs, ldbs, R) || bad_planes(groups, M, ldy, N, plane_y))
         return OZB_EARG;
     if (groups > 1024) return OZB_ESIZE;
     return run_mx4({2, groups, M, N, R, type, offsets, A, lda, As, ldas, B, ldb, 0, Bs, ldbs, 0, Y, ldy, plane_y}, stream);
@@ -1024,7 +1033,7 @@ OZB_API int ozb_expert_mx4(int T, int top, int experts, int N, int K, const void
                            int align, int *offsets, int *rows, int *slots, void *Z, long long ldz, void *Y, long long ldy, void *work, size_t work_bytes,
                            void *stream) {
     if (bad_layer(T, top, experts, N, K, type) || align <= 0 || align > 256 || !X || off_type(X, type) || ldx < K || (id_bytes != 4 && id_bytes != 8) || !ids ||
-        off(ids, id_bytes) || off(weights, 4) || bad_mx4(W, ldw, Ws, ldws, K) || (experts > 1 && ((plane_w & 15) || (plane_ws & 15))) || !Y || off_type(Y, type) ||
+        off(ids, id_bytes) || off(weights, 4) || bad_mx4(W, ldw, Ws, ldws, K) || bad_stack(experts, N, K, ldw, plane_w, plane_ws) || !Y || off_type(Y, type) ||
         ldy < N || !work || off(work, 16) || (Z && (ldz < N || off_type(Z, type))) || off(offsets, 4) || off(rows, 4) || off(slots, 4) ||
         !offsets != !rows || !rows != !slots)
         return OZB_EARG;
@@ -1053,9 +1062,9 @@ OZB_API int ozb_expert_mx4_grad(int T, int top, int experts, int N, int K, int R
                                 size_t plane_wts, const int *offsets, const int *rows, const int *slots, const float *weights, void *dX, long long lddx,
                                 float *dweights, void *dW, long long lddw, size_t plane_dw, void *work, size_t work_bytes, void *stream) {
     if (bad_layer(T, top, experts, N, K, type) || R <= 0 || R > MAX_LEN || !dY || !X || !Z || off_type(dY, type) || off_type(X, type) || off_type(Z, type) ||
-        lddy < N || ldx < K || ldz < N || bad_mx4(Wt, ldwt, Wts, ldwts, N) || (experts > 1 && ((plane_wt & 15) || (plane_wts & 15))) || !offsets || !rows ||
+        lddy < N || ldx < K || ldz < N || bad_mx4(Wt, ldwt, Wts, ldwts, N) || bad_stack(experts, K, N, ldwt, plane_wt, plane_wts) || !offsets || !rows ||
         !slots || off(offsets, 4) || off(rows, 4) || off(slots, 4) || off(weights, 4) || !dX || off_type(dX, type) || lddx < K || !dweights || off(dweights, 4) ||
-        !dW || off_type(dW, type) || lddw < K || !work || off(work, 16))
+        !dW || off_type(dW, type) || lddw < K || bad_planes(experts, N, lddw, K, plane_dw) || !work || off(work, 16))
         return OZB_EARG;
     if (experts > 1024) return OZB_ESIZE;
     if (work_bytes < carve_gradient(nullptr, N, K, type, R).bytes) return OZB_EARG;

@@ -48,6 +48,21 @@ def test_products():
     assert call(groups=1025) == SIZE
 
 
+def test_planes_in_one_another():
+    """Several matrices do not overlap: neither results, which would be written twice, nor the codes of weights."""
+    assert _quantize(planes=2, plane_x=256, plane_q=112, plane_s=64) == ARG and _quantize(planes=2, plane_x=256, plane_q=128, plane_s=48) == ARG
+    stack = lambda planes: lib.ozb_mx4_gemm_grouped(2, 4, 4, 64, P, P, 32, P, 16, P, 32, planes[0], P, 16, planes[1], P, 0, 4, None)  # noqa: E731
+    assert stack((0, 64)) == stack((112, 64)) == ARG
+    for plane in (0, 15):
+        assert lib.ozb_mx4_gemm_segments(2, 4, 4, 64, P, P, 32, P, 16, P, 32, P, 16, P, 0, 4, plane, None) == ARG
+    need = lib.ozb_expert_mx4_work(3, 2, 4, 8, 64, 0, 64)
+    layer = lambda planes: lib.ozb_expert_mx4(3, 2, 4, 8, 64, P, 0, 64, P, 4, None, P, 32, planes[0], P, 16, planes[1], 64, None, None, None, None, 0, P, 8, P, need, None)  # noqa: E731
+    assert layer((0, 128)) == layer((240, 128)) == ARG
+    need = lib.ozb_expert_mx4_grad_work(256, 8, 64, 0)
+    grad = lambda planes: lib.ozb_expert_mx4_grad(3, 2, 4, 8, 64, 256, P, 0, 8, P, 64, P, 8, P, 16, planes[0], P, 16, planes[1], P, P, P, None, P, 64, P, P, 64, planes[2], P, need, None)  # noqa: E731
+    assert grad((0, 1024, 512)) == grad((1008, 1024, 512)) == grad((1024, 1024, 0)) == grad((1024, 1024, 511)) == ARG
+
+
 def test_sort():
     assert lib.ozb_expert_sort_rows(3, 2, 4, 1) == 6
     assert lib.ozb_expert_sort_rows(3, 2, 4, 64) == (6 + 4 * 63) // 64 * 64      # four segments of at most 64
