@@ -189,10 +189,9 @@ __global__ void __launch_bounds__(256) mx4_rows(const T *X, int nvec, int len, l
 
 // Blocks down the columns of a row-major X (len x nvec): vector c is column c, and comes out as a row. A block of threads takes 256
 // rows of 64 (FP32) or 128 columns: warp w holds rows 32w .. 32w+31, 8 bytes of columns to a lane (single columns are loaded one by
-// one where groups are not aligned, two to a lane), in registers, so that a lane has a
-// whole block of each of its columns and 32 loads of 256 contiguous bytes are in flight to a warp (with 4 bytes to a lane 16-bit
-// matrices came at 4.0 TB/s where FP32 ones reached 6.5). The codes turn through shared memory into 128 contiguous bytes for each
-// column.
+// one where groups are not aligned, two to a lane), in registers, so that a lane has a whole block of each of its columns and 32
+// loads of 256 contiguous bytes are in flight to a warp (with 4 bytes to a lane 16-bit matrices came at 4.0 TB/s where FP32 ones
+// reached 6.5). The codes turn through shared memory into 128 contiguous bytes for each column.
 constexpr int CT_ROWS = 256, CT_PITCH = 128 + 16;
 template <class T, bool VEC> struct Columns { static constexpr int LANE = VEC ? 8 / (int)sizeof(T) : 2, TILE = 32 * LANE; };
 template <class T, bool VEC>

@@ -70,20 +70,21 @@ def _codes(q, role, dims, index):
     codes, scales, length = q
     blocks = (length + 31) >> 5
     have, bytes_, at, steps = codes.shape, scales.shape, codes.stride(), scales.stride()
-    if (codes.dtype is torch.uint8 and scales.dtype is torch.uint8 and len(have) == dims and have[:-1] == bytes_[:-1] and have[-2] > 1 and at[-1] == 1 and steps[-1] == 1
+    if (codes.dtype is torch.uint8 and scales.dtype is torch.uint8 and len(have) == dims and have[:-1] == bytes_[:-1] and at[-1] == 1 and steps[-1] == 1
             and have[-1] >= 16 * blocks and bytes_[-1] >= (blocks + 15) & ~15 and codes.get_device() == index == scales.get_device() and index >= 0):
-        return codes.data_ptr(), at[-2], scales.data_ptr(), steps[-2]
-    # a single vector, whose pitch may be anything, or something to refuse
-    ldq, lds = _pitch(codes, role, dims), _pitch(scales, role, dims)
+        if have[-2] > 1:
+            return codes.data_ptr(), at[-2], scales.data_ptr(), steps[-2]
+        return codes.data_ptr(), max(at[-2], have[-1]), scales.data_ptr(), max(steps[-2], bytes_[-1])   # one vector has any pitch
+    # something is wrong: say what
+    _pitch(codes, role, dims)
+    _pitch(scales, role, dims)
     if codes.dtype is not torch.uint8 or scales.dtype is not torch.uint8:
         raise TypeError(f"{role}: codes and scales are uint8, not {codes.dtype} and {scales.dtype}")
     if have[:-1] != bytes_[:-1]:
         raise ValueError(f"{role}: codes {tuple(have)} and scales {tuple(bytes_)} are of different vectors")
     if have[-1] < 16 * blocks or bytes_[-1] < (blocks + 15) & ~15:
         raise ValueError(f"{role}: rows of {have[-1]} and {bytes_[-1]} bytes do not hold {length} values")
-    if codes.get_device() != index or scales.get_device() != index:
-        raise ValueError(f"{role} must be on cuda:{index} with the other operands")
-    return codes.data_ptr(), ldq, scales.data_ptr(), lds
+    raise ValueError(f"{role} must be on cuda:{index} with the other operands")
 
 
 def _result(like, out, shape, dtype, dims=2):
