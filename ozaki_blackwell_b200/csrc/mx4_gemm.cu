@@ -229,15 +229,6 @@ __device__ __forceinline__ void store_wide(const CUtensorMap *map, bool whole_wo
                                            int group, Piece &piece) {
     if (j >= j1 || i0 >= i1) return;
     constexpr int N = Vec16<T>::N, COLS = 4 * N;   // columns to 16 and to 64 bytes
-    if (!whole_words) {
-        if (i0 + lane < i1) {
-            T *dst = Y + (size_t)(i0 + lane) * ldy + j;
-#pragma unroll
-            for (int c = 0; c < 32; c++)
-                if (j + c < j1) dst[c] = from_f32<T>(__uint_as_float(v[c]));
-        }
-        return;
-    }
 #pragma unroll
     for (int h = 0; h < 32; h += COLS) {
         if (j + h >= j1) break;
@@ -251,7 +242,16 @@ __device__ __forceinline__ void store_wide(const CUtensorMap *map, bool whole_wo
             for (int e = 0; e < N; e++) f[e] = __uint_as_float(v[h + c * N + e]);
             *reinterpret_cast<uint4 *>(buf + lane * 64 + 16 * (c ^ (lane >> 1 & 3))) = Vec16<T>::pack(f);
         }
-        if (i0 + 32 <= i1) {   // columns behind the last are cut by the tensor map
+        if (!whole_words) {   // COLS lanes to a row, value by value
+            __syncwarp();
+            const int c = lane % COLS, col = j + h + c;
+#pragma unroll 8
+            for (int r = lane / COLS; r < 32; r += 32 / COLS) {
+                const T x = *reinterpret_cast<const T *>(buf + r * 64 + 16 * (c / N ^ (r >> 1 & 3)) + c % N * sizeof(T));
+                if (i0 + r < i1 && col < j1) Y[(size_t)(i0 + r) * ldy + col] = x;
+            }
+            __syncwarp();
+        } else if (i0 + 32 <= i1) {   // columns behind the last are cut by the tensor map
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) {
