@@ -15,7 +15,7 @@ from typing import NamedTuple
 import torch
 
 from ._lib import lib as _lib
-from .mx4 import _call, _codes, _pitch, _result, _routed, _type
+from .mx4 import _call, _codes, _offsets, _pitch, _result, _routed, _type
 
 __all__ = ["Routing", "sort", "gather", "combine", "combine_grad", "matmul", "matmul_grad"]
 
@@ -132,7 +132,7 @@ def matmul_grad(dy, x, z, wt, routing, weights=None):
     experts = wt.codes.shape[0]
     if not dy.dtype is z.dtype is x.dtype or dy.shape != (tokens, n) or x.shape[0] != tokens or r != routing.slots.shape[0] or dy.get_device() != index or z.get_device() != index:
         raise ValueError(f"dy {tuple(dy.shape)}, x {tuple(x.shape)} and z {tuple(z.shape)} do not fit a routing of {tokens} tokens and {routing.slots.shape[0]} rows, or differ in type")
-    if wt.length != n or wt.codes.shape[1] != k or routing.offsets.shape[0] != experts + 1:
+    if _offsets(routing.offsets, index) != experts or wt.length != n or wt.codes.shape[1] != k:
         raise ValueError(f"wt must be a stack of {routing.offsets.shape[0] - 1} matrices of {k} vectors of {n}")
     factors = _weights(weights, routing.rows.shape, index)
     need = _lib.ozb_expert_mx4_grad_work(r, n, k, kind)

@@ -105,8 +105,8 @@ def _offsets(offsets, index):
 
 
 def _routed(r, index):
-    """Checks a Routing (of experts.sort) on device `index`; (tokens, top)."""
-    for name, t in (("offsets", r.offsets), ("rows", r.rows), ("slots", r.slots)):
+    """Checks the maps of a Routing (of experts.sort) on device `index`; (tokens, top)."""
+    for name, t in (("rows", r.rows), ("slots", r.slots)):
         if t.dtype is not torch.int32 or not t.is_contiguous() or t.get_device() != index:
             raise ValueError(f"routing.{name} must be contiguous int32 on cuda:{index}")
     if r.rows.dim() != 2:

@@ -281,3 +281,16 @@ def test_refusals():
         ex.gather(x, ex.Routing(r.offsets, r.rows.long(), r.slots))
     with pytest.raises(ValueError):
         ex.matmul_grad(x, x, z, None, r)      # segments that are not padded to 64
+
+
+def test_gradient_refuses_offsets_of_other_experts():
+    from ozaki_blackwell_b200 import mx4
+    ex = _experts()
+    ids = torch.zeros(4, 2, dtype=torch.int32, device="cuda")
+    x, dy, w = torch.randn(4, 64, device="cuda"), torch.randn(4, 32, device="cuda"), torch.randn(3, 32, 64, device="cuda")
+    wt = mx4.quantize(w, dim=-2)
+    _, z, r = ex.matmul(x, mx4.quantize(w), ids, keep=True)
+    for offsets in (r.offsets.long(), r.offsets[:-1], r.offsets.cpu(), r.offsets.reshape(1, -1)):
+        with pytest.raises(ValueError):
+            ex.matmul_grad(dy, x, z, wt, ex.Routing(offsets, r.rows, r.slots, r.align))
+    assert len(ex.matmul_grad(dy, x, z, wt, r)) == 3
