@@ -17,6 +17,7 @@
 //              and writes the 4 x 4 words turned: four 16-byte loads and stores for 128 rows by 512 values, without bank conflicts.
 //   warp 2     one thread; tcgen05.cp of a stage's turned scales into tensor memory, its completion counted by the stage's barrier
 //   warp 1     issuer: one thread; four tcgen05.mma kind::mxf4 (K = 64) to a stage
+//   warp 11    in a pair: tells the leader of the slots that the peer has turned
 //   warps 4-7, 12-15  epilogue: tensor memory to registers to global memory, 32 columns at a time in turns, while the next tile
 //              accumulates
 // An instruction of tcgen05 takes 20 to 60 cycles to issue, whatever it does; with the four to six copies of a stage's scales in
@@ -49,7 +50,7 @@ namespace m4 {
 constexpr int BP = 128;            // rows of P to a CTA
 constexpr int BK = 256, BKB = 128; // k of a stage, in values and in bytes
 constexpr int UK = 64;             // k of one tcgen05.mma kind::mxf4
-constexpr int THREADS = 512;       // warp 11 is idle: the epilogue's second four must be warps 0 .. 3 modulo 4
+constexpr int THREADS = 512;       // warp 11 is idle but in a pair's peer: the epilogue's second four must be warps 0 .. 3 modulo 4
 constexpr int MAX_GROUPS = 1024;
 constexpr int AHEAD = 48;          // tiles of a CTA that are worked out before it starts
 
@@ -295,7 +296,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm(const __grid_constant__ C
     const uint32_t slots = base + S::STAGES * S::STAGE, bars = slots + S::SLOTS * S::SLOT + S::TURN;
     auto full_bar = [&](int s) { return bars + 8u * s; };                                        // codes are there, and the scales in tensor memory (in a pair: both CTAs', at the leader)
     auto empty_bar = [&](int s) { return bars + 8u * (S::STAGES + s); };                         // the stage has been used up
-    auto turned_bar = [&](int s) { return bars + 8u * (2 * S::STAGES + s); };                    // a slot's scales are turned (in a pair: both CTAs', at the leader)
+    auto turned_bar = [&](int s) { return bars + 8u * (2 * S::STAGES + s); };                    // a slot's scales are turned (at the leader of a pair: both CTAs')
     auto slot_bar = [&](int s) { return bars + 8u * (2 * S::STAGES + S::SLOTS + s); };           // the slot has been used up
     auto accfull_bar = [&](int a) { return bars + 8u * (2 * S::STAGES + 2 * S::SLOTS + a); };
     auto accempty_bar = [&](int a) { return bars + 8u * (2 * S::STAGES + 2 * S::SLOTS + 2 + a); };
@@ -313,7 +314,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm(const __grid_constant__ C
     if (threadIdx.x == 0) {
         abort_flag = 0;
         for (int s = 0; s < S::STAGES; s++) { mbar_init(full_bar(s), 2); mbar_init(empty_bar(s), 1); }
-        for (int s = 0; s < S::SLOTS; s++) { mbar_init(turned_bar(s), pair ? 2 : 1); mbar_init(slot_bar(s), 1); }
+        for (int s = 0; s < S::SLOTS; s++) { mbar_init(turned_bar(s), pair && rank == 0 ? 2 : 1); mbar_init(slot_bar(s), 1); }
         for (int a = 0; a < 2; a++) { mbar_init(accfull_bar(a), 1); mbar_init(accempty_bar(a), pair ? 16 : 8); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -580,14 +581,29 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm(const __grid_constant__ C
                 if constexpr (S::Q_TILES == 2) turn(a, 2);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the tensor core reads these through the async proxy
                 __syncwarp();
-                // In a pair the leader's thread starts the copies of both CTAs. What the peer wrote is read by its own tensor core, behind the
-                // fence above, so a plain remote arrive passes it on; a release at cluster scope holds the warp for 1800 cycles.
-                if (lane < S::HALVES) {
-                    if (pair && rank) mbar_arrive_cluster(map_to_cta(turned_bar(r + lane), 0));
-                    else mbar_arrive(turned_bar(r + lane));
-                }
+                if (lane < S::HALVES) mbar_arrive(turned_bar(r + lane));
             }
             if (!ok) break;
+        }
+    } else if (pair && warp == 11) {
+        // The leader's thread starts the copies of both CTAs, so what the peer's warps turned must be ordered before it: their arrivals
+        // here (at the scope of the CTA), then a release at the scope of the cluster at the leader, which acquires at that scope. The
+        // release holds a warp for 1800 cycles, so the warps that turn leave it to this one, a window of 2300 at a time.
+        if (rank == 1) {
+            uint32_t n = 0;
+            for (int w = first; w < total && !__any_sync(~0u, *abortp); w += step, n++) {
+                const Tile t = tile_at(w, n);
+                bool ok = true;
+                for (int at = t.s0 & ~(S::WINDOW - 1); at < t.s1; at += S::WINDOW, sl += S::HALVES) {
+                    const int r = sl % S::SLOTS;
+                    const uint32_t parity = (sl / S::SLOTS) & 1u;
+                    for (int h = 0; h < S::HALVES && ok; h++) ok = warp_wait(turned_bar(r + h), parity, abortp, 0x141);
+                    if (!ok) break;
+                    if (lane < S::HALVES) mbar_arrive_release_cluster(map_to_cta(turned_bar(r + lane), 0));
+                    __syncwarp();
+                }
+                if (!ok) break;
+            }
         }
     } else if ((warp >= 4 && warp < 8) || warp >= 12) {
         const int quarter = warp & 3, half = warp >= 12;   // lanes 32 quarter .. +31, every other 32 columns
