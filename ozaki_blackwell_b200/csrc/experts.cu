@@ -371,7 +371,7 @@ __global__ void __launch_bounds__(256) combine_grad_rows(const T *dY, long long 
         };
         int c0 = 0;
         if constexpr (VEC) {
-            for (; c0 + U * 32 * N <= H; c0 += U * 32 * N) {
+            for (; H - c0 >= U * 32 * N; c0 += U * 32 * N) {   // (a sum may pass 31 bits behind the last piece of the widest rows)
                 uint4 qa[U], qb[U];
 #pragma unroll
                 for (int u = 0; u < U; u++) {
@@ -389,7 +389,7 @@ __global__ void __launch_bounds__(256) combine_grad_rows(const T *dY, long long 
             }
         }
         if constexpr (VEC) {
-            for (; c0 + 32 * N <= H; c0 += 32 * N) {
+            for (; H - c0 >= 32 * N; c0 += 32 * N) {
                 float a[N], b[N];
                 Vec16<T>::unpack(*reinterpret_cast<const uint4 *>(dy + c0 + lane * N), a);
                 Vec16<T>::unpack(__ldcs(reinterpret_cast<const uint4 *>(z + c0 + lane * N)), b);
