@@ -250,7 +250,8 @@ int ozb_mx4_gemm_grouped(int groups, int R, int N, int K, const int *offsets, co
                          const uint8_t *W, long long ldw, size_t plane_w, const uint8_t *Ws, long long ldws, size_t plane_ws, void *Y, int type,
                          long long ldy, void *stream);
 /* Y[g] = A[:, offsets[g] : offsets[g + 1]] B[:, the same]^T: A is M x R, B is N x R, blocks along R; Y[g] is M x N, plane_y elements
- * from one to the next, zeros for an empty segment. The offsets are multiples of 64 (they are rounded down to one). At most 1024. */
+ * from one to the next, zeros for an empty segment. The offsets are multiples of 64; the end of a segment may also be R. Of a segment
+ * that is not so, Y[g] is NaN, and ozb_status reports OZB_EARG. At most 1024. */
 int ozb_mx4_gemm_segments(int groups, int M, int N, int R, const int *offsets, const uint8_t *A, long long lda, const uint8_t *As, long long ldas,
                           const uint8_t *B, long long ldb, const uint8_t *Bs, long long ldbs, void *Y, int type, long long ldy, size_t plane_y,
                           void *stream);
@@ -286,7 +287,7 @@ int ozb_expert_mx4(int T, int top, int experts, int N, int K, const void *X, int
                    void *stream);
 /* Its gradients for dY (T x N): dX (T x K), dweights [T][top], and dW [experts] of N x K (plane_dw elements from one to the next), all
  * but dweights of `type`. Wt: the weights with blocks along N, [experts] of K x N; Z and the maps as ozb_expert_mx4 left them (segments
- * padded to 64). dZ = ozb_expert_combine_grad is rounded to `type`, then to the 4-bit format by rows for dX and by columns, as X, for
+ * padded to 64; dW of an expert whose segment is not comes out as ozb_mx4_gemm_segments says). dZ = ozb_expert_combine_grad is rounded to `type`, then to the 4-bit format by rows for dX and by columns, as X, for
  * dW; the gradient passes through the roundings. `work`: ozb_expert_mx4_grad_work bytes, 16-byte aligned. */
 size_t ozb_expert_mx4_grad_work(int R, int N, int K, int type);
 int ozb_expert_mx4_grad(int T, int top, int experts, int N, int K, int R, const void *dY, int type, long long lddy, const void *X, long long ldx,
@@ -353,7 +354,8 @@ int ozb_selftest_wait_expiry(int budget_ms);
 int ozb_bounds_report(unsigned long long out[4]);
 int ozb_selftest_bounds(void);
 /* Status of the stage calls above (they share one status word per device) and of the cached plans behind ozb_dgemm_ex,
- * ozb_dgemm_norm and ozb_ddgemm_ex on the current device: 0 or OZB_ETIMEOUT. Synchronises the device. */
+ * ozb_dgemm_norm and ozb_ddgemm_ex on the current device since the last call: 0, OZB_ETIMEOUT, or OZB_EARG (a product of 4-bit operands
+ * along k was given offsets that it refuses). Synchronises the device. */
 int ozb_status(void);
 
 #ifdef __cplusplus

@@ -349,7 +349,8 @@ static int plan_dgemm_host(ozb_plan *p, const double *A, const double *B, double
     return (int)e3;
 }
 
-// status words: [0] the first wait code of a launch that gave up (0 = none), [1..63] per-CTA codes for diagnostics
+// status words: [0] the first wait code of a launch that gave up (0 = none; STATUS_OFFSETS: a product that refused its segments),
+// [1..63] per-CTA codes for diagnostics
 static int read_status(int *dev_words) {
     int h[64] = {};
     if (cudaError_t e = cudaMemcpy(h, dev_words, sizeof h, cudaMemcpyDeviceToHost)) return (int)e;
@@ -358,6 +359,7 @@ static int read_status(int *dev_words) {
                 h[14], h[15]);
     if (!h[0]) return 0;
     cudaMemset(dev_words, 0, sizeof h);
+    if (h[0] == STATUS_OFFSETS) return OZB_EARG;
     if (getenv("OZ_DEBUG")) {
         fprintf(stderr, "ozb: a wait expired, first code 0x%x; per CTA:", h[0]);
         for (int i = 1; i < 64; i++) if (h[i]) fprintf(stderr, " [%d]=0x%x", i - 1, h[i]);

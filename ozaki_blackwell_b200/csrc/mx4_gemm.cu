@@ -5,7 +5,9 @@
 // X are the tokens, W the weights. Three walks over groups g:
 //     dense      one group
 //     by rows    group g owns the rows [offsets[g], offsets[g + 1]) of X and Y and multiplies them by its own W[g]
-//     along k    group g owns the k in [offsets[g], offsets[g + 1]) (multiples of 64); X and W are shared, Y[g] is its own
+//     along k    group g owns the k in [offsets[g], offsets[g + 1]) (multiples of 64, or K for an end); X and W are shared, Y[g] is its
+//                own. An instruction takes 64 of k: a segment that begins or ends inside them would take a neighbour's values or lose
+//                some of its own, so its Y[g] is NaN and the status word is raised.
 // The offsets live on the device. Accumulation is in FP32 in tensor memory, one rounding to the output type at the end.
 //
 // One kernel, warp-specialised: a tile is 128 rows of P, which are the lanes of the accumulator, by BN rows of Q, its columns; 256
@@ -55,6 +57,7 @@ constexpr int MAX_GROUPS = 1024;
 constexpr int AHEAD = 48;          // tiles of a CTA that are worked out before it starts
 
 enum { DENSE = 0, BY_ROWS = 1, ALONG_K = 2 };
+constexpr uint32_t NOT_A_NUMBER = 0x7fffffffu;
 enum { NARROW = 0, SPLIT = 1, WIDE = 2, PAIR = 3 };
 
 struct Params {
@@ -145,6 +148,7 @@ struct Tile {
     int p0, p1, q0, q1;      // rows of P and of Q: from the first, and where they end (this group's, not the tile's)
     int k0, k1;              // range along k
     int s0, s1;              // stages [s0, s1) of 256 that cover it (or this CTA's share of them)
+    int refused;             // the range along k begins or ends inside an instruction's 64
 };
 
 // The range along k or of rows that `offsets` gives group g. Offsets that are out of order or out of range are cut to what is there.
@@ -162,6 +166,7 @@ __device__ __forceinline__ Tile decode(const Params &p, const int *cum, int w) {
     int nt, lo = 0, hi = p.tokens, idx;
     t.k0 = 0;
     t.k1 = p.K;
+    t.refused = 0;
     if (p.mode == BY_ROWS) {
         int a = 0, b = p.groups;   // the last group whose first item is not behind w
         while (b - a > 1) {
@@ -179,8 +184,9 @@ __device__ __forceinline__ Tile decode(const Params &p, const int *cum, int w) {
         idx = w - t.group * per_group;
         if (p.mode == ALONG_K) {
             segment(p, t.group, p.K, t.k0, t.k1);
-            t.k0 &= ~(UK - 1);
-            t.k1 &= ~(UK - 1);
+            if (t.k1 > t.k0) t.refused = t.k0 % UK != 0 || (t.k1 % UK != 0 && t.k1 != p.K);
+            if (t.refused || t.k1 == t.k0) t.k1 = t.k0;   // no stage
+            else t.k1 = (t.k1 + UK - 1) & ~(UK - 1);      // what lies behind K is zero
         }
     }
     const int np = S::wide ? nt : nw, nq = S::wide ? nw : nt;
@@ -374,7 +380,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm(const __grid_constant__ C
     for (int n = threadIdx.x; n < AHEAD && n * (long long)step + first < total; n += THREADS) {
         const Tile t = decode<S>(p, cum, first + n * step);
         ahead[2 * n] = make_int4(t.group, t.p0, t.p1, t.q0);
-        ahead[2 * n + 1] = make_int4(t.q1, t.k0, t.k1, 0);
+        ahead[2 * n + 1] = make_int4(t.q1, t.k0, t.k1, t.refused);
     }
     __syncthreads();
     auto tile_at = [&](int w, uint32_t n) {   // the n-th tile of this CTA, item w
@@ -382,7 +388,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm(const __grid_constant__ C
         if (n < AHEAD) {
             const int4 a = ahead[2 * n], b = ahead[2 * n + 1];
             t.group = a.x; t.p0 = a.y; t.p1 = a.z; t.q0 = a.w;
-            t.q1 = b.x; t.k0 = b.y; t.k1 = b.z;
+            t.q1 = b.x; t.k0 = b.y; t.k1 = b.z; t.refused = b.w;
         } else t = decode<S>(p, cum, w);
         t.s0 = t.k0 / BK;
         t.s1 = t.k1 > t.k0 ? (t.k1 + BK - 1) / BK : t.s0;
@@ -616,7 +622,9 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm(const __grid_constant__ C
             if (!warp_wait(accfull_bar(acc), (n >> 1) & 1u, abortp, 0x150)) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * BN;
-            const bool some = t.s1 > t.s0;   // no stage: nothing was accumulated, the tile is zero
+            const bool some = t.s1 > t.s0;   // no stage: nothing was accumulated, the tile is zero (or refused)
+            const uint32_t nothing = uniform(t.refused) ? NOT_A_NUMBER : 0u;
+            if (nothing && quarter == 0 && !half && lane == 0) atomicCAS(p.status, 0, STATUS_OFFSETS);
             const int i0 = t.p0 + (pair ? (int)rank * BP : 0) + quarter * 32;   // the warp's first row of P
             if constexpr (FORM != SPLIT) {
                 T *Y = reinterpret_cast<T *>(p.Y) + (p.mode == ALONG_K ? (size_t)t.group * p.plane_y : 0);
@@ -628,7 +636,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm(const __grid_constant__ C
                     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
                     if (!some) {
 #pragma unroll
-                        for (int e = 0; e < 32; e++) v[e] = 0;
+                        for (int e = 0; e < 32; e++) v[e] = nothing;
                     }
                     const int j1 = min(t.q1, t.q0 + BN);   // a tile of 16 columns: the other 16 are not its own
                     if constexpr (S::wide) store_wide<T>(&mapY, p.whole_words, Y, p.ldy, v, i0, lane, t.p1, t.q0 + c, j1, p.mode == ALONG_K ? t.group : 0, piece);

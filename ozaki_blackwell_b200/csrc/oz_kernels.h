@@ -75,6 +75,7 @@ struct Mx4Product {
     long long ldy;
     size_t plane_y;
 };
+constexpr int STATUS_OFFSETS = 0x200;   // in the status word: segments along k that are not whole instructions (the last byte of a wait code is not 0)
 cudaError_t mx4_product(const Mx4Product &g, int *status, cudaStream_t st);
 
 // tokens by expert and back (experts.cu)

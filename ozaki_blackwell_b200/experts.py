@@ -122,7 +122,8 @@ def matmul(x, w, ids, weights=None, keep=False):
 def matmul_grad(dy, x, z, wt, routing, weights=None):
     """The gradients of matmul(..., keep=True): (dx, dweights, dw) with dw [experts, n, k] of x's type, in one call of the library. wt: the
     weights with blocks along n, mx4.quantize(W, dim=-2), a stack [experts, k, ...]. Operands of the products are rounded to the 4-bit
-    format, gradients pass through that rounding."""
+    format, gradients pass through that rounding. dw of an expert whose segment is not padded to 64, which only a Routing of unknown
+    padding can bring here, is NaN."""
     if routing.align % 64:
         raise ValueError(f"the segments are padded to {routing.align}: products along the tokens need multiples of 64 (matmul with keep=True)")
     lddy, ldx, ldz, index = _pitch(dy, "dy"), _pitch(x, "x"), _pitch(z, "z"), x.get_device()

@@ -192,7 +192,8 @@ def grouped_matmul(x, w, offsets, dtype=torch.bfloat16, out=None):
 
 
 def segment_matmul(a, b, offsets, dtype=torch.bfloat16, out=None):
-    """Y[g] = A[:, offsets[g] : offsets[g + 1]] B[:, the same]^T, [groups, rows of a, rows of b]; the offsets are multiples of 64."""
+    """Y[g] = A[:, offsets[g] : offsets[g + 1]] B[:, the same]^T, [groups, rows of a, rows of b]; the offsets are multiples of 64 (an end
+    may also be the vectors' length). Y[g] of a segment that is not so is NaN."""
     r, like = _common_length(a, b), a.codes
     index = like.get_device()
     groups = _offsets(offsets, index)
