@@ -67,10 +67,12 @@ def gather(x, routing, out=None):
 
 
 def combine(z, routing, weights=None, out=None):
-    """y[t] = sum over j of weights[t, j] z[rows[t, j]] (weights None: 1), in FP32, rounded once to z's type."""
+    """y[t] = sum over j of weights[t, j] z[rows[t, j]] (weights None: 1), in FP32, rounded once to z's type. z has all of the routing's rows."""
     ldz, index = _pitch(z, "z"), z.get_device()
     tokens, top = _routed(routing, index)
     kind, (r, h), w = _type(z.dtype), z.shape, _weights(weights, routing.rows.shape, index)
+    if r < routing.slots.shape[0]:
+        raise ValueError(f"z has {r} rows, the routing {routing.slots.shape[0]} rows")
     y, ldy = _result(z, out, (tokens, h), z.dtype)
     _call(index, _lib.ozb_expert_combine, tokens, top, h, z.data_ptr(), kind, r, ldz, routing.rows.data_ptr(), w, y.data_ptr(), ldy)
     return y
