@@ -287,8 +287,9 @@ int ozb_expert_mx4(int T, int top, int experts, int N, int K, const void *X, int
                    void *stream);
 /* Its gradients for dY (T x N): dX (T x K), dweights [T][top], and dW [experts] of N x K (plane_dw elements from one to the next), all
  * but dweights of `type`. Wt: the weights with blocks along N, [experts] of K x N; Z and the maps as ozb_expert_mx4 left them (segments
- * padded to 64; dW of an expert whose segment is not comes out as ozb_mx4_gemm_segments says). dZ = ozb_expert_combine_grad is rounded to `type`, then to the 4-bit format by rows for dX and by columns, as X, for
- * dW; the gradient passes through the roundings. `work`: ozb_expert_mx4_grad_work bytes, 16-byte aligned. */
+ * padded to 64; dW of an expert whose segment is not comes out as ozb_mx4_gemm_segments says). dZ = ozb_expert_combine_grad is rounded
+ * to `type`, then to the 4-bit format by rows for dX and by columns, as X, for dW; the gradient passes through the roundings. dX may be
+ * X, or dY or Z where the sizes let it. `work`: ozb_expert_mx4_grad_work bytes, 16-byte aligned. */
 size_t ozb_expert_mx4_grad_work(int R, int N, int K, int type);
 int ozb_expert_mx4_grad(int T, int top, int experts, int N, int K, int R, const void *dY, int type, long long lddy, const void *X, long long ldx,
                         const void *Z, long long ldz, const uint8_t *Wt, long long ldwt, size_t plane_wt, const uint8_t *Wts, long long ldwts,
