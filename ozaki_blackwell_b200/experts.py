@@ -8,7 +8,8 @@
     matmul_grad(dy, x, z, wt, routing, weights)       its gradients: (dx, dweights, dw)
 
 The gradient of gather is combine without weights. What each computes, index by index, is in include/ozb.h (ozb_expert_*). Every call
-is asynchronous on the current stream of the operands' device and may be captured into a CUDA graph.
+is asynchronous on the current stream of the operands' device and may be captured into a CUDA graph; mx4.status() tells whether the
+products of the last two did all that they were asked for.
 """
 from typing import NamedTuple
 

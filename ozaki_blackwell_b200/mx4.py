@@ -5,10 +5,13 @@
     matmul(x, w, dtype)                               Y = X W^T
     grouped_matmul(x, w, offsets, dtype)              rows offsets[g] .. offsets[g + 1] of X with W[g]
     segment_matmul(a, b, offsets, dtype)              Y[g] = A[:, segment g] B[:, segment g]^T
+    status(device=None)                               raises what products so far could not tell when they were called
 
 The format and the exact meaning of each are in include/ozb.h (ozb_mx4_*). Every call is asynchronous on the current stream of the
-operands' device and may be captured into a CUDA graph; results are new tensors unless out= is given. The backward pass of a
-product is two products: from y = matmul(quantize(x), quantize(w)) with a gradient dy,
+operands' device and may be captured into a CUDA graph; results are new tensors unless out= is given. So a call returns before its
+kernels have run, and a wait that expires in one of them (its result is then not valid) is only heard of from status().
+
+The backward pass of a product is two products: from y = matmul(quantize(x), quantize(w)) with a gradient dy,
 dx = matmul(quantize(dy), quantize(w, dim=-2)) and dw = matmul(quantize(dy, dim=-2), quantize(x, dim=-2)).
 """
 from typing import NamedTuple
@@ -21,7 +24,7 @@ from ._lib import lib as _lib
 _current_device = torch.cuda.current_device
 _raw_stream = torch._C._cuda_getCurrentRawStream   # the number behind torch.cuda.current_stream(index), without making the object
 
-__all__ = ["Mx4", "quantize", "dequantize", "matmul", "grouped_matmul", "segment_matmul"]
+__all__ = ["Mx4", "quantize", "dequantize", "matmul", "grouped_matmul", "segment_matmul", "status"]
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _RULES = {"floor": 0, "ceil": 1}
@@ -155,6 +158,18 @@ def dequantize(q, dtype=torch.float32, out=None):
     y, ldy = _result(like, out, (n, length), dtype)
     _call(index, _lib.ozb_mx4_dequantize, codes, ldq, scales, lds, n, length, y.data_ptr(), _type(dtype), ldy)
     return y
+
+
+def status(device=None):
+    """Waits for `device` (default: the current one) and raises OzakiError if, since the last call, a bounded wait of a product on it
+    expired, whose result is then not valid, or a product along the vectors refused its segments, whose results are NaN."""
+    if device is None:
+        code = _lib.ozb_status()
+    else:
+        with torch.cuda.device(device):
+            code = _lib.ozb_status()
+    if code:
+        raise OzakiError(code)
 
 
 def _common_length(a, b):

@@ -37,3 +37,15 @@ def test_combine_needs_a_row_for_each_of_the_routing(gpu):
     for rows in (8, 9):     # more do no harm
         assert experts.combine(gpu(rows, 16), r).shape == (4, 16)
     assert len(gpu.calls) == 2
+
+
+def test_status_is_the_library_s(monkeypatch):
+    """mx4.status: nothing where all went well, the library's error where a wait expired or segments were refused."""
+    from ozaki_blackwell_b200 import OzakiError
+    codes = iter([0, 10004, 10001])
+    monkeypatch.setattr(mx4, "_lib", type("Library", (), {"ozb_status": staticmethod(lambda: next(codes))}))
+    assert mx4.status() is None
+    for code in (10004, 10001):
+        with pytest.raises(OzakiError) as e:
+            mx4.status()
+        assert e.value.code == code
