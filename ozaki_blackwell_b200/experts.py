@@ -9,14 +9,14 @@
 
 The gradient of gather is combine without weights. What each computes, index by index, is in include/ozb.h (ozb_expert_*). Every call
 is asynchronous on the current stream of the operands' device and may be captured into a CUDA graph; mx4.status() tells whether the
-products of the last two did all that they were asked for.
+products of the last two did all that they were asked for. None takes part in autograd; they warn where an operand requires a gradient.
 """
 from typing import NamedTuple
 
 import torch
 
 from ._lib import lib as _lib
-from .mx4 import _call, _codes, _offsets, _pitch, _result, _routed, _type
+from .mx4 import _call, _codes, _cut, _offsets, _pitch, _result, _routed, _type
 
 __all__ = ["Routing", "sort", "gather", "combine", "combine_grad", "matmul", "matmul_grad"]
 
@@ -61,6 +61,8 @@ def gather(x, routing, out=None):
     tokens, top = _routed(routing, index)
     if x.shape[0] != tokens:
         raise ValueError(f"x has {x.shape[0]} rows, the routing {tokens} tokens")
+    if x.requires_grad:
+        _cut("gather")
     kind, r, h = _type(x.dtype), routing.slots.shape[0], x.shape[1]
     y, ldy = _result(x, out, (r, h), x.dtype)
     _call(index, _lib.ozb_expert_gather, tokens, top, h, x.data_ptr(), kind, ldx, r, routing.rows.data_ptr(), routing.slots.data_ptr(), y.data_ptr(), ldy)
@@ -74,6 +76,8 @@ def combine(z, routing, weights=None, out=None):
     kind, (r, h), w = _type(z.dtype), z.shape, _weights(weights, routing.rows.shape, index)
     if r < routing.slots.shape[0]:
         raise ValueError(f"z has {r} rows, the routing {routing.slots.shape[0]} rows")
+    if z.requires_grad or w is not None and weights.requires_grad:
+        _cut("combine")
     y, ldy = _result(z, out, (tokens, h), z.dtype)
     _call(index, _lib.ozb_expert_combine, tokens, top, h, z.data_ptr(), kind, r, ldz, routing.rows.data_ptr(), w, y.data_ptr(), ldy)
     return y
@@ -87,6 +91,8 @@ def combine_grad(dy, z, routing, weights=None):
     if dy.dtype is not z.dtype or dy.shape != (tokens, h) or r != routing.slots.shape[0] or dy.get_device() != index:
         raise ValueError(f"dy {tuple(dy.shape)} of {dy.dtype} and z {tuple(z.shape)} of {z.dtype} do not fit a routing of {tokens} tokens and {routing.slots.shape[0]} rows")
     kind, w = _type(z.dtype), _weights(weights, routing.rows.shape, index)
+    if dy.requires_grad or z.requires_grad or w is not None and weights.requires_grad:
+        _cut("combine_grad")
     dz, dweights = z.new_empty(r, h), z.new_empty(tokens, top, dtype=torch.float32)
     _call(index, _lib.ozb_expert_combine_grad, tokens, top, h, dy.data_ptr(), kind, lddy, z.data_ptr(), ldz, r, routing.rows.data_ptr(),
           routing.slots.data_ptr(), w, dz.data_ptr(), h, dweights.data_ptr())
@@ -106,6 +112,8 @@ def matmul(x, w, ids, weights=None, keep=False):
         raise ValueError(f"cannot multiply rows of {k} by vectors of {w.length}")
     (experts, n), top = w.codes.shape[:2], ids.shape[1]
     factors = _weights(weights, ids.shape, index)
+    if x.requires_grad or factors is not None and weights.requires_grad:
+        _cut("matmul")
     align = 64 if keep else 1
     need = _lib.ozb_expert_mx4_work(tokens, top, experts, n, k, kind, align)
     if not need:
@@ -139,6 +147,8 @@ def matmul_grad(dy, x, z, wt, routing, weights=None):
     if _offsets(routing.offsets, index) != experts or wt.length != n or wt.codes.shape[1] != k:
         raise ValueError(f"wt must be a stack of {routing.offsets.shape[0] - 1} matrices of {k} vectors of {n}")
     factors = _weights(weights, routing.rows.shape, index)
+    if dy.requires_grad or x.requires_grad or z.requires_grad or factors is not None and weights.requires_grad:
+        _cut("matmul_grad")
     need = _lib.ozb_expert_mx4_grad_work(r, n, k, kind)
     dx, dweights = x.new_empty(tokens, k), x.new_empty(tokens, top, dtype=torch.float32)
     dw, work = x.new_empty(experts, n, k), x.new_empty(need, dtype=torch.uint8)

@@ -12,8 +12,10 @@ operands' device and may be captured into a CUDA graph; results are new tensors 
 kernels have run, and a wait that expires in one of them (its result is then not valid) is only heard of from status().
 
 The backward pass of a product is two products: from y = matmul(quantize(x), quantize(w)) with a gradient dy,
-dx = matmul(quantize(dy), quantize(w, dim=-2)) and dw = matmul(quantize(dy, dim=-2), quantize(x, dim=-2)).
+dx = matmul(quantize(dy), quantize(w, dim=-2)) and dw = matmul(quantize(dy, dim=-2), quantize(x, dim=-2)). The calls take no part in
+autograd, and warn where an operand requires a gradient.
 """
+import warnings
 from typing import NamedTuple
 
 import torch
@@ -53,6 +55,13 @@ def _call(index, entry, *args):
             status = entry(*args, _raw_stream(index))
     if status:
         raise OzakiError(status)
+
+
+def _cut(name):
+    """An operand requires a gradient that the result will not carry."""
+    if torch.is_grad_enabled():
+        warnings.warn(f"{name} takes no part in autograd and an operand requires a gradient, which ends here: call it from the forward of a "
+                      "torch.autograd.Function whose backward makes the gradients' calls, or under torch.no_grad()", UserWarning, stacklevel=3)
 
 
 def _pitch(x, role, dims=2):
@@ -128,6 +137,8 @@ def quantize(x, dim=-1, rule="floor", routing=None):
     if dims not in (2, 3):
         raise ValueError(f"x must be a matrix or a stack of matrices, not {dims}-dimensional")
     ldx, index = _pitch(x, "x", dims), x.get_device()
+    if x.requires_grad:
+        _cut("quantize")
     rows, cols = shape[-2:]
     maps = None, None, 0, 0
     if routing is not None:

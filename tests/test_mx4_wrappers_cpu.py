@@ -49,3 +49,31 @@ def test_status_is_the_library_s(monkeypatch):
         with pytest.raises(OzakiError) as e:
             mx4.status()
         assert e.value.code == code
+
+
+def _stack(gpu, experts_, n, k):
+    u8 = dict(dtype=torch.uint8)
+    return mx4.Mx4(gpu(experts_, n, k // 2, **u8), gpu(experts_, n, 16, **u8), k)
+
+
+def test_a_gradient_that_is_cut_is_said(gpu, recwarn):
+    """The calls take no part in autograd: on an operand that requires a gradient they warn, unless autograd is off."""
+    x, dy, z = gpu(4, 64), gpu(4, 32), gpu(8, 32)
+    ids, weights, r = gpu(4, 2, dtype=torch.int32), gpu(4, 2), _routing(gpu)
+    w, wt, padded = _stack(gpu, 3, 32, 64), _stack(gpu, 3, 64, 32), _routing(gpu)._replace(align=64)
+    calls = {"quantize": (lambda: mx4.quantize(x), [x]), "gather": (lambda: experts.gather(x, r), [x]), "combine": (lambda: experts.combine(z, r, weights), [z, weights]),
+             "combine_grad": (lambda: experts.combine_grad(dy, z, r, weights), [dy, z, weights]),
+             "matmul": (lambda: experts.matmul(x, w, ids, weights), [x, weights]),
+             "matmul_grad": (lambda: experts.matmul_grad(dy, x, z, wt, padded, weights), [dy, x, z, weights])}
+    cut = lambda: [str(v.message) for v in recwarn.list if "autograd" in str(v.message)]  # noqa: E731
+    for name, (call, operands) in calls.items():
+        call()
+        assert not cut(), name                      # nothing requires a gradient
+        for t in operands:
+            t.requires_grad_()
+            with torch.no_grad():
+                call()
+            assert not cut(), name                  # as inside a torch.autograd.Function
+            with pytest.warns(UserWarning, match=f"{name} takes no part in autograd"):
+                call()
+            t.requires_grad_(False)
