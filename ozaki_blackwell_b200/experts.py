@@ -16,7 +16,7 @@ from typing import NamedTuple
 import torch
 
 from ._lib import lib as _lib
-from .mx4 import _call, _codes, _cut, _offsets, _pitch, _result, _routed, _type
+from .mx4 import _MOST, _call, _codes, _cut, _offsets, _pitch, _result, _routed, _type
 
 __all__ = ["Routing", "sort", "gather", "combine", "combine_grad", "matmul", "matmul_grad"]
 
@@ -44,7 +44,7 @@ def sort(ids, experts, align=1):
     if ids.dtype not in (torch.int32, torch.int64) or ids.dim() != 2 or not ids.is_contiguous() or not ids.is_cuda:
         raise ValueError("ids must be a contiguous [tokens, top] matrix of int32 or int64 on a GPU")
     tokens, top = ids.shape
-    size = _lib.ozb_expert_sort_rows(tokens, top, experts, align)
+    size = _lib.ozb_expert_sort_rows(tokens, top, experts, align) if max(ids.numel(), experts, align) <= _MOST else -1
     if size < 0:
         raise ValueError(f"cannot sort {tokens} x {top} slots over {experts} experts in segments of {align}: sizes are positive, at most 1024 experts, align at most 256")
     need = _lib.ozb_expert_sort_scratch(tokens, top, experts)
@@ -105,7 +105,7 @@ def matmul(x, w, ids, weights=None, keep=False):
     along the rows of x. keep: returns (y, z, routing) for matmul_grad, with segments padded to 64."""
     ldx, index = _pitch(x, "x"), x.get_device()
     kind, (tokens, k) = _type(x.dtype), x.shape
-    if (ids.dtype is not torch.int32 and ids.dtype is not torch.int64) or ids.dim() != 2 or ids.shape[0] != tokens or not ids.is_contiguous() or ids.get_device() != index:
+    if (ids.dtype is not torch.int32 and ids.dtype is not torch.int64) or ids.dim() != 2 or ids.shape[0] != tokens or not ids.is_contiguous() or ids.get_device() != index or ids.numel() > _MOST:
         raise ValueError(f"ids must be a contiguous [{tokens}, top] matrix of int32 or int64 on cuda:{index}")
     wc, ldw, ws, ldws = _codes(w, "w", 3, index)
     if w.length != k:

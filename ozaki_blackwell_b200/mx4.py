@@ -30,6 +30,7 @@ __all__ = ["Mx4", "quantize", "dequantize", "matmul", "grouped_matmul", "segment
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _RULES = {"floor": 0, "ceil": 1}
+_MOST = 2 ** 31 - 1   # of rows, columns, vectors, values: the library counts in 32 bits (where memory is large enough for more)
 
 
 class Mx4(NamedTuple):
@@ -64,6 +65,11 @@ def _cut(name):
                       "torch.autograd.Function whose backward makes the gradients' calls, or under torch.no_grad()", UserWarning, stacklevel=3)
 
 
+def _few(role, sizes):
+    if max(sizes) > _MOST:
+        raise ValueError(f"{role} of sizes {tuple(sizes)}: none may pass {_MOST}")
+
+
 def _pitch(x, role, dims=2):
     """Checks that x is a matrix (or a stack of them) on a GPU whose rows are contiguous; elements from one row to the next (a single row
     has any stride)."""
@@ -74,6 +80,8 @@ def _pitch(x, role, dims=2):
         raise TypeError(f"{role} must be on a GPU")
     if stride[-1] != 1 and shape[-1] != 1:
         raise ValueError(f"the rows of {role} must be contiguous; make it contiguous first")
+    if x.numel() > _MOST:
+        _few(role, shape)
     return stride[-2] if shape[-2] > 1 else max(stride[-2], shape[-1])
 
 
@@ -84,6 +92,8 @@ def _codes(q, role, dims, index):
     have, bytes_, at, steps = codes.shape, scales.shape, codes.stride(), scales.stride()
     if (codes.dtype is torch.uint8 and scales.dtype is torch.uint8 and len(have) == dims and have[:-1] == bytes_[:-1] and at[-1] == 1 and steps[-1] == 1
             and have[-1] >= 16 * blocks and bytes_[-1] >= (blocks + 15) & ~15 and codes.get_device() == index == scales.get_device() and index >= 0):
+        if length > _MOST or codes.numel() > _MOST:
+            _few(role, (*have[:-1], length))
         if have[-2] > 1:
             return codes.data_ptr(), at[-2], scales.data_ptr(), steps[-2]
         return codes.data_ptr(), max(at[-2], have[-1]), scales.data_ptr(), max(steps[-2], bytes_[-1])   # one vector has any pitch
@@ -121,6 +131,8 @@ def _routed(r, index):
     for name, t in (("rows", r.rows), ("slots", r.slots)):
         if t.dtype is not torch.int32 or not t.is_contiguous() or t.get_device() != index:
             raise ValueError(f"routing.{name} must be contiguous int32 on cuda:{index}")
+        if t.numel() > _MOST:
+            raise ValueError(f"routing.{name} has {t.numel()} numbers, which may not pass {_MOST}")
     if r.rows.dim() != 2:
         raise ValueError("routing.rows has a row for each token")
     return r.rows.shape

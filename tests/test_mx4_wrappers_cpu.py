@@ -77,3 +77,21 @@ def test_a_gradient_that_is_cut_is_said(gpu, recwarn):
             with pytest.warns(UserWarning, match=f"{name} takes no part in autograd"):
                 call()
             t.requires_grad_(False)
+
+
+def test_sizes_past_32_bits_are_refused(gpu):
+    """The library counts in 32 bits; a larger size is refused here, not cut to its low bits."""
+    much, u8, i32 = 2 ** 32 + 4, dict(dtype=torch.uint8), dict(dtype=torch.int32)
+    x, ids, r = gpu(4, 64), gpu(4, 2, **i32), _routing(gpu)
+    codes = lambda n, k: mx4.Mx4(gpu(n, max(16, k // 2), **u8), gpu(n, max(16, k // 32), **u8), k)  # noqa: E731
+    for call in (lambda: mx4.quantize(gpu(much, 1)), lambda: mx4.quantize(gpu(much, 1), dim=-2), lambda: mx4.quantize(gpu(1, much)), lambda: mx4.quantize(gpu(much, 1, 1)),
+                 lambda: mx4.quantize(x, routing=r._replace(slots=gpu(much, **i32))),
+                 lambda: mx4.dequantize(codes(much, 32)), lambda: mx4.dequantize(codes(1, much)),
+                 lambda: mx4.matmul(codes(much, 32), codes(4, 32)), lambda: mx4.matmul(codes(4, 32), codes(much, 32)), lambda: mx4.matmul(codes(1, much), codes(1, much)),
+                 lambda: experts.sort(ids, much), lambda: experts.sort(ids, 4, much), lambda: experts.sort(gpu(much, 1, **i32), 4), lambda: experts.sort(gpu(1, much, **i32), 4),
+                 lambda: experts.gather(x, r._replace(slots=gpu(much, **i32))), lambda: experts.gather(gpu(much, 1), r._replace(rows=gpu(much, 1, **i32))),
+                 lambda: experts.combine(gpu(much, 1), r), lambda: experts.combine(gpu(8, much), r),
+                 lambda: experts.matmul(gpu(much, 64), _stack(gpu, 3, 32, 64), gpu(much, 1, **i32)), lambda: experts.matmul(x, _stack(gpu, 3, 32, 64), gpu(4, much, **i32))):
+        with pytest.raises(ValueError):
+            call()
+    assert not gpu.calls
