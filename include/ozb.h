@@ -21,7 +21,7 @@ extern "C" {
 #endif
 
 enum {
-    OZB_EARG = 10001,     /* python/capi.cu:17 -- M, N, K not positive, or moduli outside 8..16 */
+    OZB_EARG = 10001,     /* python/capi.cu:17 -- M, N, K not positive, or moduli outside 8..16; additions: any argument that an entry point's text rules out */
     OZB_EK = 10002,       /* python/capi.cu:17 -- K >= 131072: the int32 accumulators of the INT8 GEMMs would overflow */
     OZB_EARCH = 10003,    /* python/capi.cu:17 -- unsupported GPU; here: anything that is not compute capability 10.x */
     OZB_ETIMEOUT = 10004, /* addition: a bounded wait inside the GEMM kernel expired; the result is not valid */

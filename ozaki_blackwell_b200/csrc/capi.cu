@@ -462,7 +462,7 @@ OZB_API const char *ozb_version(void) { return OZB_VERSION; }
 OZB_API const char *ozb_error(int e) {
     switch (e) {
     case 0: return "ok";
-    case OZB_EARG: return "M, N and K must be positive, and every other argument there, aligned and in its range";
+    case OZB_EARG: return "an argument is refused: sizes (M, N, K, ...) must be positive, pointers there and aligned, pitches and planes wide enough that rows and matrices do not overlap, segments whole, every other argument in its range";
     case OZB_EK: return "K must be below 131072 (the int32 accumulators of the INT8 GEMMs)";
     case OZB_EARCH: return "this build runs on compute capability 10.x GPUs (B200, sm_100a: tcgen05 tensor cores) only";
     case OZB_ETIMEOUT: return "a bounded wait inside a GEMM kernel expired; the result is not valid";

@@ -95,3 +95,10 @@ def test_sizes_past_32_bits_are_refused(gpu):
         with pytest.raises(ValueError):
             call()
     assert not gpu.calls
+
+
+def test_the_text_of_a_refusal_names_what_is_refused():
+    """One code stands for every refused argument: a misaligned row and an overlapping stack too."""
+    from ozaki_blackwell_b200 import OzakiError
+    text = str(OzakiError(10001))
+    assert all(word in text for word in ("positive", "aligned", "overlap", "segments"))
