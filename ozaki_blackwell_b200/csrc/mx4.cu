@@ -66,7 +66,8 @@ __device__ __forceinline__ uint32_t scale_byte(uint32_t amax_bits, int rule) {
     const int field = (int)((amax_bits + (rule ? 0x3fffffu : 0u)) >> 23);   // mantissa above 1.5: the next power of two
     return field > 2 ? (uint32_t)(field - 2) : 0u;
 }
-// 2^-e for the byte e + 127; 0 for a block that is not a number, whose codes are then 0 (its values are cleared first)
+// 2^-e for the byte e + 127, which is at most 253 (e of the largest number is 126). For 255, a block that is not a number, it
+// is minus infinity, and the codes that come of it are cleared.
 __device__ __forceinline__ float inverse_scale(uint32_t byte) { return __uint_as_float((254u - byte) << 23); }
 __device__ __forceinline__ float scale_of(uint32_t byte) {
     return __uint_as_float(byte == 255 ? 0x7fffffffu : byte ? byte << 23 : 0x00400000u);
@@ -333,7 +334,7 @@ cudaError_t mx4_quantize_rows(const void *X, int type, int nvec, int len, long l
     const bool vec = !(reinterpret_cast<uintptr_t>(X) & 15) && !(ldx * size & 15) && !(plane_x * size & 15) && !((long long)len * size & 15);
     const long long vectors = slots ? tokens : (long long)planes * nvec;
     const int load = 512 / size;   // values that a warp loads at a time
-    const bool few = vectors * ((len + load - 1) / load) < 148 * 16;
+    const bool few = vectors * ((len + load - 1) / load) < 16LL * multiprocessors();   // loads in all
     const int unit = few ? load : load * UNITS;
     const int grid = warp_grid(vectors * ((len + unit - 1) / unit) + (slots ? nvec / 32 : 0));
     cudaError_t e = cudaErrorInvalidValue;
@@ -341,7 +342,9 @@ cudaError_t mx4_quantize_rows(const void *X, int type, int nvec, int len, long l
         using T = decltype(t);
         auto go = [&](auto vec_, auto routed_) {
             constexpr bool v = decltype(vec_)::value, r = decltype(routed_)::value;
-            // four loads in flight to a warp, or one where there are few: (16, 4096) values 2.4 and 1.9 us, (2048, 7168) 8.6 and 13.4
+            // Four loads in flight to a warp, or one where there are few. BF16 in us, four : one: (16, 4096) 2.1 : 1.4, (128, 4096) 2.15 : 1.7,
+            // (1024, 4096) 4.0 : 4.2, (2048, 7168) 8.5 : 11.3; between 16 and 64 loads to an SM, where it is four, one would be the shorter:
+            // (512, 4096) 3.4 : 2.7.
             e = few ? launch_behind(mx4_rows<T, v, r, 1>, grid, 256, 0, 1, st, (const T *)X, nvec, len, ldx, plane_x, planes, rule, rows, slots, top, tokens, codes, ldq,
                                     plane_q, scales, lds, plane_s)
                     : launch_behind(mx4_rows<T, v, r, UNITS>, grid, 256, 0, 1, st, (const T *)X, nvec, len, ldx, plane_x, planes, rule, rows, slots, top, tokens, codes,

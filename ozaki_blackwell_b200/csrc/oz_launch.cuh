@@ -14,6 +14,12 @@ __device__ __forceinline__ void behind_predecessors() {
     asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
+inline int multiprocessors() {   // of the current device
+    int dev = 0, n = 0;
+    if (cudaGetDevice(&dev) || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev)) cudaGetLastError();
+    return n;
+}
+
 template <class... P, class... A>
 cudaError_t launch_behind(void (*kernel)(P...), int grid, int block, size_t smem, int cluster, cudaStream_t st, A &&...args) {
     cudaLaunchConfig_t cfg = {};
