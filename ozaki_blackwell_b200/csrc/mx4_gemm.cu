@@ -657,7 +657,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm(const __grid_constant__ C
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
             if (lane == 0) {
-                if constexpr (pair) mbar_arrive_cluster(map_to_cta(accempty_bar(acc), 0));
+                if constexpr (pair) mbar_arrive_cluster(map_to_cta(accempty_bar(acc), 0));   // hands over no data: what was read is in registers
                 else mbar_arrive(accempty_bar(acc));
             }
         }
@@ -820,6 +820,8 @@ cudaError_t mx4_product(const Mx4Product &g, int *status, cudaStream_t st) {
     p.tokens = g.tokens;
     p.weights = g.weights;
     p.K = g.K;
+    // 2048 x 18432 x 7168 in us with 4 : 8 : 16 : 32 : 64: 115 : 109 : 109 : 110 : 121; 8192^3, under the power limit, and 1024 x 8192 x 8192 the
+    // same from 8 on
     p.band = 16;
     p.offsets = g.offsets;
     p.Y = g.y; p.ldy = g.ldy; p.plane_y = g.plane_y;
