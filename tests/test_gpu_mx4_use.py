@@ -1,0 +1,158 @@
+"""Calls as programs make them: captured over forked streams, replayed two at a time, on operands that are views, at the ends of the
+scales' range, over more than 2^31 elements, on routings that leave experts without tokens or one with all of them."""
+import pytest
+import torch
+
+import mx4_ref as ref
+
+pytestmark = pytest.mark.gpu
+TABLE = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0, -0.0, -0.5, -1.0, -1.5, -2.0, -3.0, -4.0, -6.0)
+
+
+def _codes(seed, *shape):
+    """Values that the format holds exactly, whatever the largest of a block."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return torch.tensor(TABLE, device="cuda")[torch.randint(0, 16, shape, generator=g, device="cuda")]
+
+
+def test_capture_over_forked_streams():
+    from ozaki_blackwell_b200 import mx4
+    m, n, k = 70, 300, 500
+    x, w = _codes(1, m, k), _codes(2, n, k)
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        main = torch.cuda.current_stream()
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            q = mx4.quantize(w)
+        p = mx4.quantize(x)
+        main.wait_stream(side)
+        y = mx4.matmul(p, q, torch.float32)
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            back = mx4.dequantize(mx4.quantize(y, dim=-2))
+        yt = mx4.matmul(q, p, torch.float32)
+        main.wait_stream(side)
+    for seed in range(3, 8):
+        x.copy_(_codes(seed, m, k))
+        w.copy_(_codes(seed + 10, n, k))
+        graph.replay()
+        want = x.double() @ w.double().t()
+        assert torch.equal(y, want.float()) and torch.equal(yt, y.t())
+        assert torch.equal(back, mx4.dequantize(mx4.quantize(y, dim=-2)))
+
+
+def test_two_graphs_at_once():
+    """Each has its own maps and workspaces: replayed side by side they do not meet."""
+    from ozaki_blackwell_b200 import experts as ex
+    from ozaki_blackwell_b200 import mx4
+    tokens, top, experts, n, k = 200, 2, 6, 320, 256
+    streams, graphs, held, got, want = [torch.cuda.Stream() for _ in range(2)], [], [], [], []
+    w = _codes(1, experts, n, k)
+    wq, wt = mx4.quantize(w), mx4.quantize(w, dim=-2)
+    weights = torch.full((tokens, top), 2.0, device="cuda")
+    for i in range(2):
+        x, dy = _codes(10 + i, tokens, k), _codes(20 + i, tokens, n)
+        ids = torch.randint(0, experts, (tokens, top), generator=torch.Generator().manual_seed(i)).cuda()
+        held.append((x, dy, ids))
+
+        def step(x=x, dy=dy, ids=ids):
+            y, z, r = ex.matmul(x, wq, ids, weights, keep=True)
+            return (y, *ex.matmul_grad(dy, x, z, wt, r, weights))
+
+        want.append([t.clone() for t in step()])
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got.append(step())
+        graphs.append(graph)
+    torch.cuda.synchronize()
+    for _ in range(30):
+        for t in (*got[0], *got[1]):
+            t.fill_(9)
+        torch.cuda.synchronize()
+        for s, graph in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+@pytest.mark.parametrize("far", [40, 100, 126])
+@pytest.mark.parametrize("m,n,k", [(9, 140, 200), (300, 9600, 96), (2, 70, 16384)])
+def test_scales_at_opposite_ends(m, n, k, far):
+    """2^far on one side and 2^-far on the other: the products are those of the codes."""
+    from ozaki_blackwell_b200 import mx4
+    x, w = _codes(1, m, k), _codes(2, n, k)
+    p, q = mx4.quantize(x), mx4.quantize(w)
+    for a, b in ((p, q), (q, p)):
+        up, down = (mx4.Mx4(t.codes, (t.scales.int() + d).clamp(0, 254).to(torch.uint8), t.length) for t, d in ((a, far), (b, -far)))
+        # a block whose scale is cut at the lowest or highest stands for other values: take them as they are
+        want = (mx4.dequantize(mx4.Mx4(up.codes, (up.scales.int() - far).to(torch.uint8), k)).double()
+                @ mx4.dequantize(mx4.Mx4(down.codes, (down.scales.int() + far).to(torch.uint8), k)).double().t())
+        assert torch.equal(mx4.matmul(up, down, torch.float32), want.float())
+
+
+def test_operands_that_are_views():
+    from ozaki_blackwell_b200 import experts as ex
+    from ozaki_blackwell_b200 import mx4
+    tokens, top, experts, n, k = 33, 2, 4, 70, 96
+    x, w = _codes(1, tokens, k + 40)[:, 5: 5 + k], _codes(2, experts, n, k)
+    ids = torch.randint(0, experts, (tokens, top), generator=torch.Generator().manual_seed(1)).cuda()
+    wide = mx4.quantize(_codes(3, experts + 2, n + 9, k))
+    part = mx4.Mx4(wide.codes[1: 1 + experts, 4: 4 + n], wide.scales[1: 1 + experts, 4: 4 + n], k)
+    whole = mx4.Mx4(part.codes.contiguous(), part.scales.contiguous(), k)
+    assert torch.equal(ex.matmul(x, part, ids), ex.matmul(x.contiguous(), whole, ids))
+    # a matrix's columns and a single row of it; every second matrix of a stack
+    got, want = mx4.quantize(w[::2], dim=-2), mx4.quantize(w[::2].contiguous(), dim=-2)
+    assert all(torch.equal(a, b) for a, b in zip(ref.unpack(got), ref.unpack(want)))   # the scales' bytes behind the last block are nobody's
+    one = x[7: 8]
+    assert torch.equal(mx4.matmul(mx4.quantize(one), mx4.quantize(w[0]), torch.float32), (one.double() @ w[0].double().t()).float())
+    # one matrix for all planes: read again and again
+    many = w[:1].expand(3, n, k)
+    q = mx4.quantize(many)
+    assert all(torch.equal(q.codes[i], mx4.quantize(w[0]).codes) for i in range(3))
+
+
+@pytest.mark.parametrize("ids", ["one expert", "all dropped", "the last expert alone has one"])
+@pytest.mark.parametrize("tokens,experts,n,k", [(600, 8, 500, 320), (2, 64, 130, 8000)])
+def test_routings_far_from_even(ids, tokens, experts, n, k):
+    from ozaki_blackwell_b200 import experts as ex
+    from ozaki_blackwell_b200 import mx4
+    top = 2
+    chosen = torch.full((tokens, top), 3 if ids == "one expert" else -1, device="cuda")
+    if ids == "the last expert alone has one":
+        chosen[tokens - 1, 1] = experts - 1
+    x, dy, w = _codes(1, tokens, k), _codes(2, tokens, n), _codes(3, experts, n, k)
+    weights = torch.full((tokens, top), 0.5, device="cuda")
+    y, z, r = ex.matmul(x, mx4.quantize(w), chosen, weights, keep=True)
+    assert torch.equal(y, ex.matmul(x, mx4.quantize(w), chosen, weights))
+    dx, dweights, dw = ex.matmul_grad(dy, x, z, mx4.quantize(w, dim=-2), r, weights)
+    for e in range(experts):
+        times = (chosen == e).double().sum(1, keepdim=True) * 0.5
+        assert torch.equal(dw[e], ((times * dy.double()).t() @ x.double()).float())
+    times = [(chosen == e).double().sum(1, keepdim=True) * 0.5 for e in range(experts)]
+    assert torch.equal(y, sum(t * (x.double() @ w[e].double().t()) for e, t in enumerate(times)).float())
+    assert torch.equal(dx, sum(t * (dy.double() @ w[e].double()) for e, t in enumerate(times)).float())
+    assert bool((dweights[chosen < 0] == 0).all()) and mx4.status() is None
+
+
+def test_rows_past_31_bits():
+    """More than 2^31 elements gathered, added up again and rounded by columns."""
+    from ozaki_blackwell_b200 import experts as ex
+    from ozaki_blackwell_b200 import mx4
+    tokens, top, h = 140000, 8, 2056
+    assert tokens * top * h > 2 ** 31
+    x = torch.tensor(TABLE, device="cuda", dtype=torch.bfloat16)[torch.randint(0, 8, (tokens, h), generator=torch.Generator(device="cuda").manual_seed(1), device="cuda")]
+    ids = torch.randint(0, 16, (tokens, top), generator=torch.Generator(device="cuda").manual_seed(2), device="cuda")
+    r = ex.sort(ids, 16)
+    z = ex.gather(x, r)
+    for row in (0, 1, tokens * top // 2, tokens * top - 2, tokens * top - 1):
+        assert torch.equal(z[row], x[r.slots[row].item() // top])
+    assert torch.equal(ex.combine(z, r), 8 * x)              # eight times a number of three bits
+    dz, dweights = ex.combine_grad(x, z, r)
+    assert torch.equal(dz, z)
+    assert bool((dweights == dweights[:, :1]).all())         # the same products in the same order
+    del dz
+    q, one = mx4.quantize(z, dim=-2), mx4.quantize(z[-64:].contiguous(), dim=-2)
+    assert q.length % 64 == 0 and torch.equal(q.codes[:, -32:], one.codes[:, :32])
