@@ -146,9 +146,8 @@ __device__ __forceinline__ uint4 first_bytes(uint4 v, int n) {
 struct Tile {
     int group;
     int p0, p1, q0, q1;      // rows of P and of Q: from the first, and where they end (this group's, not the tile's)
-    int k0, k1;              // range along k
+    int k0, k1;              // range along k; k1 = -1: it begins or ends inside an instruction's 64 and is refused
     int s0, s1;              // stages [s0, s1) of 256 that cover it (or this CTA's share of them)
-    int refused;             // the range along k begins or ends inside an instruction's 64
 };
 
 // The range along k or of rows that `offsets` gives group g. Offsets that are out of order or out of range are cut to what is there.
@@ -166,7 +165,6 @@ __device__ __forceinline__ Tile decode(const Params &p, const int *cum, int w) {
     int nt, lo = 0, hi = p.tokens, idx;
     t.k0 = 0;
     t.k1 = p.K;
-    t.refused = 0;
     if (p.mode == BY_ROWS) {
         int a = 0, b = p.groups;   // the last group whose first item is not behind w
         while (b - a > 1) {
@@ -184,9 +182,7 @@ __device__ __forceinline__ Tile decode(const Params &p, const int *cum, int w) {
         idx = w - t.group * per_group;
         if (p.mode == ALONG_K) {
             segment(p, t.group, p.K, t.k0, t.k1);
-            if (t.k1 > t.k0) t.refused = t.k0 % UK != 0 || (t.k1 % UK != 0 && t.k1 != p.K);
-            if (t.refused || t.k1 == t.k0) t.k1 = t.k0;   // no stage
-            else t.k1 = (t.k1 + UK - 1) & ~(UK - 1);      // what lies behind K is zero
+            if (t.k1 > t.k0) t.k1 = t.k0 % UK || (t.k1 % UK && t.k1 != p.K) ? -1 : (t.k1 + UK - 1) & ~(UK - 1);   // what lies behind K is zero
         }
     }
     const int np = S::wide ? nt : nw, nq = S::wide ? nw : nt;
@@ -380,7 +376,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm(const __grid_constant__ C
     for (int n = threadIdx.x; n < AHEAD && n * (long long)step + first < total; n += THREADS) {
         const Tile t = decode<S>(p, cum, first + n * step);
         ahead[2 * n] = make_int4(t.group, t.p0, t.p1, t.q0);
-        ahead[2 * n + 1] = make_int4(t.q1, t.k0, t.k1, t.refused);
+        ahead[2 * n + 1] = make_int4(t.q1, t.k0, t.k1, 0);
     }
     __syncthreads();
     auto tile_at = [&](int w, uint32_t n) {   // the n-th tile of this CTA, item w
@@ -388,7 +384,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm(const __grid_constant__ C
         if (n < AHEAD) {
             const int4 a = ahead[2 * n], b = ahead[2 * n + 1];
             t.group = a.x; t.p0 = a.y; t.p1 = a.z; t.q0 = a.w;
-            t.q1 = b.x; t.k0 = b.y; t.k1 = b.z; t.refused = b.w;
+            t.q1 = b.x; t.k0 = b.y; t.k1 = b.z;
         } else t = decode<S>(p, cum, w);
         t.s0 = t.k0 / BK;
         t.s1 = t.k1 > t.k0 ? (t.k1 + BK - 1) / BK : t.s0;
@@ -623,7 +619,7 @@ __global__ void __launch_bounds__(THREADS, 1) mx4_gemm(const __grid_constant__ C
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * BN;
             const bool some = t.s1 > t.s0;   // no stage: nothing was accumulated, the tile is zero (or refused)
-            const uint32_t nothing = uniform(t.refused) ? NOT_A_NUMBER : 0u;
+            const uint32_t nothing = t.k1 < 0 ? NOT_A_NUMBER : 0u;
             if (nothing && quarter == 0 && !half && lane == 0) atomicCAS(p.status, 0, STATUS_OFFSETS);
             const int i0 = t.p0 + (pair ? (int)rank * BP : 0) + quarter * 32;   // the warp's first row of P
             if constexpr (FORM != SPLIT) {
