@@ -1077,13 +1077,15 @@ OZB_API int ozb_expert_mx4_grad(int T, int top, int experts, int N, int K, int R
     cudaStream_t st = (cudaStream_t)stream;
     cudaError_t e = expert_combine_grad(T, top, N, dY, type, lddy, Z, ldz, R, rows, slots, weights, g.dz, N, dweights, st);
     if (!e) e = mx4_quantize_rows(g.dz, type, R, N, N, 0, 1, 0, nullptr, nullptr, 0, 0, g.rows.codes, g.rows.ldq, 0, g.rows.scales, g.rows.lds, 0, st);
-    if (!e) e = mx4_product({1, experts, R, K, N, type, offsets, g.rows.codes, g.rows.ldq, g.rows.scales, g.rows.lds, Wt, ldwt, plane_wt, Wts, ldwts, plane_wts,
-                             g.dxs, K, 0}, status, st);
     if (!e) e = mx4_quantize_cols(g.dz, type, N, R, N, 0, 1, 0, nullptr, nullptr, 0, 0, g.dzt.codes, g.dzt.ldq, 0, g.dzt.scales, g.dzt.lds, 0, st);
     if (!e) e = mx4_quantize_cols(X, type, K, R, ldx, 0, 1, 0, rows, slots, top, T, g.xt.codes, g.xt.ldq, 0, g.xt.scales, g.xt.lds, 0, st);
-    if (!e) e = expert_combine(T, top, K, g.dxs, type, R, K, rows, nullptr, dX, lddx, st);   // behind the last use of X, Z and dY: dX may be one of them
     if (!e) e = mx4_product({2, experts, N, K, R, type, offsets, g.dzt.codes, g.dzt.ldq, g.dzt.scales, g.dzt.lds, g.xt.codes, g.xt.ldq, 0, g.xt.scales, g.xt.lds, 0,
                              dW, lddw, plane_dw}, status, st);
+    if (!e) e = mx4_product({1, experts, R, K, N, type, offsets, g.rows.codes, g.rows.ldq, g.rows.scales, g.rows.lds, Wt, ldwt, plane_wt, Wts, ldwts, plane_wts,
+                             g.dxs, K, 0}, status, st);
+    // dX may be X, Z or dY: it is written last. (In the other orders that allow it, 2048 tokens x 4 of 16 experts, 1536 x 2048, took 119 to 122
+    // us, this one 112: dz is read twice from the L2, and so are the rows that this adds up.)
+    if (!e) e = expert_combine(T, top, K, g.dxs, type, R, K, rows, nullptr, dX, lddx, st);
     return e == cudaErrorInvalidValue ? OZB_ESIZE : (int)e;
 }
 OZB_API int ozb_int8_peak(int iters, int pair, float *ms, double *tops) {
