@@ -23,13 +23,14 @@ import torch
 from . import OzakiError
 from ._lib import lib as _lib
 
-_current_device = torch.cuda.current_device
+_current_device = torch._C._cuda_getDevice         # torch.cuda.current_device where CUDA is in use already, as it is behind a tensor on a GPU
 _raw_stream = torch._C._cuda_getCurrentRawStream   # the number behind torch.cuda.current_stream(index), without making the object
 
 __all__ = ["Mx4", "quantize", "dequantize", "matmul", "grouped_matmul", "segment_matmul", "status"]
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _RULES = {"floor": 0, "ceil": 1}
+_INT32 = torch.int32
 _MOST = 2 ** 31 - 1   # of rows, columns, vectors, values: the library counts in 32 bits (where memory is large enough for more)
 
 
@@ -80,7 +81,7 @@ def _pitch(x, role, dims=2):
         raise TypeError(f"{role} must be on a GPU")
     if stride[-1] != 1 and shape[-1] != 1:
         raise ValueError(f"the rows of {role} must be contiguous; make it contiguous first")
-    if x.numel() > _MOST:
+    if shape[0] > _MOST or shape[-2] > _MOST or shape[-1] > _MOST:
         _few(role, shape)
     return stride[-2] if shape[-2] > 1 else max(stride[-2], shape[-1])
 
@@ -128,14 +129,17 @@ def _offsets(offsets, index):
 
 def _routed(r, index):
     """Checks the maps of a Routing (of experts.sort) on device `index`; (tokens, top)."""
-    for name, t in (("rows", r.rows), ("slots", r.slots)):
-        if t.dtype is not torch.int32 or not t.is_contiguous() or t.get_device() != index:
-            raise ValueError(f"routing.{name} must be contiguous int32 on cuda:{index}")
-        if t.numel() > _MOST:
-            raise ValueError(f"routing.{name} has {t.numel()} numbers, which may not pass {_MOST}")
-    if r.rows.dim() != 2:
+    _, rows, slots, _ = r
+    if not (rows.dtype is _INT32 is slots.dtype and rows.is_contiguous() and slots.is_contiguous() and rows.get_device() == index == slots.get_device()
+            and rows.numel() <= _MOST and slots.numel() <= _MOST):
+        for name, t in (("rows", rows), ("slots", slots)):
+            if t.dtype is not _INT32 or not t.is_contiguous() or t.get_device() != index:
+                raise ValueError(f"routing.{name} must be contiguous int32 on cuda:{index}")
+            _few(f"routing.{name}", (t.numel(),))
+    shape = rows.shape
+    if len(shape) != 2:
         raise ValueError("routing.rows has a row for each token")
-    return r.rows.shape
+    return shape
 
 
 def quantize(x, dim=-1, rule="floor", routing=None):
