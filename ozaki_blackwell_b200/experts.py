@@ -102,7 +102,7 @@ def combine_grad(dy, z, routing, weights=None):
 def matmul(x, w, ids, weights=None, keep=False):
     """y[t] = sum over j of weights[t, j] W[ids[t, j]] x[t]: tokens sorted by expert, rounded to the 4-bit format as they are gathered, one
     product for all experts, and the rows added up by token, in one call of the library. w: Mx4 stack [experts, n, ...] with blocks
-    along the rows of x. keep: returns (y, z, routing) for matmul_grad, with segments padded to 64."""
+    along the rows of x. keep: returns (y, z, routing) for matmul_grad, with segments padded to 64; z's rows behind the last segment are not written."""
     ldx, index = _pitch(x, "x"), x.get_device()
     kind, (tokens, k) = _type(x.dtype), x.shape
     if (ids.dtype is not torch.int32 and ids.dtype is not torch.int64) or ids.dim() != 2 or ids.shape[0] != tokens or not ids.is_contiguous() or ids.get_device() != index or ids.numel() > _MOST:

@@ -156,3 +156,43 @@ def test_rows_past_31_bits():
     del dz
     q, one = mx4.quantize(z, dim=-2), mx4.quantize(z[-64:].contiguous(), dim=-2)
     assert q.length % 64 == 0 and torch.equal(q.codes[:, -32:], one.codes[:, :32])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("tokens,top,experts,h,f", [(5, 2, 7, 96, 80), (300, 3, 5, 256, 200)])
+def test_two_projections_with_a_gate_between(dtype, tokens, top, experts, h, f):
+    """An experts' layer of two products, call by call: rows behind the last segment are nobody's, whatever lies there.
+
+    The first product's rows come from codes, so they are exact (rounded once to `dtype`); what is rounded of them is compared bit for
+    bit; the second product's sums are off by f 2^-23 of their magnitudes and half a unit, the sum over the choices by (top + 1) 2^-24."""
+    from ozaki_blackwell_b200 import experts as ex
+    from ozaki_blackwell_b200 import mx4
+    x, w1, w2 = _codes(1, tokens, h).to(dtype), _codes(2, experts, 2 * f, h) / 8, _codes(3, experts, h, f)
+    g = torch.Generator().manual_seed(4)
+    ids, weights = torch.randint(-1, experts, (tokens, top), generator=g).cuda(), torch.rand(tokens, top, generator=g).cuda()
+    r = ex.sort(ids, experts, 32)
+    rows = r.slots.numel()
+    z = mx4.grouped_matmul(mx4.quantize(x, routing=r), mx4.quantize(w1), r.offsets, dtype, out=torch.full((rows, 2 * f), float("nan"), dtype=dtype, device="cuda"))
+    a = torch.relu(z[:, :f]) * z[:, f:]
+    q = mx4.quantize(a)
+    u = mx4.grouped_matmul(q, mx4.quantize(w2), r.offsets, dtype, out=torch.full((rows, h), float("nan"), dtype=dtype, device="cuda"))
+    y = ex.combine(u, r, weights)
+
+    end, half = r.offsets[-1].item(), torch.finfo(dtype).eps / 2
+    assert bool(torch.isnan(z[end:]).all()) and bool(torch.isnan(u[end:]).all()) and not bool(torch.isnan(z[:end]).any())
+    slots, at = r.slots.cpu().long(), r.rows.cpu().long()
+    want, bound = torch.zeros(tokens, h, dtype=torch.float64), torch.zeros(tokens, h, dtype=torch.float64)
+    xs, w1s, w2s, av = x.cpu().double(), w1.cpu().double(), w2.cpu().double(), ref.values(*ref.quantize(a[:end].float()), f)
+    codes, scales = ref.unpack(mx4.Mx4(q.codes[:end], q.scales[:end], f))
+    assert all(torch.equal(p, s) for p, s in zip((codes, scales), ref.quantize(a[:end].float())))
+    for t in range(tokens):
+        for j in range(top):
+            e, i, c = ids[t, j].item(), at[t, j].item(), weights[t, j].item()
+            if e < 0:
+                continue
+            assert slots[i] == t * top + j and torch.equal(z[i].cpu(), (w1s[e] @ xs[t]).float().to(dtype))
+            part, size = w2s[e] @ av[i], w2s[e].abs() @ av[i].abs()
+            want[t] += c * part
+            bound[t] += c * (f * 2.0 ** -23 * size + half * part.abs())
+            bound[t] += (top + 1) * 2.0 ** -24 * c * (1 + half) * size
+    assert bool(((y.cpu().double() - want).abs() <= bound * (1 + half) + half * want.abs() + torch.finfo(dtype).tiny).all())
