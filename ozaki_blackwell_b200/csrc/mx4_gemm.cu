@@ -34,8 +34,8 @@
 // and turns its own tokens' and all the weights' scales.
 //
 // What bounds it: for one token HBM (18432 x 7168 in 10.4 us, 6.7 TB/s with the weights partly in L2; 14.1 us from HBM); for many, what
-// the L2 delivers. At 2048 x 18432 x 7168 (107 us, 5040 TFLOP/s, 0.76 of four times the measured burst rate of BF16, 0.89 of four times
-// the sustained one) the CTAs fetch 1.2 GB of operands, 11 TB/s, and every other many-token shape comes to the same rate; the clock is
+// the L2 delivers. At 2048 x 18432 x 7168 (109 us, 4980 TFLOP/s, 0.75 of four times the measured burst rate of BF16, 0.88 of four times
+// the sustained one) the CTAs fetch 1.2 GB of operands, 11 TB/s, and every other dense many-token shape comes to the same rate; the clock is
 // then at 1.5 GHz under the power limit. WIDE fetches 40 KB to a stage of 128 x 192, PAIR 56 KB to one of 256 x 192.
 // Every wait is bounded: on expiry the CTA raises the status word, stops, frees its tensor memory and returns.
 #include <type_traits>
