@@ -220,9 +220,9 @@ __device__ __forceinline__ void store_narrow(T *Y, long long ldy, const uint32_t
 // WIDE: Y's row is the lane's. Whole 64-byte pieces of 32 rows go to the warp's shared memory (16-byte words permuted by their row, as
 // the TMA unit's 64-byte swizzle has them, so that no two lanes meet in a bank) and from there by TMA, which takes them while the warp
 // goes on: with stores of its own the warp held its accumulator until the L2 had taken them (segments of 512 tokens: 39 us for 100
-// MB). Where the group's rows end inside the piece, four lanes store 64 contiguous bytes of each row that is there. Rows that do not
-// start on 16 bytes leave the piece value by value, 64 contiguous bytes to a row (14 segments of 289 x 798 BF16: 14 us; from the lanes that
-// have the rows, a sector to a value, about 60).
+// MB). Where the group's rows end inside the piece, or Y's columns inside 16 bytes of it (the unit writes whole ones), four lanes store
+// 64 contiguous bytes of each row that is there. Rows that do not start on 16 bytes leave the piece value by value, 64 contiguous bytes
+// to a row (14 segments of 289 x 798 BF16: 14 us; from the lanes that have the rows, a sector to a value, about 60).
 struct Piece {
     uint8_t *buffer;       // two of 2048 bytes
     uint32_t used;         // pieces so far
@@ -255,7 +255,7 @@ __device__ __forceinline__ void store_wide(const CUtensorMap *map, bool whole_wo
                 if (i0 + r < i1 && col < j1) Y[(size_t)(i0 + r) * ldy + col] = x;
             }
             __syncwarp();
-        } else if (i0 + 32 <= i1) {   // columns behind the last are cut by the tensor map
+        } else if (i0 + 32 <= i1 && (j + h + COLS <= j1 || (j1 - j - h) % N == 0)) {   // columns behind the last are cut by the tensor map, 16 bytes at a time
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) {

@@ -163,3 +163,33 @@ def test_the_layer_and_its_gradients(tokens, top, experts, n, k):
         assert _same(dw[e], (2 * times * dy.double()).t() @ x.double())
     assert _same(y, want_y) and _same(dx, want_dx)
     _status()
+
+
+# pairs with fewer weights than a CTA's half of a tile; rows of Y with a pitch, whose last columns end inside 16 bytes: tokens as lanes, pairs, few tokens
+@gpu
+@pytest.mark.parametrize("m,n,k,pitch", [(20000, 50, 700, 50), (20000, 97, 90, 104), (300, 9601, 300, 9608), (150, 9503, 300, 9504), (1100, 3001, 1090, 3016), (40, 1001, 300, 1008)])
+def test_results_with_a_pitch(m, n, k, pitch):
+    from ozaki_blackwell_b200 import mx4
+    (x, xv), (w, wv) = _operand(k, m, m), _operand(k, n, n)
+    exact = xv @ wv.t()
+    for dtype in TYPES:
+        out = torch.full((m + 2, pitch), 5.0, dtype=dtype, device="cuda")
+        mx4.matmul(x, w, dtype, out=out[1: m + 1, :n])
+        assert _same(out[1: m + 1, :n], exact)
+        assert bool((out[0] == 5).all()) and bool((out[m + 1] == 5).all()) and bool((out[:, n:] == 5).all())
+    _status()
+
+
+@gpu
+@pytest.mark.parametrize("m,n,pitch,gap", [(140, 1501, 1504, 0), (140, 1501, 1504, 3), (1100, 3001, 3008, 2), (20, 301, 304, 1)])
+def test_segments_with_a_pitch(m, n, pitch, gap):
+    from ozaki_blackwell_b200 import mx4
+    offsets = [0, 64, 64, 320, 384, 640, 704, 768, 790]
+    (a, av), (b, bv) = _operand(790, m, m), _operand(790, n, n)
+    for dtype in TYPES:
+        out = torch.full((8, m + gap, pitch), 5.0, dtype=dtype, device="cuda")
+        mx4.segment_matmul(a, b, torch.tensor(offsets, dtype=torch.int32, device="cuda"), dtype, out=out[:, :m, :n])
+        for g in range(8):
+            assert _same(out[g, :m, :n], av[:, offsets[g]: offsets[g + 1]] @ bv[:, offsets[g]: offsets[g + 1]].t())
+        assert bool((out[:, m:] == 5).all()) and bool((out[:, :, n:] == 5).all())
+    _status()
