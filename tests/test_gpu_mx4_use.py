@@ -196,3 +196,40 @@ def test_two_projections_with_a_gate_between(dtype, tokens, top, experts, h, f):
             bound[t] += c * (f * 2.0 ** -23 * size + half * part.abs())
             bound[t] += (top + 1) * 2.0 ** -24 * c * (1 + half) * size
     assert bool(((y.cpu().double() - want).abs() <= bound * (1 + half) + half * want.abs() + torch.finfo(dtype).tiny).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("h,pitch,shift", [(1, 3, 0), (96, 96, 0), (97, 104, 0), (97, 104, 5), (1030, 1032, 0), (1032, 1040, 8), (2050, 2056, 1)])
+def test_nothing_is_written_beside_the_results(dtype, h, pitch, shift):
+    """Results into views: what lies before, behind and between their rows stays as it was. (Every sum is a multiple of 1/4 below 2^22: the
+    order of addition, which alignment changes, does not show.)"""
+    from ozaki_blackwell_b200 import experts as ex
+    from ozaki_blackwell_b200 import mx4
+    from ozaki_blackwell_b200._lib import lib
+    tokens, top, experts = 37, 3, 5
+    x = _codes(1, tokens, h).to(dtype)
+    r = ex.sort(torch.randint(-1, experts, (tokens, top), generator=torch.Generator().manual_seed(2)).cuda(), experts, 8)
+    rows, kind = r.slots.numel(), {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}[dtype]
+
+    def view(n):
+        flat = torch.full((shift + n * pitch + 64,), 7.0, dtype=dtype, device="cuda")
+        return flat, flat[shift: shift + n * pitch].view(n, pitch)[:, :h]
+
+    def untouched(flat, n):
+        part = flat[shift: shift + n * pitch].view(n, pitch)
+        return bool((flat[:shift] == 7).all()) and bool((flat[shift + n * pitch:] == 7).all()) and bool((part[:, h:] == 7).all())
+
+    flat, out = view(rows)
+    z = ex.gather(x, r, out=out)
+    assert torch.equal(z, ex.gather(x, r)) and untouched(flat, rows)
+    flat, out = view(tokens)
+    assert torch.equal(ex.combine(z, r, out=out), ex.combine(z.contiguous(), r)) and untouched(flat, tokens)
+    flat, out = view(rows)
+    weights, dw = torch.full((tokens, top), 0.5, device="cuda"), torch.empty(tokens, top, device="cuda")
+    assert lib.ozb_expert_combine_grad(tokens, top, h, x.data_ptr(), kind, h, z.data_ptr(), z.stride(0), rows, r.rows.data_ptr(), r.slots.data_ptr(), weights.data_ptr(),
+                                       out.data_ptr(), pitch, dw.data_ptr(), torch.cuda.current_stream().cuda_stream) == 0
+    dz, dweights = ex.combine_grad(x, z.contiguous(), r, weights)
+    assert torch.equal(out, dz) and torch.equal(dw, dweights) and untouched(flat, rows)
+    q = mx4.quantize(x)
+    flat, out = view(tokens)
+    assert torch.equal(mx4.dequantize(q, dtype, out=out), x) and untouched(flat, tokens)
